@@ -452,6 +452,96 @@ int quintrit_b200_batch_prefill(quintrit_b200_batch_t* batch, uint32_t sequence,
 int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint32_t* sequences, size_t count, const uint32_t* tokens, uint32_t* out_tokens, float* logits,
                              size_t logits_capacity);
 
+/* ---- a key / value cache in pages, shared by many sequences, and its attention -----------------------------------------
+ * A cache holds `pages` pages of page_tokens positions for each of `layers` layers: keys and values of kv_heads heads of head_dim values, in
+ * F16, BF16, or Q8 (8-bit codes rint(x / d) with one F32 scale d = max|x| / 127 per position and head). Which pages a sequence owns, and in
+ * what order, is the caller's: a page table per sequence. The reference has one contiguous F16 cache per session
+ * (quintrit-runtime/src/kv_cache.rs:24-46) and no counterpart of these functions.
+ *
+ * A call works on a set of rows (quintrit_b200_paged_rows_t): the new tokens of `sequences` sequences, packed one sequence after the other. d_starts,
+ * d_lengths and d_table lie in device memory and are read when the call runs on the GPU: a call captured into a CUDA graph serves what they hold
+ * when it is replayed. The functions enqueue on `stream` (a cudaStream_t of the cache's device, NULL = its default stream) and do not wait; they allocate
+ * nothing. Calls that write the same positions, or read what another writes, are ordered by the caller; otherwise calls may overlap.
+ *
+ * Device data that is out of range (a page number, a token or length outside the table, the angles or the packed rows; a chunk longer than max_new) is
+ * skipped, and quintrit_b200_paged_cache_status reports it. The rows behind the last sequence (d_starts[sequences] and up) are left as they were. */
+#define QUINTRIT_B200_F32 0
+#define QUINTRIT_B200_F16 1
+#define QUINTRIT_B200_BF16 2
+#define QUINTRIT_B200_Q8 3
+
+typedef struct quintrit_b200_paged_cache quintrit_b200_paged_cache_t;
+
+/* page_tokens: 16, 32, 64, 128 or 256; head_dim: 64, 128 or 256; type: F16, BF16 or Q8. A new cache holds zeros. */
+int quintrit_b200_paged_cache_create(uint32_t device_index, uint32_t layers, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, int32_t type,
+                                     quintrit_b200_paged_cache_t** out_cache);
+int quintrit_b200_paged_cache_free(quintrit_b200_paged_cache_t* cache);
+/* The bytes the cache occupies in device memory, and its device (either pointer may be NULL). */
+int quintrit_b200_paged_cache_info(const quintrit_b200_paged_cache_t* cache, size_t* out_device_bytes, uint32_t* out_device);
+/* Whether the calls that have finished on the GPU met anything out of range, since the last call of this function: QUINTRIT_ERR_INVALID_VALUE for a page or position
+ * outside its range, or for a value that was not finite or too large for the stored type (it was stored as the nearest finite value, a NaN as zero: the cache holds finite
+ * values only, so that what a mask hides has no effect); QUINTRIT_ERR_DEVICE if a kernel gave up waiting. Synchronise the streams in question first. */
+int quintrit_b200_paged_cache_status(quintrit_b200_paged_cache_t* cache);
+
+typedef struct quintrit_b200_paged_rows {
+    uint32_t struct_size;
+    uint32_t sequences;        /* 1 to 65535 */
+    uint32_t tokens;           /* rows that the packed arrays of the call have */
+    uint32_t max_new;          /* no sequence has more new tokens than this */
+    uint32_t max_length;       /* no sequence is longer than this, as far as the caller knows: used to divide the work, a longer one is served too */
+    uint32_t table_stride;     /* pages that a sequence's row of the table has room for */
+    const int32_t* d_starts;   /* [sequences + 1], ascending: sequence s has the packed tokens d_starts[s] .. d_starts[s + 1] - 1 (none is allowed) */
+    const int32_t* d_lengths;  /* [sequences]: cached positions, the new tokens included; the last new token is at position d_lengths[s] - 1 */
+    const int32_t* d_table;    /* [sequences][table_stride]: position p lies in page d_table[s][p / page_tokens] */
+} quintrit_b200_paged_rows_t;
+
+/* Appends the new tokens: each query and key head is RMS-normalised with d_q_norm / d_k_norm (head_dim F32 weights; NULL: not), its first rope_dims values are rotated by its
+ * position's row of d_cos_sin ([positions][rope_dims] F32: cos at 2 i, sin at 2 i + 1; NULL: not) in pairs (2 i, 2 i + 1), or (i, i + rope_dims / 2) with neox, and keys and
+ * values are stored, queries written to d_q_out. In F32 arithmetic, rounded once. d_q may be NULL (keys and values only). Strides count elements; pointers and strides are
+ * multiples of 16 bytes; the values of a head are consecutive. d_q_out may be d_q if type and strides agree. */
+typedef struct quintrit_b200_paged_append {
+    uint32_t struct_size;
+    int32_t type;              /* of d_q, d_k and d_v: F32, F16 or BF16 */
+    int32_t q_out_type;        /* F32, F16 or BF16 */
+    uint32_t q_heads;
+    const void *d_q, *d_k, *d_v;
+    size_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    void* d_q_out;
+    size_t out_token_stride, out_head_stride;
+    const float *d_q_norm, *d_k_norm;
+    float norm_eps;
+    const float* d_cos_sin;
+    uint32_t positions, rope_dims;
+    int32_t neox;
+} quintrit_b200_paged_append_t;
+int quintrit_b200_paged_append_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, const quintrit_b200_paged_append_t* args, void* stream);
+
+/* The new tokens' rows of the cache as dense arrays [tokens][kv_heads][head_dim] of `type` (F32, F16 or BF16), 16-byte aligned; either may be NULL. With d_starts counting up by
+ * whole lengths: everything that is cached. */
+int quintrit_b200_paged_read_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, int32_t type, void* d_k, void* d_v, void* stream);
+
+/* Attention of the new tokens over the cached positions up to their own: out = softmax(z) v with z_j = scale q.k_j, or cap tanh(scale q.k_j / cap) with cap > 0, over j <= p and,
+ * with window > 0, j > p - window; query head h reads KV head h / (q_heads / kv_heads). A token that sees nothing gives zeros. q_type: that of the cache, or any of F32, F16,
+ * BF16 over a Q8 cache; out_type: F32, F16 or BF16. Products of 16-bit operands (weights rounded to the cache's type, F16 for Q8) with F32 sums.
+ * d_workspace: quintrit_b200_paged_attention_workspace bytes, 16-byte aligned, not shared with a call that may overlap; need not be kept or cleared. */
+typedef struct quintrit_b200_paged_attention {
+    uint32_t struct_size;
+    int32_t q_type, out_type;
+    uint32_t q_heads;
+    const void* d_q;
+    size_t q_token_stride, q_head_stride;
+    void* d_out;
+    size_t out_token_stride, out_head_stride;
+    float scale, cap;
+    uint32_t window;
+    void* d_workspace;
+    size_t workspace_bytes;
+} quintrit_b200_paged_attention_t;
+/* Enough for every attention call over `cache` with these rows' tokens, sequences, max_new and max_length (the device pointers are not looked at) and that many query heads. */
+int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged_cache_t* cache, const quintrit_b200_paged_rows_t* rows, uint32_t q_heads, size_t* out_bytes);
+int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, const quintrit_b200_paged_attention_t* args,
+                                         void* stream);
+
 /* ---- batched projection on the tensor cores: out[b][n] = sum_k trit[n][k] * act[b][k] for `batch` int8 activation vectors
  * ([batch][cols], row-major), the integers quintrit_b200_gemv_i32 gives vector by vector (so every vector may carry its own
  * activation scale, as the tokens of a prompt do: quintrit-runtime/src/layer.rs:123-177 per token). out is [batch][rows]. The

@@ -35,3 +35,4 @@ from .api import (  # noqa: F401
     selftest_barrier,
     version,
 )
+from .paged import PagedCache, PagedRows  # noqa: F401

@@ -95,24 +95,6 @@ int check_plan(const quintrit_b200_plan* p) {
     return QUINTRIT_OK;
 }
 
-int device_props(int index, cudaDeviceProp* prop) {
-    int n = 0;
-    cudaError_t e = cudaGetDeviceCount(&n);
-    if (e != cudaSuccess) return fail(QUINTRIT_ERR_DEVICE, "no usable CUDA device: %s", cudaGetErrorString(e));
-    if (index < 0 || index >= n) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "GPU index %d does not exist (%d devices)", index, n);
-    QTB_CUDA(cudaGetDeviceProperties(prop, index));
-    return QUINTRIT_OK;
-}
-
-int require_b200(int index, cudaDeviceProp* prop) {
-    int rc = device_props(index, prop);
-    if (rc != QUINTRIT_OK) return rc;
-    if (prop->major != 10)
-        return fail(QUINTRIT_ERR_UNSUPPORTED, "GPU %d (%s, compute capability %d.%d) is not supported: the kernels are built for sm_100a only", index,
-                    prop->name, prop->major, prop->minor);
-    return QUINTRIT_OK;
-}
-
 // Tiles per work item. A table fill costs about as much shared-memory time as streaming 8 row tiles, so items are
 // kept well above that; the environment variable is an experiment knob.
 int item_tiles_override() {
@@ -230,17 +212,6 @@ int check_kernel_status(unsigned int* d_counters) {  // after a synchronisation
     QTB_CUDA(cudaMemcpy(&flag, d_counters + 2, sizeof flag, cudaMemcpyDeviceToHost));
     return gemv_status_error(flag, d_counters);
 }
-
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        cudaGetDevice(&prev);
-        if (prev != dev) cudaSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        if (prev >= 0) cudaSetDevice(prev);
-    }
-};
 
 }  // namespace
 

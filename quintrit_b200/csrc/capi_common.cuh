@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <exception>
+#include <new>
 #include <string>
 
 #include <cuda_runtime.h>
@@ -63,9 +65,45 @@ inline int guard(F&& body) {
     }
 }
 
+inline int device_props(int index, cudaDeviceProp* prop) {
+    int n = 0;
+    cudaError_t e = cudaGetDeviceCount(&n);
+    if (e != cudaSuccess) return fail(QUINTRIT_ERR_DEVICE, "no usable CUDA device: %s", cudaGetErrorString(e));
+    if (index < 0 || index >= n) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "GPU index %d does not exist (%d devices)", index, n);
+    QTB_CUDA(cudaGetDeviceProperties(prop, index));
+    return QUINTRIT_OK;
+}
+
+inline int require_b200(int index, cudaDeviceProp* prop) {
+    int rc = device_props(index, prop);
+    if (rc != QUINTRIT_OK) return rc;
+    if (prop->major != 10)
+        return fail(QUINTRIT_ERR_UNSUPPORTED, "GPU %d (%s, compute capability %d.%d) is not supported: the kernels are built for sm_100a only", index,
+                    prop->name, prop->major, prop->minor);
+    return QUINTRIT_OK;
+}
+
+struct DeviceGuard {
+    int prev = -1;
+    explicit DeviceGuard(int dev) {
+        cudaGetDevice(&prev);
+        if (prev != dev) cudaSetDevice(dev);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
 constexpr uint32_t kMagicMatrix = 0x5154424Du;  // "QTBM"
 constexpr uint32_t kMagicPlan = 0x51544250u;    // "QTBP"
 
 thread_local inline uint64_t g_launches = 0;
+
+#define QTB_LAUNCH_CHECK()                                   \
+    do {                                                     \
+        ++g_launches;                                        \
+        cudaError_t qtb_e_ = cudaGetLastError();             \
+        if (qtb_e_ != cudaSuccess) return cuda_fail(qtb_e_, "kernel launch"); \
+    } while (0)
 
 }  // namespace qtb

@@ -201,13 +201,6 @@ inline void launch_attention(quintrit_b200_decoder* d, AttnArgs at, int n, cudaS
         attention_kernel<<<dim3(d->q_heads, 4, n), kAttnThreads, attention_smem(d->head_dim), s>>>(at);
 }
 
-#define QTB_LAUNCH_CHECK()                                   \
-    do {                                                     \
-        ++g_launches;                                        \
-        cudaError_t qtb_e_ = cudaGetLastError();             \
-        if (qtb_e_ != cudaSuccess) return cuda_fail(qtb_e_, "kernel launch"); \
-    } while (0)
-
 // The launch sequence of one token (gpu.rs:389-453 reshaped: 4 GEMV launches and 5 float kernels per layer).
 inline int enqueue_token(quintrit_b200_decoder* d, bool with_head) {
     if (d->lay) return layered_enqueue_token(d, with_head);

@@ -1,0 +1,340 @@
+// C ABI of the paged key / value cache (declared in include/quintrit_b200.h): handles, checks of arguments, launches.
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "capi_common.cuh"
+#include "paged.hpp"
+#include "paged_attention.cuh"
+#include "paged_rows.cuh"
+
+using namespace qtb;
+
+namespace {
+
+constexpr uint32_t kMagicPaged = 0x51545047u;  // "QTPG"
+constexpr unsigned int kPagedSpin = 1u << 20;  // tries of a wait (up to 20 us each) before it gives up
+
+int check_cache(const quintrit_b200_paged_cache* c) {
+    if (c == nullptr || c->magic != kMagicPaged) return fail(QUINTRIT_ERR_INVALID_HANDLE, "paged cache handle is NULL, freed or of the wrong type");
+    return QUINTRIT_OK;
+}
+int check_layer(const quintrit_b200_paged_cache* c, uint32_t layer) {
+    if (layer >= c->layers) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "layer %u of %u", layer, c->layers);
+    return QUINTRIT_OK;
+}
+int check_rows(const quintrit_b200_paged_cache*, const quintrit_b200_paged_rows_t* r, bool pointers) {
+    if (r == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "rows is NULL");
+    if (r->struct_size < sizeof(quintrit_b200_paged_rows_t)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.struct_size %u is too small", r->struct_size);
+    if (r->sequences == 0 || r->sequences > 65535) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "sequences must be in [1, 65535], got %u", r->sequences);
+    if (r->tokens > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "at most 2^24 tokens, got %u", r->tokens);
+    if (r->table_stride == 0 || r->table_stride > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "table_stride must be in [1, 2^24], got %u", r->table_stride);
+    if (r->tokens != 0 && (r->max_new == 0 || r->max_new > r->tokens)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_new %u must be in [1, tokens = %u]", r->max_new, r->tokens);
+    if (r->max_length > 0x7fff0000u) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_length %u is too large", r->max_length);
+    if (pointers && (r->d_starts == nullptr || r->d_lengths == nullptr || r->d_table == nullptr)) return fail(QUINTRIT_ERR_NULL_POINTER, "rows.d_starts, d_lengths or d_table is NULL");
+    if (pointers && (reinterpret_cast<uintptr_t>(r->d_starts) % 4 != 0 || reinterpret_cast<uintptr_t>(r->d_lengths) % 4 != 0 || reinterpret_cast<uintptr_t>(r->d_table) % 4 != 0))
+        return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.d_starts, d_lengths and d_table must be 4-byte aligned");
+    return QUINTRIT_OK;
+}
+bool dense_type(int32_t t) { return t == kPagedF32 || t == kPagedF16 || t == kPagedBf16; }
+int check_array(const char* name, const void* p, int32_t type, std::initializer_list<size_t> strides) {
+    if (p == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "%s is NULL", name);
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned", name);
+    for (size_t s : strides)
+        if (s * paged_size_of(type) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "%s: a stride of %zu elements is not a multiple of 16 bytes", name, s);
+    return QUINTRIT_OK;
+}
+
+PagedView view_of(const quintrit_b200_paged_cache* c, uint32_t layer) {
+    PagedView v{};
+    v.k = c->k + layer * c->layer_bytes, v.v = c->v + layer * c->layer_bytes;
+    if (c->type == kPagedQ8) v.ks = c->ks + layer * c->layer_scales, v.vs = c->vs + layer * c->layer_scales;
+    int log2 = 0;
+    while ((1u << log2) < c->page_tokens) ++log2;
+    v.pages = static_cast<int>(c->pages), v.page_log2 = log2, v.kv_heads = static_cast<int>(c->kv_heads), v.blocks = static_cast<int>(c->head_dim) / kPagedBlock;
+    v.status = c->status;
+    return v;
+}
+RowsView view_of(const quintrit_b200_paged_rows_t* r) {
+    RowsView v{};
+    v.starts = r->d_starts, v.lengths = r->d_lengths, v.table = r->d_table;
+    v.sequences = static_cast<int>(r->sequences), v.tokens = static_cast<int>(r->tokens), v.stride = static_cast<int>(r->table_stride);
+    return v;
+}
+void destroy(quintrit_b200_paged_cache* c) {
+    if (c == nullptr) return;
+    DeviceGuard g(c->device);
+    cudaFree(c->k);
+    cudaFree(c->v);
+    cudaFree(c->ks);
+    cudaFree(c->vs);
+    cudaFree(c->status);
+    c->magic = 0;
+    delete c;
+}
+
+// How the positions are cut into ranges: enough blocks of threads to fill the device, ranges of at least four tiles.
+struct PagedCut {
+    int splits, split, most;  // most: no window makes more ranges of it
+};
+PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, int row_tiles) {
+    long long span = std::max<uint32_t>(r->max_length, 1);
+    if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
+    const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_tiles;
+    const long long want = std::max<long long>(1, std::min<long long>({(4LL * c->sm_count + items - 1) / items, (tiles + 3) / 4, 128}));
+    const long long per = (tiles + want - 1) / want;
+    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile), static_cast<int>(want)};
+}
+
+template <int TYPE, int BLOCKS, int RT>
+int launch_few(const PagedAttnArgs& a, dim3 grid, cudaStream_t s) {
+    constexpr int smem = paged_few_smem<TYPE, BLOCKS, RT>();
+    static_assert(smem <= 227 * 1024, "the ring does not fit");
+    QTB_CUDA(cudaFuncSetAttribute(paged_few_kernel<TYPE, BLOCKS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    paged_few_kernel<TYPE, BLOCKS, RT><<<grid, 32 + 128 * RT, smem, s>>>(a);
+    QTB_LAUNCH_CHECK();
+    return QUINTRIT_OK;
+}
+template <int TYPE, int BLOCKS>
+int launch_few_rows(const PagedAttnArgs& a, int rt, dim3 grid, cudaStream_t s) {
+    return rt == 1 ? launch_few<TYPE, BLOCKS, 1>(a, grid, s) : launch_few<TYPE, BLOCKS, 2>(a, grid, s);
+}
+template <int TYPE>
+int launch_few_type(const PagedAttnArgs& a, int rt, dim3 grid, cudaStream_t s) {
+    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, rt, grid, s) : launch_few_rows<TYPE, 4>(a, rt, grid, s);
+}
+int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a block of threads
+
+}  // namespace
+
+extern "C" int quintrit_b200_paged_cache_create(uint32_t device_index, uint32_t layers, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, int32_t type,
+                                                quintrit_b200_paged_cache_t** out_cache) {
+    return guard([&]() -> int {
+        if (out_cache == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "out_cache is NULL");
+        *out_cache = nullptr;
+        if (layers == 0 || layers > 4096) return fail(QUINTRIT_ERR_INVALID_SHAPE, "layers must be in [1, 4096], got %u", layers);
+        if (pages == 0 || pages > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_SHAPE, "pages must be in [1, 2^24], got %u", pages);
+        if (page_tokens < 16 || page_tokens > 256 || (page_tokens & (page_tokens - 1)) != 0) return fail(QUINTRIT_ERR_INVALID_SHAPE, "page_tokens must be 16, 32, 64, 128 or 256, got %u", page_tokens);
+        if (kv_heads == 0 || kv_heads > 1024) return fail(QUINTRIT_ERR_INVALID_SHAPE, "kv_heads must be in [1, 1024], got %u", kv_heads);
+        if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(QUINTRIT_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256, got %u", head_dim);
+        if (type != kPagedF16 && type != kPagedBf16 && type != kPagedQ8) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "cache type %d: F16, BF16 or Q8", type);
+        cudaDeviceProp prop;
+        int rc = require_b200(static_cast<int>(device_index), &prop);
+        if (rc != QUINTRIT_OK) return rc;
+        DeviceGuard g(static_cast<int>(device_index));
+        quintrit_b200_paged_cache* c = new quintrit_b200_paged_cache();
+        c->magic = kMagicPaged, c->device = static_cast<int>(device_index), c->sm_count = prop.multiProcessorCount;
+        c->layers = layers, c->pages = pages, c->page_tokens = page_tokens, c->kv_heads = kv_heads, c->head_dim = head_dim, c->type = type;
+        c->layer_scales = static_cast<size_t>(pages) * kv_heads * page_tokens;
+        c->layer_bytes = c->layer_scales * head_dim * paged_size_of(type);
+        auto alloc = [&](void** p, size_t bytes, int fill = 0) -> cudaError_t {
+            cudaError_t e = cudaMalloc(p, bytes);
+            if (e == cudaSuccess) e = cudaMemset(*p, fill, bytes);
+            c->device_bytes += bytes;
+            return e;
+        };
+        cudaError_t e = alloc(reinterpret_cast<void**>(&c->k), layers * c->layer_bytes);
+        if (e == cudaSuccess) e = alloc(reinterpret_cast<void**>(&c->v), layers * c->layer_bytes);
+        if (e == cudaSuccess && type == kPagedQ8) e = alloc(reinterpret_cast<void**>(&c->ks), layers * c->layer_scales * sizeof(float), kPagedFreshScale);
+        if (e == cudaSuccess && type == kPagedQ8) e = alloc(reinterpret_cast<void**>(&c->vs), layers * c->layer_scales * sizeof(float), kPagedFreshScale);
+        if (e == cudaSuccess) e = alloc(reinterpret_cast<void**>(&c->status), 16);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // the zeros are there before a call on any stream
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            destroy(c);
+            return cuda_fail(e, "cudaMalloc(paged cache)");
+        }
+        *out_cache = c;
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_paged_cache_free(quintrit_b200_paged_cache_t* cache) {
+    return guard([&]() -> int {
+        if (cache == nullptr) return ok();
+        const int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK) return rc;
+        destroy(cache);
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_paged_cache_info(const quintrit_b200_paged_cache_t* cache, size_t* out_device_bytes, uint32_t* out_device) {
+    return guard([&]() -> int {
+        const int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK) return rc;
+        if (out_device_bytes) *out_device_bytes = cache->device_bytes;
+        if (out_device) *out_device = static_cast<uint32_t>(cache->device);
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_paged_cache_status(quintrit_b200_paged_cache_t* cache) {
+    return guard([&]() -> int {
+        const int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK) return rc;
+        DeviceGuard g(cache->device);
+        unsigned int bits = 0;
+        QTB_CUDA(cudaMemcpy(&bits, cache->status, sizeof bits, cudaMemcpyDeviceToHost));
+        if (bits == 0) return ok();
+        QTB_CUDA(cudaMemset(cache->status, 0, sizeof bits));
+        if (bits & kPagedGaveUp) return fail(QUINTRIT_ERR_DEVICE, "the paged attention kernel on the CUDA device gave up waiting for its copies");
+        if (bits & kPagedBadPage) return fail(QUINTRIT_ERR_INVALID_VALUE, "a page table named a page that the cache does not have (%u pages)", cache->pages);
+        if (bits & kPagedBadPosition) return fail(QUINTRIT_ERR_INVALID_VALUE, "a token or length lay outside the page table, the angles or the packed rows, or a chunk was longer than announced");
+        return fail(QUINTRIT_ERR_INVALID_VALUE, "a key or value was not finite or too large for the cache's type");
+    });
+}
+
+extern "C" int quintrit_b200_paged_append_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, const quintrit_b200_paged_append_t* args,
+                                                 void* stream) {
+    return guard([&]() -> int {
+        int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK || (rc = check_layer(cache, layer)) != QUINTRIT_OK || (rc = check_rows(cache, rows, true)) != QUINTRIT_OK) return rc;
+        if (args == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "args is NULL");
+        if (args->struct_size < sizeof(quintrit_b200_paged_append_t)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "args.struct_size %u is too small", args->struct_size);
+        if (!dense_type(args->type)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "type %d: F32, F16 or BF16", args->type);
+        if (rows->tokens == 0) return ok();
+        PagedAppendArgs a{};
+        if (args->d_q != nullptr) {
+            if (!dense_type(args->q_out_type)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "q_out_type %d: F32, F16 or BF16", args->q_out_type);
+            if (args->q_heads == 0 || args->q_heads > 65536) return fail(QUINTRIT_ERR_INVALID_SHAPE, "q_heads must be in [1, 65536], got %u", args->q_heads);
+            if ((rc = check_array("d_q", args->d_q, args->type, {args->q_token_stride, args->q_head_stride})) != QUINTRIT_OK ||
+                (rc = check_array("d_q_out", args->d_q_out, args->q_out_type, {args->out_token_stride, args->out_head_stride})) != QUINTRIT_OK)
+                return rc;
+            if (args->d_q == args->d_q_out && (args->type != args->q_out_type || args->q_token_stride != args->out_token_stride || args->q_head_stride != args->out_head_stride))
+                return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_q_out may be d_q only with the same type and strides");
+            a.q_heads = static_cast<int>(args->q_heads);
+        }
+        if ((rc = check_array("d_k", args->d_k, args->type, {args->k_token_stride, args->k_head_stride})) != QUINTRIT_OK ||
+            (rc = check_array("d_v", args->d_v, args->type, {args->v_token_stride, args->v_head_stride})) != QUINTRIT_OK)
+            return rc;
+        for (const float* w : {args->d_q_norm, args->d_k_norm})
+            if (reinterpret_cast<uintptr_t>(w) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_q_norm and d_k_norm must be 16-byte aligned");
+        if ((args->d_q_norm != nullptr || args->d_k_norm != nullptr) && !(args->norm_eps >= 0.0f && std::isfinite(args->norm_eps)))
+            return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "norm_eps must be finite and not negative");
+        if (args->d_cos_sin != nullptr) {
+            if (args->rope_dims < 2 || args->rope_dims % 2 != 0 || args->rope_dims > cache->head_dim)
+                return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rope_dims must be even and in [2, head_dim = %u], got %u", cache->head_dim, args->rope_dims);
+            if (args->positions == 0 || args->positions > 0x7fffffffu) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "positions must be in [1, 2^31 - 1], got %u", args->positions);
+            if (reinterpret_cast<uintptr_t>(args->d_cos_sin) % 4 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_cos_sin must be 4-byte aligned");
+        }
+        DeviceGuard g(cache->device);
+        a.c = view_of(cache, layer), a.r = view_of(rows);
+        a.type = cache->type, a.in_type = args->type, a.q_type = args->q_out_type;
+        a.q = args->d_q, a.k = args->d_k, a.v = args->d_v, a.q_out = args->d_q_out;
+        a.q_token = args->q_token_stride, a.q_head = args->q_head_stride, a.k_token = args->k_token_stride, a.k_head = args->k_head_stride, a.v_token = args->v_token_stride,
+        a.v_head = args->v_head_stride, a.o_token = args->out_token_stride, a.o_head = args->out_head_stride;
+        a.q_norm = args->d_q_norm, a.k_norm = args->d_k_norm, a.eps = args->norm_eps;
+        a.cos_sin = args->d_cos_sin, a.rope = static_cast<int>(args->rope_dims), a.positions = static_cast<int>(args->positions), a.neox = args->neox;
+        const int lanes = static_cast<int>(cache->head_dim) / 8, per_warp = 32 / lanes, heads = a.q_heads + 2 * a.c.kv_heads;
+        const long long warps = static_cast<long long>(rows->tokens) * ((heads + per_warp - 1) / per_warp), blocks = (warps + 7) / 8;
+        if (warps > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", rows->tokens, heads);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        auto kernel = lanes == 8 ? paged_append_kernel<8> : lanes == 16 ? paged_append_kernel<16> : paged_append_kernel<32>;
+        kernel<<<static_cast<unsigned int>(blocks), kPagedRowThreads, 0, s>>>(a);
+        QTB_LAUNCH_CHECK();
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_paged_read_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, int32_t type, void* d_k, void* d_v, void* stream) {
+    return guard([&]() -> int {
+        int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK || (rc = check_layer(cache, layer)) != QUINTRIT_OK || (rc = check_rows(cache, rows, true)) != QUINTRIT_OK) return rc;
+        if (!dense_type(type)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "type %d: F32, F16 or BF16", type);
+        if (rows->tokens == 0) return ok();
+        if (d_k == nullptr && d_v == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_k and d_v are NULL");
+        if ((d_k != nullptr && (rc = check_array("d_k", d_k, type, {})) != QUINTRIT_OK) || (d_v != nullptr && (rc = check_array("d_v", d_v, type, {})) != QUINTRIT_OK)) return rc;
+        DeviceGuard g(cache->device);
+        PagedReadArgs a{};
+        a.c = view_of(cache, layer), a.r = view_of(rows), a.type = cache->type, a.out_type = type, a.k = d_k, a.v = d_v;
+        const int lanes = static_cast<int>(cache->head_dim) / 8, per_warp = 32 / lanes, heads = 2 * a.c.kv_heads;
+        const long long warps = static_cast<long long>(rows->tokens) * ((heads + per_warp - 1) / per_warp), blocks = (warps + 7) / 8;
+        if (warps > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", rows->tokens, heads);
+        auto kernel = lanes == 8 ? paged_read_kernel<8> : lanes == 16 ? paged_read_kernel<16> : paged_read_kernel<32>;
+        kernel<<<static_cast<unsigned int>(blocks), kPagedRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+        QTB_LAUNCH_CHECK();
+        return ok();
+    });
+}
+
+namespace {
+int check_heads(const quintrit_b200_paged_cache* c, uint32_t q_heads) {
+    if (q_heads == 0 || q_heads % c->kv_heads != 0 || q_heads > 65536) return fail(QUINTRIT_ERR_INVALID_SHAPE, "q_heads %u must be a multiple of kv_heads = %u", q_heads, c->kv_heads);
+    return QUINTRIT_OK;
+}
+size_t workspace_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, int splits) {
+    return splits > 1 ? static_cast<size_t>(splits) * r->tokens * q_heads * (c->head_dim * sizeof(float) + sizeof(float2)) : 0;
+}
+}  // namespace
+
+extern "C" int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged_cache_t* cache, const quintrit_b200_paged_rows_t* rows, uint32_t q_heads, size_t* out_bytes) {
+    return guard([&]() -> int {
+        int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK) return rc;
+        if (out_bytes == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "out_bytes is NULL");
+        *out_bytes = 0;
+        if ((rc = check_rows(cache, rows, false)) != QUINTRIT_OK || (rc = check_heads(cache, q_heads)) != QUINTRIT_OK) return rc;
+        if (rows->tokens == 0) return ok();
+        const int most = static_cast<int>(rows->max_new * (q_heads / cache->kv_heads)), rt = row_tiles_of(most), tiles = (most + 16 * rt - 1) / (16 * rt);
+        *out_bytes = workspace_of(cache, rows, q_heads, cut_of(cache, rows, 0, tiles).most);
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, const quintrit_b200_paged_attention_t* args,
+                                                    void* stream) {
+    return guard([&]() -> int {
+        int rc = check_cache(cache);
+        if (rc != QUINTRIT_OK || (rc = check_layer(cache, layer)) != QUINTRIT_OK || (rc = check_rows(cache, rows, true)) != QUINTRIT_OK) return rc;
+        if (args == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "args is NULL");
+        if (args->struct_size < sizeof(quintrit_b200_paged_attention_t)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "args.struct_size %u is too small", args->struct_size);
+        if (!dense_type(args->q_type) || (cache->type != kPagedQ8 && args->q_type != cache->type))
+            return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "q_type %d: the cache's type, or F32, F16 or BF16 over a Q8 cache", args->q_type);
+        if (!dense_type(args->out_type)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "out_type %d: F32, F16 or BF16", args->out_type);
+        if ((rc = check_heads(cache, args->q_heads)) != QUINTRIT_OK) return rc;
+        if (!std::isfinite(args->scale)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "scale must be finite");
+        if (!(args->cap >= 0.0f) || !std::isfinite(args->cap)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "cap must be finite and not negative (0: none)");
+        if (args->window > 0x7fffffffu) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "window %u is too large", args->window);
+        if (rows->tokens == 0) return ok();
+        if ((rc = check_array("d_q", args->d_q, args->q_type, {args->q_token_stride, args->q_head_stride})) != QUINTRIT_OK ||
+            (rc = check_array("d_out", args->d_out, args->out_type, {args->out_token_stride, args->out_head_stride})) != QUINTRIT_OK)
+            return rc;
+        const int group = static_cast<int>(args->q_heads / cache->kv_heads);
+        const long long most = static_cast<long long>(rows->max_new) * group;
+        const int rt = row_tiles_of(static_cast<int>(std::min<long long>(most, 1 << 30)));
+        const long long tiles = (most + 16 * rt - 1) / (16 * rt);
+        if (tiles * cache->kv_heads > 65535) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
+        const PagedCut cut = cut_of(cache, rows, args->window, static_cast<int>(tiles));
+        const size_t need = workspace_of(cache, rows, args->q_heads, cut.splits);
+        if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);
+        if (need > args->workspace_bytes) return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "the workspace holds %zu bytes, %zu are needed", args->workspace_bytes, need);
+        if (need > 0 && reinterpret_cast<uintptr_t>(args->d_workspace) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_workspace must be 16-byte aligned");
+        DeviceGuard g(cache->device);
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        PagedAttnArgs a{};
+        a.c = view_of(cache, layer), a.r = view_of(rows);
+        a.q = args->d_q, a.q_token = args->q_token_stride, a.q_head = args->q_head_stride, a.q_type = args->q_type;
+        a.out = args->d_out, a.o_token = args->out_token_stride, a.o_head = args->out_head_stride, a.out_type = args->out_type;
+        a.group = group;
+        a.scale = args->cap > 0.0f ? args->scale / args->cap : args->scale * kLog2e;
+        a.cap = args->cap * kLog2e;
+        a.window = static_cast<int>(args->window);
+        a.splits = cut.splits, a.split = cut.split;
+        a.part_o = static_cast<float*>(args->d_workspace);
+        if (need > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(cut.splits) * rows->tokens * args->q_heads * cache->head_dim);
+        a.few = 1, a.many = a.most = static_cast<int>(rows->max_new);
+        a.spin_limit = kPagedSpin;
+        const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cache->kv_heads * tiles), rows->sequences);
+        rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, rt, grid, s) : launch_few_type<kPagedQ8>(a, rt, grid, s);
+        if (rc != QUINTRIT_OK) return rc;
+        if (cut.splits > 1) {
+            const long long items = static_cast<long long>(rows->tokens) * args->q_heads;
+            const unsigned blocks = static_cast<unsigned>((items + 7) / 8);
+            auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
+            kernel<<<blocks, 256, 0, s>>>(a);
+            QTB_LAUNCH_CHECK();
+        }
+        return ok();
+    });
+}
