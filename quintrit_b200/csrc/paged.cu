@@ -1,7 +1,9 @@
 // C ABI of the paged key / value cache (declared in include/quintrit_b200.h): handles, checks of arguments, launches.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 #include "capi_common.cuh"
 #include "paged.hpp"
@@ -73,6 +75,25 @@ void destroy(quintrit_b200_paged_cache* c) {
     delete c;
 }
 
+struct AppendKernel {
+    template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_append_kernel<LANES, TYPE, U>; }
+};
+struct ReadKernel {
+    template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_read_kernel<LANES, TYPE, U>; }
+};
+// A warp takes four groups of heads where that leaves a few warps for every place of the device, else one.
+template <typename Kernel, int LANES, int TYPE, typename Args>
+int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void* stream) {
+    constexpr int kHeads = 32 / LANES, kWarps = kPagedRowThreads / 32;
+    const long long one = static_cast<long long>(tokens) * ((heads + kHeads - 1) / kHeads), four = static_cast<long long>(tokens) * ((heads + 4 * kHeads - 1) / (4 * kHeads));
+    if (one > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", tokens, heads);
+    const bool many = four >= 64LL * sm_count;
+    auto kernel = many ? Kernel::template of<LANES, TYPE, 4>() : Kernel::template of<LANES, TYPE, 1>();
+    kernel<<<static_cast<unsigned int>(((many ? four : one) + kWarps - 1) / kWarps), kPagedRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    QTB_LAUNCH_CHECK();
+    return QUINTRIT_OK;
+}
+
 // How the positions are cut into ranges: enough blocks of threads to fill the device, ranges of at least four tiles.
 struct PagedCut {
     int splits, split, most;  // most: no window makes more ranges of it
@@ -86,22 +107,34 @@ PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_ro
     return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile), static_cast<int>(want)};
 }
 
+// The shared memory a kernel may ask for, raised once per device (`done`: a bit per device; two threads at once set the same).
+template <typename Kernel>
+int allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t>& done) {
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit) != 0) return QUINTRIT_OK;
+    QTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return QUINTRIT_OK;
+}
+
 template <int TYPE, int BLOCKS, int RT>
-int launch_few(const PagedAttnArgs& a, dim3 grid, cudaStream_t s) {
+int launch_few(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
     constexpr int smem = paged_few_smem<TYPE, BLOCKS, RT>();
     static_assert(smem <= 227 * 1024, "the ring does not fit");
-    QTB_CUDA(cudaFuncSetAttribute(paged_few_kernel<TYPE, BLOCKS, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<uint64_t> done{0};
+    const int rc = allow_smem(paged_few_kernel<TYPE, BLOCKS, RT>, smem, device, done);
+    if (rc != QUINTRIT_OK) return rc;
     paged_few_kernel<TYPE, BLOCKS, RT><<<grid, 32 + 128 * RT, smem, s>>>(a);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
 template <int TYPE, int BLOCKS>
-int launch_few_rows(const PagedAttnArgs& a, int rt, dim3 grid, cudaStream_t s) {
-    return rt == 1 ? launch_few<TYPE, BLOCKS, 1>(a, grid, s) : launch_few<TYPE, BLOCKS, 2>(a, grid, s);
+int launch_few_rows(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
+    return rt == 1 ? launch_few<TYPE, BLOCKS, 1>(a, device, grid, s) : launch_few<TYPE, BLOCKS, 2>(a, device, grid, s);
 }
 template <int TYPE>
-int launch_few_type(const PagedAttnArgs& a, int rt, dim3 grid, cudaStream_t s) {
-    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, rt, grid, s) : launch_few_rows<TYPE, 4>(a, rt, grid, s);
+int launch_few_type(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
+    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, rt, grid, s) : launch_few_rows<TYPE, 4>(a, device, rt, grid, s);
 }
 int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a block of threads
 
@@ -225,14 +258,17 @@ extern "C" int quintrit_b200_paged_append_device(quintrit_b200_paged_cache_t* ca
         a.q_token = args->q_token_stride, a.q_head = args->q_head_stride, a.k_token = args->k_token_stride, a.k_head = args->k_head_stride, a.v_token = args->v_token_stride,
         a.v_head = args->v_head_stride, a.o_token = args->out_token_stride, a.o_head = args->out_head_stride;
         a.q_norm = args->d_q_norm, a.k_norm = args->d_k_norm, a.eps = args->norm_eps;
-        a.cos_sin = args->d_cos_sin, a.rope = static_cast<int>(args->rope_dims), a.positions = static_cast<int>(args->positions), a.neox = args->neox;
-        const int lanes = static_cast<int>(cache->head_dim) / 8, per_warp = 32 / lanes, heads = a.q_heads + 2 * a.c.kv_heads;
-        const long long warps = static_cast<long long>(rows->tokens) * ((heads + per_warp - 1) / per_warp), blocks = (warps + 7) / 8;
-        if (warps > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", rows->tokens, heads);
-        cudaStream_t s = static_cast<cudaStream_t>(stream);
-        auto kernel = lanes == 8 ? paged_append_kernel<8> : lanes == 16 ? paged_append_kernel<16> : paged_append_kernel<32>;
-        kernel<<<static_cast<unsigned int>(blocks), kPagedRowThreads, 0, s>>>(a);
-        QTB_LAUNCH_CHECK();
+        a.cos_sin = args->d_cos_sin, a.rope = static_cast<int>(args->rope_dims), a.positions = static_cast<int>(args->positions), a.neox = args->neox != 0;
+        a.vector = a.rope % (a.neox ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0;
+        auto launch = [&](auto type) {
+            constexpr int T = decltype(type)::value;
+            return cache->head_dim == 64 ? launch_rows_of<AppendKernel, 8, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream)
+                 : cache->head_dim == 128 ? launch_rows_of<AppendKernel, 16, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream)
+                                          : launch_rows_of<AppendKernel, 32, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream);
+        };
+        rc = args->type == kPagedF32 ? launch(std::integral_constant<int, kPagedF32>()) : args->type == kPagedF16 ? launch(std::integral_constant<int, kPagedF16>())
+                                                                                                                  : launch(std::integral_constant<int, kPagedBf16>());
+        if (rc != QUINTRIT_OK) return rc;
         return ok();
     });
 }
@@ -248,12 +284,15 @@ extern "C" int quintrit_b200_paged_read_device(quintrit_b200_paged_cache_t* cach
         DeviceGuard g(cache->device);
         PagedReadArgs a{};
         a.c = view_of(cache, layer), a.r = view_of(rows), a.type = cache->type, a.out_type = type, a.k = d_k, a.v = d_v;
-        const int lanes = static_cast<int>(cache->head_dim) / 8, per_warp = 32 / lanes, heads = 2 * a.c.kv_heads;
-        const long long warps = static_cast<long long>(rows->tokens) * ((heads + per_warp - 1) / per_warp), blocks = (warps + 7) / 8;
-        if (warps > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", rows->tokens, heads);
-        auto kernel = lanes == 8 ? paged_read_kernel<8> : lanes == 16 ? paged_read_kernel<16> : paged_read_kernel<32>;
-        kernel<<<static_cast<unsigned int>(blocks), kPagedRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-        QTB_LAUNCH_CHECK();
+        auto launch = [&](auto of) {
+            constexpr int T = decltype(of)::value;
+            return cache->head_dim == 64 ? launch_rows_of<ReadKernel, 8, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream)
+                 : cache->head_dim == 128 ? launch_rows_of<ReadKernel, 16, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream)
+                                          : launch_rows_of<ReadKernel, 32, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream);
+        };
+        rc = cache->type == kPagedF16 ? launch(std::integral_constant<int, kPagedF16>()) : cache->type == kPagedBf16 ? launch(std::integral_constant<int, kPagedBf16>())
+                                                                                                                     : launch(std::integral_constant<int, kPagedQ8>());
+        if (rc != QUINTRIT_OK) return rc;
         return ok();
     });
 }
@@ -326,7 +365,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         a.few = 1, a.many = a.most = static_cast<int>(rows->max_new);
         a.spin_limit = kPagedSpin;
         const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cache->kv_heads * tiles), rows->sequences);
-        rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, rt, grid, s) : launch_few_type<kPagedQ8>(a, rt, grid, s);
+        rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, cache->device, rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, cache->device, rt, grid, s) : launch_few_type<kPagedQ8>(a, cache->device, rt, grid, s);
         if (rc != QUINTRIT_OK) return rc;
         if (cut.splits > 1) {
             const long long items = static_cast<long long>(rows->tokens) * args->q_heads;

@@ -7,8 +7,9 @@
 // Reading (paged_read_kernel): the same rows back, code times scale, rounded to the output type.
 //
 // Eight values to a thread (16 bytes of a 16-bit type, 8 codes), 8 to 32 threads to a head: norm and maximum are exchanges within those threads, and a
-// row of the cache is written once. Both are bound by the bytes they move, small calls by their latency: the addresses need four dependent reads
-// (starts, length, page, row), behind which the head's values are already on their way.
+// row of the cache is written once. A warp takes U such groups of heads of one token. Both kernels are bound by the bytes they move, small calls by
+// their latency: a row's address needs four dependent reads (starts, length, page), so the heads' values are asked for before them, and where there are
+// tokens enough for it, four groups of heads share one address (U = 4).
 #pragma once
 #include "paged_cache.cuh"
 
@@ -29,117 +30,179 @@ struct PagedAppendArgs {
     float eps;
     const float* cos_sin;            // [positions][rope]: cos at 2 i, sin at 2 i + 1; nullptr: no rotation
     int rope, positions, neox;
+    int vector;                      // eight values of a thread share 16-byte pieces of an angles' row: rope a multiple of 8, with neox of 16, rows on 16-byte boundaries
     int q_heads;                     // 0 where q is nullptr
 };
 
-template <int LANES>  // threads of a head: head_dim / 8
+// A token's place in the cache, by a whole warp: page < 0 where the token is behind the last sequence or something is out of range (then reported).
+struct PagedPlace {
+    int pos, page, row;
+};
+__device__ __forceinline__ PagedPlace paged_place(const PagedView& c, const RowsView& r, int t, int positions) {
+    PagedPlace p{0, -1, 0};
+    const int s = paged_sequence_of(r, t);
+    if (s < 0) return p;
+    const PagedSequence sq = paged_sequence(c, r, s);
+    if (!sq.ok || t < sq.first || t >= sq.first + sq.news) return p;
+    p.pos = sq.length - sq.news + (t - sq.first);
+    if (p.pos < 0 || p.pos >= positions) {
+        if ((threadIdx.x & 31) == 0) atomicOr(c.status, kPagedBadPosition);
+        return p;
+    }
+    p.row = p.pos & ((1 << c.page_log2) - 1), p.page = r.table[static_cast<size_t>(s) * r.stride + (p.pos >> c.page_log2)];
+    if (p.page < 0 || p.page >= c.pages) {
+        if ((threadIdx.x & 31) == 0) atomicOr(c.status, kPagedBadPage);
+        p.page = -1;
+    }
+    return p;
+}
+
+// Eight values of a head as they lie in memory, and as 32-bit values.
+template <int TYPE> struct PagedRaw { uint4 v[TYPE == kPagedF32 ? 2 : 1]; };
+template <int TYPE>
+__device__ __forceinline__ PagedRaw<TYPE> paged_raw(const void* base, size_t element) {
+    PagedRaw<TYPE> r;
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + element * paged_size_of(TYPE));
+    r.v[0] = *p;
+    if constexpr (TYPE == kPagedF32) r.v[1] = p[1];
+    return r;
+}
+
+template <int LANES, int TYPE, int U>  // threads of a head: head_dim / 8; type of q, k and v; groups of heads of a warp
 __global__ void __launch_bounds__(kPagedRowThreads) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
-    constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a warp
-    __shared__ float exchange[kPagedRowThreads / 32][kHeads][HD];  // NEOX pairs lie half a rotation apart
+    constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a group
+    __shared__ __align__(16) float exchange[kPagedRowThreads / 32][kHeads][HD];  // NEOX pairs lie half a rotation apart
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, piece = lane % LANES;
-    const int heads = a.q_heads + 2 * a.c.kv_heads, groups = (heads + kHeads - 1) / kHeads;
+    const int heads = a.q_heads + 2 * a.c.kv_heads, groups = (heads + U * kHeads - 1) / (U * kHeads);
     const int item = blockIdx.x * (kPagedRowThreads / 32) + warp, t = item / groups;
     if (t >= a.r.tokens) return;
-    const int head = item % groups * kHeads + sub, kind = head < a.q_heads ? 0 : head < a.q_heads + a.c.kv_heads ? 1 : 2;  // query, key, value
-    const bool live = head < heads;
-    const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.c.kv_heads;
-    float x[8];
+    const int head0 = item % groups * U * kHeads + sub;
+    PagedRaw<TYPE> raw[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (live) {
+    for (int u = 0; u < U; ++u) {
+        const int head = min(head0 + u * kHeads, heads - 1), kind = head < a.q_heads ? 0 : head < a.q_heads + a.c.kv_heads ? 1 : 2;  // query, key, value
+        const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.c.kv_heads;
         const size_t at = kind == 0 ? t * a.q_token + h * a.q_head : kind == 1 ? t * a.k_token + h * a.k_head : t * a.v_token + h * a.v_head;
-        const void* base = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-        paged_load8(static_cast<const unsigned char*>(base) + (at + piece * 8) * paged_size_of(a.in_type), a.in_type, x);
+        raw[u] = paged_raw<TYPE>(kind == 0 ? a.q : kind == 1 ? a.k : a.v, at + piece * 8);
     }
-    const int s = paged_sequence_of(a.r, t);
-    if (s < 0) return;  // a row behind the last sequence is left as it was
-    const PagedSequence sq = paged_sequence(a.c, a.r, s);
-    if (!sq.ok || t < sq.first || t >= sq.first + sq.news) return;
-    const int pos = sq.length - sq.news + (t - sq.first);
-    if (pos < 0 || (a.cos_sin != nullptr && pos >= a.positions)) {
-        if (lane == 0) atomicOr(a.c.status, kPagedBadPosition);
-        return;
-    }
-    const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-    float sum = 0.0f;
+    const PagedPlace place = paged_place(a.c, a.r, t, a.cos_sin != nullptr ? a.positions : 0x7fffffff);
+    // (a query of a token whose page does not exist is left as it was, like its row of the cache)
+    if (place.page < 0) return;
+    // this thread's factors of the rotation: x_i cos_i + partner_i sin_i
+    float cs[8], sn[8];
+    const int half = a.rope / 2, e0 = piece * 8;
+    const bool neox = a.cos_sin != nullptr && a.neox != 0, whole = a.vector != 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
+    if (a.cos_sin != nullptr && e0 < a.rope) {
+        const float* row = a.cos_sin + static_cast<size_t>(place.pos) * a.rope;
+        if (a.vector && a.neox) {  // eight pairs, all first or all second values
+            const bool second = e0 >= half;
+            const float4* at = reinterpret_cast<const float4*>(row + 2 * (second ? e0 - half : e0));
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (w != nullptr) {
-        const float inv = 1.0f / sqrtf(sum / HD + a.eps);
-        float g[8];
-        paged_load8(w + piece * 8, kPagedF32, g);
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = at[i];
+                cs[2 * i] = v.x, sn[2 * i] = second ? v.y : -v.y, cs[2 * i + 1] = v.z, sn[2 * i + 1] = second ? v.w : -v.w;
+            }
+        } else if (a.vector) {  // four pairs
+            const float4* at = reinterpret_cast<const float4*>(row + e0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-    }
-    if (a.cos_sin != nullptr) {
-        const float* cs = a.cos_sin + static_cast<size_t>(pos) * a.rope;
-        if (!a.neox) {
-            if (kind != 2) {
-#pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                    if (piece * 8 + i < a.rope) {
-                        const float c = cs[piece * 8 + i], sn = cs[piece * 8 + i + 1], x0 = x[i], x1 = x[i + 1];
-                        x[i] = x0 * c - x1 * sn, x[i + 1] = x0 * sn + x1 * c;
-                    }
+            for (int i = 0; i < 2; ++i) {
+                const float4 v = at[i];
+                cs[4 * i] = cs[4 * i + 1] = v.x, sn[4 * i] = -v.y, sn[4 * i + 1] = v.y, cs[4 * i + 2] = cs[4 * i + 3] = v.z, sn[4 * i + 2] = -v.w, sn[4 * i + 3] = v.w;
             }
         } else {
-            float* row = exchange[warp][sub];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) row[piece * 8 + i] = x[i];
-            __syncwarp();
-            if (kind != 2) {
-                const int half = a.rope / 2;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = piece * 8 + i;
-                    if (e >= a.rope) continue;
-                    const bool second = e >= half;
-                    const int p = second ? e - half : e;
-                    const float c = cs[2 * p], sn = cs[2 * p + 1], other = row[second ? p : p + half];
-                    x[i] = second ? other * sn + x[i] * c : x[i] * c - other * sn;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                if (e >= a.rope) continue;
+                const bool second = a.neox ? e >= half : (e & 1) != 0;
+                const int p = a.neox ? (second ? e - half : e) : e >> 1;
+                cs[i] = row[2 * p], sn[i] = second ? row[2 * p + 1] : -row[2 * p + 1];
             }
         }
     }
-    if (live && kind == 0) {
-        paged_store8(static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + piece * 8) * paged_size_of(a.q_type), a.q_type, x);
-        if (a.type != kPagedQ8) return;  // (the exchanges below are for whole warps)
-    }
-    if (a.type != kPagedQ8 && !live) return;
-    // what is not finite, or does not fit the type, becomes the nearest value that does, and a value that is none becomes zero
     const float most_finite = a.type == kPagedF16 ? 65504.0f : a.type == kPagedBf16 ? 3.3895313892515355e38f : 8.507059173023462e37f;  // (Q8: 2^126, so that 127 d does not overflow)
-    bool odd = false;
-    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (!(fabsf(x[i]) <= most_finite)) odd = true, x[i] = isnan(x[i]) ? 0.0f : copysignf(most_finite, x[i]);
-        amax = fmaxf(amax, fabsf(x[i]));
-    }
-    if (odd && live && kind != 0) atomicOr(a.c.status, kPagedSaturated);
-    const int row = pos & ((1 << a.c.page_log2) - 1), page = a.r.table[static_cast<size_t>(s) * a.r.stride + (pos >> a.c.page_log2)];
-    const bool there = page >= 0 && page < a.c.pages;
-    if (!there && lane == 0) atomicOr(a.c.status, kPagedBadPage);
-    unsigned char* store = kind == 1 ? a.c.k : a.c.v;
-    if (a.type != kPagedQ8) {
-        if (there)
-            paged_store8(store + paged_block_at(a.c, a.type, page, h, piece >> 3) + row * 128 + paged_piece(a.type, row, piece & 7) * 16, a.type, x);
-        return;
-    }
+    for (int u = 0; u < U; ++u) {
+        const int head = head0 + u * kHeads, kind = head < a.q_heads ? 0 : head < a.q_heads + a.c.kv_heads ? 1 : 2;
+        const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.c.kv_heads;
+        const bool live = head < heads;
+        if (head0 - sub + u * kHeads >= heads) break;  // (the whole warp)
+        float x[8];
+        paged_load8(raw[u].v, TYPE, x);
+        const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+        if (a.q_norm != nullptr || a.k_norm != nullptr) {
+            float sum = 0.0f;
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!live || kind == 0 || !there) return;
-    const float d = fmaxf(amax / 127.0f, kPagedMinScale);
-    uint32_t code[2] = {0u, 0u};
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // (127 / d rounds to 127 at most, as d is at least the rounded amax / 127: |x| / d <= 127 (1 + 2^-23), and rint gives 127)
-        const int q = max(-127, min(127, __float2int_rn(x[i] / d)));
-        code[i >> 2] |= static_cast<uint32_t>(q & 0xff) << (8 * (i & 3));
+            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (w != nullptr) {
+                const float inv = 1.0f / sqrtf(sum / HD + a.eps);
+                float g[8];
+                paged_load8(w + e0, kPagedF32, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
+            }
+        }
+        float y[8];  // the other one of each pair
+        if (neox) {
+            float* row = exchange[warp][sub];
+            __syncwarp();
+            paged_store8(row + e0, kPagedF32, x);
+            __syncwarp();
+            const int from = e0 >= half ? e0 - half : e0 + half;
+            if (whole) {
+                paged_load8(row + (e0 < a.rope ? from : e0), kPagedF32, y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = row[e0 + i >= a.rope ? e0 + i : e0 + i >= half ? e0 + i - half : e0 + i + half];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+        }
+        if (kind != 2) {
+            float r[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = sn[i] == 0.0f && cs[i] == 1.0f ? x[i] : fmaf(x[i], cs[i], y[i] * sn[i]);  // (nothing of a partner that is no number where there is no rotation)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = r[i];
+        }
+        if (live && kind == 0) paged_store8(static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.q_type), a.q_type, x);
+        // what is not finite, or does not fit the type, becomes the nearest value that does, and a value that is none becomes zero
+        bool odd = false;
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i])), odd = odd || !(fabsf(x[i]) <= most_finite);
+        if (odd) {
+            amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!(fabsf(x[i]) <= most_finite)) x[i] = isnan(x[i]) ? 0.0f : copysignf(most_finite, x[i]);
+                amax = fmaxf(amax, fabsf(x[i]));
+            }
+            if (live && kind != 0) atomicOr(a.c.status, kPagedSaturated);
+        }
+        unsigned char* block = (kind == 1 ? a.c.k : a.c.v) + paged_block_at(a.c, a.type, place.page, h, piece >> 3);
+        if (a.type != kPagedQ8) {
+            if (live && kind != 0) paged_store8(block + place.row * 128 + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
+            continue;
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (!live || kind == 0) continue;
+        const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = 1.0f / d;
+        uint32_t code[2] = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // (|x| / d <= 127 (1 + 2^-22), which rounds to 127; x (1 / d) is off x / d by 2^-16 of a step at most)
+            const int q = __float2int_rn(x[i] * inv);
+            code[i >> 2] |= static_cast<uint32_t>(q & 0xff) << (8 * (i & 3));
+        }
+        *reinterpret_cast<uint2*>(block + place.row * 64 + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
+        if (piece == 0) (kind == 1 ? a.c.ks : a.c.vs)[paged_scales_at(a.c, place.page, h) + place.row] = d;
     }
-    *reinterpret_cast<uint2*>(store + paged_block_at(a.c, a.type, page, h, piece >> 3) + row * 64 + paged_piece(a.type, row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) =
-        make_uint2(code[0], code[1]);
-    if (piece == 0) (kind == 1 ? a.c.ks : a.c.vs)[paged_scales_at(a.c, page, h) + row] = d;
 }
 
 struct PagedReadArgs {
@@ -149,43 +212,48 @@ struct PagedReadArgs {
     void *k, *v;  // [token][kv_heads][head_dim]; either may be nullptr
 };
 
-template <int LANES>
+template <int LANES, int TYPE, int U>  // TYPE: of the cache
 __global__ void __launch_bounds__(kPagedRowThreads) paged_read_kernel(const __grid_constant__ PagedReadArgs a) {
     constexpr int kHeads = 32 / LANES, HD = LANES * 8;
     const int lane = threadIdx.x & 31, sub = lane / LANES, piece = lane % LANES;
-    const int heads = 2 * a.c.kv_heads, groups = (heads + kHeads - 1) / kHeads;
+    const int heads = 2 * a.c.kv_heads, groups = (heads + U * kHeads - 1) / (U * kHeads);
     const int item = blockIdx.x * (kPagedRowThreads / 32) + (threadIdx.x >> 5), t = item / groups;
     if (t >= a.r.tokens) return;
-    const int head = item % groups * kHeads + sub;
-    const bool value = head >= a.c.kv_heads;
-    const int h = value ? head - a.c.kv_heads : head;
-    const int s = paged_sequence_of(a.r, t);
-    if (s < 0) return;
-    const PagedSequence sq = paged_sequence(a.c, a.r, s);
-    if (!sq.ok || t < sq.first || t >= sq.first + sq.news) return;
-    const int pos = sq.length - sq.news + (t - sq.first);
-    if (pos < 0) {
-        if (lane == 0) atomicOr(a.c.status, kPagedBadPosition);
-        return;
-    }
-    const int row = pos & ((1 << a.c.page_log2) - 1), page = a.r.table[static_cast<size_t>(s) * a.r.stride + (pos >> a.c.page_log2)];
-    if (page < 0 || page >= a.c.pages) {
-        if (lane == 0) atomicOr(a.c.status, kPagedBadPage);
-        return;
-    }
-    void* out = value ? a.v : a.k;
-    if (head >= heads || out == nullptr) return;
-    const unsigned char* store = (value ? a.c.v : a.c.k) + paged_block_at(a.c, a.type, page, h, piece >> 3);
-    float x[8];
-    if (a.type == kPagedQ8) {
-        const uint2 code = *reinterpret_cast<const uint2*>(store + row * 64 + paged_piece(a.type, row, (piece & 7) >> 1) * 16 + (piece & 1) * 8);
-        const float d = (value ? a.c.vs : a.c.ks)[paged_scales_at(a.c, page, h) + row];
+    const int head0 = item % groups * U * kHeads + sub;
+    const PagedPlace place = paged_place(a.c, a.r, t, 0x7fffffff);
+    if (place.page < 0) return;
+    uint4 raw[U];
+    float d[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? code.x : code.y) >> (8 * (i & 3)))) * d;
-    } else {
-        paged_load8(store + row * 128 + paged_piece(a.type, row, piece & 7) * 16, a.type, x);
+    for (int u = 0; u < U; ++u) {
+        const int head = min(head0 + u * kHeads, heads - 1);
+        const bool value = head >= a.c.kv_heads;
+        const int h = value ? head - a.c.kv_heads : head;
+        const unsigned char* block = (value ? a.c.v : a.c.k) + paged_block_at(a.c, TYPE, place.page, h, piece >> 3);
+        if constexpr (TYPE == kPagedQ8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(block + place.row * 64 + paged_piece(TYPE, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8);
+            raw[u] = make_uint4(v.x, v.y, 0, 0);
+            d[u] = (value ? a.c.vs : a.c.ks)[paged_scales_at(a.c, place.page, h) + place.row];
+        } else {
+            raw[u] = *reinterpret_cast<const uint4*>(block + place.row * 128 + paged_piece(TYPE, place.row, piece & 7) * 16);
+        }
     }
-    paged_store8(static_cast<unsigned char*>(out) + ((static_cast<size_t>(t) * a.c.kv_heads + h) * HD + piece * 8) * paged_size_of(a.out_type), a.out_type, x);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int head = head0 + u * kHeads;
+        const bool value = head >= a.c.kv_heads;
+        const int h = value ? head - a.c.kv_heads : head;
+        void* out = value ? a.v : a.k;
+        if (head >= heads || out == nullptr) continue;
+        float x[8];
+        if constexpr (TYPE == kPagedQ8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? raw[u].x : raw[u].y) >> (8 * (i & 3)))) * d[u];
+        } else {
+            paged_load8(&raw[u], TYPE, x);
+        }
+        paged_store8(static_cast<unsigned char*>(out) + ((static_cast<size_t>(t) * a.c.kv_heads + h) * HD + piece * 8) * paged_size_of(a.out_type), a.out_type, x);
+    }
 }
 
 }  // namespace qtb

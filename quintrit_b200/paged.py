@@ -8,6 +8,7 @@ device (or the ``stream`` given) and do not wait; ``status()`` reports what they
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import api as _api
 
@@ -33,6 +34,11 @@ class _AttentionC(C.Structure):
                 ("out_token_stride", _sz), ("out_head_stride", _sz), ("scale", _f32), ("cap", _f32), ("window", _u32), ("d_workspace", _vp), ("workspace_bytes", _sz)]
 
 
+# The same layouts packed in one go: a call's arguments as bytes (a third of the time that filling the structures takes, on a path that a step walks once per layer).
+_APPEND = struct.Struct("@IiiIPPPNNNNNNPNNPPfPIIi0P")
+_ATTENTION = struct.Struct("@IiiIPNNPNNffIPN")
+assert _APPEND.size == C.sizeof(_AppendC) and _ATTENTION.size == C.sizeof(_AttentionC)
+
 _bound = None
 
 
@@ -44,23 +50,30 @@ def _lib():
         lib.quintrit_b200_paged_cache_free.argtypes = [_vp]
         lib.quintrit_b200_paged_cache_info.argtypes = [_vp, C.POINTER(_sz), C.POINTER(_u32)]
         lib.quintrit_b200_paged_cache_status.argtypes = [_vp]
-        lib.quintrit_b200_paged_append_device.argtypes = [_vp, _u32, C.POINTER(_RowsC), C.POINTER(_AppendC), _vp]
-        lib.quintrit_b200_paged_read_device.argtypes = [_vp, _u32, C.POINTER(_RowsC), _i32, _vp, _vp, _vp]
-        lib.quintrit_b200_paged_attention_workspace.argtypes = [_vp, C.POINTER(_RowsC), _u32, C.POINTER(_sz)]
-        lib.quintrit_b200_paged_attention_device.argtypes = [_vp, _u32, C.POINTER(_RowsC), C.POINTER(_AttentionC), _vp]
+        lib.quintrit_b200_paged_append_device.argtypes = [_vp, _u32, _vp, _vp, _vp]
+        lib.quintrit_b200_paged_read_device.argtypes = [_vp, _u32, _vp, _i32, _vp, _vp, _vp]
+        lib.quintrit_b200_paged_attention_workspace.argtypes = [_vp, _vp, _u32, C.POINTER(_sz)]
+        lib.quintrit_b200_paged_attention_device.argtypes = [_vp, _u32, _vp, _vp, _vp]
         _bound = lib
     return _bound
 
 
-_dtypes = None
+_dtypes = {}
+_torch_stream = None
+
+
+def _torch():
+    """torch, asked for on first use: the rest of the package works without it."""
+    global _torch_stream
+    import torch
+
+    _dtypes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _torch_stream = raw if raw is not None else lambda device: torch.cuda.current_stream(device).cuda_stream
+    return torch
 
 
 def _type_of(t) -> int:
-    global _dtypes
-    if _dtypes is None:
-        import torch
-
-        _dtypes = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
     try:
         return _dtypes[t.dtype]
     except KeyError:
@@ -74,8 +87,7 @@ class PagedRows:
     more new tokens; ``max_length``: no sequence is longer, as far as is known (it divides the work)."""
 
     def __init__(self, starts, lengths, table, tokens: int, max_new: int, max_length: int):
-        import torch
-
+        torch = _torch()
         for name, t, dim in (("starts", starts, 1), ("lengths", lengths, 1), ("table", table, 2)):
             if t.dtype != torch.int32 or t.dim() != dim or not t.is_cuda or (t.numel() > 1 and t.stride(-1) != 1):
                 raise ValueError(f"{name} is a {dim}-dimensional int32 CUDA tensor with consecutive values")
@@ -89,8 +101,9 @@ class PagedRows:
         self.starts, self.lengths, self.table, self.tokens = starts, lengths, table, tokens
         # (the rows of a table may lie further apart than they are long: what lies between is not the sequence's, but pages beyond a length are never looked at)
         self._c = _RowsC(C.sizeof(_RowsC), n, tokens, max_new, max_length, table.stride(0) if n > 1 else table.shape[1], starts.data_ptr(), lengths.data_ptr(), table.data_ptr())
-        self._p = C.byref(self._c)
+        self._p = C.addressof(self._c)
         self.device = starts.device
+        self._device = starts.get_device()
 
 
 class PagedCache:
@@ -102,6 +115,7 @@ class PagedCache:
         if dtype not in _CACHE_TYPES:
             raise ValueError(f"a paged cache is stored as {', '.join(_CACHE_TYPES)}, got {dtype!r}")
         self._lib = _lib()
+        _torch()
         _api._check(self._lib.quintrit_b200_paged_cache_create(device, layers, pages, page_tokens, kv_heads, head_dim, _CACHE_TYPES[dtype], C.byref(self._h)))
         self.layers, self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.dtype, self.device = layers, pages, page_tokens, kv_heads, head_dim, dtype, device
 
@@ -111,112 +125,102 @@ class PagedCache:
         _api._check(self._lib.quintrit_b200_paged_cache_info(self._h, C.byref(n), None))
         return n.value
 
-    def _stream(self, stream):
-        if stream is not None:
-            return stream
-        import torch
-
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def _heads(self, name, t, tokens, heads=None):
-        if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads) or t.stride(2) != 1:
-            raise ValueError(f"{name} is [{tokens}][{'heads' if heads is None else heads}][{self.head_dim}] with the values of a head side by side, got {tuple(t.shape)}, strides {t.stride()}")
+    def _heads(self, name, t, tokens, heads):
+        """Checks [tokens][heads][head_dim] (heads None: any number) on this device; returns (type, heads, token stride, head stride)."""
+        shape, strides, kind = t.shape, t.stride(), _dtypes.get(t.dtype)
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != self.head_dim or (heads is not None and shape[1] != heads) or strides[2] != 1:
+            raise ValueError(f"{name} is [{tokens}][{'heads' if heads is None else heads}][{self.head_dim}] with the values of a head side by side, got {tuple(shape)}, strides {strides}")
         if t.get_device() != self.device:
             raise ValueError(f"{name} is not on the cache's device {self.device}")
-        return t
+        if kind is None:
+            raise ValueError(f"{name} is float32, float16 or bfloat16, got {t.dtype}")
+        return kind, shape[1], strides[0], strides[1]
+
+    def _call(self, rc):
+        if rc != 0:
+            _api._check(rc)
 
     def _rows(self, rows):
-        if rows.device.index != self.device:
+        if rows._device != self.device:
             raise ValueError(f"the rows' tensors are not on the cache's device {self.device}")
-        return rows
+        return rows._p
 
     def append(self, layer: int, rows: PagedRows, q, k, v, *, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, cos_sin=None, neox: bool = False, stream=None):
         """Normalises and rotates the new tokens' query and key heads, writes keys and values to the cache and returns the queries (``q_out``, by default new
         and of the queries' type; None if ``q`` is None). ``q_norm`` / ``k_norm``: float32 weights [head_dim]; ``cos_sin``: float32 [positions][rotated values]
         with cos at 2 i and sin at 2 i + 1; ``neox``: pairs (i, i + half) instead of (2 i, 2 i + 1)."""
-        import torch
-
-        rows, n = self._rows(rows), rows.tokens
-        k, v = self._heads("k", k, n, self.kv_heads), self._heads("v", v, n, self.kv_heads)
-        a = _AppendC(C.sizeof(_AppendC))
-        a.type = _type_of(k)
-        if _type_of(v) != a.type or (q is not None and _type_of(q) != a.type):
-            raise ValueError("q, k and v have the same type")
+        at, n = self._rows(rows), rows.tokens
+        kind, _, k_token, k_head = self._heads("k", k, n, self.kv_heads)
+        v_kind, _, v_token, v_head = self._heads("v", v, n, self.kv_heads)
+        q_heads = q_token = q_head = o_token = o_head = q_at = o_at = o_kind = 0
+        q_kind = kind
         if q is not None:
-            self._heads("q", q, n)
+            q_kind, q_heads, q_token, q_head = self._heads("q", q, n, None)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            self._heads("q_out", q_out, n, q.shape[1])
-            a.q_out_type, a.q_heads, a.d_q, a.d_q_out = _type_of(q_out), q.shape[1], q.data_ptr(), q_out.data_ptr()
-            a.q_token_stride, a.q_head_stride = q.stride(0), q.stride(1)
-            a.out_token_stride, a.out_head_stride = q_out.stride(0), q_out.stride(1)
+                q_out = q.new_empty(q.shape)
+            o_kind, _, o_token, o_head = self._heads("q_out", q_out, n, q_heads)
+            q_at, o_at = q.data_ptr(), q_out.data_ptr()
         else:
             q_out = None
-        a.d_k, a.k_token_stride, a.k_head_stride = k.data_ptr(), k.stride(0), k.stride(1)
-        a.d_v, a.v_token_stride, a.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
-        if q_norm is not None or k_norm is not None:
-            for w in (q_norm, k_norm):
-                if w is not None and (w.dtype != torch.float32 or w.shape != (self.head_dim,) or not w.is_contiguous() or w.get_device() != self.device):
-                    raise ValueError(f"norm weights are float32 [{self.head_dim}] on the cache's device")
-            a.d_q_norm = None if q_norm is None else q_norm.data_ptr()
-            a.d_k_norm = None if k_norm is None else k_norm.data_ptr()
-            a.norm_eps = eps
+        if not kind == v_kind == q_kind:
+            raise ValueError("q, k and v have the same type")
+        wq = wk = cs = positions = rope = 0
+        for w in (q_norm, k_norm):
+            if w is not None and (_dtypes.get(w.dtype) != F32 or w.shape != (self.head_dim,) or not w.is_contiguous() or w.get_device() != self.device):
+                raise ValueError(f"norm weights are float32 [{self.head_dim}] on the cache's device")
+        if q_norm is not None:
+            wq = q_norm.data_ptr()
+        if k_norm is not None:
+            wk = k_norm.data_ptr()
         if cos_sin is not None:
-            if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.get_device() != self.device:
+            if _dtypes.get(cos_sin.dtype) != F32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.get_device() != self.device:
                 raise ValueError("cos_sin is a contiguous float32 [positions][rotated values] on the cache's device")
-            a.d_cos_sin, a.positions, a.rope_dims, a.neox = cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1], int(neox)
-        rc = self._lib.quintrit_b200_paged_append_device(self._h, layer, rows._p, C.byref(a), self._stream(stream))
-        if rc != 0:
-            _api._check(rc)
+            cs, (positions, rope) = cos_sin.data_ptr(), cos_sin.shape
+        a = _APPEND.pack(_APPEND.size, kind, o_kind, q_heads, q_at, k.data_ptr(), v.data_ptr(), q_token, q_head, k_token, k_head, v_token, v_head, o_at, o_token, o_head, wq, wk, eps, cs,
+                         positions, rope, neox)
+        self._call(self._lib.quintrit_b200_paged_append_device(self._h, layer, at, a, _torch_stream(self.device) if stream is None else stream))
         return q_out
 
     def read(self, layer: int, rows: PagedRows, *, k_out=None, v_out=None, dtype=None, stream=None):
         """The new tokens' rows of the cache, dense: (keys, values), each [tokens][kv_heads][head_dim]. With whole sequences as "new" tokens: all that is cached.
         ``dtype``: of the results where they are not given (default float16)."""
-        import torch
-
-        rows, n = self._rows(rows), rows.tokens
+        at, n = self._rows(rows), rows.tokens
         if k_out is None and v_out is None:
+            torch = _torch()
             k_out, v_out = (torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype or torch.float16, device=rows.device) for _ in range(2))
-        given = [t for t in (k_out, v_out) if t is not None]
-        for t in given:
-            self._heads("an output", t, n, self.kv_heads)
-            if not t.is_contiguous() or t.dtype != given[0].dtype:
-                raise ValueError("outputs are contiguous and of one type")
-        rc = self._lib.quintrit_b200_paged_read_device(self._h, layer, rows._p, _type_of(given[0]), None if k_out is None else k_out.data_ptr(),
-                                                       None if v_out is None else v_out.data_ptr(), self._stream(stream))
-        if rc != 0:
-            _api._check(rc)
+        kind = None
+        for t in (k_out, v_out):
+            if t is not None:
+                t_kind = self._heads("an output", t, n, self.kv_heads)[0]
+                if not t.is_contiguous() or (kind is not None and t_kind != kind):
+                    raise ValueError("outputs are contiguous and of one type")
+                kind = t_kind
+        self._call(self._lib.quintrit_b200_paged_read_device(self._h, layer, at, kind, None if k_out is None else k_out.data_ptr(), None if v_out is None else v_out.data_ptr(),
+                                                             _torch_stream(self.device) if stream is None else stream))
         return k_out, v_out
 
     def attend_workspace(self, rows: PagedRows, q_heads: int):
         """Scratch memory for ``attend`` on these rows with that many query heads (a uint8 tensor, perhaps empty). Calls that may overlap need one each."""
-        import torch
-
-        n = _sz(0)
-        _api._check(self._lib.quintrit_b200_paged_attention_workspace(self._h, rows._p, q_heads, C.byref(n)))
+        torch, n = _torch(), _sz(0)
+        _api._check(self._lib.quintrit_b200_paged_attention_workspace(self._h, self._rows(rows), q_heads, C.byref(n)))
         return torch.empty(n.value, dtype=torch.uint8, device=rows.device)
 
     def attend(self, layer: int, rows: PagedRows, q, *, out=None, scale: float | None = None, cap: float = 0.0, window: int = 0, workspace=None, stream=None):
         """Attention of the new tokens' queries [tokens][query heads][head_dim] over the cached positions up to their own (the last ``window`` of them, if that
         is not 0), scores times ``scale`` (default head_dim ** -0.5), capped to ``cap`` tanh(score / ``cap``) if that is not 0. Returns ``out`` (by default
         new, of the queries' type). ``workspace``: from ``attend_workspace``, by default allocated by torch for this call on its current stream."""
-        import torch
-
-        rows, n = self._rows(rows), rows.tokens
-        self._heads("q", q, n)
+        at, n = self._rows(rows), rows.tokens
+        kind, heads, q_token, q_head = self._heads("q", q, n, None)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._heads("out", out, n, q.shape[1])
+            out = q.new_empty(q.shape)
+        o_kind, _, o_token, o_head = self._heads("out", out, n, heads)
         if workspace is None:
-            workspace = self.attend_workspace(rows, q.shape[1])
+            workspace = self.attend_workspace(rows, heads)
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("the workspace is a contiguous tensor on the cache's device")
-        a = _AttentionC(C.sizeof(_AttentionC), _type_of(q), _type_of(out), q.shape[1], q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                        self.head_dim ** -0.5 if scale is None else scale, cap, window, workspace.data_ptr(), workspace.numel() * workspace.element_size())
-        rc = self._lib.quintrit_b200_paged_attention_device(self._h, layer, rows._p, C.byref(a), self._stream(stream))
-        if rc != 0:
-            _api._check(rc)
+        a = _ATTENTION.pack(_ATTENTION.size, kind, o_kind, heads, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, self.head_dim ** -0.5 if scale is None else scale, cap,
+                            window, workspace.data_ptr(), workspace.nbytes)
+        self._call(self._lib.quintrit_b200_paged_attention_device(self._h, layer, at, a, _torch_stream(self.device) if stream is None else stream))
         return out
 
     def status(self) -> None:

@@ -41,7 +41,7 @@ def attention(**more):
 
 def call(name, *args):
     lib = paged._lib()
-    rc = getattr(lib, "quintrit_b200_paged_" + name)(*[C.byref(a) if isinstance(a, C.Structure) else a for a in args])
+    rc = getattr(lib, "quintrit_b200_paged_" + name)(*[C.addressof(a) if isinstance(a, C.Structure) else a for a in args])
     assert rc == lib.quintrit_last_error_code() and (rc == 0) == (lib.quintrit_last_error_message() == b"")
     return rc
 
@@ -61,13 +61,13 @@ def test_create_without_an_out_pointer_and_handles():
     junk = handle()
     junk.magic = 5
     for h in (None, junk):
-        p = None if h is None else C.byref(h)
+        p = None if h is None else C.addressof(h)
         assert call("cache_info", p, None, None) == HANDLE
         assert call("cache_status", p) == HANDLE
         assert call("append_device", p, 0, rows(), append(), None) == HANDLE
         assert call("attention_device", p, 0, rows(), attention(), None) == HANDLE
         assert call("read_device", p, 0, rows(), F16, 0x10000, 0x20000, None) == HANDLE
-    assert call("cache_free", C.byref(junk)) == HANDLE
+    assert call("cache_free", C.addressof(junk)) == HANDLE
 
 
 BAD_ROWS = [(dict(struct_size=8), ARG), (dict(sequences=0), ARG), (dict(sequences=65536), ARG), (dict(tokens=(1 << 24) + 1), ARG), (dict(max_new=0), ARG), (dict(max_new=7), ARG),

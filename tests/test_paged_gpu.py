@@ -34,7 +34,7 @@ def filled(cache_type, kvh, hd, new, lengths, page, seed=1, **more):
 # ---- rows in and out -------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("cache_type,hd,page,in_type", [("f16", 64, 16, "f32"), ("f16", 128, 64, "f16"), ("bf16", 256, 32, "bf16"), ("q8", 64, 256, "f16"), ("q8", 128, 16, "bf16"),
                                                          ("q8", 256, 64, "f32"), ("bf16", 64, 128, "f32")])
-@pytest.mark.parametrize("norm,rope,neox", [(False, 0, False), (True, 1.0, False), (True, 0.5, True), (False, 1.0, True)])
+@pytest.mark.parametrize("norm,rope,neox", [(False, 0, False), (True, 64, False), (True, 32, True), (False, 64, True), (True, 22, True), (False, 22, False), (False, 2, True), (False, 8, True)])
 def test_append_and_read(cache_type, hd, page, in_type, norm, rope, neox):
     new, lengths, qh, kvh = [1, 5, 0, 40, page + 1], [1, 70, 33, 40, 3 * page], 6, 3  # a first token, the middle of a page, no token, a whole sequence, over a page's end
     rows, pages, _ = make_rows(q, new, lengths, page, seed=3)
@@ -43,7 +43,7 @@ def test_append_and_read(cache_type, hd, page, in_type, norm, rope, neox):
     x = randn(T, qh + 2 * kvh, hd, seed=7, dtype=dt) * 3
     qs, ks, vs = x[:, :qh], x[:, qh:qh + kvh], x[:, qh + kvh:]
     wq, wk = (1 + 0.3 * randn(hd, seed=9), 1 + 0.3 * randn(hd, seed=10)) if norm else (None, None)
-    cs = angles(max(lengths), int(hd * rope)) if rope else None
+    cs = angles(max(lengths), rope * hd // 64 if rope > 22 else rope) if rope else None
     out = cache.append(1, rows, qs, ks, vs, q_norm=wq, k_norm=wk, eps=1e-5, cos_sin=cs, neox=neox)
     pos = torch.tensor([p for _, p in places(rows)], device="cuda")
     # 32-bit arithmetic: a sum of hd squares, a root, a division, four products and a sum: under (hd / 2 + 16) half steps of the pair's magnitude
