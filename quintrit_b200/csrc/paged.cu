@@ -8,6 +8,7 @@
 #include "capi_common.cuh"
 #include "paged.hpp"
 #include "paged_attention.cuh"
+#include "paged_attention_tc.cuh"
 #include "paged_rows.cuh"
 
 using namespace qtb;
@@ -15,7 +16,7 @@ using namespace qtb;
 namespace {
 
 constexpr uint32_t kMagicPaged = 0x51545047u;  // "QTPG"
-constexpr unsigned int kPagedSpin = 1u << 20;  // tries of a wait (up to 20 us each) before it gives up
+constexpr unsigned int kPagedSpin = 1u << 17;  // tries of a wait (up to 20 us each) before it gives up
 
 int check_cache(const quintrit_b200_paged_cache* c) {
     if (c == nullptr || c->magic != kMagicPaged) return fail(QUINTRIT_ERR_INVALID_HANDLE, "paged cache handle is NULL, freed or of the wrong type");
@@ -76,16 +77,19 @@ void destroy(quintrit_b200_paged_cache* c) {
 }
 
 struct AppendKernel {
+    static int groups(const PagedAppendArgs& a, int heads) { return (a.q_heads + heads - 1) / heads + 2 * ((a.c.kv_heads + heads - 1) / heads); }
     template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_append_kernel<LANES, TYPE, U>; }
 };
 struct ReadKernel {
+    static int groups(const PagedReadArgs& a, int heads) { return (2 * a.c.kv_heads + heads - 1) / heads; }
     template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_read_kernel<LANES, TYPE, U>; }
 };
 // A warp takes four groups of heads where that leaves a few warps for every place of the device, else one.
 template <typename Kernel, int LANES, int TYPE, typename Args>
 int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void* stream) {
     constexpr int kHeads = 32 / LANES, kWarps = kPagedRowThreads / 32;
-    const long long one = static_cast<long long>(tokens) * ((heads + kHeads - 1) / kHeads), four = static_cast<long long>(tokens) * ((heads + 4 * kHeads - 1) / (4 * kHeads));
+    const int groups = Kernel::groups(a, kHeads);
+    const long long one = static_cast<long long>(tokens) * groups, four = static_cast<long long>(tokens) * ((groups + 3) / 4);
     if (one > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", tokens, heads);
     const bool many = four >= 64LL * sm_count;
     auto kernel = many ? Kernel::template of<LANES, TYPE, 4>() : Kernel::template of<LANES, TYPE, 1>();
@@ -98,7 +102,7 @@ int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void
 struct PagedCut {
     int splits, split, most;  // most: no window makes more ranges of it
 };
-PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, int row_tiles) {
+PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles) {
     long long span = std::max<uint32_t>(r->max_length, 1);
     if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
     const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_tiles;
@@ -136,7 +140,51 @@ template <int TYPE>
 int launch_few_type(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
     return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, rt, grid, s) : launch_few_rows<TYPE, 4>(a, device, rt, grid, s);
 }
+template <int TYPE, int BLOCKS>
+int launch_many_of(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
+    using M = PagedMany<TYPE, BLOCKS>;
+    static_assert(M::kSmem <= 227 * 1024, "the rings do not fit");
+    static std::atomic<uint64_t> done{0};
+    const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS>, M::kSmem, device, done);
+    if (rc != QUINTRIT_OK) return rc;
+    paged_many_kernel<TYPE, BLOCKS><<<grid, M::kThreads, M::kSmem, s>>>(a);
+    QTB_LAUNCH_CHECK();
+    return QUINTRIT_OK;
+}
+template <int TYPE>
+int launch_many_type(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
+    return a.c.blocks == 1 ? launch_many_of<TYPE, 1>(a, device, grid, s) : a.c.blocks == 2 ? launch_many_of<TYPE, 2>(a, device, grid, s) : launch_many_of<TYPE, 4>(a, device, grid, s);
+}
 int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a block of threads
+
+// How a call is served: sequences of up to `few_new` new tokens by the kernel for few rows, the others by the one for many; either may have nothing to do.
+struct PagedPlan {
+    int few_new;             // 0: all by the kernel for many rows
+    bool many;
+    int rt;                  // few: row tiles of a block, blocks per head
+    long long few_tiles, many_tiles;
+    PagedCut few_cut, many_cut;
+    int most_splits() const { return std::max(few_new > 0 ? few_cut.most : 1, many ? many_cut.most : 1); }
+    int splits() const { return std::max(few_new > 0 ? few_cut.splits : 1, many ? many_cut.splits : 1); }
+};
+PagedPlan plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window) {
+    PagedPlan p{};
+    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = 64;
+    p.many = most > limit;
+    p.few_new = static_cast<int>(!p.many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(limit / group, r->max_new - 1));  // (a sequence alone is the longest)
+    if (p.few_new > 0) {
+        const long long rows = p.few_new * group;
+        p.rt = row_tiles_of(static_cast<int>(rows));
+        p.few_tiles = (rows + 16 * p.rt - 1) / (16 * p.rt);
+        p.few_cut = cut_of(c, r, window, p.few_tiles);
+    }
+    if (p.many) {
+        const int block = c->head_dim == 256 ? 128 : 256;
+        p.many_tiles = (most + block - 1) / block;
+        p.many_cut = cut_of(c, r, window, p.many_tiles);
+    }
+    return p;
+}
 
 }  // namespace
 
@@ -315,8 +363,7 @@ extern "C" int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged
         *out_bytes = 0;
         if ((rc = check_rows(cache, rows, false)) != QUINTRIT_OK || (rc = check_heads(cache, q_heads)) != QUINTRIT_OK) return rc;
         if (rows->tokens == 0) return ok();
-        const int most = static_cast<int>(rows->max_new * (q_heads / cache->kv_heads)), rt = row_tiles_of(most), tiles = (most + 16 * rt - 1) / (16 * rt);
-        *out_bytes = workspace_of(cache, rows, q_heads, cut_of(cache, rows, 0, tiles).most);
+        *out_bytes = workspace_of(cache, rows, q_heads, plan_of(cache, rows, q_heads, 0).most_splits());
         return ok();
     });
 }
@@ -340,12 +387,11 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             (rc = check_array("d_out", args->d_out, args->out_type, {args->out_token_stride, args->out_head_stride})) != QUINTRIT_OK)
             return rc;
         const int group = static_cast<int>(args->q_heads / cache->kv_heads);
-        const long long most = static_cast<long long>(rows->max_new) * group;
-        const int rt = row_tiles_of(static_cast<int>(std::min<long long>(most, 1 << 30)));
-        const long long tiles = (most + 16 * rt - 1) / (16 * rt);
-        if (tiles * cache->kv_heads > 65535) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
-        const PagedCut cut = cut_of(cache, rows, args->window, static_cast<int>(tiles));
-        const size_t need = workspace_of(cache, rows, args->q_heads, cut.splits);
+        const PagedPlan plan = plan_of(cache, rows, args->q_heads, args->window);
+        if (std::max(plan.few_tiles, plan.many_tiles) * cache->kv_heads > 65535)
+            return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
+        const int splits = plan.splits();
+        const size_t need = workspace_of(cache, rows, args->q_heads, splits);
         if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);
         if (need > args->workspace_bytes) return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "the workspace holds %zu bytes, %zu are needed", args->workspace_bytes, need);
         if (need > 0 && reinterpret_cast<uintptr_t>(args->d_workspace) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_workspace must be 16-byte aligned");
@@ -359,19 +405,31 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         a.scale = args->cap > 0.0f ? args->scale / args->cap : args->scale * kLog2e;
         a.cap = args->cap * kLog2e;
         a.window = static_cast<int>(args->window);
-        a.splits = cut.splits, a.split = cut.split;
         a.part_o = static_cast<float*>(args->d_workspace);
-        if (need > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(cut.splits) * rows->tokens * args->q_heads * cache->head_dim);
-        a.few = 1, a.many = a.most = static_cast<int>(rows->max_new);
+        if (need > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(splits) * rows->tokens * args->q_heads * cache->head_dim);
+        a.most = static_cast<int>(rows->max_new);
         a.spin_limit = kPagedSpin;
-        const dim3 grid(static_cast<unsigned>(cut.splits), static_cast<unsigned>(cache->kv_heads * tiles), rows->sequences);
-        rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, cache->device, rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, cache->device, rt, grid, s) : launch_few_type<kPagedQ8>(a, cache->device, rt, grid, s);
-        if (rc != QUINTRIT_OK) return rc;
-        if (cut.splits > 1) {
+        PagedAttnArgs few = a, many = a;
+        few.few = 1, few.many = plan.few_new, few.splits = std::max(1, plan.few_cut.splits), few.split = plan.few_cut.split;
+        many.few = plan.many ? plan.few_new + 1 : 0x7fffffff, many.many = a.most, many.splits = std::max(1, plan.many_cut.splits), many.split = plan.many_cut.split;
+        const int device = cache->device;
+        if (plan.many) {
+            const dim3 grid(static_cast<unsigned>(many.splits), static_cast<unsigned>(cache->kv_heads * plan.many_tiles), rows->sequences);
+            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(many, device, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(many, device, grid, s)
+                                                                                                                          : launch_many_type<kPagedQ8>(many, device, grid, s);
+            if (rc != QUINTRIT_OK) return rc;
+        }
+        if (plan.few_new > 0) {
+            const dim3 grid(static_cast<unsigned>(few.splits), static_cast<unsigned>(cache->kv_heads * plan.few_tiles), rows->sequences);
+            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(few, device, plan.rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(few, device, plan.rt, grid, s)
+                                                                                                                                  : launch_few_type<kPagedQ8>(few, device, plan.rt, grid, s);
+            if (rc != QUINTRIT_OK) return rc;
+        }
+        if (splits > 1) {
             const long long items = static_cast<long long>(rows->tokens) * args->q_heads;
             const unsigned blocks = static_cast<unsigned>((items + 7) / 8);
             auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
-            kernel<<<blocks, 256, 0, s>>>(a);
+            kernel<<<blocks, 256, 0, s>>>(few, many);
             QTB_LAUNCH_CHECK();
         }
         return ok();

@@ -1,0 +1,428 @@
+// Attention of many new tokens over a paged cache on the 5th-generation tensor cores (the mathematics: paged_attention.cuh).
+//
+// A block of threads takes one KV head of one sequence, 256 rows of queries (128 where a head has 256 values; a row is a (token, head of the group)) and a
+// range of positions, in tiles of 128 positions (64). Units of work alternate between two score buffers in tensor memory: the two row tiles of a tile of positions,
+// or the one row tile of successive tiles. For a unit one thread issues S = Q K^T (tcgen05.mma, operands in shared memory; Q of 256 values in tensor memory), a warpgroup
+// with a row per thread turns S into weights (maximum, exponentials, sum: no exchange between threads) and writes them as 16-bit values over S, and O += P V takes them from
+// there. The tensor cores work on the other buffer meanwhile: score products of unit u + 2 follow the value products of unit u. O stays in tensor memory and is rescaled, by its
+// warpgroup, only when a row's maximum grew by more than 2^8.
+//
+// F16 / BF16: one warp brings the pages' rows by bulk copies straight into the operands' places, since they lie in the cache in the 128-byte swizzle already (keys as a K-major,
+// values as an MN-major operand). Q8: it brings codes and scales to a ring of their own, and four warps widen the codes to F16 operands and prepare the scales.
+//
+// Bound by the tensor cores (4 head_dim flops per row and position) and, for heads of up to 128 values, as much by the exponentials: 16 a clock and
+// multiprocessor, so that 128 x 128 scores of a unit take 1024 cycles, and the two products 8 head_dim.
+#pragma once
+#include "packed_f32.cuh"
+#include "paged_attention.cuh"
+
+namespace qtb {
+
+template <int TYPE, int BLOCKS>
+struct PagedMany {
+    static constexpr bool Q8 = TYPE == kPagedQ8, BF = TYPE == kPagedBf16;
+    static constexpr int HD = BLOCKS * kPagedBlock, NT = BLOCKS == 4 ? 1 : 2;  // row tiles of a block
+    static constexpr int KT = BLOCKS == 4 ? 64 : 128;                          // positions of a tile
+    static constexpr int kRows = 128 * NT;
+    static constexpr int kSlot = KT * HD * 2, kSlots = Q8 ? 3 : 4;             // operand tiles: keys and values in turn
+    static constexpr int kRaw = KT * HD, kRaws = Q8 ? 3 : 0;                   // Q8: the codes; those of keys with the scales of keys and values
+    static constexpr int kRawStride = Q8 ? kRaw + KT * 8 : 0;
+    static constexpr int kFactors = Q8 ? 4 : 0;                                // sets of KT x (key scale, log2 of the value scale, its reciprocal)
+    static constexpr bool kQTmem = BLOCKS == 4;
+    static constexpr int kQBytes = kQTmem ? 0 : NT * 128 * HD * 2;
+    static constexpr int kSoftWarps = 4 * NT, kLoadWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
+    static constexpr int kThreads = (kSoftWarps + 4 + (Q8 ? 4 : 0)) * 32;
+    // registers per thread where the warpgroups with the scores need more than their share: launched with 168 (384 threads) or 128 (512 threads)
+    static constexpr bool kSplitRegs = NT == 2;
+    static constexpr int kSoftRegs = Q8 ? 200 : 216, kRestRegs = Q8 ? 56 : 72;
+    static constexpr int kBars = 2 * kSlots + 2 * kRaws + 2 * 3 + 2;
+    static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + kBars * 8 + 16;
+    static constexpr int kSmem = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one block per multiprocessor: it takes all of its tensor memory
+    static constexpr int kOCol = 0, kSCol = 256, kQCol = 384;  // tensor memory columns: O (of row tile i at 128 i), S (buffer b at KT b behind), Q
+};
+
+namespace paged_detail {
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+          "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// kind::f16: F32 accumulator (1 at bit 4), A and B F16 or BF16 (1 at bits 7 and 10), B transposed (MN-major) at bit 16, N / 8 at bit 17, M / 16 at bit 24.
+__host__ __device__ constexpr uint32_t instr_desc_16(bool bf16, bool b_mn, int n) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+}  // namespace paged_detail
+
+template <int TYPE, int BLOCKS>
+__global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a) {
+    using namespace gemm_detail;
+    using namespace paged_detail;
+    using M = PagedMany<TYPE, BLOCKS>;
+    constexpr bool Q8 = M::Q8;
+    constexpr int HD = M::HD, NT = M::NT, KT = M::KT, RS = M::kSlots, RW = Q8 ? M::kRaws : 1, kRow = paged_row_bytes(TYPE);
+    extern __shared__ unsigned char many_smem_raw[];
+    const uint32_t base = (smem_u32(many_smem_raw) + 1023u) & ~1023u;
+    unsigned char* smem = many_smem_raw + (base - smem_u32(many_smem_raw));
+    const uint32_t q_at = base, slots = base + M::kQBytes, raws = slots + RS * M::kSlot;
+    unsigned char* raw_smem = smem + M::kQBytes + RS * M::kSlot;
+    float* factors = reinterpret_cast<float*>(raw_smem + M::kRaws * M::kRawStride);  // [kFactors][3][KT]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(factors + M::kFactors * 3 * KT);
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };                       // an operand tile is there
+    auto empty = [&](int s) { return bar0 + 8u * (RS + s); };               // the products that read it are done
+    auto raw_full = [&](int s) { return bar0 + 8u * (2 * RS + s); };
+    auto raw_empty = [&](int s) { return bar0 + 8u * (2 * RS + M::kRaws + s); };
+    const uint32_t tail = bar0 + 8u * (2 * RS + 2 * M::kRaws);
+    auto s_full = [&](int b) { return tail + 8u * b; };                     // scores of a buffer
+    auto p_full = [&](int b) { return tail + 8u * (2 + b); };               // weights of a buffer
+    auto o_done = [&](int i) { return tail + 8u * (4 + i); };               // value products of a row tile so far
+    const uint32_t q_full = tail + 8u * 6, drained = tail + 8u * 7;
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + M::kBars);
+    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    const int seq = blockIdx.z, kvh = blockIdx.y % a.c.kv_heads, block = static_cast<int>(gridDim.y) / a.c.kv_heads - 1 - static_cast<int>(blockIdx.y) / a.c.kv_heads;  // the last rows, which see most, first
+    const PagedSequence sq = paged_sequence(a.c, a.r, seq);
+    if (!sq.ok || sq.news < a.few || sq.news > a.many) {
+        if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
+        return;
+    }
+    const int rows = sq.news * a.group, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);
+    if (r0 >= rows) return;
+    if (static_cast<int>(blockIdx.x) >= paged_splits_used(a, sq)) return;
+    const PagedRange range = paged_range(a, sq, r0 / a.group, (r1 - 1) / a.group + 1, blockIdx.x);
+    const int p0 = sq.length - sq.news, tiles = range.end > range.begin ? (range.end - range.begin + KT - 1) / KT : 0, units = tiles * NT;
+
+    if (tid == 0) {
+        for (int s = 0; s < RS; ++s) mbar_init(full(s), Q8 ? 4 : 1), mbar_init(empty(s), 1);
+        for (int s = 0; s < M::kRaws; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4);
+        for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4), mbar_init(o_done(b), 1);
+        mbar_init(q_full, M::kSoftWarps);
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == M::kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(const_cast<uint32_t*>(tmem_slot))), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp >= M::kSoftWarps) {
+        if constexpr (M::kSplitRegs) registers_down<M::kRestRegs>();
+        if (warp == M::kLoadWarp) {
+            // ---- pages to shared memory: per tile of positions the keys' rows, then the values' ----
+            const int* table = a.r.table + static_cast<size_t>(seq) * a.r.stride;
+            const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
+            constexpr int kRing = Q8 ? RW : RS;
+            auto page_of = [&](int k0) {  // lane i: the page of the tile's piece i
+                const int k = k0 + lane * PR;
+                if (lane * PR >= KT || k >= range.end) return 0;
+                int page = table[k >> a.c.page_log2];
+                if (page < 0 || page >= a.c.pages) {
+                    atomicOr(a.c.status, kPagedBadPage);
+                    page = 0;
+                }
+                return page;
+            };
+            int next = tiles > 0 ? page_of(range.begin) : 0, n = 0;
+            bool okay = true;
+            for (int j = 0; j < tiles && okay; ++j) {
+                const int k0 = range.begin + j * KT, pages = next, pieces = (min(KT, range.end - k0) + PR - 1) / PR;
+                if (j + 1 < tiles) next = page_of(k0 + KT);
+                for (int value = 0; value < 2; ++value, ++n) {
+                    const int s = n % kRing;
+                    const uint32_t bar = Q8 ? raw_full(s) : full(s), to = Q8 ? raws + s * M::kRawStride : slots + s * M::kSlot;
+                    if (!(okay = __all_sync(0xffffffffu, mbar_wait(Q8 ? raw_empty(s) : empty(s), ((n / kRing) & 1) ^ 1, abort_flag, a.spin_limit)))) break;
+                    if (!Q8 && value && pieces * PR < KT) {  // rows that no page brings: their weights are zeros, their values must be numbers
+                        for (int i = pieces * PR * 8 + lane; i < KT * 8; i += 32)
+                            for (int b = 0; b < BLOCKS; ++b)
+                                *reinterpret_cast<uint4*>(smem + (to - base) + (b * KT + (i >> 3)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        fence_async_shared();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_expect_tx(bar, pieces * PR * (BLOCKS * kRow + (Q8 && !value ? 8 : 0)));
+                    __syncwarp();
+                    const unsigned char* store = value ? a.c.v : a.c.k;
+                    for (int i0 = 0; i0 < pieces * BLOCKS; i0 += 32) {
+                        const int i = i0 + lane, piece = i / BLOCKS, b = i % BLOCKS, page = __shfl_sync(0xffffffffu, pages, min(piece, 31));
+                        if (i < pieces * BLOCKS)
+                            bulk_load(to + (b * KT + piece * PR) * kRow, store + paged_block_at(a.c, TYPE, page, kvh, b) + static_cast<size_t>((k0 + piece * PR) & (P - 1)) * kRow, PR * kRow, bar);
+                    }
+                    if constexpr (Q8) {
+                        if (!value && lane < pieces) {
+                            const size_t from = paged_scales_at(a.c, pages, kvh) + ((k0 + lane * PR) & (P - 1));
+                            bulk_load(to + M::kRaw + lane * PR * 4, a.c.ks + from, PR * 4, bar);
+                            bulk_load(to + M::kRaw + (KT + lane * PR) * 4, a.c.vs + from, PR * 4, bar);
+                        }
+                    }
+                }
+            }
+            for (int back = max(0, n - kRing); back < n; ++back) mbar_wait(Q8 ? raw_full(back % kRing) : full(back % kRing), (back / kRing) & 1, abort_flag, a.spin_limit, false);
+        } else if (warp == M::kMmaWarp) {
+            // ---- one thread issues all products ----
+            if (lane == 0) {
+                constexpr uint32_t kScores = instr_desc_16(M::BF, false, KT), kValues = instr_desc_16(M::BF, true, HD);
+                bool okay = units == 0 || mbar_wait(q_full, 0, abort_flag, a.spin_limit);
+                fence_after();
+                int have = 0;  // operand tiles waited for: tile n of the sequence keys 0, values 0, keys 1, ...
+                auto need = [&](int n) {
+                    for (; okay && have <= n; ++have) okay = mbar_wait(full(have % RS), (have / RS) & 1, abort_flag, a.spin_limit);
+                    fence_after();
+                    return okay;
+                };
+                auto scores = [&](int u) {  // S of unit u; the keys are given back behind the last unit that reads them
+                    const int j = u / NT, i = u % NT, b = u & 1;
+                    if (!need(2 * j)) return;
+                    const uint32_t keys = slots + (2 * j % RS) * M::kSlot, d = tmem + M::kSCol + b * KT;
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint64_t kd = smem_desc(keys + (k >> 2) * KT * 128, 16, 1024, 2) + 2 * (k & 3);
+                        if constexpr (M::kQTmem) mma_ts(d, tmem + M::kQCol + k * 8, kd, kScores, k > 0);
+                        else mma_ss(d, smem_desc(q_at + (i * BLOCKS + (k >> 2)) * 128 * 128, 16, 1024, 2) + 2 * (k & 3), kd, kScores, k > 0);
+                    }
+                    mma_commit(s_full(b));
+                    if (i == NT - 1) mma_commit(empty(2 * j % RS));
+                };
+                if (units > 0) scores(0);
+                if (okay && units > 1) scores(1);
+                for (int u = 0; u < units && okay; ++u) {
+                    const int j = u / NT, i = u % NT, b = u & 1;
+                    if (!need(2 * j + 1) || !(okay = mbar_wait(p_full(b), (u >> 1) & 1, abort_flag, a.spin_limit))) break;
+                    fence_after();
+                    const uint32_t values = slots + ((2 * j + 1) % RS) * M::kSlot;
+#pragma unroll
+                    for (int k = 0; k < KT / 16; ++k)
+                        mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, smem_desc(values + k * 16 * 128, KT * 128, 1024, 2), kValues, j > 0 || k > 0);
+                    mma_commit(o_done(i));
+                    if (i == NT - 1) mma_commit(empty((2 * j + 1) % RS));
+                    if (u + 2 < units) scores(u + 2);
+                }
+                mma_commit(drained);  // nothing is under way when the block leaves
+                mbar_wait(drained, 0, abort_flag, a.spin_limit, false);
+            }
+            __syncwarp();
+        } else if (Q8 && warp >= M::kWidenWarp) {
+            // ---- codes to F16 operands ----
+            if constexpr (Q8) {
+                const int w = tid - M::kWidenWarp * 32;
+                bool okay = true;
+                for (int n = 0; n < 2 * tiles && okay; ++n) {
+                    const int j = n >> 1, value = n & 1, rs = n % RW, s = n % RS, left = range.end - (range.begin + j * KT);  // rows of the tile that are there
+                    okay = __all_sync(0xffffffffu, mbar_wait(raw_full(rs), (n / RW) & 1, abort_flag, a.spin_limit) && mbar_wait(empty(s), ((n / RS) & 1) ^ 1, abort_flag, a.spin_limit));
+                    if (!okay) break;
+                    const uint32_t from = raws + rs * M::kRawStride;
+                    unsigned char* to = smem + M::kQBytes + s * M::kSlot;
+                    if (!value && w < KT) {
+                        const float* d = reinterpret_cast<const float*>(raw_smem + rs * M::kRawStride + M::kRaw) + w;
+                        float* f = factors + (j & 3) * 3 * KT + w;
+                        f[0] = w < left ? d[0] : 0.0f, f[KT] = w < left ? lg2(d[KT]) : 0.0f, f[2 * KT] = w < left ? rcp(d[KT]) : 0.0f;
+                    }
+#pragma unroll 4
+                    for (int i = w; i < KT * BLOCKS * 4; i += 128) {  // a piece of sixteen codes
+                        const int row = i >> 2, r = row % KT, c = (i & 3) ^ ((r >> 1) & 3);
+                        uint32_t v[4], o[8];
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(from + i * 16) : "memory");
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t u = r < left ? v[e] ^ 0x80808080u : 0x80808080u;
+                            o[2 * e] = codes_to_half2(u, 0x4140), o[2 * e + 1] = codes_to_half2(u, 0x4342);
+                        }
+                        *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full(s)), mbar_arrive(raw_empty(rs));
+                }
+            }
+        }
+    } else {
+        if constexpr (M::kSplitRegs) registers_up<M::kSoftRegs>();
+        // ---- a row of queries per thread ----
+        const int i = warp >> 2, local = (warp & 3) * 32 + lane, r = r0 + i * 128 + local, t = r / a.group, h = kvh * a.group + r % a.group;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const bool live = r < r1;
+        float rowf;  // what the row's scores are multiplied by: never negative, the queries take the sign
+        {
+            const unsigned char* src = static_cast<const unsigned char*>(a.q) + ((static_cast<size_t>(sq.first) + (live ? t : 0)) * a.q_token + (live ? h : kvh * a.group) * a.q_head) * paged_size_of(a.q_type);
+            float f = a.scale < 0.0f ? -1.0f : 1.0f;
+            rowf = fabsf(a.scale);
+            if constexpr (Q8) {
+                float m = 0.0f;
+#pragma unroll 4
+                for (int e = 0; e < HD; e += 8) {
+                    float x[8];
+                    paged_load8(src + e * paged_size_of(a.q_type), a.q_type, x);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+                }
+                const uint32_t ex = __float_as_uint(m) >> 23;
+                if (ex > 1 && ex < 254) rowf *= __uint_as_float(ex << 23), f *= __uint_as_float((254 - ex) << 23);
+            }
+#pragma unroll 2
+            for (int e = 0; e < HD; e += 64) {
+                uint32_t v[32];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float x[8];
+                    paged_load8(src + (e + k * 8) * paged_size_of(a.q_type), a.q_type, x);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k * 4 + c] = live ? paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x[2 * c] * f, x[2 * c + 1] * f) : 0u;
+                }
+                if constexpr (M::kQTmem) {
+                    tmem_store32(tmem + lanes + M::kQCol + e / 2, v);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        *reinterpret_cast<uint4*>(smem + ((i * BLOCKS + e / 64) * 128 + local) * 128 + ((k ^ (local & 7)) << 4)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                }
+            }
+            if constexpr (M::kQTmem) tmem_wait_store();
+            else fence_async_shared();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const int p = p0 + t, last = live ? min(p, range.end - 1) : -1, first = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        float m = -INFINITY, l = 0.0f;
+        bool okay = true;
+        for (int j = 0; j < tiles; ++j) {
+            const int u = j * NT + i, b = u & 1, k0 = range.begin + j * KT;
+            const uint32_t s_at = tmem + lanes + M::kSCol + b * KT;
+            okay = __all_sync(0xffffffffu, mbar_wait(s_full(b), (u >> 1) & 1, abort_flag, a.spin_limit));
+            if (!okay) break;
+            fence_after();
+            uint32_t s[KT / 32][32];
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c) tmem_load32(s_at + c * 32, s[c]);
+            tmem_wait_load();
+            const float* f = factors + (j & 3) * 3 * KT;
+            const bool masked = __any_sync(0xffffffffu, k0 + KT - 1 > last || k0 < first);
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    float x = __uint_as_float(s[c][e]);
+                    if constexpr (Q8) x *= f[c * 32 + e];
+                    x *= rowf;
+                    if (a.cap > 0.0f) x = a.cap * tanh_of(x);
+                    if constexpr (Q8) x += f[KT + c * 32 + e];
+                    if (masked) x = k0 + c * 32 + e >= first && k0 + c * 32 + e <= last ? x : -INFINITY;
+                    s[c][e] = __float_as_uint(x);
+                    top = fmaxf(top, x);
+                }
+            const bool grew = top > m + kPagedLazy || (m == -INFINITY && top > -INFINITY);
+            if (__any_sync(0xffffffffu, grew)) {
+                const float keep = grew ? ex2(m - top) : 1.0f;  // 0 the first time
+                if (grew) m = top, l *= keep;
+                if (j > 0) {
+                    okay = __all_sync(0xffffffffu, mbar_wait(o_done(i), (j - 1) & 1, abort_flag, a.spin_limit));
+                    if (!okay) break;
+                    fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        tmem_store32(tmem + lanes + M::kOCol + i * 128 + c, o);
+                    }
+                }
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int c = 0; c < KT / 64; ++c) {
+                uint32_t w[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int k = 2 * e, cc = c * 2 + k / 32;
+                    const float x0 = ex2(__uint_as_float(s[cc][k % 32]) - ref), x1 = ex2(__uint_as_float(s[cc][k % 32 + 1]) - ref);
+                    if constexpr (Q8) l = fmaf(x0, f[2 * KT + c * 64 + k], l), l = fmaf(x1, f[2 * KT + c * 64 + k + 1], l);
+                    else l += x0 + x1;
+                    w[e] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x0, x1);
+                }
+                tmem_store32(s_at + c * 32, w);
+            }
+            tmem_wait_store();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(b));
+        }
+        if (okay && tiles > 0) okay = __all_sync(0xffffffffu, mbar_wait(o_done(i), (tiles - 1) & 1, abort_flag, a.spin_limit));
+        okay = __all_sync(0xffffffffu, okay && *abort_flag == 0);
+        if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
+        if (okay) {
+            fence_after();
+            const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+            const int heads = a.c.kv_heads * a.group;
+            const size_t token = static_cast<size_t>(sq.first) + t, row = (static_cast<size_t>(blockIdx.x) * a.r.tokens + token) * heads + h;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                if (tiles > 0) {
+                    tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
+                    tmem_wait_load();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (!live) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    float x[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(o[e + k]);
+                    if (a.splits == 1) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) x[k] *= inv;
+                        paged_store8(static_cast<unsigned char*>(a.out) + (token * a.o_token + h * a.o_head + c + e) * paged_size_of(a.out_type), a.out_type, x);
+                    } else {
+                        paged_store8(a.part_o + row * HD + c + e, kPagedF32, x);
+                    }
+                }
+            }
+            if (live && a.splits > 1) a.part_ml[row] = make_float2(m, l);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == M::kMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace qtb

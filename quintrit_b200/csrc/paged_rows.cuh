@@ -69,32 +69,32 @@ __device__ __forceinline__ PagedRaw<TYPE> paged_raw(const void* base, size_t ele
 }
 
 template <int LANES, int TYPE, int U>  // threads of a head: head_dim / 8; type of q, k and v; groups of heads of a warp
-__global__ void __launch_bounds__(kPagedRowThreads) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
-    constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a group
+__global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
+    constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a group: all of them queries, keys or values
     __shared__ __align__(16) float exchange[kPagedRowThreads / 32][kHeads][HD];  // NEOX pairs lie half a rotation apart
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, piece = lane % LANES;
-    const int heads = a.q_heads + 2 * a.c.kv_heads, groups = (heads + U * kHeads - 1) / (U * kHeads);
-    const int item = blockIdx.x * (kPagedRowThreads / 32) + warp, t = item / groups;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, piece = lane % LANES, e0 = piece * 8;
+    const int q_groups = (a.q_heads + kHeads - 1) / kHeads, kv_groups = (a.c.kv_heads + kHeads - 1) / kHeads, all = q_groups + 2 * kv_groups, units = (all + U - 1) / U;
+    const int item = blockIdx.x * (kPagedRowThreads / 32) + warp, t = item / units;
     if (t >= a.r.tokens) return;
-    const int head0 = item % groups * U * kHeads + sub;
+    const int g0 = item % units * U;
+    // group u of this warp: its kind (0 queries, 1 keys, 2 values) and this thread's head, the last one where there are no more
+    auto kind_of = [&](int g) { return g < q_groups ? 0 : g < q_groups + kv_groups ? 1 : 2; };
+    auto head_of = [&](int g, int kind) { return (g - (kind == 0 ? 0 : kind == 1 ? q_groups : q_groups + kv_groups)) * kHeads + sub; };
     PagedRaw<TYPE> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int head = min(head0 + u * kHeads, heads - 1), kind = head < a.q_heads ? 0 : head < a.q_heads + a.c.kv_heads ? 1 : 2;  // query, key, value
-        const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.c.kv_heads;
-        const size_t at = kind == 0 ? t * a.q_token + h * a.q_head : kind == 1 ? t * a.k_token + h * a.k_head : t * a.v_token + h * a.v_head;
-        raw[u] = paged_raw<TYPE>(kind == 0 ? a.q : kind == 1 ? a.k : a.v, at + piece * 8);
+        const int g = min(g0 + u, all - 1), kind = kind_of(g), h = min(head_of(g, kind), (kind == 0 ? a.q_heads : a.c.kv_heads) - 1);
+        raw[u] = kind == 0 ? paged_raw<TYPE>(a.q, t * a.q_token + h * a.q_head + e0) : kind == 1 ? paged_raw<TYPE>(a.k, t * a.k_token + h * a.k_head + e0)
+                                                                                               : paged_raw<TYPE>(a.v, t * a.v_token + h * a.v_head + e0);
     }
     const PagedPlace place = paged_place(a.c, a.r, t, a.cos_sin != nullptr ? a.positions : 0x7fffffff);
     // (a query of a token whose page does not exist is left as it was, like its row of the cache)
     if (place.page < 0) return;
     // this thread's factors of the rotation: x_i cos_i + partner_i sin_i
     float cs[8], sn[8];
-    const int half = a.rope / 2, e0 = piece * 8;
-    const bool neox = a.cos_sin != nullptr && a.neox != 0, whole = a.vector != 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) cs[i] = 1.0f, sn[i] = 0.0f;
-    if (a.cos_sin != nullptr && e0 < a.rope) {
+    const int half = a.rope / 2;
+    const bool turns = a.cos_sin != nullptr && g0 < q_groups + kv_groups, rotate = turns && e0 < a.rope;
+    if (rotate) {
         const float* row = a.cos_sin + static_cast<size_t>(place.pos) * a.rope;
         if (a.vector && a.neox) {  // eight pairs, all first or all second values
             const bool second = e0 >= half;
@@ -114,8 +114,7 @@ __global__ void __launch_bounds__(kPagedRowThreads) paged_append_kernel(const __
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int e = e0 + i;
-                if (e >= a.rope) continue;
+                const int e = min(e0 + i, a.rope - 1);
                 const bool second = a.neox ? e >= half : (e & 1) != 0;
                 const int p = a.neox ? (second ? e - half : e) : e >> 1;
                 cs[i] = row[2 * p], sn[i] = second ? row[2 * p + 1] : -row[2 * p + 1];
@@ -125,75 +124,78 @@ __global__ void __launch_bounds__(kPagedRowThreads) paged_append_kernel(const __
     const float most_finite = a.type == kPagedF16 ? 65504.0f : a.type == kPagedBf16 ? 3.3895313892515355e38f : 8.507059173023462e37f;  // (Q8: 2^126, so that 127 d does not overflow)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int head = head0 + u * kHeads, kind = head < a.q_heads ? 0 : head < a.q_heads + a.c.kv_heads ? 1 : 2;
-        const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.c.kv_heads;
-        const bool live = head < heads;
-        if (head0 - sub + u * kHeads >= heads) break;  // (the whole warp)
+        const int g = g0 + u, kind = kind_of(g), h = head_of(g, kind);
+        if (g >= all) break;
+        const bool live = h < (kind == 0 ? a.q_heads : a.c.kv_heads);
         float x[8];
         paged_load8(raw[u].v, TYPE, x);
         const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-        if (a.q_norm != nullptr || a.k_norm != nullptr) {
-            float sum = 0.0f;
+        if (w != nullptr) {
+            float sum = 0.0f, f[8];
+            paged_load8(w + e0, kPagedF32, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (w != nullptr) {
-                const float inv = 1.0f / sqrtf(sum / HD + a.eps);
-                float g[8];
-                paged_load8(w + e0, kPagedF32, g);
+            const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);  // (off by 2^-22 at most)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-            }
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * f[i];
         }
-        float y[8];  // the other one of each pair
-        if (neox) {
-            float* row = exchange[warp][sub];
-            __syncwarp();
-            paged_store8(row + e0, kPagedF32, x);
-            __syncwarp();
-            const int from = e0 >= half ? e0 - half : e0 + half;
-            if (whole) {
-                paged_load8(row + (e0 < a.rope ? from : e0), kPagedF32, y);
+        if (turns && kind != 2) {
+            float y[8];  // the other one of each pair
+            if (a.neox) {
+                float* row = exchange[warp][sub];
+                __syncwarp();
+                paged_store8(row + e0, kPagedF32, x);
+                __syncwarp();
+                if (a.vector) {
+                    if (rotate) paged_load8(row + (e0 >= half ? e0 - half : e0 + half), kPagedF32, y);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = row[e0 + i >= a.rope ? e0 + i : e0 + i >= half ? e0 + i - half : e0 + i + half];
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = row[e0 + i >= a.rope ? e0 + i : e0 + i >= half ? e0 + i - half : e0 + i + half];
+                for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
             }
-        } else {
+            if (rotate && a.vector) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
+                for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], cs[i], y[i] * sn[i]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = y[i];
+            } else if (rotate) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = e0 + i < a.rope ? fmaf(x[i], cs[i], y[i] * sn[i]) : x[i];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = y[i];
+            }
         }
-        if (kind != 2) {
-            float r[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = sn[i] == 0.0f && cs[i] == 1.0f ? x[i] : fmaf(x[i], cs[i], y[i] * sn[i]);  // (nothing of a partner that is no number where there is no rotation)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = r[i];
+        if (kind == 0) {
+            if (live) paged_store8(static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.q_type), a.q_type, x);
+            continue;
         }
-        if (live && kind == 0) paged_store8(static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.q_type), a.q_type, x);
-        // what is not finite, or does not fit the type, becomes the nearest value that does, and a value that is none becomes zero
-        bool odd = false;
         float amax = 0.0f;
+        bool fits = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i])), odd = odd || !(fabsf(x[i]) <= most_finite);
-        if (odd) {
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i])), fits = fits && fabsf(x[i]) <= most_finite;
+        if (!fits) {  // the nearest value that is finite and fits the type; zero for what is no number
             amax = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (!(fabsf(x[i]) <= most_finite)) x[i] = isnan(x[i]) ? 0.0f : copysignf(most_finite, x[i]);
                 amax = fmaxf(amax, fabsf(x[i]));
             }
-            if (live && kind != 0) atomicOr(a.c.status, kPagedSaturated);
+            if (live) atomicOr(a.c.status, kPagedSaturated);
         }
         unsigned char* block = (kind == 1 ? a.c.k : a.c.v) + paged_block_at(a.c, a.type, place.page, h, piece >> 3);
         if (a.type != kPagedQ8) {
-            if (live && kind != 0) paged_store8(block + place.row * 128 + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
+            if (live) paged_store8(block + place.row * 128 + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
             continue;
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (!live || kind == 0) continue;
-        const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = 1.0f / d;
+        if (!live) continue;
+        const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = __fdividef(1.0f, d);
         uint32_t code[2] = {0u, 0u};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // (|x| / d <= 127 (1 + 2^-22), which rounds to 127; x (1 / d) is off x / d by 2^-16 of a step at most)
