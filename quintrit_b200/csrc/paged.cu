@@ -100,15 +100,15 @@ int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void
 
 // How the positions are cut into ranges: enough blocks of threads to fill the device, ranges of at least four tiles.
 struct PagedCut {
-    int splits, split, most;  // most: no window makes more ranges of it
+    int splits, split;
 };
-PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles) {
+PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles, int limit) {
     long long span = std::max<uint32_t>(r->max_length, 1);
     if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
     const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_tiles;
-    const long long want = std::max<long long>(1, std::min<long long>({(4LL * c->sm_count + items - 1) / items, (tiles + 3) / 4, 128}));
+    const long long want = std::max<long long>(1, std::min<long long>({(4LL * c->sm_count + items - 1) / items, (tiles + 3) / 4, limit}));
     const long long per = (tiles + want - 1) / want;
-    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile), static_cast<int>(want)};
+    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile)};
 }
 
 // The shared memory a kernel may ask for, raised once per device (`done`: a bit per device; two threads at once set the same).
@@ -140,6 +140,23 @@ template <int TYPE>
 int launch_few_type(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
     return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, rt, grid, s) : launch_few_rows<TYPE, 4>(a, device, rt, grid, s);
 }
+// The same for the kernel for many rows, one block of threads per multiprocessor: waves of blocks, each as long as its tiles and a start that costs about four, and what writing and reading
+// the ranges' results costs, in tiles of about 0.6 us.
+PagedCut cut_of_many(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, long long row_blocks, int limit) {
+    long long span = std::max<uint32_t>(r->max_length, 1);
+    if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
+    const int tile = c->head_dim == 256 ? 64 : 128;
+    const long long tiles = (span + tile - 1) / tile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_blocks;
+    const double part = static_cast<double>(r->tokens) * q_heads * c->head_dim * 8.0 / 4.0e12 / 0.6e-6;
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= limit && s <= std::max<long long>(1, tiles / 2); ++s) {
+        const double cost = static_cast<double>((items * s + c->sm_count - 1) / c->sm_count) * ((tiles + s - 1) / s + 4) + (s > 1 ? 4 + s * part : 0);
+        if (cost < least * 0.97) best = s, least = cost;
+    }
+    const long long per = (tiles + best - 1) / best;
+    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * tile)};
+}
 template <int TYPE, int BLOCKS>
 int launch_many_of(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
     using M = PagedMany<TYPE, BLOCKS>;
@@ -164,7 +181,6 @@ struct PagedPlan {
     int rt;                  // few: row tiles of a block, blocks per head
     long long few_tiles, many_tiles;
     PagedCut few_cut, many_cut;
-    int most_splits() const { return std::max(few_new > 0 ? few_cut.most : 1, many ? many_cut.most : 1); }
     int splits() const { return std::max(few_new > 0 ? few_cut.splits : 1, many ? many_cut.splits : 1); }
 };
 PagedPlan plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window) {
@@ -176,12 +192,14 @@ PagedPlan plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_
         const long long rows = p.few_new * group;
         p.rt = row_tiles_of(static_cast<int>(rows));
         p.few_tiles = (rows + 16 * p.rt - 1) / (16 * p.rt);
-        p.few_cut = cut_of(c, r, window, p.few_tiles);
+        p.few_cut = cut_of(c, r, 0, p.few_tiles, 128);
+        if (window > 0) p.few_cut = cut_of(c, r, window, p.few_tiles, p.few_cut.splits);  // (no window takes more of the workspace than none)
     }
     if (p.many) {
         const int block = c->head_dim == 256 ? 128 : 256;
         p.many_tiles = (most + block - 1) / block;
-        p.many_cut = cut_of(c, r, window, p.many_tiles);
+        p.many_cut = cut_of_many(c, r, q_heads, 0, p.many_tiles, 32);
+        if (window > 0) p.many_cut = cut_of_many(c, r, q_heads, window, p.many_tiles, p.many_cut.splits);
     }
     return p;
 }
@@ -363,7 +381,7 @@ extern "C" int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged
         *out_bytes = 0;
         if ((rc = check_rows(cache, rows, false)) != QUINTRIT_OK || (rc = check_heads(cache, q_heads)) != QUINTRIT_OK) return rc;
         if (rows->tokens == 0) return ok();
-        *out_bytes = workspace_of(cache, rows, q_heads, plan_of(cache, rows, q_heads, 0).most_splits());
+        *out_bytes = workspace_of(cache, rows, q_heads, plan_of(cache, rows, q_heads, 0).splits());
         return ok();
     });
 }

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     const uint32_t tail = bar0 + 8u * (2 * RS + 2 * M::kRaws);
     auto s_full = [&](int b) { return tail + 8u * b; };                     // scores of a buffer
     auto p_full = [&](int b) { return tail + 8u * (2 + b); };               // weights of a buffer
-    auto o_done = [&](int i) { return tail + 8u * (4 + i); };               // value products of a row tile so far
+    auto o_done = [&](int b) { return tail + 8u * (4 + b); };               // the value products of a buffer's weights
     const uint32_t q_full = tail + 8u * 6, drained = tail + 8u * 7;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + M::kBars);
     volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1);
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k)
                         mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, smem_desc(values + k * 16 * 128, KT * 128, 1024, 2), kValues, j > 0 || k > 0);
-                    mma_commit(o_done(i));
+                    mma_commit(o_done(b));
                     if (i == NT - 1) mma_commit(empty((2 * j + 1) % RS));
                     if (u + 2 < units) scores(u + 2);
                 }
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
         {
             const unsigned char* src = static_cast<const unsigned char*>(a.q) + ((static_cast<size_t>(sq.first) + (live ? t : 0)) * a.q_token + (live ? h : kvh * a.group) * a.q_head) * paged_size_of(a.q_type);
             float f = a.scale < 0.0f ? -1.0f : 1.0f;
-            rowf = fabsf(a.scale);
+            rowf = fmaxf(fabsf(a.scale), 1e-37f);  // (times minus infinity, where a mask hides a score, it stays that)
             if constexpr (Q8) {
                 float m = 0.0f;
 #pragma unroll 4
@@ -317,6 +317,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
         const int p = p0 + t, last = live ? min(p, range.end - 1) : -1, first = a.window > 0 ? max(0, p - a.window + 1) : 0;
         float m = -INFINITY, l = 0.0f;
         bool okay = true;
+        // The value products of unit u. A wait tells phases apart by their parity alone, so each buffer has a barrier: those of unit u - 2, the phase before, are done, as the scores
+        // of unit u (asked for behind them) were waited for, and those of unit u + 2 cannot have begun.
+        auto values_done = [&](int u) { return mbar_wait(o_done(u & 1), (u >> 1) & 1, abort_flag, a.spin_limit); };
         for (int j = 0; j < tiles; ++j) {
             const int u = j * NT + i, b = u & 1, k0 = range.begin + j * KT;
             const uint32_t s_at = tmem + lanes + M::kSCol + b * KT;
@@ -327,28 +330,57 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c) tmem_load32(s_at + c * 32, s[c]);
             tmem_wait_load();
-            const float* f = factors + (j & 3) * 3 * KT;
-            const bool masked = __any_sync(0xffffffffu, k0 + KT - 1 > last || k0 < first);
-            float top = -INFINITY;
+            // v in s, so that a weight is 2^(v mul - m): the products themselves, where only the scale is to come; else the whole exponent
+            float mul = 1.0f;
+            const float4* f = reinterpret_cast<const float4*>(factors + (j & 3) * 3 * KT);
+            auto pair = [&](int c, int e) { return pack_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])); };
+            auto put = [&](int c, int e, unsigned long long v) {
+                const float2 x = unpack_f32x2(v);
+                s[c][e] = __float_as_uint(x.x), s[c][e + 1] = __float_as_uint(x.y);
+            };
+            const unsigned long long row2 = pack_f32x2(rowf, rowf);
+            if (a.cap > 0.0f) {
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        float x = __uint_as_float(s[c][e]);
+                        if constexpr (Q8) x *= reinterpret_cast<const float*>(f)[c * 32 + e];
+                        x = a.cap * tanh_of(x * rowf);
+                        if constexpr (Q8) x += reinterpret_cast<const float*>(f)[KT + c * 32 + e];
+                        s[c][e] = __float_as_uint(x);
+                    }
+            } else if constexpr (Q8) {
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 ks = f[(c * 32 + e) / 4], lv = f[(KT + c * 32 + e) / 4];
+                        put(c, e, fma_f32x2(mul_f32x2(pair(c, e), pack_f32x2(ks.x, ks.y)), row2, pack_f32x2(lv.x, lv.y)));
+                        put(c, e + 2, fma_f32x2(mul_f32x2(pair(c, e + 2), pack_f32x2(ks.z, ks.w)), row2, pack_f32x2(lv.z, lv.w)));
+                    }
+            } else {
+                mul = rowf;
+            }
+            if (__any_sync(0xffffffffu, k0 + KT - 1 > last || k0 < first)) {
+                const int lo = first - k0, hi = last - k0;
+#pragma unroll
+                for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e >= lo && c * 32 + e <= hi ? s[c][e] : 0xff800000u;  // minus infinity
+            }
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four at a time: a chain of maxima or sums takes four cycles a link
 #pragma unroll
             for (int c = 0; c < KT / 32; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float x = __uint_as_float(s[c][e]);
-                    if constexpr (Q8) x *= f[c * 32 + e];
-                    x *= rowf;
-                    if (a.cap > 0.0f) x = a.cap * tanh_of(x);
-                    if constexpr (Q8) x += f[KT + c * 32 + e];
-                    if (masked) x = k0 + c * 32 + e >= first && k0 + c * 32 + e <= last ? x : -INFINITY;
-                    s[c][e] = __float_as_uint(x);
-                    top = fmaxf(top, x);
-                }
+                for (int e = 0; e < 32; ++e) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[c][e]));
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
             const bool grew = top > m + kPagedLazy || (m == -INFINITY && top > -INFINITY);
             if (__any_sync(0xffffffffu, grew)) {
                 const float keep = grew ? ex2(m - top) : 1.0f;  // 0 the first time
                 if (grew) m = top, l *= keep;
                 if (j > 0) {
-                    okay = __all_sync(0xffffffffu, mbar_wait(o_done(i), (j - 1) & 1, abort_flag, a.spin_limit));
+                    okay = __all_sync(0xffffffffu, values_done(u - NT));
                     if (!okay) break;
                     fence_after();
 #pragma unroll 1
@@ -362,26 +394,36 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     }
                 }
             }
-            const float ref = m == -INFINITY ? 0.0f : m;
+            const float ref = m == -INFINITY ? 0.0f : -m;
+            const unsigned long long mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(ref, ref);
+            unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < KT / 64; ++c) {
                 uint32_t w[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
+                for (int e = 0; e < 32; e += 2) {
                     const int k = 2 * e, cc = c * 2 + k / 32;
-                    const float x0 = ex2(__uint_as_float(s[cc][k % 32]) - ref), x1 = ex2(__uint_as_float(s[cc][k % 32 + 1]) - ref);
-                    if constexpr (Q8) l = fmaf(x0, f[2 * KT + c * 64 + k], l), l = fmaf(x1, f[2 * KT + c * 64 + k + 1], l);
-                    else l += x0 + x1;
-                    w[e] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x0, x1);
+                    float2 x = unpack_f32x2(fma_f32x2(pair(cc, k % 32), mul2, ref2)), y = unpack_f32x2(fma_f32x2(pair(cc, k % 32 + 2), mul2, ref2));
+                    x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
+                    if constexpr (Q8) {
+                        const float4 iv = f[(2 * KT + c * 64 + k) / 4];
+                        sums[0] = fma_f32x2(pack_f32x2(x.x, x.y), pack_f32x2(iv.x, iv.y), sums[0]);
+                        sums[1] = fma_f32x2(pack_f32x2(y.x, y.y), pack_f32x2(iv.z, iv.w), sums[1]);
+                    } else {
+                        sums[0] = add_f32x2(sums[0], pack_f32x2(x.x, x.y)), sums[1] = add_f32x2(sums[1], pack_f32x2(y.x, y.y));
+                    }
+                    w[e] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x.x, x.y), w[e + 1] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, y.x, y.y);
                 }
                 tmem_store32(s_at + c * 32, w);
             }
+            const float2 sum = unpack_f32x2(add_f32x2(sums[0], sums[1]));
+            l += sum.x + sum.y;
             tmem_wait_store();
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full(b));
         }
-        if (okay && tiles > 0) okay = __all_sync(0xffffffffu, mbar_wait(o_done(i), (tiles - 1) & 1, abort_flag, a.spin_limit));
+        if (okay && tiles > 0) okay = __all_sync(0xffffffffu, values_done((tiles - 1) * NT + i));
         okay = __all_sync(0xffffffffu, okay && *abort_flag == 0);
         if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
         if (okay) {
@@ -391,6 +433,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             const size_t token = static_cast<size_t>(sq.first) + t, row = (static_cast<size_t>(blockIdx.x) * a.r.tokens + token) * heads + h;
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
+                if (tiles == 0 && a.splits > 1) break;
                 uint32_t o[32];
                 if (tiles > 0) {
                     tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
@@ -414,7 +457,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     }
                 }
             }
-            if (live && a.splits > 1) a.part_ml[row] = make_float2(m, l);
+            if (live && a.splits > 1) a.part_ml[row] = make_float2(m, l);  // (of a range in which the row sees nothing this is all that is read)
         }
     }
     fence_before();
