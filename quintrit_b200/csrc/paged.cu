@@ -140,37 +140,69 @@ template <int TYPE>
 int launch_few_type(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
     return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, rt, grid, s) : launch_few_rows<TYPE, 4>(a, device, rt, grid, s);
 }
-// The same for the kernel for many rows, one block of threads per multiprocessor: waves of blocks, each as long as its tiles and a start that costs about four, and what writing and reading
-// the ranges' results costs, in tiles of about 0.6 us.
-PagedCut cut_of_many(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, long long row_blocks, int limit) {
-    long long span = std::max<uint32_t>(r->max_length, 1);
-    if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
-    const int tile = c->head_dim == 256 ? 64 : 128;
-    const long long tiles = (span + tile - 1) / tile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_blocks;
-    const double part = static_cast<double>(r->tokens) * q_heads * c->head_dim * 8.0 / 4.0e12 / 0.6e-6;
+// The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles and a start and an end of
+// about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. Where the sequences' chunks differ, as in a step that carries one
+// prompt, fewer row blocks are there than the longest chunk times the sequences: their number is taken from the tokens.
+size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, size_t limit, PagedSchedule* g) {
+    constexpr double kStart = 4.0, kJoin = 3.0;
+    const int rows = c->head_dim == 256 ? 128 : 256, tile = c->head_dim == 256 ? 64 : 128, sms = c->sm_count;
+    const long long most = static_cast<long long>(r->max_new) * group, blocks = (most + rows - 1) / rows, kvh = c->kv_heads;
+    const long long all = static_cast<long long>(r->tokens) * group, m = std::max<long long>(kvh, kvh * ((all + rows - 1) / rows) / blocks);  // blocks of an order, likely
+    // tiles that the row block of an order sees, if its sequence has the length that was announced
+    auto tiles_of = [&](long long order) -> long long {
+        const long long first = (blocks - 1 - order) * rows / group, last = std::min<long long>(((blocks - order) * rows - 1) / group, r->max_new - 1), before = static_cast<long long>(r->max_length) - r->max_new;
+        const long long high = std::max<long long>(before + last + 1, 1), low = window > 0 ? std::max<long long>(before + first - window + 1, 0) : 0;
+        return std::max<long long>(1, (high - low + tile - 1) / tile);
+    };
+    g->m = static_cast<int>(kvh * r->sequences), g->mapped = 0, g->whole = static_cast<int>(blocks), g->cut = 1;
+    if (blocks * m < sms) {
+        // Ranges of at most `length` tiles, the shortest for which they are there at once.
+        const size_t per_range = static_cast<size_t>(all) * kvh;
+        const long long longest = tiles_of(0);
+        long long best = longest;
+        for (long long length = longest - 1; length >= 2; --length) {
+            long long parts = 0;
+            for (long long o = 0; o < blocks && parts * m <= sms; ++o) parts += (tiles_of(o) + length - 1) / length;
+            if (parts * m > sms || parts > kPagedMapped || static_cast<size_t>((longest + length - 1) / length) * per_range > limit) break;
+            best = length;
+        }
+        if (best + kJoin >= longest) return 0;
+        int x = 0;
+        for (long long o = 0; o < blocks; ++o) {
+            const int ranges = static_cast<int>((tiles_of(o) + best - 1) / best);
+            for (int i = 0; i < ranges; ++i, ++x) g->order[x] = static_cast<unsigned char>(o), g->range[x] = static_cast<unsigned char>(i), g->ranges[x] = static_cast<unsigned char>(ranges);
+        }
+        g->mapped = x, g->whole = 0;
+        return static_cast<size_t>((longest + best - 1) / best) * per_range;
+    }
+    const long long whole = blocks * m / sms * sms / m, left = blocks - whole;  // row blocks that fill whole waves, and those that do not
+    if (left == 0) return 0;
+    const double tiles = static_cast<double>(tiles_of(whole));
+    const long long room = sms + (blocks * m / sms * sms - whole * m);
     int best = 1;
     double least = 1e30;
-    for (int s = 1; s <= limit && s <= std::max<long long>(1, tiles / 2); ++s) {
-        const double cost = static_cast<double>((items * s + c->sm_count - 1) / c->sm_count) * ((tiles + s - 1) / s + 4) + (s > 1 ? 4 + s * part : 0);
+    for (int s = 1; s <= 24 && (s == 1 || (static_cast<size_t>(left) * g->m * s * rows <= limit && tiles / s >= 2.0)); ++s) {
+        const double cost = static_cast<double>((left * m * s + room - 1) / room) * (std::ceil(tiles / s) + kStart) + (s > 1 ? kJoin : 0.0);
         if (cost < least * 0.97) best = s, least = cost;
     }
-    const long long per = (tiles + best - 1) / best;
-    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * tile)};
+    if (best == 1) return 0;
+    g->whole = static_cast<int>(whole), g->cut = best;
+    return static_cast<size_t>(left) * g->m * best * rows;
 }
 template <int TYPE, int BLOCKS>
-int launch_many_of(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
+int launch_many_of(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
     using M = PagedMany<TYPE, BLOCKS>;
     static_assert(M::kSmem <= 227 * 1024, "the rings do not fit");
     static std::atomic<uint64_t> done{0};
     const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS>, M::kSmem, device, done);
     if (rc != QUINTRIT_OK) return rc;
-    paged_many_kernel<TYPE, BLOCKS><<<grid, M::kThreads, M::kSmem, s>>>(a);
+    paged_many_kernel<TYPE, BLOCKS><<<grid, M::kThreads, M::kSmem, s>>>(a, g);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
 template <int TYPE>
-int launch_many_type(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
-    return a.c.blocks == 1 ? launch_many_of<TYPE, 1>(a, device, grid, s) : a.c.blocks == 2 ? launch_many_of<TYPE, 2>(a, device, grid, s) : launch_many_of<TYPE, 4>(a, device, grid, s);
+int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
+    return a.c.blocks == 1 ? launch_many_of<TYPE, 1>(a, g, device, grid, s) : a.c.blocks == 2 ? launch_many_of<TYPE, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 4>(a, g, device, grid, s);
 }
 int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a block of threads
 
@@ -178,32 +210,40 @@ int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a blo
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
     bool many;
-    int rt;                  // few: row tiles of a block, blocks per head
-    long long few_tiles, many_tiles;
-    PagedCut few_cut, many_cut;
-    int splits() const { return std::max(few_new > 0 ? few_cut.splits : 1, many ? many_cut.splits : 1); }
+    int rt;                  // few: row tiles of a block, blocks per head, ranges
+    long long few_tiles;
+    PagedCut few_cut;
+    PagedSchedule schedule;  // many: which blocks, their number, slots of the workspace
+    long long many_blocks;
+    size_t part_rows;
+    size_t few_bytes, many_bytes;  // of the workspace
 };
-PagedPlan plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window) {
-    PagedPlan p{};
+constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {
     const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = 64;
-    p.many = most > limit;
-    p.few_new = static_cast<int>(!p.many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(limit / group, r->max_new - 1));  // (a sequence alone is the longest)
-    if (p.few_new > 0) {
-        const long long rows = p.few_new * group;
-        p.rt = row_tiles_of(static_cast<int>(rows));
-        p.few_tiles = (rows + 16 * p.rt - 1) / (16 * p.rt);
-        p.few_cut = cut_of(c, r, 0, p.few_tiles, 128);
-        if (window > 0) p.few_cut = cut_of(c, r, window, p.few_tiles, p.few_cut.splits);  // (no window takes more of the workspace than none)
+    p->many = most > limit;
+    p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(limit / group, r->max_new - 1));  // (a sequence alone is the longest)
+    p->few_tiles = 0, p->few_cut = PagedCut{1, kPagedTile}, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
+    const size_t row_bytes = c->head_dim * sizeof(float) + sizeof(float2);
+    if (p->few_new > 0) {
+        const long long rows = p->few_new * group;
+        p->rt = row_tiles_of(static_cast<int>(rows));
+        p->few_tiles = (rows + 16 * p->rt - 1) / (16 * p->rt);
+        p->few_cut = cut_of(c, r, 0, p->few_tiles, 128);
+        if (window > 0) p->few_cut = cut_of(c, r, window, p->few_tiles, p->few_cut.splits);  // (no window takes more of the workspace than none)
+        if (p->few_cut.splits > 1) p->few_bytes = up16(p->few_cut.splits * static_cast<size_t>(r->tokens) * q_heads * row_bytes);
     }
-    if (p.many) {
-        const int block = c->head_dim == 256 ? 128 : 256;
-        p.many_tiles = (most + block - 1) / block;
-        p.many_cut = cut_of_many(c, r, q_heads, 0, p.many_tiles, 32);
-        if (window > 0) p.many_cut = cut_of_many(c, r, q_heads, window, p.many_tiles, p.many_cut.splits);
+    if (p->many) {
+        const int rows = c->head_dim == 256 ? 128 : 256;
+        // (up to four results for every row of a block of threads on every multiprocessor, about 80 MB; no window takes more than none)
+        p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), 0, static_cast<size_t>(4) * c->sm_count * rows, &p->schedule);
+        if (window > 0) p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), window, p->part_rows, &p->schedule);
+        p->many_bytes = up16(p->part_rows * row_bytes);
+        const PagedSchedule& g = p->schedule;
+        const long long blocks = (most + rows - 1) / rows;
+        p->many_blocks = (g.mapped ? g.mapped : g.whole + (blocks - g.whole) * g.cut) * static_cast<long long>(g.m);
     }
-    return p;
 }
-
 }  // namespace
 
 extern "C" int quintrit_b200_paged_cache_create(uint32_t device_index, uint32_t layers, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, int32_t type,
@@ -368,9 +408,6 @@ int check_heads(const quintrit_b200_paged_cache* c, uint32_t q_heads) {
     if (q_heads == 0 || q_heads % c->kv_heads != 0 || q_heads > 65536) return fail(QUINTRIT_ERR_INVALID_SHAPE, "q_heads %u must be a multiple of kv_heads = %u", q_heads, c->kv_heads);
     return QUINTRIT_OK;
 }
-size_t workspace_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, int splits) {
-    return splits > 1 ? static_cast<size_t>(splits) * r->tokens * q_heads * (c->head_dim * sizeof(float) + sizeof(float2)) : 0;
-}
 }  // namespace
 
 extern "C" int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged_cache_t* cache, const quintrit_b200_paged_rows_t* rows, uint32_t q_heads, size_t* out_bytes) {
@@ -381,7 +418,9 @@ extern "C" int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged
         *out_bytes = 0;
         if ((rc = check_rows(cache, rows, false)) != QUINTRIT_OK || (rc = check_heads(cache, q_heads)) != QUINTRIT_OK) return rc;
         if (rows->tokens == 0) return ok();
-        *out_bytes = workspace_of(cache, rows, q_heads, plan_of(cache, rows, q_heads, 0).splits());
+        PagedPlan plan;
+        plan_of(cache, rows, q_heads, 0, &plan);
+        *out_bytes = plan.few_bytes + plan.many_bytes;
         return ok();
     });
 }
@@ -405,11 +444,11 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             (rc = check_array("d_out", args->d_out, args->out_type, {args->out_token_stride, args->out_head_stride})) != QUINTRIT_OK)
             return rc;
         const int group = static_cast<int>(args->q_heads / cache->kv_heads);
-        const PagedPlan plan = plan_of(cache, rows, args->q_heads, args->window);
-        if (std::max(plan.few_tiles, plan.many_tiles) * cache->kv_heads > 65535)
+        PagedPlan plan;
+        plan_of(cache, rows, args->q_heads, args->window, &plan);
+        if (plan.few_tiles * cache->kv_heads > 65535 || plan.many_blocks > 0x7fffffffLL)
             return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
-        const int splits = plan.splits();
-        const size_t need = workspace_of(cache, rows, args->q_heads, splits);
+        const size_t need = plan.few_bytes + plan.many_bytes;
         if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);
         if (need > args->workspace_bytes) return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "the workspace holds %zu bytes, %zu are needed", args->workspace_bytes, need);
         if (need > 0 && reinterpret_cast<uintptr_t>(args->d_workspace) % 16 != 0) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "d_workspace must be 16-byte aligned");
@@ -423,32 +462,39 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         a.scale = args->cap > 0.0f ? args->scale / args->cap : args->scale * kLog2e;
         a.cap = args->cap * kLog2e;
         a.window = static_cast<int>(args->window);
-        a.part_o = static_cast<float*>(args->d_workspace);
-        if (need > 0) a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(splits) * rows->tokens * args->q_heads * cache->head_dim);
         a.most = static_cast<int>(rows->max_new);
         a.spin_limit = kPagedSpin;
-        PagedAttnArgs few = a, many = a;
-        few.few = 1, few.many = plan.few_new, few.splits = std::max(1, plan.few_cut.splits), few.split = plan.few_cut.split;
-        many.few = plan.many ? plan.few_new + 1 : 0x7fffffff, many.many = a.most, many.splits = std::max(1, plan.many_cut.splits), many.split = plan.many_cut.split;
         const int device = cache->device;
+        unsigned char* workspace = static_cast<unsigned char*>(args->d_workspace);
         if (plan.many) {
-            const dim3 grid(static_cast<unsigned>(many.splits), static_cast<unsigned>(cache->kv_heads * plan.many_tiles), rows->sequences);
-            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(many, device, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(many, device, grid, s)
-                                                                                                                          : launch_many_type<kPagedQ8>(many, device, grid, s);
+            a.few = plan.few_new + 1, a.many = a.most;
+            PagedSchedule& g = plan.schedule;
+            g.part_o = reinterpret_cast<float*>(workspace + plan.few_bytes), g.part_ml = reinterpret_cast<float2*>(g.part_o + plan.part_rows * cache->head_dim);
+            const unsigned grid = static_cast<unsigned>(plan.many_blocks);
+            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(a, g, device, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(a, g, device, grid, s)
+                                                                                                                         : launch_many_type<kPagedQ8>(a, g, device, grid, s);
             if (rc != QUINTRIT_OK) return rc;
+            if (plan.part_rows > 0) {
+                const int block = cache->head_dim == 256 ? 128 : 256, blocks = static_cast<int>((static_cast<long long>(rows->max_new) * group + block - 1) / block);
+                auto kernel = a.c.blocks == 1 ? paged_join_kernel<1> : a.c.blocks == 2 ? paged_join_kernel<2> : paged_join_kernel<4>;
+                kernel<<<dim3(block / 8, static_cast<unsigned>(g.m), static_cast<unsigned>(blocks - g.whole)), 256, 0, s>>>(a, g);
+                QTB_LAUNCH_CHECK();
+            }
         }
         if (plan.few_new > 0) {
-            const dim3 grid(static_cast<unsigned>(few.splits), static_cast<unsigned>(cache->kv_heads * plan.few_tiles), rows->sequences);
-            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(few, device, plan.rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(few, device, plan.rt, grid, s)
-                                                                                                                                  : launch_few_type<kPagedQ8>(few, device, plan.rt, grid, s);
+            a.few = 1, a.many = plan.few_new, a.splits = plan.few_cut.splits, a.split = plan.few_cut.split;
+            a.part_o = reinterpret_cast<float*>(workspace);
+            a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(a.splits) * rows->tokens * args->q_heads * cache->head_dim);
+            const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(cache->kv_heads * plan.few_tiles), rows->sequences);
+            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.rt, grid, s)
+                                                                                                                                : launch_few_type<kPagedQ8>(a, device, plan.rt, grid, s);
             if (rc != QUINTRIT_OK) return rc;
-        }
-        if (splits > 1) {
-            const long long items = static_cast<long long>(rows->tokens) * args->q_heads;
-            const unsigned blocks = static_cast<unsigned>((items + 7) / 8);
-            auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
-            kernel<<<blocks, 256, 0, s>>>(few, many);
-            QTB_LAUNCH_CHECK();
+            if (a.splits > 1) {
+                const long long items = static_cast<long long>(rows->tokens) * args->q_heads;
+                auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
+                kernel<<<static_cast<unsigned>((items + 7) / 8), 256, 0, s>>>(a);
+                QTB_LAUNCH_CHECK();
+            }
         }
         return ok();
     });

@@ -486,20 +486,18 @@ __global__ void __launch_bounds__(32 + 128 * RT, 1) paged_few_kernel(const __gri
     }
 }
 
-// Joins the ranges of the sequences that were cut (by the launch for few rows, or the one for many): a warp per (token, query head), in the order of the ranges.
+// Joins the ranges of a sequence: a warp per (token, query head), in the order of the ranges.
 template <int BLOCKS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnArgs few, const __grid_constant__ PagedAttnArgs many) {
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
     using namespace paged_detail;
     constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
-    const int heads = few.c.kv_heads * few.group, lane = threadIdx.x & 31;
+    const int heads = a.c.kv_heads * a.group, lane = threadIdx.x & 31;
     const int item = blockIdx.x * 8 + (threadIdx.x >> 5), t = item / heads, h = item % heads;
-    if (t >= few.r.tokens) return;
-    const int s = paged_sequence_of(few.r, t);
+    if (t >= a.r.tokens) return;
+    const int s = paged_sequence_of(a.r, t);
     if (s < 0) return;
-    const PagedSequence sq = paged_sequence(few.c, few.r, s);
-    if (!sq.ok || t < sq.first || t >= sq.first + sq.news || sq.news > few.most) return;
-    const PagedAttnArgs& a = sq.news >= many.few ? many : few;  // the launch that served it
-    if (a.splits == 1) return;
+    const PagedSequence sq = paged_sequence(a.c, a.r, s);
+    if (!sq.ok || t < sq.first || t >= sq.first + sq.news || sq.news < a.few || sq.news > a.many) return;
     const int used = paged_splits_used(a, sq);
     const size_t step = static_cast<size_t>(a.r.tokens) * heads, row = static_cast<size_t>(t) * heads + h;
     float top = -INFINITY;

@@ -3,9 +3,10 @@
 // A block of threads takes one KV head of one sequence, 256 rows of queries (128 where a head has 256 values; a row is a (token, head of the group)) and a
 // range of positions, in tiles of 128 positions (64). Units of work alternate between two score buffers in tensor memory: the two row tiles of a tile of positions,
 // or the one row tile of successive tiles. For a unit one thread issues S = Q K^T (tcgen05.mma, operands in shared memory; Q of 256 values in tensor memory), a warpgroup
-// with a row per thread turns S into weights (maximum, exponentials, sum: no exchange between threads) and writes them as 16-bit values over S, and O += P V takes them from
+// with a row per thread (two warpgroups where there is one row tile: two threads per row, half of the positions each, which speak to each other when a maximum grew) turns S into
+// weights (maximum, exponentials, sum) and writes them as 16-bit values over S, and O += P V takes them from
 // there. The tensor cores work on the other buffer meanwhile: score products of unit u + 2 follow the value products of unit u. O stays in tensor memory and is rescaled, by its
-// warpgroup, only when a row's maximum grew by more than 2^8.
+// warpgroups, only when a row's maximum grew by more than 2^8.
 //
 // F16 / BF16: one warp brings the pages' rows by bulk copies straight into the operands' places, since they lie in the cache in the 128-byte swizzle already (keys as a K-major,
 // values as an MN-major operand). Q8: it brings codes and scales to a ring of their own, and four warps widen the codes to F16 operands and prepare the scales.
@@ -17,6 +18,37 @@
 #include "paged_attention.cuh"
 
 namespace qtb {
+
+// Which rows and ranges the blocks of a launch take. Row blocks count from the last one of a sequence, which sees most (order 0, 1, ...); m = KV heads x sequences of each. One block of threads
+// per multiprocessor, so that what matters is the last of them to end: as long as row blocks fill whole waves they are taken whole; the rest, or all where there are too few,
+// are cut into ranges of equal length, whose results meet in the workspace.
+constexpr int kPagedMapped = 160;  // most (row block, range) pairs of a mapped schedule
+struct PagedSchedule {
+    int m, whole, cut;                       // blocks x m: order x < whole, all of its range; else order whole + (x - whole) / cut, range (x - whole) % cut of cut
+    int mapped;                              // few row blocks, of different lengths: order[x], range[x] of ranges[x] instead
+    unsigned char order[kPagedMapped], range[kPagedMapped], ranges[kPagedMapped];
+    float* part_o;                           // [x - whole][m][rows of a block][head_dim] for what is cut; mapped: [range][KV head][packed tokens x group][head_dim]
+    float2* part_ml;
+};
+struct PagedPart {
+    int order, range, ranges, slot;  // slot: of the workspace
+};
+__device__ __forceinline__ PagedPart paged_part(const PagedSchedule& g, int x) {
+    if (g.mapped) return PagedPart{g.order[x], g.range[x], g.ranges[x], x};
+    if (x < g.whole) return PagedPart{x, 0, 1, 0};
+    return PagedPart{g.whole + (x - g.whole) / g.cut, (x - g.whole) % g.cut, g.cut, x - g.whole};
+}
+// The row of the workspace that has the result of row r (`local` of its block) for a part.
+__device__ __forceinline__ size_t paged_part_row(const PagedAttnArgs& a, const PagedSchedule& g, const PagedSequence& q, const PagedPart& part, int which, int kvh, int r, int local, int rows) {
+    if (g.mapped) return (static_cast<size_t>(part.range) * a.c.kv_heads + kvh) * (static_cast<size_t>(a.r.tokens) * a.group) + static_cast<size_t>(q.first) * a.group + r;
+    return (static_cast<size_t>(part.slot) * g.m + which) * rows + local;
+}
+// Range `part` of `parts` of what rows of tokens [t0, t1) see; begin is a multiple of 64.
+__device__ __forceinline__ PagedRange paged_part_range(const PagedAttnArgs& a, const PagedSequence& q, int t0, int t1, int part, int parts, int tile) {
+    const int p0 = q.length - q.news, low = a.window > 0 ? max(0, p0 + t0 - a.window + 1) & ~(kPagedTile - 1) : 0, high = max(low, max(0, p0 + t1));
+    const int tiles = (high - low + tile - 1) / tile, per = (tiles + parts - 1) / parts;
+    return PagedRange{min(high, low + part * per * tile), min(high, low + (part + 1) * per * tile)};
+}
 
 template <int TYPE, int BLOCKS>
 struct PagedMany {
@@ -30,13 +62,15 @@ struct PagedMany {
     static constexpr int kFactors = Q8 ? 4 : 0;                                // sets of KT x (key scale, log2 of the value scale, its reciprocal)
     static constexpr bool kQTmem = BLOCKS == 4;
     static constexpr int kQBytes = kQTmem ? 0 : NT * 128 * HD * 2;
-    static constexpr int kSoftWarps = 4 * NT, kLoadWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
+    static constexpr int SIDES = BLOCKS == 4 ? 2 : 1;                          // threads of a row
+    static constexpr int kSoftWarps = 4 * NT * SIDES, kLoadWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
     static constexpr int kThreads = (kSoftWarps + 4 + (Q8 ? 4 : 0)) * 32;
-    // registers per thread where the warpgroups with the scores need more than their share: launched with 168 (384 threads) or 128 (512 threads)
+    // registers: 384 threads are launched with 168 each, 512 with 128; the warpgroups with the scores of two row tiles take some of the others'
     static constexpr bool kSplitRegs = NT == 2;
-    static constexpr int kSoftRegs = Q8 ? 200 : 216, kRestRegs = Q8 ? 56 : 72;
+    static constexpr int kLaunchRegs = Q8 ? 128 : 168, kSoftRegs = Q8 ? 200 : 216, kRestRegs = Q8 ? 56 : 72;
+    static_assert(!kSplitRegs || kSoftWarps * 32 * kSoftRegs + (kThreads - kSoftWarps * 32) * kRestRegs <= kThreads * kLaunchRegs, "more registers than the block was launched with");
     static constexpr int kBars = 2 * kSlots + 2 * kRaws + 2 * 3 + 2;
-    static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + kBars * 8 + 16;
+    static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + (SIDES == 2 ? 2048 : 0) + kBars * 8 + 16;
     static constexpr int kSmem = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one block per multiprocessor: it takes all of its tensor memory
     static constexpr int kOCol = 0, kSCol = 256, kQCol = 384;  // tensor memory columns: O (of row tile i at 128 i), S (buffer b at KT b behind), Q
 };
@@ -51,6 +85,11 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
           "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
           "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -81,19 +120,20 @@ template <int N> __device__ __forceinline__ void registers_down() { asm volatile
 }  // namespace paged_detail
 
 template <int TYPE, int BLOCKS>
-__global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
     using namespace gemm_detail;
     using namespace paged_detail;
     using M = PagedMany<TYPE, BLOCKS>;
     constexpr bool Q8 = M::Q8;
-    constexpr int HD = M::HD, NT = M::NT, KT = M::KT, RS = M::kSlots, RW = Q8 ? M::kRaws : 1, kRow = paged_row_bytes(TYPE);
+    constexpr int HD = M::HD, NT = M::NT, SIDES = M::SIDES, KT = M::KT, RS = M::kSlots, RW = Q8 ? M::kRaws : 1, kRow = paged_row_bytes(TYPE);
     extern __shared__ unsigned char many_smem_raw[];
     const uint32_t base = (smem_u32(many_smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = many_smem_raw + (base - smem_u32(many_smem_raw));
     const uint32_t q_at = base, slots = base + M::kQBytes, raws = slots + RS * M::kSlot;
     unsigned char* raw_smem = smem + M::kQBytes + RS * M::kSlot;
     float* factors = reinterpret_cast<float*>(raw_smem + M::kRaws * M::kRawStride);  // [kFactors][3][KT]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(factors + M::kFactors * 3 * KT);
+    float2* exchange = reinterpret_cast<float2*>(factors + M::kFactors * 3 * KT);  // [2][128]: between the two threads of a row
+    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + (SIDES == 2 ? 256 : 0));
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };                       // an operand tile is there
     auto empty = [&](int s) { return bar0 + 8u * (RS + s); };               // the products that read it are done
@@ -108,22 +148,22 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    const int seq = blockIdx.z, kvh = blockIdx.y % a.c.kv_heads, block = static_cast<int>(gridDim.y) / a.c.kv_heads - 1 - static_cast<int>(blockIdx.y) / a.c.kv_heads;  // the last rows, which see most, first
+    const PagedPart part = paged_part(g, static_cast<int>(blockIdx.x) / g.m);
+    const int which = static_cast<int>(blockIdx.x) % g.m, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
     const PagedSequence sq = paged_sequence(a.c, a.r, seq);
     if (!sq.ok || sq.news < a.few || sq.news > a.many) {
         if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
         return;
     }
-    const int rows = sq.news * a.group, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);
-    if (r0 >= rows) return;
-    if (static_cast<int>(blockIdx.x) >= paged_splits_used(a, sq)) return;
-    const PagedRange range = paged_range(a, sq, r0 / a.group, (r1 - 1) / a.group + 1, blockIdx.x);
+    const int rows = sq.news * a.group, block = (rows + M::kRows - 1) / M::kRows - 1 - part.order, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);
+    if (block < 0) return;
+    const PagedRange range = paged_part_range(a, sq, r0 / a.group, (r1 - 1) / a.group + 1, part.range, part.ranges, KT);
     const int p0 = sq.length - sq.news, tiles = range.end > range.begin ? (range.end - range.begin + KT - 1) / KT : 0, units = tiles * NT;
 
     if (tid == 0) {
         for (int s = 0; s < RS; ++s) mbar_init(full(s), Q8 ? 4 : 1), mbar_init(empty(s), 1);
         for (int s = 0; s < M::kRaws; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4);
-        for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4), mbar_init(o_done(b), 1);
+        for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4 * SIDES), mbar_init(o_done(b), 1);
         mbar_init(q_full, M::kSoftWarps);
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -269,11 +309,23 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
         }
     } else {
         if constexpr (M::kSplitRegs) registers_up<M::kSoftRegs>();
-        // ---- a row of queries per thread ----
-        const int i = warp >> 2, local = (warp & 3) * 32 + lane, r = r0 + i * 128 + local, t = r / a.group, h = kvh * a.group + r % a.group;
+        // ---- a row of queries for a thread, or for two, which have half of a tile's positions each: warps w and w + 4 ----
+        const int i = SIDES == 2 ? 0 : warp >> 2, side = SIDES == 2 ? warp >> 2 : 0, local = (warp & 3) * 32 + lane, r = r0 + i * 128 + local, t = r / a.group, h = kvh * a.group + r % a.group;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const bool live = r < r1;
-        float rowf;  // what the row's scores are multiplied by: never negative, the queries take the sign
+        constexpr int KH = KT / SIDES, HH = HD / SIDES;
+        // the two warps meet at a barrier of their own; both come to it the same number of times whatever happens, as all other waits end by themselves
+        const int meet = 1 + (warp & 3);
+        volatile float2* mine = exchange + side * 128 + local;
+        volatile float2* theirs = exchange + (side ^ 1) * 128 + local;
+        auto meet_sync = [&]() { asm volatile("barrier.cta.sync %0, 64;" ::"r"(meet) : "memory"); };
+        auto meet_any = [&](bool x) {
+            if constexpr (SIDES == 1) return __any_sync(0xffffffffu, x) != 0;
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(x ? 1u : 0u), "r"(meet) : "memory");
+            return any != 0;
+        };
+        float rowf;  // what the row's scores are multiplied by: positive, the queries take the sign
         {
             const unsigned char* src = static_cast<const unsigned char*>(a.q) + ((static_cast<size_t>(sq.first) + (live ? t : 0)) * a.q_token + (live ? h : kvh * a.group) * a.q_head) * paged_size_of(a.q_type);
             float f = a.scale < 0.0f ? -1.0f : 1.0f;
@@ -290,22 +342,22 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                 const uint32_t ex = __float_as_uint(m) >> 23;
                 if (ex > 1 && ex < 254) rowf *= __uint_as_float(ex << 23), f *= __uint_as_float((254 - ex) << 23);
             }
-#pragma unroll 2
-            for (int e = 0; e < HD; e += 64) {
-                uint32_t v[32];
+#pragma unroll 1
+            for (int e = side * HH; e < (side + 1) * HH; e += 32) {
+                uint32_t v[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < 4; ++k) {
                     float x[8];
                     paged_load8(src + (e + k * 8) * paged_size_of(a.q_type), a.q_type, x);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) v[k * 4 + c] = live ? paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x[2 * c] * f, x[2 * c + 1] * f) : 0u;
                 }
                 if constexpr (M::kQTmem) {
-                    tmem_store32(tmem + lanes + M::kQCol + e / 2, v);
+                    tmem_store16(tmem + lanes + M::kQCol + e / 2, v);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        *reinterpret_cast<uint4*>(smem + ((i * BLOCKS + e / 64) * 128 + local) * 128 + ((k ^ (local & 7)) << 4)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint4*>(smem + ((i * BLOCKS + e / 64) * 128 + local) * 128 + ((((e & 32) / 8 + k) ^ (local & 7)) << 4)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 }
             }
             if constexpr (M::kQTmem) tmem_wait_store();
@@ -315,24 +367,24 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             if (lane == 0) mbar_arrive(q_full);
         }
         const int p = p0 + t, last = live ? min(p, range.end - 1) : -1, first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f;  // l: over this thread's positions
         bool okay = true;
         // The value products of unit u. A wait tells phases apart by their parity alone, so each buffer has a barrier: those of unit u - 2, the phase before, are done, as the scores
         // of unit u (asked for behind them) were waited for, and those of unit u + 2 cannot have begun.
-        auto values_done = [&](int u) { return mbar_wait(o_done(u & 1), (u >> 1) & 1, abort_flag, a.spin_limit); };
+        auto values_done = [&](int u) { return __all_sync(0xffffffffu, mbar_wait(o_done(u & 1), (u >> 1) & 1, abort_flag, a.spin_limit)); };
+#pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
-            const int u = j * NT + i, b = u & 1, k0 = range.begin + j * KT;
+            const int u = j * NT + i, b = u & 1, k0 = range.begin + j * KT + side * KH;
             const uint32_t s_at = tmem + lanes + M::kSCol + b * KT;
-            okay = __all_sync(0xffffffffu, mbar_wait(s_full(b), (u >> 1) & 1, abort_flag, a.spin_limit));
-            if (!okay) break;
+            if (okay) okay = __all_sync(0xffffffffu, mbar_wait(s_full(b), (u >> 1) & 1, abort_flag, a.spin_limit));
             fence_after();
-            uint32_t s[KT / 32][32];
+            uint32_t s[KH / 32][32];
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c) tmem_load32(s_at + c * 32, s[c]);
+            for (int c = 0; c < KH / 32; ++c) tmem_load32(s_at + side * KH + c * 32, s[c]);
             tmem_wait_load();
             // v in s, so that a weight is 2^(v mul - m): the products themselves, where only the scale is to come; else the whole exponent
             float mul = 1.0f;
-            const float4* f = reinterpret_cast<const float4*>(factors + (j & 3) * 3 * KT);
+            const float4* f = reinterpret_cast<const float4*>(factors + (j & 3) * 3 * KT + side * KH);
             auto pair = [&](int c, int e) { return pack_f32x2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])); };
             auto put = [&](int c, int e, unsigned long long v) {
                 const float2 x = unpack_f32x2(v);
@@ -341,7 +393,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             const unsigned long long row2 = pack_f32x2(rowf, rowf);
             if (a.cap > 0.0f) {
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
+                for (int c = 0; c < KH / 32; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
                         float x = __uint_as_float(s[c][e]);
@@ -352,7 +404,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     }
             } else if constexpr (Q8) {
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
+                for (int c = 0; c < KH / 32; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 ks = f[(c * 32 + e) / 4], lv = f[(KT + c * 32 + e) / 4];
@@ -362,29 +414,38 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             } else {
                 mul = rowf;
             }
-            if (__any_sync(0xffffffffu, k0 + KT - 1 > last || k0 < first)) {
+            if (__any_sync(0xffffffffu, k0 + KH - 1 > last || k0 < first)) {
                 const int lo = first - k0, hi = last - k0;
 #pragma unroll
-                for (int c = 0; c < KT / 32; ++c)
+                for (int c = 0; c < KH / 32; ++c)
 #pragma unroll
                     for (int e = 0; e < 32; ++e) s[c][e] = c * 32 + e >= lo && c * 32 + e <= hi ? s[c][e] : 0xff800000u;  // minus infinity
             }
             float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four at a time: a chain of maxima or sums takes four cycles a link
 #pragma unroll
-            for (int c = 0; c < KT / 32; ++c)
+            for (int c = 0; c < KH / 32; ++c)
 #pragma unroll
                 for (int e = 0; e < 32; ++e) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(s[c][e]));
-            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
-            const bool grew = top > m + kPagedLazy || (m == -INFINITY && top > -INFINITY);
-            if (__any_sync(0xffffffffu, grew)) {
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mul;
+            // (also: both have read their scores, so that the weights may be written over them)
+            if (meet_any(!okay || top > m + kPagedLazy || (m == -INFINITY && top > -INFINITY))) {
+                if constexpr (SIDES == 2) {
+                    mine->x = top, mine->y = okay ? 0.0f : 1.0f;
+                    meet_sync();
+                    const float other = theirs->x, theirs_okay = theirs->y;
+                    meet_sync();  // before either writes the next one
+                    okay = __all_sync(0xffffffffu, okay && theirs_okay == 0.0f);  // the same in both warps: a warp is of one mind, and hears of the other's
+                    top = fmaxf(top, other);
+                }
+                if (!okay) break;
+                const bool grew = top > m + kPagedLazy || (m == -INFINITY && top > -INFINITY);
                 const float keep = grew ? ex2(m - top) : 1.0f;  // 0 the first time
                 if (grew) m = top, l *= keep;
-                if (j > 0) {
-                    okay = __all_sync(0xffffffffu, values_done(u - NT));
-                    if (!okay) break;
+                if (j > 0 && __any_sync(0xffffffffu, grew)) {
+                    okay = values_done(u - NT);
                     fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
+                    for (int c = side * HH; c < (side + 1) * HH; c += 32) {
                         uint32_t o[32];
                         tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
                         tmem_wait_load();
@@ -398,15 +459,15 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             const unsigned long long mul2 = pack_f32x2(mul, mul), ref2 = pack_f32x2(ref, ref);
             unsigned long long sums[2] = {0ull, 0ull};
 #pragma unroll
-            for (int c = 0; c < KT / 64; ++c) {
-                uint32_t w[32];
+            for (int c = 0; c < KH / 32; ++c) {
+                uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const int k = 2 * e, cc = c * 2 + k / 32;
-                    float2 x = unpack_f32x2(fma_f32x2(pair(cc, k % 32), mul2, ref2)), y = unpack_f32x2(fma_f32x2(pair(cc, k % 32 + 2), mul2, ref2));
+                for (int e = 0; e < 16; e += 2) {
+                    const int k = 2 * e;
+                    float2 x = unpack_f32x2(fma_f32x2(pair(c, k), mul2, ref2)), y = unpack_f32x2(fma_f32x2(pair(c, k + 2), mul2, ref2));
                     x.x = ex2(x.x), x.y = ex2(x.y), y.x = ex2(y.x), y.y = ex2(y.y);
                     if constexpr (Q8) {
-                        const float4 iv = f[(2 * KT + c * 64 + k) / 4];
+                        const float4 iv = f[(2 * KT + c * 32 + k) / 4];
                         sums[0] = fma_f32x2(pack_f32x2(x.x, x.y), pack_f32x2(iv.x, iv.y), sums[0]);
                         sums[1] = fma_f32x2(pack_f32x2(y.x, y.y), pack_f32x2(iv.z, iv.w), sums[1]);
                     } else {
@@ -414,26 +475,31 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     }
                     w[e] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x.x, x.y), w[e + 1] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, y.x, y.y);
                 }
-                tmem_store32(s_at + c * 32, w);
+                tmem_store16(s_at + side * (KH / 2) + c * 16, w);
             }
             const float2 sum = unpack_f32x2(add_f32x2(sums[0], sums[1]));
             l += sum.x + sum.y;
             tmem_wait_store();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(b));
+            if (lane == 0 && okay) mbar_arrive(p_full(b));
         }
-        if (okay && tiles > 0) okay = __all_sync(0xffffffffu, values_done((tiles - 1) * NT + i));
+        if (okay && tiles > 0) okay = values_done((tiles - 1) * NT + i);
         okay = __all_sync(0xffffffffu, okay && *abort_flag == 0);
+        if constexpr (SIDES == 2) {
+            mine->x = l, mine->y = okay ? 0.0f : 1.0f;
+            meet_sync();
+            okay = __all_sync(0xffffffffu, okay && theirs->y == 0.0f);
+            l += theirs->x;
+        }
         if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
         if (okay) {
             fence_after();
             const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-            const int heads = a.c.kv_heads * a.group;
-            const size_t token = static_cast<size_t>(sq.first) + t, row = (static_cast<size_t>(blockIdx.x) * a.r.tokens + token) * heads + h;
+            const size_t token = static_cast<size_t>(sq.first) + t, row = paged_part_row(a, g, sq, part, which, kvh, r, i * 128 + local, M::kRows);
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                if (tiles == 0 && a.splits > 1) break;
+            for (int c = side * HH; c < (side + 1) * HH; c += 32) {
+                if (tiles == 0 && part.ranges > 1) break;
                 uint32_t o[32];
                 if (tiles > 0) {
                     tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
@@ -448,16 +514,16 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     float x[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(o[e + k]);
-                    if (a.splits == 1) {
+                    if (part.ranges == 1) {
 #pragma unroll
                         for (int k = 0; k < 8; ++k) x[k] *= inv;
                         paged_store8(static_cast<unsigned char*>(a.out) + (token * a.o_token + h * a.o_head + c + e) * paged_size_of(a.out_type), a.out_type, x);
                     } else {
-                        paged_store8(a.part_o + row * HD + c + e, kPagedF32, x);
+                        paged_store8(g.part_o + row * HD + c + e, kPagedF32, x);
                     }
                 }
             }
-            if (live && a.splits > 1) a.part_ml[row] = make_float2(m, l);  // (of a range in which the row sees nothing this is all that is read)
+            if (live && part.ranges > 1 && side == 0) g.part_ml[row] = make_float2(m, l);  // (of a range in which the row sees nothing this is all that is read)
         }
     }
     fence_before();
@@ -465,6 +531,52 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     if (warp == M::kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Joins the ranges of the row blocks that were cut: a warp per row, in the order of the ranges. Grid (rows / 8, m, row blocks that were cut, mapped: all of them).
+template <int BLOCKS>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
+    using namespace paged_detail;
+    constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32, kRows = BLOCKS == 4 ? 128 : 256;
+    const int lane = threadIdx.x & 31, local = blockIdx.x * 8 + (threadIdx.x >> 5), which = blockIdx.y, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
+    int x = 0, order = blockIdx.z, ranges = g.cut;
+    if (g.mapped) {
+        while (g.order[x] != order) ++x;
+        ranges = g.ranges[x];
+    } else {
+        x = order * g.cut, order += g.whole;
+    }
+    if (ranges == 1) return;
+    const PagedSequence sq = paged_sequence(a.c, a.r, seq);
+    if (!sq.ok || sq.news < a.few || sq.news > a.many) return;
+    const int rows = sq.news * a.group, block = (rows + kRows - 1) / kRows - 1 - order, r = block * kRows + local;
+    if (block < 0 || r >= rows) return;
+    const size_t row = paged_part_row(a, g, sq, PagedPart{order, 0, ranges, x}, which, kvh, r, local, kRows), step = paged_part_row(a, g, sq, PagedPart{order, 1, ranges, x + 1}, which, kvh, r, local, kRows) - row;
+    float top = -INFINITY;
+    for (int i = lane; i < ranges; i += 32) top = fmaxf(top, g.part_ml[i * step + row].x);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f, v[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = 0.0f;
+    for (int i = 0; i < ranges; ++i) {
+        const float2 ml = g.part_ml[i * step + row];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing visible there
+        const float w = ex2(ml.x - top);
+        sum = fmaf(w, ml.y, sum);
+        const float* from = g.part_o + (i * step + row) * HD + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[e] = fmaf(w, from[e], v[e]);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    const size_t token = static_cast<size_t>(sq.first) + r / a.group;
+    unsigned char* out = static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + r % a.group) * a.o_head + lane * kPer) * paged_size_of(a.out_type);
+    if (a.out_type == kPagedF32) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) reinterpret_cast<float*>(out)[e] = v[e] * inv;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = paged_pack2(a.out_type, v[e] * inv, v[e + 1] * inv);
     }
 }
 
