@@ -98,16 +98,23 @@ int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void
     return QUINTRIT_OK;
 }
 
-// How the positions are cut into ranges: enough blocks of threads to fill the device, ranges of at least four tiles.
+// How the kernel for few rows cuts the positions into ranges: blocks of threads come in waves of `places`, each as long as its tiles and a start and an end of about five more; ranges cost another
+// launch. (Sequences are taken to be as long as announced: shorter ones leave blocks without work, which end at once.)
 struct PagedCut {
     int splits, split;
 };
-PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles, int limit) {
+PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles, int places, int limit) {
+    constexpr double kStart = 5.0, kJoin = 4.0;
     long long span = std::max<uint32_t>(r->max_length, 1);
     if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
     const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_tiles;
-    const long long want = std::max<long long>(1, std::min<long long>({(4LL * c->sm_count + items - 1) / items, (tiles + 3) / 4, limit}));
-    const long long per = (tiles + want - 1) / want;
+    long long best = 1;
+    double least = 1e30;
+    for (long long s = 1; s <= limit && s <= std::max<long long>(1, tiles / 2); ++s) {
+        const double cost = static_cast<double>((items * s + places - 1) / places) * (static_cast<double>((tiles + s - 1) / s) + kStart) + (s > 1 ? kJoin : 0.0);
+        if (cost < least * 0.98) best = s, least = cost;
+    }
+    const long long per = (tiles + best - 1) / best;
     return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile)};
 }
 
@@ -121,25 +128,40 @@ int allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t>& done
     return QUINTRIT_OK;
 }
 
-template <int TYPE, int BLOCKS, int RT>
+template <int TYPE, int BLOCKS, int NT>
 int launch_few(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
-    constexpr int smem = paged_few_smem<TYPE, BLOCKS, RT>();
-    static_assert(smem <= 227 * 1024, "the ring does not fit");
+    using F = PagedFew<TYPE, BLOCKS, NT>;
+    static_assert(F::kSmem <= 227 * 1024, "the ring does not fit");
     static std::atomic<uint64_t> done{0};
-    const int rc = allow_smem(paged_few_kernel<TYPE, BLOCKS, RT>, smem, device, done);
+    const int rc = allow_smem(paged_few_kernel<TYPE, BLOCKS, NT>, F::kSmem, device, done);
     if (rc != QUINTRIT_OK) return rc;
-    paged_few_kernel<TYPE, BLOCKS, RT><<<grid, 32 + 128 * RT, smem, s>>>(a);
+    paged_few_kernel<TYPE, BLOCKS, NT><<<grid, F::kThreads, F::kSmem, s>>>(a);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
 template <int TYPE, int BLOCKS>
-int launch_few_rows(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
-    return rt == 1 ? launch_few<TYPE, BLOCKS, 1>(a, device, grid, s) : launch_few<TYPE, BLOCKS, 2>(a, device, grid, s);
+int launch_few_rows(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
+    if (nt == 1) return launch_few<TYPE, BLOCKS, 1>(a, device, grid, s);
+    if constexpr (BLOCKS < 4)
+        if (nt > 2) return launch_few<TYPE, BLOCKS, BLOCKS == 1 ? 4 : 3>(a, device, grid, s);
+    return launch_few<TYPE, BLOCKS, 2>(a, device, grid, s);
 }
 template <int TYPE>
-int launch_few_type(const PagedAttnArgs& a, int device, int rt, dim3 grid, cudaStream_t s) {
-    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, rt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, rt, grid, s) : launch_few_rows<TYPE, 4>(a, device, rt, grid, s);
+int launch_few_type(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
+    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, nt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, nt, grid, s) : launch_few_rows<TYPE, 4>(a, device, nt, grid, s);
 }
+// Tiles of 8 rows of a block of threads: as many as its registers hold the sums of; and such blocks on all multiprocessors.
+int row_tiles_of(const quintrit_b200_paged_cache* c, long long rows) { return rows <= 8 ? 1 : rows <= 16 || c->head_dim == 256 ? 2 : c->head_dim == 128 ? 3 : 4; }
+template <int TYPE>
+int blocks_per_sm(int head_dim, int nt) {
+    return head_dim == 64 ? (nt == 1 ? PagedFew<TYPE, 1, 1>::kBlocksPerSm : nt == 2 ? PagedFew<TYPE, 1, 2>::kBlocksPerSm : PagedFew<TYPE, 1, 4>::kBlocksPerSm)
+         : head_dim == 128 ? (nt == 1 ? PagedFew<TYPE, 2, 1>::kBlocksPerSm : nt == 2 ? PagedFew<TYPE, 2, 2>::kBlocksPerSm : PagedFew<TYPE, 2, 3>::kBlocksPerSm)
+                           : (nt == 1 ? PagedFew<TYPE, 4, 1>::kBlocksPerSm : PagedFew<TYPE, 4, 2>::kBlocksPerSm);
+}
+int places_of(const quintrit_b200_paged_cache* c, int nt) {
+    return c->sm_count * (c->type == kPagedQ8 ? blocks_per_sm<kPagedQ8>(static_cast<int>(c->head_dim), nt) : blocks_per_sm<kPagedF16>(static_cast<int>(c->head_dim), nt));
+}
+
 // The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles and a start and an end of
 // about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. Where the sequences' chunks differ, as in a step that carries one
 // prompt, fewer row blocks are there than the longest chunk times the sequences: their number is taken from the tokens.
@@ -204,13 +226,11 @@ template <int TYPE>
 int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
     return a.c.blocks == 1 ? launch_many_of<TYPE, 1>(a, g, device, grid, s) : a.c.blocks == 2 ? launch_many_of<TYPE, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 4>(a, g, device, grid, s);
 }
-int row_tiles_of(int rows) { return rows <= 16 ? 1 : 2; }  // row tiles of a block of threads
-
 // How a call is served: sequences of up to `few_new` new tokens by the kernel for few rows, the others by the one for many; either may have nothing to do.
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
     bool many;
-    int rt;                  // few: row tiles of a block, blocks per head, ranges
+    int nt;                  // few: tiles of 8 rows of a block, blocks per head, ranges
     long long few_tiles;
     PagedCut few_cut;
     PagedSchedule schedule;  // many: which blocks, their number, slots of the workspace
@@ -227,10 +247,11 @@ void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_
     const size_t row_bytes = c->head_dim * sizeof(float) + sizeof(float2);
     if (p->few_new > 0) {
         const long long rows = p->few_new * group;
-        p->rt = row_tiles_of(static_cast<int>(rows));
-        p->few_tiles = (rows + 16 * p->rt - 1) / (16 * p->rt);
-        p->few_cut = cut_of(c, r, 0, p->few_tiles, 128);
-        if (window > 0) p->few_cut = cut_of(c, r, window, p->few_tiles, p->few_cut.splits);  // (no window takes more of the workspace than none)
+        p->nt = row_tiles_of(c, rows);
+        p->few_tiles = (rows + 8 * p->nt - 1) / (8 * p->nt);
+        const int places = places_of(c, p->nt);
+        p->few_cut = cut_of(c, r, 0, p->few_tiles, places, 128);
+        if (window > 0) p->few_cut = cut_of(c, r, window, p->few_tiles, places, p->few_cut.splits);  // (no window takes more of the workspace than none)
         if (p->few_cut.splits > 1) p->few_bytes = up16(p->few_cut.splits * static_cast<size_t>(r->tokens) * q_heads * row_bytes);
     }
     if (p->many) {
@@ -486,13 +507,15 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             a.part_o = reinterpret_cast<float*>(workspace);
             a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(a.splits) * rows->tokens * args->q_heads * cache->head_dim);
             const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(cache->kv_heads * plan.few_tiles), rows->sequences);
-            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.rt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.rt, grid, s)
-                                                                                                                                : launch_few_type<kPagedQ8>(a, device, plan.rt, grid, s);
+            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.nt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.nt, grid, s)
+                                                                                                                                : launch_few_type<kPagedQ8>(a, device, plan.nt, grid, s);
             if (rc != QUINTRIT_OK) return rc;
             if (a.splits > 1) {
-                const long long items = static_cast<long long>(rows->tokens) * args->q_heads;
-                auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
-                kernel<<<static_cast<unsigned>((items + 7) / 8), 256, 0, s>>>(a);
+                const unsigned items = static_cast<unsigned>(rows->tokens) * args->q_heads;  // (below 2^31: a workspace of that many results was asked for)
+                const bool wide = a.splits > 8;
+                auto kernel = a.c.blocks == 1 ? (wide ? paged_combine_kernel<1, 8> : paged_combine_kernel<1, 1>) : a.c.blocks == 2 ? (wide ? paged_combine_kernel<2, 8> : paged_combine_kernel<2, 1>)
+                                                                                                                                 : (wide ? paged_combine_kernel<4, 8> : paged_combine_kernel<4, 1>);
+                kernel<<<items, wide ? 256 : 32, 0, s>>>(a);
                 QTB_LAUNCH_CHECK();
             }
         }

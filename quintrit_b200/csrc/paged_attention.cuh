@@ -10,10 +10,12 @@
 // So the weights that are rounded to F16 lie in [0, 256] whatever the scales are. Queries are scaled by a power of two per row to a maximum in [1, 2),
 // which is exact, so BF16 and F32 queries of any size meet F16 codes.
 //
-// Bound by the rows' bytes: 2 G flops per byte of a 16-bit cache. A block of threads takes one KV head of one sequence and a range of its positions; one
-// warp brings the pages, tile by tile of 64 positions, into a ring in shared memory with bulk copies; every other warp has 16 positions of the tiles and
-// 16 rows of queries (rows are (token, head of the group)), its own m, l and sums, all in registers of matrix instructions (m16n8k16); at the end
-// the warps of a row tile join. Long sequences are cut into ranges for several blocks, whose results meet in the caller's workspace
+// Bound by the rows' bytes: 2 G flops per byte of a 16-bit cache. A block of threads takes one KV head of one sequence, up to 32 rows of queries (24 or 16 where a head has 128 or 256 values; a row
+// is a (token, head of the group)) and a range of its positions; one warp brings the pages, tile by tile of 64 positions, into a ring in shared memory with bulk copies;
+// two groups of four warps take the tiles in turn, a warp 16 positions of a tile against all rows. Matrix instructions (m16n8k16) with the positions, and then the values, as the
+// 16 rows of the left operand and the queries as the 8 columns of the right one: S^T = K Q^T and O^T += V^T P^T, so that one query head or eight cost the same, a fragment of codes is
+// widened once for all rows, and the sums of eight rows take head_dim / 4 registers. A score's row is the same in both products' registers; only the weights are transposed (movmatrix).
+// Every warp has its own m, l and sums; at the end the eight warps join. Long sequences are cut into ranges for several blocks, whose results meet in the caller's workspace
 // (paged_combine_kernel), in the order of the ranges: no atomics.
 #pragma once
 #include "paged_cache.cuh"
@@ -119,22 +121,29 @@ __device__ __forceinline__ int paged_splits_used(const PagedAttnArgs& a, const P
     return max(1, min(a.splits, static_cast<int>((static_cast<long long>(q.length) - low_all + a.split - 1) / a.split)));
 }
 
-template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_q_pitch() { return BLOCKS * kPagedBlock * 2 + (TYPE == kPagedQ8 ? 32 : 16); }  // bytes: eight rows fall into different banks
 template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_rows_bytes() { return kPagedTile * BLOCKS * paged_row_bytes(TYPE); }  // keys or values of a tile
-template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_stage_bytes() { return 2 * paged_rows_bytes<TYPE, BLOCKS>() + (TYPE == kPagedQ8 ? 2 * kPagedTile * 4 : 0); }
-template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_stages() { return paged_stage_bytes<TYPE, BLOCKS>() > 40000 ? 3 : paged_stage_bytes<TYPE, BLOCKS>() > 20000 ? 3 : 4; }
-template <int TYPE, int BLOCKS, int RT> __host__ __device__ constexpr int paged_few_smem() {
-    const int ring = paged_stages<TYPE, BLOCKS>() * paged_stage_bytes<TYPE, BLOCKS>(), join = RT * 4 * 16 * (BLOCKS * kPagedBlock * 4 + 16);
-    return 1024 + (ring > join ? ring : join) + RT * 16 * paged_q_pitch<TYPE, BLOCKS>() + RT * 16 * 4 + 256;
-}
+template <int TYPE, int BLOCKS, int NT>  // NT: tiles of 8 rows
+struct PagedFew {
+    static constexpr int HD = BLOCKS * kPagedBlock, kRows = NT * 8, kThreads = 32 * 9;
+    // A unit holds the keys of a tile (Q8: and the scales of keys and values) or the values. Each group has a ring of its own, so that its waits see every phase of its barriers: a wait tells
+    // phases apart by their parity alone, and a group that skipped the other's phases would take an old one for its own.
+    static constexpr int kUnit = paged_rows_bytes<TYPE, BLOCKS>() + (TYPE == kPagedQ8 ? 2 * kPagedTile * 4 : 0);
+    static constexpr int kFit = 50 * 1024 / kUnit, kUnits = kFit > 8 ? 8 : kFit < 3 ? 3 : kFit;  // about 100 KB under way per block, two blocks per multiprocessor
+    static constexpr int kPitch = HD * 2 + (TYPE == kPagedQ8 ? 32 : 16);  // bytes of a row of queries: eight rows fall into different banks
+    static constexpr int kJoinPitch = HD + 4, kJoin = 8 * kRows * (kJoinPitch * 4 + 8);
+    static constexpr int kBody = 2 * kUnits * kUnit > kJoin ? 2 * kUnits * kUnit : kJoin;
+    static constexpr int kSmem = 1024 + kBody + kRows * kPitch + kRows * 4 + 4 * kUnits * 8 + 64;
+    static constexpr int kBlocksPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && (NT == 1 || NT * BLOCKS <= 2) ? 2 : 1;
+};
 
-// Brings the tiles of [begin, end) of one KV head into the ring, in turn; run by one whole warp. The pages' numbers of the tile after are asked for
-// before a wait. Returns with its own copies landed.
-template <int TYPE, int BLOCKS, int STAGES>
-__device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, uint32_t ring, uint32_t full, uint32_t empty,
+// Brings the tiles of [begin, end) of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one whole warp. The pages' numbers of the tile after are
+// asked for before a wait. Returns with its own copies landed.
+template <int TYPE, int BLOCKS, int NT>
+__device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, uint32_t rings, uint32_t full, uint32_t empty,
                                                  volatile unsigned int* abort_flag, unsigned int limit) {
     using namespace gemm_detail;
-    constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), kStage = paged_stage_bytes<TYPE, BLOCKS>();
+    using F = PagedFew<TYPE, BLOCKS, NT>;
+    constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
     const int lane = threadIdx.x & 31, P = 1 << c.page_log2, PR = min(P, kPagedTile);
     auto page_of = [&](int k0) {  // lane i: the page of the tile's piece i
         const int k = k0 + lane * PR;
@@ -146,49 +155,48 @@ __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* 
         }
         return page;
     };
-    int next = page_of(begin), it = 0;
-    for (int k0 = begin; k0 < end; k0 += kPagedTile, ++it) {
-        const int pages = next, s = it % STAGES, pieces = (min(kPagedTile, end - k0) + PR - 1) / PR;
+    int next = page_of(begin), tile = 0, asked0 = 0, asked1 = 0;  // units asked for, of either ring
+    bool okay = true;
+    for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
+        const int pages = next, pieces = (min(kPagedTile, end - k0) + PR - 1) / PR;
         if (k0 + kPagedTile < end) next = page_of(k0 + kPagedTile);
-        if (!__all_sync(0xffffffffu, mbar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, limit))) break;
-        const uint32_t stage = ring + s * kStage, bar = full + 8 * s;
-        if (lane == 0) mbar_expect_tx(bar, pieces * PR * (2 * BLOCKS * kRow + (TYPE == kPagedQ8 ? 8 : 0)));
-        __syncwarp();
-        for (int i0 = 0; i0 < pieces * BLOCKS * 2; i0 += 32) {  // a piece's rows of a block, keys then values
-            const int i = i0 + lane, piece = i / (2 * BLOCKS), b = i % BLOCKS, value = i / BLOCKS & 1;
-            const int page = __shfl_sync(0xffffffffu, pages, min(piece, 3));
-            if (i < pieces * BLOCKS * 2) {
-                const size_t from = paged_block_at(c, TYPE, page, head, b) + static_cast<size_t>((k0 + piece * PR) & (P - 1)) * kRow;
-                bulk_load(stage + value * kRows + (b * kPagedTile + piece * PR) * kRow, (value ? c.v : c.k) + from, PR * kRow, bar);
-            }
-        }
-        if constexpr (TYPE == kPagedQ8) {
-            const int piece = lane >> 1, value = lane & 1, page = __shfl_sync(0xffffffffu, pages, min(piece, 3));
-            if (piece < pieces) {
-                const size_t from = paged_scales_at(c, page, head) + ((k0 + piece * PR) & (P - 1));
-                bulk_load(stage + 2 * kRows + (value * kPagedTile + piece * PR) * 4, (value ? c.vs : c.ks) + from, PR * 4, bar);
+#pragma unroll
+        for (int value = 0; value < 2; ++value) {
+            const int ring = tile & 1, n = (tile >> 1) * 2 + value, slot = ring * U + n % U;
+            if (!(okay = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, ((n / U) & 1) ^ 1, abort_flag, limit)))) break;
+            const uint32_t to = rings + slot * F::kUnit, bar = full + 8 * slot;
+            if (lane == 0) mbar_expect_tx(bar, pieces * PR * (BLOCKS * kRow + (TYPE == kPagedQ8 && value == 0 ? 8 : 0)));
+            __syncwarp();
+            (ring ? asked1 : asked0) = n + 1;
+            const int piece = lane / BLOCKS, b = lane % BLOCKS, page = __shfl_sync(0xffffffffu, pages, min(piece, 3));  // (at most 4 pieces of 4 blocks)
+            if (lane < pieces * BLOCKS)
+                bulk_load(to + (b * kPagedTile + piece * PR) * kRow, (value ? c.v : c.k) + paged_block_at(c, TYPE, page, head, b) + static_cast<size_t>((k0 + piece * PR) & (P - 1)) * kRow, PR * kRow, bar);
+            if (TYPE == kPagedQ8 && value == 0 && lane < pieces) {
+                const size_t from = paged_scales_at(c, pages, head) + ((k0 + lane * PR) & (P - 1));
+                bulk_load(to + kRows + lane * PR * 4, c.ks + from, PR * 4, bar);
+                bulk_load(to + kRows + (kPagedTile + lane * PR) * 4, c.vs + from, PR * 4, bar);
             }
         }
     }
-    for (int back = max(0, it - STAGES); back < it; ++back) mbar_wait(full + 8 * (back % STAGES), (back / STAGES) & 1, abort_flag, limit, false);
+    for (int ring = 0; ring < 2; ++ring)
+        for (int asked = ring ? asked1 : asked0, n = max(0, asked - U); n < asked; ++n) mbar_wait(full + 8 * (ring * U + n % U), (n / U) & 1, abort_flag, limit, false);
 }
 
-template <int TYPE, int BLOCKS, int RT>
-__global__ void __launch_bounds__(32 + 128 * RT, 1) paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
+template <int TYPE, int BLOCKS, int NT>
+__global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew<TYPE, BLOCKS, NT>::kBlocksPerSm) paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
     using namespace gemm_detail;
     using namespace paged_detail;
-    constexpr int HD = BLOCKS * kPagedBlock, kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), kStage = paged_stage_bytes<TYPE, BLOCKS>(), S = paged_stages<TYPE, BLOCKS>();
-    constexpr int kPitch = paged_q_pitch<TYPE, BLOCKS>(), KS = HD / 16, kThreads = 32 + 128 * RT;
-    constexpr bool Q8 = TYPE == kPagedQ8, BF = TYPE == kPagedBf16, kHoldQ = BLOCKS <= 2;
+    using F = PagedFew<TYPE, BLOCKS, NT>;
+    constexpr int HD = F::HD, kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits, kPitch = F::kPitch, KS = HD / 16, kThreads = F::kThreads;
+    constexpr bool Q8 = TYPE == kPagedQ8, BF = TYPE == kPagedBf16, kHoldQ = KS * NT <= 16 && F::kBlocksPerSm * KS <= 16;
     extern __shared__ unsigned char few_smem_raw[];
     const uint32_t ring = (smem_u32(few_smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = few_smem_raw + (ring - smem_u32(few_smem_raw));
-    constexpr int kJoin = RT * 4 * 16 * (HD * 4 + 16), kBody = S * kStage > kJoin ? S * kStage : kJoin;
-    unsigned char* s_q = smem + kBody;                                          // [RT * 16][kPitch]
-    float* s_rowf = reinterpret_cast<float*>(s_q + RT * 16 * kPitch);           // [RT * 16]: what a row's score is multiplied by
-    uint64_t* bars = reinterpret_cast<uint64_t*>(s_rowf + RT * 16);
-    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 2 * S);
-    const uint32_t full = smem_u32(bars), empty = full + 8 * S;
+    unsigned char* s_q = smem + F::kBody;                                       // [kRows][kPitch]
+    float* s_rowf = reinterpret_cast<float*>(s_q + F::kRows * kPitch);          // [kRows]: what a row's score is multiplied by
+    uint64_t* bars = reinterpret_cast<uint64_t*>(s_rowf + F::kRows);
+    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U);
+    const uint32_t full = smem_u32(bars), empty = full + 16 * U;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const int seq = blockIdx.z, kvh = blockIdx.y % a.c.kv_heads, tile = blockIdx.y / a.c.kv_heads;
@@ -197,23 +205,23 @@ __global__ void __launch_bounds__(32 + 128 * RT, 1) paged_few_kernel(const __gri
         if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
         return;
     }
-    const int rows = sq.news * a.group, r0 = tile * RT * 16, r1 = min(rows, r0 + RT * 16);
+    const int rows = sq.news * a.group, r0 = tile * F::kRows, r1 = min(rows, r0 + F::kRows);
     if (r0 >= rows) return;
     if (static_cast<int>(blockIdx.x) >= paged_splits_used(a, sq)) return;
-    const PagedRange range = paged_range(a, sq, r0 / a.group, (r1 - 1) / a.group + 1, blockIdx.x);
-    const int p0 = sq.length - sq.news;
+    const int t0 = r0 / a.group, t1 = (r1 - 1) / a.group + 1, p0 = sq.length - sq.news;
+    const PagedRange range = paged_range(a, sq, t0, t1, blockIdx.x);
 
     if (tid == 0) {
-        for (int s = 0; s < S; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 4 * RT);
+        for (int s = 0; s < 2 * U; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 4);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    if (warp == 4 * RT) {
-        paged_load_tiles<TYPE, BLOCKS, S>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, abort_flag, a.spin_limit);
+    if (warp == 8) {
+        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, abort_flag, a.spin_limit);
     } else {
-        // queries: a warp takes rows warp, warp + 4 RT, ...; a lane 8 values or none
-        for (int i = warp; i < RT * 16; i += 4 * RT) {
+        // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none
+        for (int i = warp; i < F::kRows; i += 8) {
             const int r = r0 + i, t = r / a.group, h = kvh * a.group + r % a.group;
             float x[8];
 #pragma unroll
@@ -238,235 +246,243 @@ __global__ void __launch_bounds__(32 + 128 * RT, 1) paged_few_kernel(const __gri
             if (lane < HD / 8) paged_store8(s_q + i * kPitch + lane * 16, BF ? kPagedBf16 : kPagedF16, x);
             if (lane == 0) s_rowf[i] = f * a.scale;
         }
-        asm volatile("bar.sync 1, %0;" ::"n"(128 * RT) : "memory");
+        asm volatile("bar.sync 1, 256;" ::: "memory");
 
-        const int rt = warp >> 2, kg = warp & 3, g = lane >> 2, c4 = lane & 3;
-        const uint32_t q_at = smem_u32(s_q) + rt * 16 * kPitch;
-        // a fragment of the queries: F16 / BF16 as ldmatrix gives it; Q8: values 4 c .. 4 c + 3 of a slice of 16 stand where the instruction has 2 c, 2 c + 1, 2 c + 8, 2 c + 9,
-        // as the codes' bytes come
-        auto load_q = [&](uint32_t (&r)[4], int ks) {
+        const int turn = warp >> 2, kg = warp & 3, g = lane >> 2, c4 = lane & 3;  // positions g and g + 8 of the warp's 16, rows 2 c4 and 2 c4 + 1 of a row tile
+        const uint32_t q_at = smem_u32(s_q);
+        // the right operand of a slice of 16 values: values 2 c, 2 c + 1 and 2 c + 8, 2 c + 9 of row g; Q8: 4 c .. 4 c + 3, as the bytes of the codes come
+        auto load_q = [&](uint32_t (&r)[2], int ks, int n) {
             if constexpr (Q8) {
-                const uint2 u = lds64(q_at + g * kPitch + ks * 32 + c4 * 8), w = lds64(q_at + (g + 8) * kPitch + ks * 32 + c4 * 8);
-                r[0] = u.x, r[1] = w.x, r[2] = u.y, r[3] = w.y;
+                const uint2 u = lds64(q_at + (n * 8 + g) * kPitch + ks * 32 + c4 * 8);
+                r[0] = u.x, r[1] = u.y;
             } else {
-                ldsm4(r, q_at + (lane & 15) * kPitch + ks * 32 + (lane >> 4) * 16);
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(q_at + (n * 8 + g) * kPitch + ks * 32 + c4 * 4) : "memory");
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[1]) : "r"(q_at + (n * 8 + g) * kPitch + ks * 32 + 16 + c4 * 4) : "memory");
             }
         };
-        uint32_t qf[kHoldQ ? KS : 1][4];
+        uint32_t qf[kHoldQ ? KS : 1][kHoldQ ? NT : 1][2];
         if constexpr (kHoldQ) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) load_q(qf[ks], ks);
-        }
-        float rowf[2], m[2], l[2];
-        int last[2], first[2];  // the visible positions of the two rows: first <= j <= last
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + rt * 16 + g + 8 * i, p = p0 + r / a.group;
-            rowf[i] = s_rowf[rt * 16 + g + 8 * i], m[i] = -INFINITY, l[i] = 0.0f;
-            last[i] = r < r1 ? min(p, range.end - 1) : -1;
-            first[i] = a.window > 0 ? max(0, p - a.window + 1) : 0;
+                for (int n = 0; n < NT; ++n) load_q(qf[ks][n], ks, n);
         }
-        float o[KS][2][4];
+        float rowf[NT][2], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) rowf[n][i] = s_rowf[n * 8 + c4 * 2 + i], m[n][i] = -INFINITY, l[n][i] = 0.0f;
+        // positions that every row sees; outside of them the masks are worked out
+        const int all_last = p0 + t0, all_first = a.window > 0 ? p0 + t1 - a.window : 0;
+        float o[KS][NT][4];
 #pragma unroll
         for (int j = 0; j < KS; ++j)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][n][e] = 0.0f;
 
         bool okay = true;
-        int it = 0;
-        for (int k0 = range.begin; k0 < range.end; k0 += kPagedTile, ++it) {
-            const int s = it % S, key0 = k0 + kg * 16;
-            okay = __all_sync(0xffffffffu, mbar_wait(full + 8 * s, (it / S) & 1, abort_flag, a.spin_limit));
+        int n = 0;  // units of this group's ring
+        for (int k0 = range.begin + turn * kPagedTile; k0 < range.end; k0 += 2 * kPagedTile, n += 2) {
+            const int key_slot = turn * U + n % U, value_slot = turn * U + (n + 1) % U, key0 = k0 + kg * 16;
+            const uint32_t keys = ring + key_slot * F::kUnit, values = ring + value_slot * F::kUnit;
+            const bool there = key0 < range.end;  // (what lies behind the last page was not copied)
+            okay = __all_sync(0xffffffffu, mbar_wait(full + 8 * key_slot, (n / U) & 1, abort_flag, a.spin_limit));
             if (!okay) break;
-            const uint32_t stage = ring + s * kStage;
-            if (key0 < range.end) {  // (what lies behind the last page was not copied)
-                // scores of 16 rows and 16 positions
-                float sc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                if constexpr (Q8) {
-                    // four matrices: positions 0-7 and 8-15 of the first slice of 16 values, then of the second
-                    const int row = kg * 16 + (lane & 15), swz = (row >> 1) & 3;
+            const int row = kg * 16 + (lane & 15), swz = Q8 ? (row >> 1) & 3 : row & 7;
+            uint32_t pb[NT][2];
+            if (there) {
+                float sc[NT][4];
 #pragma unroll
-                    for (int b = 0; b < BLOCKS; ++b) {
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int two = 0; two < 2; ++two) {
-                            uint32_t r[4];
-                            ldsm4(r, stage + (b * kPagedTile + row) * kRow + (((two * 2 + (lane >> 4)) ^ swz) << 4));
+                    for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
+                auto score = [&](const uint32_t (&k)[4], int ks) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const int ks = b * 4 + two * 2 + h;
-                                uint32_t qa[4];
-                                if constexpr (kHoldQ) {
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) qa[e] = qf[ks][e];
-                                } else {
-                                    load_q(qa, ks);
-                                }
-#pragma unroll
-                                for (int n = 0; n < 2; ++n) {
-                                    const uint32_t u = r[h * 2 + n] ^ 0x80808080u;
-                                    mma<false>(sc[n], qa, codes_to_half2(u, 0x4140), codes_to_half2(u, 0x4342));
-                                }
-                            }
-                        }
+                    for (int n = 0; n < NT; ++n) {
+                        uint32_t b[2];
+                        if constexpr (kHoldQ) b[0] = qf[ks][n][0], b[1] = qf[ks][n][1];
+                        else load_q(b, ks, n);
+                        mma<BF>(sc[n], k, b[0], b[1]);
                     }
-                } else {
-                    const int row = kg * 16 + (lane & 7) + ((lane >> 4) << 3);
+                };
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        uint32_t r[4], qa[4];
-                        ldsm4(r, stage + ((ks >> 2) * kPagedTile + row) * kRow + ((((ks & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-                        if constexpr (kHoldQ) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) qa[e] = qf[ks][e];
-                        } else {
-                            load_q(qa, ks);
-                        }
-                        mma<BF>(sc[0], qa, r[0], r[1]);
-                        mma<BF>(sc[1], qa, r[2], r[3]);
-                    }
-                }
-                // the scores' exponents, with masks
-                float iv[2][2];
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    float kf[2] = {1.0f, 1.0f}, lv[2] = {0.0f, 0.0f};
-                    iv[n][0] = iv[n][1] = 1.0f;
-                    if constexpr (Q8) {
-                        const uint32_t at = stage + 2 * kRows + (kg * 16 + n * 8 + c4 * 2) * 4;
-                        const uint2 ku = lds64(at), vu = lds64(at + kPagedTile * 4);
-                        kf[0] = __uint_as_float(ku.x), kf[1] = __uint_as_float(ku.y);
-                        lv[0] = lg2(__uint_as_float(vu.x)), lv[1] = lg2(__uint_as_float(vu.y));
-                        iv[n][0] = rcp(__uint_as_float(vu.x)), iv[n][1] = rcp(__uint_as_float(vu.y));
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = e >> 1, j = key0 + n * 8 + c4 * 2 + (e & 1);
-                        float x = sc[n][e];
-                        if constexpr (Q8) x *= kf[e & 1];
-                        x *= rowf[i];
-                        if (a.cap > 0.0f) x = a.cap * tanh_of(x);
-                        if constexpr (Q8) x += lv[e & 1];
-                        x = j >= first[i] && j <= last[i] ? x : -INFINITY;
-                        sc[n][e] = x;
-                        top[i] = fmaxf(top[i], x);
-                    }
-                }
-                float keep[2];
-                bool grew = false;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                    keep[i] = 1.0f;
-                    if (top[i] > m[i] + kPagedLazy || (m[i] == -INFINITY && top[i] > -INFINITY)) {
-                        keep[i] = ex2(m[i] - top[i]);  // 0 the first time
-                        m[i] = top[i];
-                        l[i] *= keep[i];
-                        grew = true;
-                    }
-                }
-                if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-                    for (int j = 0; j < KS; ++j)
-#pragma unroll
-                        for (int n = 0; n < 2; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) o[j][n][e] *= keep[e >> 1];
-                }
-                uint32_t pa[4];
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = e >> 1;
-                        w[e] = sc[n][e] == -INFINITY ? 0.0f : ex2(sc[n][e] - m[i]);
-                        if constexpr (Q8) {
-                            if (!(w[e] == 0.0f)) l[i] = fmaf(w[e], iv[n][e & 1], l[i]);  // (the scales behind the last position may be anything)
-                        } else {
-                            l[i] += w[e];
-                        }
-                    }
-                    pa[n * 2] = paged_pack2(BF ? kPagedBf16 : kPagedF16, w[0], w[1]);
-                    pa[n * 2 + 1] = paged_pack2(BF ? kPagedBf16 : kPagedF16, w[2], w[3]);
-                }
-                // the weighted rows
-                const int row = kg * 16 + (lane & 15);
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
+                for (int ks = 0; ks < KS; ++ks) {
                     uint32_t r[4];
                     if constexpr (Q8) {
-                        if ((j & 1) == 0) {  // two slices of 16 values: matrices (positions 0-7, 8-15) x (slice j, j + 1)
-                            ldsm4_trans(r, stage + kRows + ((j >> 2) * kPagedTile + row) * kRow + ((((j & 3) + (lane >> 4)) ^ ((row >> 1) & 3)) << 4));
+                        if ((ks & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice ks, then of slice ks + 1
+                            ldsm4(r, keys + ((ks >> 2) * kPagedTile + row) * kRow + ((((ks & 3) + (lane >> 4)) ^ swz) << 4));
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
-                                mma<false>(o[j + h][0], pa, codes_to_half2(u0, 0x4240), codes_to_half2(u1, 0x4240));  // the even values of the slice
-                                mma<false>(o[j + h][1], pa, codes_to_half2(u0, 0x4341), codes_to_half2(u1, 0x4341));  // the odd ones
+                                const uint32_t k[4] = {codes_to_half2(u0, 0x4140), codes_to_half2(u1, 0x4140), codes_to_half2(u0, 0x4342), codes_to_half2(u1, 0x4342)};
+                                score(k, ks + h);
                             }
                         }
-                    } else {
-                        ldsm4_trans(r, stage + kRows + ((j >> 2) * kPagedTile + row) * kRow + ((((j & 3) * 2 + (lane >> 4)) ^ (row & 7)) << 4));
-                        mma<BF>(o[j][0], pa, r[0], r[1]);
-                        mma<BF>(o[j][1], pa, r[2], r[3]);
+                    } else {  // positions 0-7 and 8-15 of the slice's first 8 values, then of the others
+                        ldsm4(r, keys + ((ks >> 2) * kPagedTile + row) * kRow + ((((ks & 3) * 2 + (lane >> 4)) ^ swz) << 4));
+                        score(r, ks);
+                    }
+                }
+                // the exponents, with masks
+                float kf[2] = {1.0f, 1.0f}, lv[2] = {0.0f, 0.0f}, iv[2] = {1.0f, 1.0f};
+                if constexpr (Q8) {
+                    const float* f = reinterpret_cast<const float*>(smem + key_slot * F::kUnit + kRows) + kg * 16 + g;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float v = key0 + g + 8 * i < range.end ? f[kPagedTile + 8 * i] : 1.0f;  // (the scales behind the last page may be anything)
+                        kf[i] = f[8 * i], lv[i] = lg2(v), iv[i] = rcp(v);
+                    }
+                }
+                const bool masked = key0 + 15 > all_last || key0 + 15 >= range.end || key0 < all_first;
+                float top[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float x = sc[n][e];
+                        if constexpr (Q8) x *= kf[e >> 1];
+                        x *= rowf[n][e & 1];
+                        if (a.cap > 0.0f) x = a.cap * tanh_of(x);
+                        if constexpr (Q8) x += lv[e >> 1];
+                        sc[n][e] = x;
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int rr = r0 + n * 8 + c4 * 2 + (e & 1), p = p0 + rr / a.group, j = key0 + g + 8 * (e >> 1);
+                            if (rr >= r1 || j > p || j >= range.end || (a.window > 0 && j <= p - a.window)) sc[n][e] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) top[n][i] = fmaxf(sc[n][i], sc[n][2 + i]);
+                }
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], x));
+                bool grew = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) grew = grew || top[n][i] > m[n][i] + kPagedLazy || (m[n][i] == -INFINITY && top[n][i] > -INFINITY);
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float keep[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const bool more = top[n][i] > m[n][i] + kPagedLazy || (m[n][i] == -INFINITY && top[n][i] > -INFINITY);
+                            keep[i] = more ? ex2(m[n][i] - top[n][i]) : 1.0f;  // 0 the first time
+                            if (more) m[n][i] = top[n][i], l[n][i] *= keep[i];
+                        }
+#pragma unroll
+                        for (int j = 0; j < KS; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[j][n][e] *= keep[e & 1];
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float ref = m[n][e & 1];
+                        w[e] = sc[n][e] == -INFINITY ? 0.0f : ex2(sc[n][e] - ref);
+                        l[n][e & 1] = fmaf(w[e], iv[e >> 1], l[n][e & 1]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {  // rows 2 c, 2 c + 1 of position g (+ 8) become positions 2 c, 2 c + 1 (+ 8) of row g
+                        const uint32_t v = paged_pack2(BF ? kPagedBf16 : kPagedF16, w[2 * h], w[2 * h + 1]);
+                        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[n][h]) : "r"(v));
                     }
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty + 8 * s);
-        }
-        if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        }
-        // every tile was read (or a wait gave up, and nothing below matters): the ring becomes the place where the warps of a row tile meet
-        asm volatile("bar.sync 1, %0;" ::"n"(128 * RT) : "memory");
-        float* join = reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * 16 * HD;  // [16][HD]
-        float2* ml = reinterpret_cast<float2*>(smem + static_cast<size_t>(RT) * 4 * 16 * HD * 4) + warp * 16;
-        if (*abort_flag == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (c4 == 0) ml[g + 8 * i] = make_float2(m[i], l[i]);
-                float* to = join + (g + 8 * i) * HD;
+            if (lane == 0) mbar_arrive(empty + 8 * key_slot);
+            okay = __all_sync(0xffffffffu, mbar_wait(full + 8 * value_slot, ((n + 1) / U) & 1, abort_flag, a.spin_limit));
+            if (!okay) break;
+            if (there) {  // the weighted rows
 #pragma unroll
                 for (int j = 0; j < KS; ++j) {
-                    if constexpr (Q8) {  // (slice j: the even values 4 c, 4 c + 2 and the odd ones 4 c + 1, 4 c + 3)
-                        *reinterpret_cast<float4*>(to + ((j * 16 + c4 * 4) ^ (g << 2 & 12))) = make_float4(o[j][0][2 * i], o[j][1][2 * i], o[j][0][2 * i + 1], o[j][1][2 * i + 1]);
-                    } else {
+                    uint32_t r[4];
+                    if constexpr (Q8) {
+                        if ((j & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice j, then of slice j + 1; a pair of bytes is two values of a position
+                            ldsm4_trans(r, values + ((j >> 2) * kPagedTile + row) * kRow + ((((j & 3) + (lane >> 4)) ^ swz) << 4));
 #pragma unroll
-                        for (int n = 0; n < 2; ++n) *reinterpret_cast<float2*>(to + ((j * 16 + n * 8 + c4 * 2) ^ (g << 2 & 12))) = make_float2(o[j][n][2 * i], o[j][n][2 * i + 1]);
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
+                                const uint32_t v[4] = {codes_to_half2(u0, 0x4240), codes_to_half2(u0, 0x4341), codes_to_half2(u1, 0x4240), codes_to_half2(u1, 0x4341)};  // even values, odd values
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) mma<false>(o[j + h][n], v, pb[n][0], pb[n][1]);
+                            }
+                        }
+                    } else {  // matrices: (positions 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+                        const int vrow = kg * 16 + (lane & 7) + ((lane >> 4) << 3);
+                        ldsm4_trans(r, values + ((j >> 2) * kPagedTile + vrow) * kRow + ((((j & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<BF>(o[j][n], r, pb[n][0], pb[n][1]);
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + 8 * value_slot);
+        }
+        if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], x);
+        // every tile was read (or a wait gave up, and nothing below matters): the ring becomes the place where the warps meet
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        float* join = reinterpret_cast<float*>(smem) + static_cast<size_t>(warp) * F::kRows * F::kJoinPitch;
+        float2* ml = reinterpret_cast<float2*>(smem + 8 * F::kRows * F::kJoinPitch * 4) + warp * F::kRows;
+        if (*abort_flag == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = n * 8 + c4 * 2 + i;
+                    if (g == 0) ml[r] = make_float2(m[n][i], l[n][i]);
+                    float* to = join + r * F::kJoinPitch;
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        if constexpr (Q8) {
+                            *reinterpret_cast<float2*>(to + j * 16 + 2 * g) = make_float2(o[j][n][i], o[j][n][2 + i]);
+                        } else {
+                            to[j * 16 + g] = o[j][n][i], to[j * 16 + 8 + g] = o[j][n][2 + i];
+                        }
+                    }
+                }
         }
     }
     __syncthreads();
     if (*abort_flag != 0) return;
     // rows out: eight values to a thread
     const float* joined = reinterpret_cast<const float*>(smem);
-    const float2* mls = reinterpret_cast<const float2*>(smem + static_cast<size_t>(RT) * 4 * 16 * HD * 4);
+    const float2* mls = reinterpret_cast<const float2*>(smem + 8 * F::kRows * F::kJoinPitch * 4);
     for (int i = tid; i < (r1 - r0) * (HD / 8); i += kThreads) {
-        const int r = i / (HD / 8), e0 = i % (HD / 8) * 8, rt = r >> 4, rr = r & 15;
-        float top = -INFINITY, w[4], sum = 0.0f, x[8];
+        const int r = i / (HD / 8), e0 = i % (HD / 8) * 8;
+        float top = -INFINITY, w[8], sum = 0.0f, x[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, mls[(rt * 4 + k) * 16 + rr].x);
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, mls[k * F::kRows + r].x);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 v = mls[(rt * 4 + k) * 16 + rr];
+        for (int k = 0; k < 8; ++k) {
+            const float2 v = mls[k * F::kRows + r];
             w[k] = v.x == -INFINITY ? 0.0f : ex2(v.x - top);
             sum = fmaf(w[k], v.y, sum);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float* from = joined + (static_cast<size_t>(rt * 4 + k) * 16 + rr) * HD;
-            const float4 u = *reinterpret_cast<const float4*>(from + (e0 ^ (rr << 2 & 12))), v = *reinterpret_cast<const float4*>(from + ((e0 + 4) ^ (rr << 2 & 12)));
+        for (int k = 0; k < 8; ++k) {
+            const float* from = joined + static_cast<size_t>(k * F::kRows + r) * F::kJoinPitch + e0;
+            const float4 u = *reinterpret_cast<const float4*>(from), v = *reinterpret_cast<const float4*>(from + 4);
             x[0] = fmaf(w[k], u.x, x[0]), x[1] = fmaf(w[k], u.y, x[1]), x[2] = fmaf(w[k], u.z, x[2]), x[3] = fmaf(w[k], u.w, x[3]);
             x[4] = fmaf(w[k], v.x, x[4]), x[5] = fmaf(w[k], v.y, x[5]), x[6] = fmaf(w[k], v.z, x[6]), x[7] = fmaf(w[k], v.w, x[7]);
         }
@@ -486,44 +502,87 @@ __global__ void __launch_bounds__(32 + 128 * RT, 1) paged_few_kernel(const __gri
     }
 }
 
-// Joins the ranges of a sequence: a warp per (token, query head), in the order of the ranges.
-template <int BLOCKS>
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
+// Joins results of ranges: weights 2^(m_i - m) over `count` of them, `step` rows apart from row `row`, for the values of one warp's lanes (kPer each), by the WARPS warps of a block in turn, eight results at
+// a time so that their reads overlap; in the same order whenever it is asked for. Returns the row's normalised values, in the first warp.
+template <int HD, int WARPS>
+__device__ __forceinline__ void paged_join(const float* part_o, const float2* part_ml, size_t row, size_t step, int count, float (&x)[HD / 32], float* shared) {
     using namespace paged_detail;
+    constexpr int kPer = HD / 32;
+    const int lane = threadIdx.x & 31, warp = WARPS > 1 ? threadIdx.x >> 5 : 0;
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, part_ml[i * step + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
+    for (int i0 = warp; i0 < count; i0 += 8 * WARPS) {
+        float2 ml[8];
+        float v[8][kPer];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * WARPS;
+            ml[k] = i < count ? part_ml[i * step + row] : make_float2(-INFINITY, 0.0f);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool there = !(ml[k].x == -INFINITY && ml[k].y == 0.0f);  // a range in which nothing was visible has no values
+            const float* from = part_o + (static_cast<size_t>(i0 + k * WARPS) * step + row) * HD + lane * kPer;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[k][e] = there ? from[e] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float w = ml[k].x == -INFINITY && ml[k].y == 0.0f ? 0.0f : ex2(ml[k].x - top);
+            sum = fmaf(w, ml[k].y, sum);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x[e] = fmaf(w, v[k][e], x[e]);
+        }
+    }
+    if constexpr (WARPS > 1) {
+        float* mine = shared + (warp * 32 + lane) * (kPer + 1);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) mine[e] = x[e];
+        mine[kPer] = sum;
+        __syncthreads();
+        if (warp != 0) return;
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) {
+            const float* other = shared + (w * 32 + lane) * (kPer + 1);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) x[e] += other[e];
+            sum += other[kPer];
+        }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] *= inv;
+}
+template <int PER>
+__device__ __forceinline__ void paged_store_row(unsigned char* out, int type, const float (&x)[PER]) {
+    if (type == kPagedF32) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) reinterpret_cast<float*>(out)[e] = x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = paged_pack2(type, x[e], x[e + 1]);
+    }
+}
+
+// Joins the ranges of a sequence: a block of WARPS warps per (token, query head).
+template <int BLOCKS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
-    const int heads = a.c.kv_heads * a.group, lane = threadIdx.x & 31;
-    const int item = blockIdx.x * 8 + (threadIdx.x >> 5), t = item / heads, h = item % heads;
-    if (t >= a.r.tokens) return;
+    __shared__ float shared[WARPS > 1 ? WARPS * 32 * (kPer + 1) : 1];
+    const int heads = a.c.kv_heads * a.group, lane = threadIdx.x & 31, t = blockIdx.x / heads, h = blockIdx.x % heads;
     const int s = paged_sequence_of(a.r, t);
     if (s < 0) return;
     const PagedSequence sq = paged_sequence(a.c, a.r, s);
     if (!sq.ok || t < sq.first || t >= sq.first + sq.news || sq.news < a.few || sq.news > a.many) return;
-    const int used = paged_splits_used(a, sq);
-    const size_t step = static_cast<size_t>(a.r.tokens) * heads, row = static_cast<size_t>(t) * heads + h;
-    float top = -INFINITY;
-    for (int i = lane; i < used; i += 32) top = fmaxf(top, a.part_ml[i * step + row].x);
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f, x[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
-    for (int i = 0; i < used; ++i) {
-        const float2 v = a.part_ml[i * step + row];
-        if (v.x == -INFINITY && v.y == 0.0f) continue;  // nothing visible there
-        const float w = ex2(v.x - top);
-        sum = fmaf(w, v.y, sum);
-        const float* from = a.part_o + (i * step + row) * HD + lane * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) x[e] = fmaf(w, from[e], x[e]);
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
-    unsigned char* out = static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type);
-    if (a.out_type == kPagedF32) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) reinterpret_cast<float*>(out)[e] = x[e] * inv;
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = paged_pack2(a.out_type, x[e] * inv, x[e + 1] * inv);
-    }
+    float x[kPer];
+    paged_join<HD, WARPS>(a.part_o, a.part_ml, static_cast<size_t>(t) * heads + h, static_cast<size_t>(a.r.tokens) * heads, paged_splits_used(a, sq), x, shared);
+    if (threadIdx.x >= 32) return;
+    paged_store_row(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x);
 }
 
 }  // namespace qtb

@@ -553,31 +553,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     const int rows = sq.news * a.group, block = (rows + kRows - 1) / kRows - 1 - order, r = block * kRows + local;
     if (block < 0 || r >= rows) return;
     const size_t row = paged_part_row(a, g, sq, PagedPart{order, 0, ranges, x}, which, kvh, r, local, kRows), step = paged_part_row(a, g, sq, PagedPart{order, 1, ranges, x + 1}, which, kvh, r, local, kRows) - row;
-    float top = -INFINITY;
-    for (int i = lane; i < ranges; i += 32) top = fmaxf(top, g.part_ml[i * step + row].x);
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.0f, v[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = 0.0f;
-    for (int i = 0; i < ranges; ++i) {
-        const float2 ml = g.part_ml[i * step + row];
-        if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // nothing visible there
-        const float w = ex2(ml.x - top);
-        sum = fmaf(w, ml.y, sum);
-        const float* from = g.part_o + (i * step + row) * HD + lane * kPer;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) v[e] = fmaf(w, from[e], v[e]);
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
+    float x_row[kPer];
+    paged_join<HD, 1>(g.part_o, g.part_ml, row, step, ranges, x_row, nullptr);
     const size_t token = static_cast<size_t>(sq.first) + r / a.group;
-    unsigned char* out = static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + r % a.group) * a.o_head + lane * kPer) * paged_size_of(a.out_type);
-    if (a.out_type == kPagedF32) {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) reinterpret_cast<float*>(out)[e] = v[e] * inv;
-    } else {
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = paged_pack2(a.out_type, v[e] * inv, v[e + 1] * inv);
-    }
+    paged_store_row(static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + r % a.group) * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x_row);
 }
 
 }  // namespace qtb
