@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
 
@@ -165,9 +166,9 @@ int places_of(const quintrit_b200_paged_cache* c, int nt) {
 // The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles and a start and an end of
 // about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. Where the sequences' chunks differ, as in a step that carries one
 // prompt, fewer row blocks are there than the longest chunk times the sequences: their number is taken from the tokens.
-size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, size_t limit, PagedSchedule* g) {
+size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, int rows, size_t limit, PagedSchedule* g) {
     constexpr double kStart = 4.0, kJoin = 3.0;
-    const int rows = c->head_dim == 256 ? 128 : 256, tile = c->head_dim == 256 ? 64 : 128, sms = c->sm_count;
+    const int tile = c->head_dim == 256 ? 64 : 128, sms = c->sm_count;
     const long long most = static_cast<long long>(r->max_new) * group, blocks = (most + rows - 1) / rows, kvh = c->kv_heads;
     const long long all = static_cast<long long>(r->tokens) * group, m = std::max<long long>(kvh, kvh * ((all + rows - 1) / rows) / blocks);  // blocks of an order, likely
     // tiles that the row block of an order sees, if its sequence has the length that was announced
@@ -211,21 +212,24 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
     g->whole = static_cast<int>(whole), g->cut = best;
     return static_cast<size_t>(left) * g->m * best * rows;
 }
-template <int TYPE, int BLOCKS>
+template <int TYPE, int BLOCKS, int NT>
 int launch_many_of(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
-    using M = PagedMany<TYPE, BLOCKS>;
+    using M = PagedMany<TYPE, BLOCKS, NT>;
     static_assert(M::kSmem <= 227 * 1024, "the rings do not fit");
     static std::atomic<uint64_t> done{0};
-    const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS>, M::kSmem, device, done);
+    const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS, NT>, M::kSmem, device, done);
     if (rc != QUINTRIT_OK) return rc;
-    paged_many_kernel<TYPE, BLOCKS><<<grid, M::kThreads, M::kSmem, s>>>(a, g);
+    paged_many_kernel<TYPE, BLOCKS, NT><<<grid, M::kThreads, M::kSmem, s>>>(a, g);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
 template <int TYPE>
-int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
-    return a.c.blocks == 1 ? launch_many_of<TYPE, 1>(a, g, device, grid, s) : a.c.blocks == 2 ? launch_many_of<TYPE, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 4>(a, g, device, grid, s);
+int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device, int rows, unsigned grid, cudaStream_t s) {
+    if (a.c.blocks == 4) return launch_many_of<TYPE, 4, 1>(a, g, device, grid, s);
+    if (rows == 128) return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 1>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 1>(a, g, device, grid, s);
+    return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 2>(a, g, device, grid, s);
 }
+
 // How a call is served: sequences of up to `few_new` new tokens by the kernel for few rows, the others by the one for many; either may have nothing to do.
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
@@ -234,13 +238,15 @@ struct PagedPlan {
     long long few_tiles;
     PagedCut few_cut;
     PagedSchedule schedule;  // many: which blocks, their number, slots of the workspace
+    int many_rows;           // rows of a block of threads
     long long many_blocks;
     size_t part_rows;
     size_t few_bytes, many_bytes;  // of the workspace
 };
+int few_limit() { return std::getenv("QTB_FEW") ? std::atoi(std::getenv("QTB_FEW")) : 64; }
 constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {
-    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = 64;
+    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = few_limit();
     p->many = most > limit;
     p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(limit / group, r->max_new - 1));  // (a sequence alone is the longest)
     p->few_tiles = 0, p->few_cut = PagedCut{1, kPagedTile}, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
@@ -255,10 +261,11 @@ void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_
         if (p->few_cut.splits > 1) p->few_bytes = up16(p->few_cut.splits * static_cast<size_t>(r->tokens) * q_heads * row_bytes);
     }
     if (p->many) {
-        const int rows = c->head_dim == 256 ? 128 : 256;
+        const int rows = c->head_dim == 256 || most <= 128 ? 128 : 256;
+        p->many_rows = rows;
         // (up to four results for every row of a block of threads on every multiprocessor, about 80 MB; no window takes more than none)
-        p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), 0, static_cast<size_t>(4) * c->sm_count * rows, &p->schedule);
-        if (window > 0) p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), window, p->part_rows, &p->schedule);
+        p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), 0, rows, static_cast<size_t>(4) * c->sm_count * rows, &p->schedule);
+        if (window > 0) p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), window, rows, p->part_rows, &p->schedule);
         p->many_bytes = up16(p->part_rows * row_bytes);
         const PagedSchedule& g = p->schedule;
         const long long blocks = (most + rows - 1) / rows;
@@ -492,13 +499,13 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             PagedSchedule& g = plan.schedule;
             g.part_o = reinterpret_cast<float*>(workspace + plan.few_bytes), g.part_ml = reinterpret_cast<float2*>(g.part_o + plan.part_rows * cache->head_dim);
             const unsigned grid = static_cast<unsigned>(plan.many_blocks);
-            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(a, g, device, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(a, g, device, grid, s)
-                                                                                                                         : launch_many_type<kPagedQ8>(a, g, device, grid, s);
+            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(a, g, device, plan.many_rows, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(a, g, device, plan.many_rows, grid, s)
+                                                                                                                         : launch_many_type<kPagedQ8>(a, g, device, plan.many_rows, grid, s);
             if (rc != QUINTRIT_OK) return rc;
             if (plan.part_rows > 0) {
-                const int block = cache->head_dim == 256 ? 128 : 256, blocks = static_cast<int>((static_cast<long long>(rows->max_new) * group + block - 1) / block);
+                const int block = plan.many_rows, blocks = static_cast<int>((static_cast<long long>(rows->max_new) * group + block - 1) / block);
                 auto kernel = a.c.blocks == 1 ? paged_join_kernel<1> : a.c.blocks == 2 ? paged_join_kernel<2> : paged_join_kernel<4>;
-                kernel<<<dim3(block / 8, static_cast<unsigned>(g.m), static_cast<unsigned>(blocks - g.whole)), 256, 0, s>>>(a, g);
+                kernel<<<dim3(block / 8, static_cast<unsigned>(g.m), static_cast<unsigned>(blocks - g.whole)), 256, 0, s>>>(a, g, block);
                 QTB_LAUNCH_CHECK();
             }
         }

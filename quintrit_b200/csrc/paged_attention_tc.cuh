@@ -1,18 +1,19 @@
 // Attention of many new tokens over a paged cache on the 5th-generation tensor cores (the mathematics: paged_attention.cuh).
 //
-// A block of threads takes one KV head of one sequence, 256 rows of queries (128 where a head has 256 values; a row is a (token, head of the group)) and a
-// range of positions, in tiles of 128 positions (64). Units of work alternate between two score buffers in tensor memory: the two row tiles of a tile of positions,
-// or the one row tile of successive tiles. For a unit one thread issues S = Q K^T (tcgen05.mma, operands in shared memory; Q of 256 values in tensor memory), a warpgroup
+// A block of threads takes one KV head of one sequence, 256 rows of queries (128 where a head has 256 values, or where there are no more; a row is a (token, head of the group)) and a
+// range of positions, in tiles of 128 positions (64 where a head has 256 values). Units of work, a row tile and a tile of positions, take two score buffers in tensor memory in turn. For a unit one thread issues S = Q K^T (tcgen05.mma, operands in shared memory; Q of a single row tile in tensor memory), a warpgroup
 // with a row per thread (two warpgroups where there is one row tile: two threads per row, half of the positions each, which speak to each other when a maximum grew) turns S into
 // weights (maximum, exponentials, sum) and writes them as 16-bit values over S, and O += P V takes them from
-// there. The tensor cores work on the other buffer meanwhile: score products of unit u + 2 follow the value products of unit u. O stays in tensor memory and is rescaled, by its
+// there. The tensor cores work on the other buffer meanwhile: the score products that take a buffer next follow the value products that took its weights. O stays in tensor memory and is rescaled, by its
 // warpgroups, only when a row's maximum grew by more than 2^8.
 //
 // F16 / BF16: one warp brings the pages' rows by bulk copies straight into the operands' places, since they lie in the cache in the 128-byte swizzle already (keys as a K-major,
-// values as an MN-major operand). Q8: it brings codes and scales to a ring of their own, and four warps widen the codes to F16 operands and prepare the scales.
+// values as an MN-major operand). Q8: it brings codes and scales to a ring of their own, and four or eight warps widen the codes to F16 operands and prepare the scales.
 //
 // Bound by the tensor cores (4 head_dim flops per row and position) and, for heads of up to 128 values, as much by the exponentials: 16 a clock and
-// multiprocessor, so that 128 x 128 scores of a unit take 1024 cycles, and the two products 8 head_dim.
+// multiprocessor, so that 128 x 128 scores take 1024 cycles, and the two products 8 head_dim. (Tiles of 64
+// positions and four buffers kept the threads busier and the tensor cores less: an instruction over 64 positions took 87 cycles, one over 128 took 100. 64-value heads apart, 2048 tokens behind 14336:
+// 461 us against 318 us.)
 #pragma once
 #include "packed_f32.cuh"
 #include "paged_attention.cuh"
@@ -50,30 +51,36 @@ __device__ __forceinline__ PagedRange paged_part_range(const PagedAttnArgs& a, c
     return PagedRange{min(high, low + part * per * tile), min(high, low + (part + 1) * per * tile)};
 }
 
-template <int TYPE, int BLOCKS>
+template <int TYPE, int BLOCKS, int NT>  // NT: row tiles of a block, 1 or 2 (1 where a head has 256 values)
 struct PagedMany {
     static constexpr bool Q8 = TYPE == kPagedQ8, BF = TYPE == kPagedBf16;
-    static constexpr int HD = BLOCKS * kPagedBlock, NT = BLOCKS == 4 ? 1 : 2;  // row tiles of a block
-    static constexpr int KT = BLOCKS == 4 ? 64 : 128;                          // positions of a tile
+    static constexpr int HD = BLOCKS * kPagedBlock;
+    static constexpr int KT = BLOCKS == 4 ? 64 : 128, NB = 2;                  // positions of a tile; score buffers
     static constexpr int kRows = 128 * NT;
     static constexpr int kSlot = KT * HD * 2, kSlots = Q8 ? 3 : 4;             // operand tiles: keys and values in turn
-    static constexpr int kRaw = KT * HD, kRaws = Q8 ? 3 : 0;                   // Q8: the codes; those of keys with the scales of keys and values
+    static constexpr int kRaw = KT * HD, kRaws = Q8 ? (NT == 1 ? 4 : 3) : 0;                   // Q8: the codes; those of keys with the scales of keys and values
     static constexpr int kRawStride = Q8 ? kRaw + KT * 8 : 0;
     static constexpr int kFactors = Q8 ? 4 : 0;                                // sets of KT x (key scale, log2 of the value scale, its reciprocal)
-    static constexpr bool kQTmem = BLOCKS == 4;
-    static constexpr int kQBytes = kQTmem ? 0 : NT * 128 * HD * 2;
-    static constexpr int SIDES = BLOCKS == 4 ? 2 : 1;                          // threads of a row
+    static constexpr bool kQTmem = NT == 1;
+    // A warp's rows go through 32 rows of 144 bytes, so that they are read and written in whole pieces: queries on their way to tensor memory, results on their way out (over the queries in shared
+    // memory, which nothing reads any more by then).
+    static constexpr int kStagePitch = 144, kStageBytes = 4 * NT * (NT == 1 ? 2 : 1) * 32 * kStagePitch, kStageOwn = kQTmem ? kStageBytes : 0;
+    static constexpr int kQBytes = kQTmem ? 0 : NT * 128 * HD * 2 > kStageBytes ? NT * 128 * HD * 2 : (kStageBytes + 1023) / 1024 * 1024;
+    static constexpr int SIDES = NT == 1 ? 2 : 1;                              // threads of a row
+    static constexpr int kWidenWarps = Q8 ? 8 / NT : 0;
     static constexpr int kSoftWarps = 4 * NT * SIDES, kLoadWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
-    static constexpr int kThreads = (kSoftWarps + 4 + (Q8 ? 4 : 0)) * 32;
+    static constexpr int kThreads = (kSoftWarps + 4 + kWidenWarps) * 32;
     // registers: 384 threads are launched with 168 each, 512 with 128; the warpgroups with the scores of two row tiles take some of the others'
     static constexpr bool kSplitRegs = NT == 2;
     static constexpr int kLaunchRegs = Q8 ? 128 : 168, kSoftRegs = Q8 ? 200 : 216, kRestRegs = Q8 ? 56 : 72;
     static_assert(!kSplitRegs || kSoftWarps * 32 * kSoftRegs + (kThreads - kSoftWarps * 32) * kRestRegs <= kThreads * kLaunchRegs, "more registers than the block was launched with");
-    static constexpr int kBars = 2 * kSlots + 2 * kRaws + 2 * 3 + 2;
-    static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + (SIDES == 2 ? 2048 : 0) + kBars * 8 + 16;
+    static constexpr int kBars = 2 * kSlots + 2 * kRaws + 3 * NB + 2;
+    static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + (SIDES == 2 ? 2048 : 0) + NT * 512 + kStageOwn + kBars * 8 + 16;
     static constexpr int kSmem = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one block per multiprocessor: it takes all of its tensor memory
-    static constexpr int kOCol = 0, kSCol = 256, kQCol = 384;  // tensor memory columns: O (of row tile i at 128 i), S (buffer b at KT b behind), Q
+    static constexpr int kOCol = 0, kSCol = 256, kQCol = BLOCKS == 4 ? 384 : 128;  // tensor memory columns: O (of row tile i at 128 i), S (buffer b at KT b behind), Q
 };
+
+template <int T> struct PagedTag { static constexpr int value = T; };
 
 namespace paged_detail {
 
@@ -119,13 +126,13 @@ template <int N> __device__ __forceinline__ void registers_down() { asm volatile
 
 }  // namespace paged_detail
 
-template <int TYPE, int BLOCKS>
-__global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
+template <int TYPE, int BLOCKS, int NT>
+__global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
     using namespace gemm_detail;
     using namespace paged_detail;
-    using M = PagedMany<TYPE, BLOCKS>;
+    using M = PagedMany<TYPE, BLOCKS, NT>;
     constexpr bool Q8 = M::Q8;
-    constexpr int HD = M::HD, NT = M::NT, SIDES = M::SIDES, KT = M::KT, RS = M::kSlots, RW = Q8 ? M::kRaws : 1, kRow = paged_row_bytes(TYPE);
+    constexpr int HD = M::HD, NB = M::NB, SIDES = M::SIDES, KT = M::KT, RS = M::kSlots, RW = Q8 ? M::kRaws : 1, kRow = paged_row_bytes(TYPE);
     extern __shared__ unsigned char many_smem_raw[];
     const uint32_t base = (smem_u32(many_smem_raw) + 1023u) & ~1023u;
     unsigned char* smem = many_smem_raw + (base - smem_u32(many_smem_raw));
@@ -133,7 +140,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     unsigned char* raw_smem = smem + M::kQBytes + RS * M::kSlot;
     float* factors = reinterpret_cast<float*>(raw_smem + M::kRaws * M::kRawStride);  // [kFactors][3][KT]
     float2* exchange = reinterpret_cast<float2*>(factors + M::kFactors * 3 * KT);  // [2][128]: between the two threads of a row
-    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + (SIDES == 2 ? 256 : 0));
+    float* row_factor = reinterpret_cast<float*>(exchange + (SIDES == 2 ? 256 : 0));  // [NT * 128]
+    unsigned char* staging = M::kQTmem ? reinterpret_cast<unsigned char*>(row_factor + NT * 128) : smem;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(row_factor + NT * 128) + M::kStageOwn);
     const uint32_t bar0 = smem_u32(bars);
     auto full = [&](int s) { return bar0 + 8u * s; };                       // an operand tile is there
     auto empty = [&](int s) { return bar0 + 8u * (RS + s); };               // the products that read it are done
@@ -141,9 +150,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     auto raw_empty = [&](int s) { return bar0 + 8u * (2 * RS + M::kRaws + s); };
     const uint32_t tail = bar0 + 8u * (2 * RS + 2 * M::kRaws);
     auto s_full = [&](int b) { return tail + 8u * b; };                     // scores of a buffer
-    auto p_full = [&](int b) { return tail + 8u * (2 + b); };               // weights of a buffer
-    auto o_done = [&](int b) { return tail + 8u * (4 + b); };               // the value products of a buffer's weights
-    const uint32_t q_full = tail + 8u * 6, drained = tail + 8u * 7;
+    auto p_full = [&](int b) { return tail + 8u * (NB + b); };               // weights of a buffer
+    auto o_done = [&](int b) { return tail + 8u * (2 * NB + b); };               // the value products of a buffer's weights
+    const uint32_t q_full = tail + 8u * (3 * NB), drained = q_full + 8u;
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + M::kBars);
     volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -161,9 +170,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     const int p0 = sq.length - sq.news, tiles = range.end > range.begin ? (range.end - range.begin + KT - 1) / KT : 0, units = tiles * NT;
 
     if (tid == 0) {
-        for (int s = 0; s < RS; ++s) mbar_init(full(s), Q8 ? 4 : 1), mbar_init(empty(s), 1);
-        for (int s = 0; s < M::kRaws; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), 4);
-        for (int b = 0; b < 2; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4 * SIDES), mbar_init(o_done(b), 1);
+        for (int s = 0; s < RS; ++s) mbar_init(full(s), Q8 ? M::kWidenWarps : 1), mbar_init(empty(s), 1);
+        for (int s = 0; s < M::kRaws; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), M::kWidenWarps);
+        for (int b = 0; b < NB; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4 * SIDES), mbar_init(o_done(b), 1);
         mbar_init(q_full, M::kSoftWarps);
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -230,52 +239,61 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             }
             for (int back = max(0, n - kRing); back < n; ++back) mbar_wait(Q8 ? raw_full(back % kRing) : full(back % kRing), (back / kRing) & 1, abort_flag, a.spin_limit, false);
         } else if (warp == M::kMmaWarp) {
-            // ---- one thread issues all products ----
-            if (lane == 0) {
-                constexpr uint32_t kScores = instr_desc_16(M::BF, false, KT), kValues = instr_desc_16(M::BF, true, HD);
-                bool okay = units == 0 || mbar_wait(q_full, 0, abort_flag, a.spin_limit);
+            // ---- all products: one thread issues them, but the warp stays together, so that descriptors live in uniform registers (issued by a lane on its own, eight products took as long to issue
+            // as sixteen to run) ----
+            constexpr uint32_t kScores = instr_desc_16(M::BF, false, KT), kValues = instr_desc_16(M::BF, true, HD);
+            // descriptors: the upper word does not change
+            const uint64_t k_desc = smem_desc(0, 16, 1024, 2), v_desc = smem_desc(0, KT * 128, 1024, 2);
+            auto at = [](uint64_t desc, uint32_t addr) { return desc | static_cast<uint64_t>((addr & 0x3FFFFu) >> 4); };
+            bool okay = units == 0 || __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, a.spin_limit));
+            fence_after();
+            int have = 0;  // operand tiles waited for: tile n of the sequence keys 0, values 0, keys 1, ...
+            auto need = [&](int n) {
+                for (; okay && have <= n; ++have) okay = __all_sync(0xffffffffu, mbar_wait(full(have % RS), (have / RS) & 1, abort_flag, a.spin_limit));
                 fence_after();
-                int have = 0;  // operand tiles waited for: tile n of the sequence keys 0, values 0, keys 1, ...
-                auto need = [&](int n) {
-                    for (; okay && have <= n; ++have) okay = mbar_wait(full(have % RS), (have / RS) & 1, abort_flag, a.spin_limit);
-                    fence_after();
-                    return okay;
-                };
-                auto scores = [&](int u) {  // S of unit u; the keys are given back behind the last unit that reads them
-                    const int j = u / NT, i = u % NT, b = u & 1;
-                    if (!need(2 * j)) return;
-                    const uint32_t keys = slots + (2 * j % RS) * M::kSlot, d = tmem + M::kSCol + b * KT;
+                return okay;
+            };
+            auto scores = [&](int u) {  // S of unit u; the keys are given back behind the last unit that reads them
+                const int j = u / NT, i = u % NT, b = u % NB;
+                if (!need(2 * j)) return;
+                const uint32_t d = tmem + M::kSCol + b * KT;
+                const uint64_t keys = at(k_desc, slots + (2 * j % RS) * M::kSlot), queries = at(k_desc, q_at + i * BLOCKS * 128 * 128);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const uint64_t kd = smem_desc(keys + (k >> 2) * KT * 128, 16, 1024, 2) + 2 * (k & 3);
+                        const uint64_t kd = keys + ((k >> 2) * KT * 128 >> 4) + 2 * (k & 3);
                         if constexpr (M::kQTmem) mma_ts(d, tmem + M::kQCol + k * 8, kd, kScores, k > 0);
-                        else mma_ss(d, smem_desc(q_at + (i * BLOCKS + (k >> 2)) * 128 * 128, 16, 1024, 2) + 2 * (k & 3), kd, kScores, k > 0);
+                        else mma_ss(d, queries + ((k >> 2) * 128 * 128 >> 4) + 2 * (k & 3), kd, kScores, k > 0);
                     }
                     mma_commit(s_full(b));
                     if (i == NT - 1) mma_commit(empty(2 * j % RS));
-                };
-                if (units > 0) scores(0);
-                if (okay && units > 1) scores(1);
-                for (int u = 0; u < units && okay; ++u) {
-                    const int j = u / NT, i = u % NT, b = u & 1;
-                    if (!need(2 * j + 1) || !(okay = mbar_wait(p_full(b), (u >> 1) & 1, abort_flag, a.spin_limit))) break;
-                    fence_after();
-                    const uint32_t values = slots + ((2 * j + 1) % RS) * M::kSlot;
+                }
+                __syncwarp();
+            };
+            for (int u = 0; u < NB && u < units && okay; ++u) scores(u);
+            for (int u = 0; u < units && okay; ++u) {
+                const int j = u / NT, i = u % NT, b = u % NB;
+                if (!need(2 * j + 1) || !(okay = __all_sync(0xffffffffu, mbar_wait(p_full(b), (u / NB) & 1, abort_flag, a.spin_limit)))) break;
+                fence_after();
+                const uint64_t values = at(v_desc, slots + ((2 * j + 1) % RS) * M::kSlot);
+                const uint32_t first = j > 0;
+                if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < KT / 16; ++k)
-                        mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, smem_desc(values + k * 16 * 128, KT * 128, 1024, 2), kValues, j > 0 || k > 0);
+                    for (int k = 0; k < KT / 16; ++k) mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, values + (k * 16 * 128 >> 4), kValues, k > 0 ? 1u : first);
                     mma_commit(o_done(b));
                     if (i == NT - 1) mma_commit(empty((2 * j + 1) % RS));
-                    if (u + 2 < units) scores(u + 2);
                 }
-                mma_commit(drained);  // nothing is under way when the block leaves
-                mbar_wait(drained, 0, abort_flag, a.spin_limit, false);
+                __syncwarp();
+                if (u + NB < units) scores(u + NB);
             }
+            if (elect_one()) mma_commit(drained);  // nothing is under way when the block leaves
             __syncwarp();
+            mbar_wait(drained, 0, abort_flag, a.spin_limit, false);
         } else if (Q8 && warp >= M::kWidenWarp) {
             // ---- codes to F16 operands ----
             if constexpr (Q8) {
                 const int w = tid - M::kWidenWarp * 32;
+                const float scale = fmaxf(fabsf(a.scale), 1e-37f);
                 bool okay = true;
                 for (int n = 0; n < 2 * tiles && okay; ++n) {
                     const int j = n >> 1, value = n & 1, rs = n % RW, s = n % RS, left = range.end - (range.begin + j * KT);  // rows of the tile that are there
@@ -286,20 +304,30 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                     if (!value && w < KT) {
                         const float* d = reinterpret_cast<const float*>(raw_smem + rs * M::kRawStride + M::kRaw) + w;
                         float* f = factors + (j & 3) * 3 * KT + w;
-                        f[0] = w < left ? d[0] : 0.0f, f[KT] = w < left ? lg2(d[KT]) : 0.0f, f[2 * KT] = w < left ? rcp(d[KT]) : 0.0f;
+                        f[0] = w < left ? d[0] * scale : 0.0f, f[KT] = w < left ? lg2(d[KT]) : 0.0f, f[2 * KT] = w < left ? rcp(d[KT]) : 0.0f;
                     }
-#pragma unroll 4
-                    for (int i = w; i < KT * BLOCKS * 4; i += 128) {  // a piece of sixteen codes
-                        const int row = i >> 2, r = row % KT, c = (i & 3) ^ ((r >> 1) & 3);
-                        uint32_t v[4], o[8];
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(from + i * 16) : "memory");
+                    constexpr int kPieces = KT * BLOCKS * 4 / (M::kWidenWarps * 32), kAtOnce = kPieces > 4 ? 4 : kPieces;  // pieces of sixteen codes of a thread, and those under way together
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t u = r < left ? v[e] ^ 0x80808080u : 0x80808080u;
-                            o[2 * e] = codes_to_half2(u, 0x4140), o[2 * e + 1] = codes_to_half2(u, 0x4342);
+                    for (int k0 = 0; k0 < kPieces; k0 += kAtOnce) {
+                        uint32_t v[kAtOnce][4];
+#pragma unroll
+                        for (int k = 0; k < kAtOnce; ++k)
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v[k][0]), "=r"(v[k][1]), "=r"(v[k][2]), "=r"(v[k][3])
+                                         : "r"(from + (w + (k0 + k) * M::kWidenWarps * 32) * 16)
+                                         : "memory");
+#pragma unroll
+                        for (int k = 0; k < kAtOnce; ++k) {
+                            const int i = w + (k0 + k) * M::kWidenWarps * 32, row = i >> 2, r = row % KT, c = (i & 3) ^ ((r >> 1) & 3);
+                            uint32_t o[8];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t u = r < left ? v[k][e] ^ 0x80808080u : 0x80808080u;
+                                o[2 * e] = codes_to_half2(u, 0x4140), o[2 * e + 1] = codes_to_half2(u, 0x4342);
+                            }
+                            *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                         }
-                        *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<uint4*>(to + row * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                     }
                     fence_async_shared();
                     __syncwarp();
@@ -310,7 +338,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
     } else {
         if constexpr (M::kSplitRegs) registers_up<M::kSoftRegs>();
         // ---- a row of queries for a thread, or for two, which have half of a tile's positions each: warps w and w + 4 ----
-        const int i = SIDES == 2 ? 0 : warp >> 2, side = SIDES == 2 ? warp >> 2 : 0, local = (warp & 3) * 32 + lane, r = r0 + i * 128 + local, t = r / a.group, h = kvh * a.group + r % a.group;
+        const int i = SIDES == 2 ? 0 : warp >> 2, side = SIDES == 2 ? warp >> 2 : 0, local = (warp & 3) * 32 + lane, r = r0 + i * 128 + local, t = r / a.group;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const bool live = r < r1;
         constexpr int KH = KT / SIDES, HH = HD / SIDES;
@@ -325,59 +353,127 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
             asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(x ? 1u : 0u), "r"(meet) : "memory");
             return any != 0;
         };
-        float rowf;  // what the row's scores are multiplied by: positive, the queries take the sign
-        {
-            const unsigned char* src = static_cast<const unsigned char*>(a.q) + ((static_cast<size_t>(sq.first) + (live ? t : 0)) * a.q_token + (live ? h : kvh * a.group) * a.q_head) * paged_size_of(a.q_type);
-            float f = a.scale < 0.0f ? -1.0f : 1.0f;
-            rowf = fmaxf(fabsf(a.scale), 1e-37f);  // (times minus infinity, where a mask hides a score, it stays that)
-            if constexpr (Q8) {
-                float m = 0.0f;
-#pragma unroll 4
-                for (int e = 0; e < HD; e += 8) {
-                    float x[8];
-                    paged_load8(src + e * paged_size_of(a.q_type), a.q_type, x);
+        unsigned char* stage = staging + warp * 32 * M::kStagePitch;
+        {   // queries: lanes side by side along a row
+            constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;  // 16-byte pieces of a row; rows at once
+            const int wr = r0 + i * 128 + (warp & 3) * 32, sub = lane / kLanes, e = lane % kLanes * 8;  // the warp's first row
+            const float sign = a.scale < 0.0f ? -1.0f : 1.0f, scale = fmaxf(fabsf(a.scale), 1e-37f);  // (times minus infinity, where a mask hides a score, it stays that)
+            // the byte offset of the warp's row `lane`; the last row's where there are no more
+            const int own = min(wr + lane, r1 - 1);
+            const size_t own_at = ((static_cast<size_t>(sq.first) + own / a.group) * a.q_token + (kvh * a.group + own % a.group) * a.q_head) * paged_size_of(a.q_type);
+            auto load = [&](auto of) {  // by the queries' type, so that the loads of a batch of rows are under way together
+                constexpr int T = decltype(of)::value;
+                auto fetch = [&](int row, int e) { return paged_raw<T>(static_cast<const unsigned char*>(a.q) + __shfl_sync(0xffffffffu, own_at, row), e); };
+                auto power = [&](const float (&x)[8]) {  // of the row's maximum, as the bits of a power of two; 1 for zeros, denormals and what is not finite
+                    float top = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
-                }
-                const uint32_t ex = __float_as_uint(m) >> 23;
-                if (ex > 1 && ex < 254) rowf *= __uint_as_float(ex << 23), f *= __uint_as_float((254 - ex) << 23);
-            }
+                    for (int c = 0; c < 8; ++c) top = fmaxf(top, fabsf(x[c]));
+#pragma unroll
+                    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    const uint32_t ex = __float_as_uint(top) >> 23;
+                    return (T != kPagedF16 && ex > 1 && ex < 254 ? ex : 127u) << 23;  // (F16 queries go in as they are)
+                };
+                if constexpr (!M::kQTmem) {
+                    constexpr int kBatch = T == kPagedF32 ? 4 : 8;
 #pragma unroll 1
-            for (int e = side * HH; e < (side + 1) * HH; e += 32) {
-                uint32_t v[16];
+                    for (int k0 = 0; k0 < 32; k0 += kBatch * kAtOnce) {
+                        PagedRaw<T> raw[kBatch];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    float x[8];
-                    paged_load8(src + (e + k * 8) * paged_size_of(a.q_type), a.q_type, x);
+                        for (int k = 0; k < kBatch; ++k) raw[k] = fetch(k0 + k * kAtOnce + sub, e);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) v[k * 4 + c] = live ? paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x[2 * c] * f, x[2 * c + 1] * f) : 0u;
-                }
-                if constexpr (M::kQTmem) {
-                    tmem_store16(tmem + lanes + M::kQCol + e / 2, v);
+                        for (int k = 0; k < kBatch; ++k) {
+                            const int mine = k0 + k * kAtOnce + sub, row = (warp & 3) * 32 + mine;
+                            float x[8], f = sign, factor = Q8 ? 1.0f : scale;
+                            paged_load8(raw[k].v, T, x);
+                            if constexpr (Q8) {
+                                const uint32_t bits = power(x);
+                                factor *= __uint_as_float(bits), f *= __uint_as_float((254u << 23) - bits);  // (the reciprocal of a power of two)
+                            }
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) x[c] = wr + mine < r1 ? x[c] * f : 0.0f;
+                            paged_store8(smem + ((i * BLOCKS + e / 64) * 128 + row) * 128 + (((e / 8 & 7) ^ (row & 7)) << 4), M::BF ? kPagedBf16 : kPagedF16, x);
+                            if (lane % kLanes == 0) row_factor[i * 128 + row] = factor;
+                        }
+                    }
+                    fence_async_shared();
                 } else {
+                    if constexpr (Q8) {  // both warps of a row look at all of it
+                        constexpr int kBatch = T == kPagedF32 ? 4 : 8;
+#pragma unroll 1
+                        for (int k0 = 0; k0 < 32 && wr + k0 < r1; k0 += kBatch * kAtOnce) {
+                            PagedRaw<T> raw[kBatch];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        *reinterpret_cast<uint4*>(smem + ((i * BLOCKS + e / 64) * 128 + local) * 128 + ((((e & 32) / 8 + k) ^ (local & 7)) << 4)) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                            for (int k = 0; k < kBatch; ++k) raw[k] = fetch(min(k0 + k * kAtOnce + sub, 31), e);
+#pragma unroll
+                            for (int k = 0; k < kBatch; ++k) {
+                                float x[8];
+                                paged_load8(raw[k].v, T, x);
+                                const uint32_t bits = power(x);
+                                if (lane % kLanes == 0 && k0 + k * kAtOnce + sub < 32) reinterpret_cast<uint32_t*>(stage + (k0 + k * kAtOnce + sub) * M::kStagePitch)[32] = bits;  // behind the row's 128 bytes
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    constexpr int kPart = HH < 64 ? HH : 64, kPartLanes = kPart / 8, kRowsAtOnce = 32 / kPartLanes;  // values of a row that fit the staging's row
+#pragma unroll 1
+                    for (int c0 = side * HH; c0 < (side + 1) * HH; c0 += kPart) {
+                        PagedRaw<T> raw[kPartLanes];
+#pragma unroll
+                        for (int k = 0; k < kPartLanes; ++k) raw[k] = fetch(k * kRowsAtOnce + lane / kPartLanes, c0 + lane % kPartLanes * 8);
+#pragma unroll
+                        for (int k = 0; k < kPartLanes; ++k) {
+                            const int row = k * kRowsAtOnce + lane / kPartLanes;
+                            float x[8], f = sign;
+                            paged_load8(raw[k].v, T, x);
+                            if constexpr (Q8) f *= __uint_as_float((254u << 23) - reinterpret_cast<const uint32_t*>(stage + row * M::kStagePitch)[32]);
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) x[c] = wr + row < r1 ? x[c] * f : 0.0f;
+                            paged_store8(stage + row * M::kStagePitch + lane % kPartLanes * 16, M::BF ? kPagedBf16 : kPagedF16, x);
+                        }
+                        __syncwarp();
+                        uint32_t v[kPart / 2];
+#pragma unroll
+                        for (int k = 0; k < kPart / 8; ++k) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(stage + lane * M::kStagePitch + k * 16);
+                            v[4 * k] = w.x, v[4 * k + 1] = w.y, v[4 * k + 2] = w.z, v[4 * k + 3] = w.w;
+                        }
+                        if constexpr (kPart == 64) tmem_store32(tmem + lanes + M::kQCol + c0 / 2, v);
+                        else tmem_store16(tmem + lanes + M::kQCol + c0 / 2, v);
+                        __syncwarp();
+                    }
+                    if (side == 0) row_factor[local] = Q8 ? __uint_as_float(reinterpret_cast<const uint32_t*>(stage + lane * M::kStagePitch)[32]) : scale;
+                    tmem_wait_store();
                 }
-            }
-            if constexpr (M::kQTmem) tmem_wait_store();
-            else fence_async_shared();
+            };
+            if constexpr (TYPE != kPagedQ8) load(PagedTag<TYPE>());
+            else if (a.q_type == kPagedF16) load(PagedTag<kPagedF16>());
+            else if (a.q_type == kPagedBf16) load(PagedTag<kPagedBf16>());
+            else load(PagedTag<kPagedF32>());
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
+            if constexpr (SIDES == 2) meet_sync();
         }
+        const float rowf = row_factor[i * 128 + local];  // what the row's scores are multiplied by: positive, the queries took the sign
         const int p = p0 + t, last = live ? min(p, range.end - 1) : -1, first = a.window > 0 ? max(0, p - a.window + 1) : 0;
+        const bool some = r0 + i * 128 + (warp & 3) * 32 < r1;  // the same for the two warps that meet
         float m = -INFINITY, l = 0.0f;  // l: over this thread's positions
         bool okay = true;
-        // The value products of unit u. A wait tells phases apart by their parity alone, so each buffer has a barrier: those of unit u - 2, the phase before, are done, as the scores
-        // of unit u (asked for behind them) were waited for, and those of unit u + 2 cannot have begun.
-        auto values_done = [&](int u) { return __all_sync(0xffffffffu, mbar_wait(o_done(u & 1), (u >> 1) & 1, abort_flag, a.spin_limit)); };
+        // The value products of unit u. A wait tells phases apart by their parity alone, so each buffer has a barrier: those of unit u - NB, the phase before, are done, as the scores
+        // of unit u (asked for behind them) were waited for, and those of unit u + NB cannot have begun.
+        auto values_done = [&](int u) { return __all_sync(0xffffffffu, mbar_wait(o_done(u % NB), (u / NB) & 1, abort_flag, a.spin_limit)); };
 #pragma unroll 1
         for (int j = 0; j < tiles; ++j) {
-            const int u = j * NT + i, b = u & 1, k0 = range.begin + j * KT + side * KH;
+            const int u = j * NT + i, b = u % NB, k0 = range.begin + j * KT + side * KH;
             const uint32_t s_at = tmem + lanes + M::kSCol + b * KT;
-            if (okay) okay = __all_sync(0xffffffffu, mbar_wait(s_full(b), (u >> 1) & 1, abort_flag, a.spin_limit));
+            if (okay) okay = __all_sync(0xffffffffu, mbar_wait(s_full(b), (u / NB) & 1, abort_flag, a.spin_limit));
             fence_after();
+            if constexpr (SIDES == 2) {
+                if (!some) {  // a warp without rows of its own (they are the last ones: a few rows are in the first warp): its weights multiply nothing that is read
+                    if (lane == 0 && okay) mbar_arrive(p_full(b));
+                    continue;
+                }
+            }
             uint32_t s[KH / 32][32];
 #pragma unroll
             for (int c = 0; c < KH / 32; ++c) tmem_load32(s_at + side * KH + c * 32, s[c]);
@@ -401,6 +497,15 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
                         x = a.cap * tanh_of(x * rowf);
                         if constexpr (Q8) x += reinterpret_cast<const float*>(f)[KT + c * 32 + e];
                         s[c][e] = __float_as_uint(x);
+                    }
+            } else if (Q8 && a.q_type == kPagedF16) {  // every row's factor is 1
+#pragma unroll
+                for (int c = 0; c < KH / 32; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 ks = f[(c * 32 + e) / 4], lv = f[(KT + c * 32 + e) / 4];
+                        put(c, e, fma_f32x2(pair(c, e), pack_f32x2(ks.x, ks.y), pack_f32x2(lv.x, lv.y)));
+                        put(c, e + 2, fma_f32x2(pair(c, e + 2), pack_f32x2(ks.z, ks.w), pack_f32x2(lv.z, lv.w)));
                     }
             } else if constexpr (Q8) {
 #pragma unroll
@@ -495,35 +600,42 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
         if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
         if (okay) {
             fence_after();
-            const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-            const size_t token = static_cast<size_t>(sq.first) + t, row = paged_part_row(a, g, sq, part, which, kvh, r, i * 128 + local, M::kRows);
+            const float inv = part.ranges > 1 ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+            const int wr = r0 + i * 128 + (warp & 3) * 32;  // the warp's first row
+            const size_t row = paged_part_row(a, g, sq, part, which, kvh, r, i * 128 + local, M::kRows);
+            if (tiles > 0 || part.ranges == 1) {  // (of a range in which the rows see nothing only the sums below are read)
 #pragma unroll 1
-            for (int c = side * HH; c < (side + 1) * HH; c += 32) {
-                if (tiles == 0 && part.ranges > 1) break;
-                uint32_t o[32];
-                if (tiles > 0) {
-                    tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
-                    tmem_wait_load();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0u;
-                }
-                if (!live) continue;
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    float x[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(o[e + k]);
-                    if (part.ranges == 1) {
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) x[k] *= inv;
-                        paged_store8(static_cast<unsigned char*>(a.out) + (token * a.o_token + h * a.o_head + c + e) * paged_size_of(a.out_type), a.out_type, x);
+                for (int c = side * HH; c < (side + 1) * HH; c += 32) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_load32(tmem + lanes + M::kOCol + i * 128 + c, o);
+                        tmem_wait_load();
                     } else {
-                        paged_store8(g.part_o + row * HD + c + e, kPagedF32, x);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4*>(stage + lane * M::kStagePitch + e * 4) =
+                            make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 8) {  // four lanes a row
+                        const int rr = k + (lane >> 2), e = (lane & 3) * 8;
+                        if (wr + rr >= r1) continue;
+                        float x[8];
+                        paged_load8(stage + rr * M::kStagePitch + e * 4, kPagedF32, x);
+                        if (part.ranges == 1) {
+                            const size_t token = static_cast<size_t>(sq.first) + (wr + rr) / a.group;
+                            paged_store8(static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + (wr + rr) % a.group) * a.o_head + c + e) * paged_size_of(a.out_type), a.out_type, x);
+                        } else {
+                            paged_store8(g.part_o + (row - lane + rr) * HD + c + e, kPagedF32, x);
+                        }
                     }
                 }
             }
-            if (live && part.ranges > 1 && side == 0) g.part_ml[row] = make_float2(m, l);  // (of a range in which the row sees nothing this is all that is read)
+            if (live && part.ranges > 1 && side == 0) g.part_ml[row] = make_float2(m, l);
         }
     }
     fence_before();
@@ -536,9 +648,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS>::kThreads, 1) paged_ma
 
 // Joins the ranges of the row blocks that were cut: a warp per row, in the order of the ranges. Grid (rows / 8, m, row blocks that were cut, mapped: all of them).
 template <int BLOCKS>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g, int kRows) {
     using namespace paged_detail;
-    constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32, kRows = BLOCKS == 4 ? 128 : 256;
+    constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
     const int lane = threadIdx.x & 31, local = blockIdx.x * 8 + (threadIdx.x >> 5), which = blockIdx.y, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
     int x = 0, order = blockIdx.z, ranges = g.cut;
     if (g.mapped) {

@@ -111,4 +111,15 @@ __device__ __forceinline__ void paged_store8(void* p, int type, const float (&x)
 }
 __host__ __device__ constexpr int paged_size_of(int type) { return type == kPagedF32 ? 4 : type == kPagedQ8 ? 1 : 2; }
 
+// Eight values of a head as they lie in memory, and as 32-bit values.
+template <int TYPE> struct PagedRaw { uint4 v[TYPE == kPagedF32 ? 2 : 1]; };
+template <int TYPE>
+__device__ __forceinline__ PagedRaw<TYPE> paged_raw(const void* base, size_t element) {
+    PagedRaw<TYPE> r;
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + element * paged_size_of(TYPE));
+    r.v[0] = *p;
+    if constexpr (TYPE == kPagedF32) r.v[1] = p[1];
+    return r;
+}
+
 }  // namespace qtb

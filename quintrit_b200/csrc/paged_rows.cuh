@@ -57,17 +57,6 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedView& c, const Rows
     return p;
 }
 
-// Eight values of a head as they lie in memory, and as 32-bit values.
-template <int TYPE> struct PagedRaw { uint4 v[TYPE == kPagedF32 ? 2 : 1]; };
-template <int TYPE>
-__device__ __forceinline__ PagedRaw<TYPE> paged_raw(const void* base, size_t element) {
-    PagedRaw<TYPE> r;
-    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + element * paged_size_of(TYPE));
-    r.v[0] = *p;
-    if constexpr (TYPE == kPagedF32) r.v[1] = p[1];
-    return r;
-}
-
 template <int LANES, int TYPE, int U>  // threads of a head: head_dim / 8; type of q, k and v; groups of heads of a warp
 __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
     constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a group: all of them queries, keys or values
