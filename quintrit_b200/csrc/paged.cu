@@ -99,24 +99,14 @@ int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void
     return QUINTRIT_OK;
 }
 
-// How the kernel for few rows cuts the positions into ranges: blocks of threads come in waves of `places`, each as long as its tiles and a start and an end of about five more; ranges cost another
-// launch. (Sequences are taken to be as long as announced: shorter ones leave blocks without work, which end at once.)
-struct PagedCut {
-    int splits, split;
-};
-PagedCut cut_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_tiles, int places, int limit) {
-    constexpr double kStart = 5.0, kJoin = 4.0;
+// Whether the kernel for few rows shares its tiles out, and among how many blocks: all that the device holds, as long as each gets four tiles or so; sequences of a few tiles each, or very many
+// sequences, go one item to a block. (By the longest sequence: shorter ones leave the blocks less.)
+int few_blocks(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_blocks, int places) {
     long long span = std::max<uint32_t>(r->max_length, 1);
     if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
-    const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_tiles;
-    long long best = 1;
-    double least = 1e30;
-    for (long long s = 1; s <= limit && s <= std::max<long long>(1, tiles / 2); ++s) {
-        const double cost = static_cast<double>((items * s + places - 1) / places) * (static_cast<double>((tiles + s - 1) / s) + kStart) + (s > 1 ? kJoin : 0.0);
-        if (cost < least * 0.98) best = s, least = cost;
-    }
-    const long long per = (tiles + best - 1) / best;
-    return PagedCut{static_cast<int>((tiles + per - 1) / per), static_cast<int>(per * kPagedTile)};
+    const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_blocks, all = tiles * items;
+    if (r->sequences > kPagedShared || tiles < 6 || all > 0x7fffffffLL || items > 8LL * places) return 0;
+    return static_cast<int>(std::min<long long>(places, std::max<long long>(all / 4, 1)));
 }
 
 // The shared memory a kernel may ask for, raised once per device (`done`: a bit per device; two threads at once set the same).
@@ -193,6 +183,7 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
         int x = 0;
         for (long long o = 0; o < blocks; ++o) {
             const int ranges = static_cast<int>((tiles_of(o) + best - 1) / best);
+            g->at[o] = static_cast<unsigned char>(x);
             for (int i = 0; i < ranges; ++i, ++x) g->order[x] = static_cast<unsigned char>(o), g->range[x] = static_cast<unsigned char>(i), g->ranges[x] = static_cast<unsigned char>(ranges);
         }
         g->mapped = x, g->whole = 0;
@@ -234,9 +225,9 @@ int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device,
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
     bool many;
-    int nt;                  // few: tiles of 8 rows of a block, blocks per head, ranges
+    int nt;                  // few: tiles of 8 rows of a block, blocks of rows of the longest chunk, blocks that the tiles are shared out among (0: an item a block)
     long long few_tiles;
-    PagedCut few_cut;
+    int few_share;
     PagedSchedule schedule;  // many: which blocks, their number, slots of the workspace
     int many_rows;           // rows of a block of threads
     long long many_blocks;
@@ -248,17 +239,16 @@ constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {
     const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = few_limit();
     p->many = most > limit;
-    p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(limit / group, r->max_new - 1));  // (a sequence alone is the longest)
-    p->few_tiles = 0, p->few_cut = PagedCut{1, kPagedTile}, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
+    p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(std::max<long long>(8 / group, group <= 32 ? 1 : 0), r->max_new - 1));  // (a sequence alone is the longest)
+    p->few_tiles = 0, p->few_share = 0, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
     const size_t row_bytes = c->head_dim * sizeof(float) + sizeof(float2);
     if (p->few_new > 0) {
         const long long rows = p->few_new * group;
         p->nt = row_tiles_of(c, rows);
         p->few_tiles = (rows + 8 * p->nt - 1) / (8 * p->nt);
-        const int places = places_of(c, p->nt);
-        p->few_cut = cut_of(c, r, 0, p->few_tiles, places, 128);
-        if (window > 0) p->few_cut = cut_of(c, r, window, p->few_tiles, places, p->few_cut.splits);  // (no window takes more of the workspace than none)
-        if (p->few_cut.splits > 1) p->few_bytes = up16(p->few_cut.splits * static_cast<size_t>(r->tokens) * q_heads * row_bytes);
+        const int places = places_of(c, p->nt), share = few_blocks(c, r, 0, p->few_tiles, places);
+        p->few_share = window > 0 ? std::min(share, few_blocks(c, r, window, p->few_tiles, places)) : share;  // (no window takes more of the workspace than none)
+        p->few_bytes = up16(static_cast<size_t>(share) * 2 * 8 * p->nt * row_bytes);
     }
     if (p->many) {
         const int rows = c->head_dim == 256 || most <= 128 ? 128 : 256;
@@ -474,7 +464,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         const int group = static_cast<int>(args->q_heads / cache->kv_heads);
         PagedPlan plan;
         plan_of(cache, rows, args->q_heads, args->window, &plan);
-        if (plan.few_tiles * cache->kv_heads > 65535 || plan.many_blocks > 0x7fffffffLL)
+        if (plan.few_tiles > 65535 || plan.many_blocks > 0x7fffffffLL || static_cast<long long>(rows->tokens) * args->q_heads > 0x7fffffffLL)
             return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
         const size_t need = plan.few_bytes + plan.many_bytes;
         if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);
@@ -510,20 +500,22 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             }
         }
         if (plan.few_new > 0) {
-            a.few = 1, a.many = plan.few_new, a.splits = plan.few_cut.splits, a.split = plan.few_cut.split;
+            a.few = 1, a.many = plan.few_new, a.share = plan.few_share;
+            const int block_rows = 8 * plan.nt;
             a.part_o = reinterpret_cast<float*>(workspace);
-            a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(a.splits) * rows->tokens * args->q_heads * cache->head_dim);
-            const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(cache->kv_heads * plan.few_tiles), rows->sequences);
+            a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(plan.few_share) * 2 * block_rows * cache->head_dim);
+            const dim3 grid = plan.few_share > 0 ? dim3(static_cast<unsigned>(plan.few_share)) : dim3(static_cast<unsigned>(plan.few_tiles), cache->kv_heads, rows->sequences);
             rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.nt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.nt, grid, s)
                                                                                                                                 : launch_few_type<kPagedQ8>(a, device, plan.nt, grid, s);
             if (rc != QUINTRIT_OK) return rc;
-            if (a.splits > 1) {
-                const unsigned items = static_cast<unsigned>(rows->tokens) * args->q_heads;  // (below 2^31: a workspace of that many results was asked for)
-                const bool wide = a.splits > 8;
-                auto kernel = a.c.blocks == 1 ? (wide ? paged_combine_kernel<1, 8> : paged_combine_kernel<1, 1>) : a.c.blocks == 2 ? (wide ? paged_combine_kernel<2, 8> : paged_combine_kernel<2, 1>)
-                                                                                                                                 : (wide ? paged_combine_kernel<4, 8> : paged_combine_kernel<4, 1>);
-                kernel<<<items, wide ? 256 : 32, 0, s>>>(a);
-                QTB_LAUNCH_CHECK();
+            if (plan.few_share > 0) {
+                auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
+                cudaLaunchConfig_t cfg{};
+                cudaLaunchAttribute dependent{};
+                dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization, dependent.val.programmaticStreamSerializationAllowed = 1;
+                cfg.gridDim = dim3(rows->tokens * args->q_heads), cfg.blockDim = dim3(256), cfg.stream = s, cfg.attrs = &dependent, cfg.numAttrs = 1;
+                QTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.few_share, block_rows));
+                ++g_launches;
             }
         }
         return ok();

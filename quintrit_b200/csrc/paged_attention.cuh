@@ -15,8 +15,8 @@
 // two groups of four warps take the tiles in turn, a warp 16 positions of a tile against all rows. Matrix instructions (m16n8k16) with the positions, and then the values, as the
 // 16 rows of the left operand and the queries as the 8 columns of the right one: S^T = K Q^T and O^T += V^T P^T, so that one query head or eight cost the same, a fragment of codes is
 // widened once for all rows, and the sums of eight rows take head_dim / 4 registers. A score's row is the same in both products' registers; only the weights are transposed (movmatrix).
-// Every warp has its own m, l and sums; at the end the eight warps join. Long sequences are cut into ranges for several blocks, whose results meet in the caller's workspace
-// (paged_combine_kernel), in the order of the ranges: no atomics.
+// Every warp has its own m, l and sums; at the end the eight warps join. Where that pays, the tiles of all sequences are shared out evenly among as many blocks as the
+// device holds (PagedShare), whatever their lengths; results of cut items meet in the caller's workspace (paged_combine_kernel), in the order of the positions: no atomics.
 #pragma once
 #include "paged_cache.cuh"
 #include "tcgen05.cuh"
@@ -39,9 +39,9 @@ struct PagedAttnArgs {
     float scale;             // times log2(e); with a cap: scale / cap
     float cap;               // times log2(e); 0: none
     int window;              // 0: none
-    int splits, split;       // ranges of positions per sequence, positions of a range (a multiple of the tile)
-    float* part_o;           // [splits][tokens][q heads][head_dim], when splits > 1
-    float2* part_ml;         // [splits][tokens][q heads]
+    int share;               // 0: a block of threads takes a whole item; else the items' tiles are shared out evenly among the blocks (PagedShare)
+    float* part_o;           // [blocks][2][rows of a block][head_dim], where the tiles are shared out
+    float2* part_ml;         // [blocks][2][rows of a block]
     int few, many;           // new tokens of the sequences that this launch serves: few <= n <= many
     int most;                // new tokens of the longest chunk as announced: the grid has no rows for more
     unsigned int spin_limit;
@@ -99,26 +99,74 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased, uint32_t sel
 
 }  // namespace paged_detail
 
-// The range of positions that rows of tokens [t0, t1) of a sequence can see, cut to the range of split `i`; begin is a multiple of the tile.
 struct PagedRange {
     int begin, end;
 };
-__device__ __forceinline__ PagedRange paged_range(const PagedAttnArgs& a, const PagedSequence& q, int t0, int t1, int split) {
-    // The cuts count from the first position that any new token of the sequence sees, so that all row tiles of a sequence agree on them.
-    const int p0 = q.length - q.news, low_all = a.window > 0 ? max(0, p0 - a.window + 1) & ~(kPagedTile - 1) : 0;
-    const int low = a.window > 0 ? max(0, p0 + t0 - a.window + 1) & ~(kPagedTile - 1) : 0;
-    PagedRange g;
-    // (64 bits: a range may be as long as 2^31 positions)
-    const long long cut = low_all + static_cast<long long>(split) * a.split;
-    g.begin = static_cast<int>(max(static_cast<long long>(low), min(cut, static_cast<long long>(q.length))));
-    g.end = split + 1 < a.splits ? static_cast<int>(min(static_cast<long long>(q.length), cut + a.split)) : q.length;
-    g.end = min(g.end, max(0, p0 + t1));
-    return g;
+// The positions that any new token of a sequence sees; begin is a multiple of 64.
+__device__ __forceinline__ PagedRange paged_seen(const PagedAttnArgs& a, const PagedSequence& q) {
+    return PagedRange{a.window > 0 ? max(0, q.length - q.news - a.window + 1) & ~(kPagedTile - 1) : 0, q.length};
 }
-// Ranges of the sequence that hold anything.
-__device__ __forceinline__ int paged_splits_used(const PagedAttnArgs& a, const PagedSequence& q) {
-    const int p0 = q.length - q.news, low_all = a.window > 0 ? max(0, p0 - a.window + 1) & ~(kPagedTile - 1) : 0;
-    return max(1, min(a.splits, static_cast<int>((static_cast<long long>(q.length) - low_all + a.split - 1) / a.split)));
+
+// Work shared out: the items (a sequence's KV head and block of rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles; block b of G takes the tiles
+// [b W / G, (b + 1) W / G) of all W, whatever the lengths are. What a block has of an item is a segment: a whole item's result is written as it is, others go to the workspace, at most two of a block:
+// place 0 for the segment that its tiles begin with, place 1 for another. Every block works the items' places out for itself from the lengths (paged_share_begin), for up to kPagedShared sequences.
+constexpr int kPagedShared = 256;
+struct PagedShare {
+    long long total;
+    int* before;  // [sequences + 1] in shared memory: tiles of the items before a sequence's
+    int4* of;     // [sequences]: first token, new tokens, length, tiles of an item
+};
+struct PagedItem {
+    int seq, kvh, rows0;        // rows0: the block of rows' first
+    long long begin;            // the item's first tile among all
+    int tiles;
+    PagedSequence q;
+};
+// Tiles and items of a sequence.
+__device__ __forceinline__ void paged_weight(const PagedAttnArgs& a, const PagedSequence& q, int block_rows, int* tiles, int* items) {
+    const PagedRange g = paged_seen(a, q);
+    const bool mine = q.ok && q.news >= a.few && q.news <= a.many;
+    *tiles = max(1, (g.end - g.begin + kPagedTile - 1) / kPagedTile), *items = mine ? a.c.kv_heads * ((q.news * a.group + block_rows - 1) / block_rows) : 0;
+}
+// By all threads of a block; `before` and `of` have room for kPagedShared + 1 and kPagedShared. (32 bits hold the tiles: at most 2^16 items of 2^15 tiles, or a longer sequence alone.)
+__device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, int block_rows, int* before, int4* of, int threads) {
+    for (int s = threadIdx.x; s < a.r.sequences; s += threads) {
+        int tiles, items;
+        const PagedSequence q = paged_sequence(a.c, a.r, s);
+        paged_weight(a, q, block_rows, &tiles, &items);
+        before[s + 1] = tiles * items;
+        of[s] = make_int4(q.first, q.news, q.length, tiles);
+        if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
+    }
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int s0 = 0; s0 < a.r.sequences; s0 += 32) {
+            const int s = s0 + threadIdx.x;
+            int v = s < a.r.sequences ? before[s + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, v, o);
+                if (static_cast<int>(threadIdx.x) >= o) v += up;
+            }
+            if (s < a.r.sequences) before[s + 1] = sum + v;
+            sum += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    return PagedShare{before[a.r.sequences], before, of};
+}
+__device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const PagedShare& w, long long tile, int block_rows) {
+    int lo = 0, hi = a.r.sequences - 1;  // the last sequence whose items begin at or before the tile
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (w.before[mid] <= tile) lo = mid;
+        else hi = mid - 1;
+    }
+    const int4 of = w.of[lo];
+    const int i = static_cast<int>((tile - w.before[lo]) / of.w);
+    return PagedItem{lo, i % a.c.kv_heads, i / a.c.kv_heads * block_rows, w.before[lo] + static_cast<long long>(i) * of.w, of.w, PagedSequence{of.x, of.y, of.z, true}};
 }
 
 template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_rows_bytes() { return kPagedTile * BLOCKS * paged_row_bytes(TYPE); }  // keys or values of a tile
@@ -133,14 +181,14 @@ struct PagedFew {
     static constexpr int kJoinPitch = HD + 4, kJoin = 8 * kRows * (kJoinPitch * 4 + 8);
     static constexpr int kBody = 2 * kUnits * kUnit > kJoin ? 2 * kUnits * kUnit : kJoin;
     static constexpr int kSmem = 1024 + kBody + kRows * kPitch + kRows * 4 + 4 * kUnits * 8 + 64;
-    static constexpr int kBlocksPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && (NT == 1 || NT * BLOCKS <= 2) ? 2 : 1;
+    static constexpr int kBlocksPerSm = 2 * (kSmem + (kPagedShared + 1) * 20 + 1024 + 128) <= 228 * 1024 && (NT == 1 || NT * BLOCKS <= 2) ? 2 : 1;
 };
 
-// Brings the tiles of [begin, end) of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one whole warp. The pages' numbers of the tile after are
-// asked for before a wait. Returns with its own copies landed.
+// Brings the tiles of [begin, end) of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one whole warp. base0, base1: units that the rings have seen
+// before. The pages' numbers of the tile after are asked for before a wait. Returns with its own copies landed.
 template <int TYPE, int BLOCKS, int NT>
 __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, uint32_t rings, uint32_t full, uint32_t empty,
-                                                 volatile unsigned int* abort_flag, unsigned int limit) {
+                                                 int base0, int base1, volatile unsigned int* abort_flag, unsigned int limit) {
     using namespace gemm_detail;
     using F = PagedFew<TYPE, BLOCKS, NT>;
     constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
@@ -155,22 +203,21 @@ __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* 
         }
         return page;
     };
-    int next = page_of(begin), tile = 0, asked0 = 0, asked1 = 0;  // units asked for, of either ring
+    int next = page_of(begin), tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
     bool okay = true;
     for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
         const int pages = next, pieces = (min(kPagedTile, end - k0) + PR - 1) / PR;
         if (k0 + kPagedTile < end) next = page_of(k0 + kPagedTile);
 #pragma unroll
         for (int value = 0; value < 2; ++value) {
-            const int ring = tile & 1, n = (tile >> 1) * 2 + value, slot = ring * U + n % U;
+            const int ring = tile & 1, n = (ring ? base1 : base0) + (tile >> 1) * 2 + value, slot = ring * U + n % U;
             if (!(okay = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot, ((n / U) & 1) ^ 1, abort_flag, limit)))) break;
             const uint32_t to = rings + slot * F::kUnit, bar = full + 8 * slot;
             if (lane == 0) mbar_expect_tx(bar, pieces * PR * (BLOCKS * kRow + (TYPE == kPagedQ8 && value == 0 ? 8 : 0)));
             __syncwarp();
             (ring ? asked1 : asked0) = n + 1;
-            const int piece = lane / BLOCKS, b = lane % BLOCKS, page = __shfl_sync(0xffffffffu, pages, min(piece, 3));  // (at most 4 pieces of 4 blocks)
-            if (lane < pieces * BLOCKS)
-                bulk_load(to + (b * kPagedTile + piece * PR) * kRow, (value ? c.v : c.k) + paged_block_at(c, TYPE, page, head, b) + static_cast<size_t>((k0 + piece * PR) & (P - 1)) * kRow, PR * kRow, bar);
+            if (lane < pieces)
+                bulk_load(to + lane * PR * BLOCKS * kRow, (value ? c.v : c.k) + paged_rows_at(c, TYPE, pages, head, (k0 + lane * PR) & (P - 1)), PR * BLOCKS * kRow, bar);
             if (TYPE == kPagedQ8 && value == 0 && lane < pieces) {
                 const size_t from = paged_scales_at(c, pages, head) + ((k0 + lane * PR) & (P - 1));
                 bulk_load(to + kRows + lane * PR * 4, c.ks + from, PR * 4, bar);
@@ -179,7 +226,7 @@ __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* 
         }
     }
     for (int ring = 0; ring < 2; ++ring)
-        for (int asked = ring ? asked1 : asked0, n = max(0, asked - U); n < asked; ++n) mbar_wait(full + 8 * (ring * U + n % U), (n / U) & 1, abort_flag, limit, false);
+        for (int asked = ring ? asked1 : asked0, n = max(ring ? base1 : base0, asked - U); n < asked; ++n) mbar_wait(full + 8 * (ring * U + n % U), (n / U) & 1, abort_flag, limit, false);
 }
 
 template <int TYPE, int BLOCKS, int NT>
@@ -196,29 +243,55 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     float* s_rowf = reinterpret_cast<float*>(s_q + F::kRows * kPitch);          // [kRows]: what a row's score is multiplied by
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_rowf + F::kRows);
     volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U);
+    __shared__ int s_before[kPagedShared + 1];
+    __shared__ int4 s_of[kPagedShared];
     const uint32_t full = smem_u32(bars), empty = full + 16 * U;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-    const int seq = blockIdx.z, kvh = blockIdx.y % a.c.kv_heads, tile = blockIdx.y / a.c.kv_heads;
-    const PagedSequence sq = paged_sequence(a.c, a.r, seq);
-    if (!sq.ok || sq.news < a.few || sq.news > a.many) {
-        if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
-        return;
-    }
-    const int rows = sq.news * a.group, r0 = tile * F::kRows, r1 = min(rows, r0 + F::kRows);
-    if (r0 >= rows) return;
-    if (static_cast<int>(blockIdx.x) >= paged_splits_used(a, sq)) return;
-    const int t0 = r0 / a.group, t1 = (r1 - 1) / a.group + 1, p0 = sq.length - sq.news;
-    const PagedRange range = paged_range(a, sq, t0, t1, blockIdx.x);
 
     if (tid == 0) {
         for (int s = 0; s < 2 * U; ++s) mbar_init(full + 8 * s, 1), mbar_init(empty + 8 * s, 4);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
+    long long at = 0, until = 1, first = 0;  // this block's tiles among all
+    PagedShare shared{0, s_before, s_of};
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (a.share) {
+        shared = paged_share_begin(a, F::kRows, s_before, s_of, kThreads);
+        at = first = shared.total * blockIdx.x / gridDim.x, until = shared.total * (blockIdx.x + 1) / gridDim.x;
+    }
+    int base0 = 0, base1 = 0;  // units that the rings have seen
+    while (at < until) {
+    int seq, kvh, r0, parts_place = -1;  // place of the workspace that the segment's result goes to, or none
+    PagedSequence sq;
+    PagedRange range;
+    if (a.share) {
+        const PagedItem item = paged_item_at(a, shared, at, F::kRows);
+        seq = item.seq, kvh = item.kvh, r0 = item.rows0, sq = item.q;
+        const int t = static_cast<int>(at - item.begin), n = static_cast<int>(min(static_cast<long long>(item.tiles - t), until - at));
+        range = paged_seen(a, sq);
+        range.end = min(range.end, range.begin + (t + n) * kPagedTile), range.begin += t * kPagedTile;
+        if (n < item.tiles) parts_place = static_cast<int>(blockIdx.x) * 2 + (at == first ? 0 : 1);
+        at += n;
+    } else {
+        at = until, seq = blockIdx.z, kvh = blockIdx.y, r0 = blockIdx.x * F::kRows;
+        sq = paged_sequence(a.c, a.r, seq);
+        if (!sq.ok || sq.news < a.few || sq.news > a.many) {
+            if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
+            return;
+        }
+        range = paged_seen(a, sq);
+    }
+    const int rows = sq.news * a.group, r1 = min(rows, r0 + F::kRows);
+    if (r0 >= rows) return;  // (only where a block takes a whole item)
+    const int t0 = r0 / a.group, t1 = (r1 - 1) / a.group + 1, p0 = sq.length - sq.news;
+    // what these rows see of it
+    const int low = a.window > 0 ? max(0, p0 + t0 - a.window + 1) & ~(kPagedTile - 1) : 0;
+    range.begin = max(range.begin, low), range.end = max(range.begin, min(range.end, max(0, p0 + t1)));
+    const int tiles = (range.end - range.begin + kPagedTile - 1) / kPagedTile;
+    __syncthreads();  // the barriers are there; the segment before has left the ring
     if (warp == 8) {
-        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, abort_flag, a.spin_limit);
+        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, base0, base1, abort_flag, a.spin_limit);
     } else {
         // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none
         for (int i = warp; i < F::kRows; i += 8) {
@@ -283,7 +356,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                 for (int e = 0; e < 4; ++e) o[j][n][e] = 0.0f;
 
         bool okay = true;
-        int n = 0;  // units of this group's ring
+        int n = turn ? base1 : base0;  // units of this group's ring
         for (int k0 = range.begin + turn * kPagedTile; k0 < range.end; k0 += 2 * kPagedTile, n += 2) {
             const int key_slot = turn * U + n % U, value_slot = turn * U + (n + 1) % U, key0 = k0 + kg * 16;
             const uint32_t keys = ring + key_slot * F::kUnit, values = ring + value_slot * F::kUnit;
@@ -312,7 +385,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                     uint32_t r[4];
                     if constexpr (Q8) {
                         if ((ks & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice ks, then of slice ks + 1
-                            ldsm4(r, keys + ((ks >> 2) * kPagedTile + row) * kRow + ((((ks & 3) + (lane >> 4)) ^ swz) << 4));
+                            ldsm4(r, keys + paged_row_at(TYPE, BLOCKS, ks >> 2, row) + ((((ks & 3) + (lane >> 4)) ^ swz) << 4));
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
@@ -321,7 +394,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                             }
                         }
                     } else {  // positions 0-7 and 8-15 of the slice's first 8 values, then of the others
-                        ldsm4(r, keys + ((ks >> 2) * kPagedTile + row) * kRow + ((((ks & 3) * 2 + (lane >> 4)) ^ swz) << 4));
+                        ldsm4(r, keys + paged_row_at(TYPE, BLOCKS, ks >> 2, row) + ((((ks & 3) * 2 + (lane >> 4)) ^ swz) << 4));
                         score(r, ks);
                     }
                 }
@@ -341,12 +414,16 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float x = sc[n][e];
-                        if constexpr (Q8) x *= kf[e >> 1];
-                        x *= rowf[n][e & 1];
-                        if (a.cap > 0.0f) x = a.cap * tanh_of(x);
-                        if constexpr (Q8) x += lv[e >> 1];
-                        sc[n][e] = x;
+                        if constexpr (Q8) sc[n][e] *= kf[e >> 1];
+                        sc[n][e] *= rowf[n][e & 1];
+                    }
+                    if (a.cap > 0.0f) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[n][e] = a.cap * tanh_of(sc[n][e]);
+                    }
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[n][e] += lv[e >> 1];
                     }
                     if (masked) {
 #pragma unroll
@@ -411,7 +488,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                     uint32_t r[4];
                     if constexpr (Q8) {
                         if ((j & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice j, then of slice j + 1; a pair of bytes is two values of a position
-                            ldsm4_trans(r, values + ((j >> 2) * kPagedTile + row) * kRow + ((((j & 3) + (lane >> 4)) ^ swz) << 4));
+                            ldsm4_trans(r, values + paged_row_at(TYPE, BLOCKS, j >> 2, row) + ((((j & 3) + (lane >> 4)) ^ swz) << 4));
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
@@ -422,7 +499,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                         }
                     } else {  // matrices: (positions 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
                         const int vrow = kg * 16 + (lane & 7) + ((lane >> 4) << 3);
-                        ldsm4_trans(r, values + ((j >> 2) * kPagedTile + vrow) * kRow + ((((j & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+                        ldsm4_trans(r, values + paged_row_at(TYPE, BLOCKS, j >> 2, vrow) + ((((j & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma<BF>(o[j][n], r, pb[n][0], pb[n][1]);
                     }
@@ -488,51 +565,54 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         }
         const size_t t = static_cast<size_t>(sq.first) + (r0 + r) / a.group;
         const int h = kvh * a.group + (r0 + r) % a.group;
-        if (a.splits == 1) {
+        if (parts_place < 0) {
             const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (a sum that is no number stays one)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= inv;
             paged_store8(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.out_type), a.out_type, x);
         } else {
-            const int heads = a.c.kv_heads * a.group;
-            const size_t row = (static_cast<size_t>(blockIdx.x) * a.r.tokens + t) * heads + h;
+            const size_t row = static_cast<size_t>(parts_place) * F::kRows + r;
             paged_store8(a.part_o + row * HD + e0, kPagedF32, x);
             if (e0 == 0) a.part_ml[row] = make_float2(top, sum);
         }
     }
+    base0 += (tiles + 1) / 2 * 2, base1 += tiles / 2 * 2;
+    __syncthreads();
+    }
 }
 
-// Joins results of ranges: weights 2^(m_i - m) over `count` of them, `step` rows apart from row `row`, for the values of one warp's lanes (kPer each), by the WARPS warps of a block in turn, eight results at
+// Joins results: weights 2^(m_i - m) over `count` of them, the i-th in row row_of(i) of the workspace, for the values of one warp's lanes (kPer each), by the WARPS warps of a block in turn, a few results at
 // a time so that their reads overlap; in the same order whenever it is asked for. Returns the row's normalised values, in the first warp.
-template <int HD, int WARPS>
-__device__ __forceinline__ void paged_join(const float* part_o, const float2* part_ml, size_t row, size_t step, int count, float (&x)[HD / 32], float* shared) {
+template <int HD, int WARPS, typename RowOf>
+__device__ __forceinline__ void paged_join(const float* part_o, const float2* part_ml, RowOf row_of, int count, float (&x)[HD / 32], float* shared) {
     using namespace paged_detail;
     constexpr int kPer = HD / 32;
     const int lane = threadIdx.x & 31, warp = WARPS > 1 ? threadIdx.x >> 5 : 0;
     float top = -INFINITY;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, part_ml[i * step + row].x);
+    for (int i = lane; i < count; i += 32) top = fmaxf(top, part_ml[row_of(i)].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) x[e] = 0.0f;
-    for (int i0 = warp; i0 < count; i0 += 8 * WARPS) {
-        float2 ml[8];
-        float v[8][kPer];
+    constexpr int kBatch = HD > 128 ? 4 : 8;
+    for (int i0 = warp; i0 < count; i0 += kBatch * WARPS) {
+        float2 ml[kBatch];
+        float v[kBatch][kPer];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
             const int i = i0 + k * WARPS;
-            ml[k] = i < count ? part_ml[i * step + row] : make_float2(-INFINITY, 0.0f);
+            ml[k] = i < count ? part_ml[row_of(i)] : make_float2(-INFINITY, 0.0f);
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
             const bool there = !(ml[k].x == -INFINITY && ml[k].y == 0.0f);  // a range in which nothing was visible has no values
-            const float* from = part_o + (static_cast<size_t>(i0 + k * WARPS) * step + row) * HD + lane * kPer;
+            const float* from = part_o + row_of(min(i0 + k * WARPS, count - 1)) * HD + lane * kPer;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) v[k][e] = there ? from[e] : 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < kBatch; ++k) {
             const float w = ml[k].x == -INFINITY && ml[k].y == 0.0f ? 0.0f : ex2(ml[k].x - top);
             sum = fmaf(w, ml[k].y, sum);
 #pragma unroll
@@ -569,18 +649,31 @@ __device__ __forceinline__ void paged_store_row(unsigned char* out, int type, co
     }
 }
 
-// Joins the ranges of a sequence: a block of WARPS warps per (token, query head).
-template <int BLOCKS, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
+// The block of G whose share of W tiles has tile x.
+__device__ __forceinline__ int paged_block_of(long long x, long long total, int blocks) { return static_cast<int>(((x + 1) * blocks - 1) / total); }
+// Joins the segments of the items that were cut: a block of 8 warps per (token, query head); `blocks`, `block_rows`: of the launch whose tiles were shared out.
+template <int BLOCKS>
+__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a, int blocks, int block_rows) {
     constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
-    __shared__ float shared[WARPS > 1 ? WARPS * 32 * (kPer + 1) : 1];
+    __shared__ float shared[8 * 32 * (kPer + 1)];
+    __shared__ int before[kPagedShared + 1];
+    __shared__ int4 of[kPagedShared];
     const int heads = a.c.kv_heads * a.group, lane = threadIdx.x & 31, t = blockIdx.x / heads, h = blockIdx.x % heads;
     const int s = paged_sequence_of(a.r, t);
+    const PagedShare w = paged_share_begin(a, block_rows, before, of, 256);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the segments are still being worked on; what was read above is input. Every block waits, so that none ends before them
     if (s < 0) return;
     const PagedSequence sq = paged_sequence(a.c, a.r, s);
     if (!sq.ok || t < sq.first || t >= sq.first + sq.news || sq.news < a.few || sq.news > a.many) return;
+    int tiles, items;
+    paged_weight(a, sq, block_rows, &tiles, &items);
+    const int kvh = h / a.group, r = (t - sq.first) * a.group + h % a.group;
+    const long long begin = w.before[s] + static_cast<long long>(r / block_rows * a.c.kv_heads + kvh) * tiles;
+    const int b0 = paged_block_of(begin, w.total, blocks), b1 = paged_block_of(begin + tiles - 1, w.total, blocks), row = r % block_rows;
+    if (b0 == b1) return;  // it was whole
+    const int place0 = w.total * b0 / blocks == begin ? 0 : 1;
     float x[kPer];
-    paged_join<HD, WARPS>(a.part_o, a.part_ml, static_cast<size_t>(t) * heads + h, static_cast<size_t>(a.r.tokens) * heads, paged_splits_used(a, sq), x, shared);
+    paged_join<HD, 8>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + row; }, b1 - b0 + 1, x, shared);
     if (threadIdx.x >= 32) return;
     paged_store_row(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x);
 }

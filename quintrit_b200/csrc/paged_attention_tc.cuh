@@ -27,7 +27,7 @@ constexpr int kPagedMapped = 160;  // most (row block, range) pairs of a mapped 
 struct PagedSchedule {
     int m, whole, cut;                       // blocks x m: order x < whole, all of its range; else order whole + (x - whole) / cut, range (x - whole) % cut of cut
     int mapped;                              // few row blocks, of different lengths: order[x], range[x] of ranges[x] instead
-    unsigned char order[kPagedMapped], range[kPagedMapped], ranges[kPagedMapped];
+    unsigned char order[kPagedMapped], range[kPagedMapped], ranges[kPagedMapped], at[kPagedMapped];  // at: the first x of an order
     float* part_o;                           // [x - whole][m][rows of a block][head_dim] for what is cut; mapped: [range][KV head][packed tokens x group][head_dim]
     float2* part_ml;
 };
@@ -216,18 +216,14 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     if (!Q8 && value && pieces * PR < KT) {  // rows that no page brings: their weights are zeros, their values must be numbers
                         for (int i = pieces * PR * 8 + lane; i < KT * 8; i += 32)
                             for (int b = 0; b < BLOCKS; ++b)
-                                *reinterpret_cast<uint4*>(smem + (to - base) + (b * KT + (i >> 3)) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4*>(smem + (to - base) + paged_row_at(TYPE, BLOCKS, b, i >> 3) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
                         fence_async_shared();
                         __syncwarp();
                     }
                     if (lane == 0) mbar_expect_tx(bar, pieces * PR * (BLOCKS * kRow + (Q8 && !value ? 8 : 0)));
                     __syncwarp();
                     const unsigned char* store = value ? a.c.v : a.c.k;
-                    for (int i0 = 0; i0 < pieces * BLOCKS; i0 += 32) {
-                        const int i = i0 + lane, piece = i / BLOCKS, b = i % BLOCKS, page = __shfl_sync(0xffffffffu, pages, min(piece, 31));
-                        if (i < pieces * BLOCKS)
-                            bulk_load(to + (b * KT + piece * PR) * kRow, store + paged_block_at(a.c, TYPE, page, kvh, b) + static_cast<size_t>((k0 + piece * PR) & (P - 1)) * kRow, PR * kRow, bar);
-                    }
+                    if (lane < pieces) bulk_load(to + lane * PR * BLOCKS * kRow, store + paged_rows_at(a.c, TYPE, pages, kvh, (k0 + lane * PR) & (P - 1)), PR * BLOCKS * kRow, bar);
                     if constexpr (Q8) {
                         if (!value && lane < pieces) {
                             const size_t from = paged_scales_at(a.c, pages, kvh) + ((k0 + lane * PR) & (P - 1));
@@ -243,7 +239,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             // as sixteen to run) ----
             constexpr uint32_t kScores = instr_desc_16(M::BF, false, KT), kValues = instr_desc_16(M::BF, true, HD);
             // descriptors: the upper word does not change
-            const uint64_t k_desc = smem_desc(0, 16, 1024, 2), v_desc = smem_desc(0, KT * 128, 1024, 2);
+            const uint64_t q_desc = smem_desc(0, 16, 1024, 2), k_desc = smem_desc(0, 16, BLOCKS * 1024, 2), v_desc = smem_desc(0, 1024, BLOCKS * 1024, 2);
             auto at = [](uint64_t desc, uint32_t addr) { return desc | static_cast<uint64_t>((addr & 0x3FFFFu) >> 4); };
             bool okay = units == 0 || __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, a.spin_limit));
             fence_after();
@@ -257,11 +253,11 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                 const int j = u / NT, i = u % NT, b = u % NB;
                 if (!need(2 * j)) return;
                 const uint32_t d = tmem + M::kSCol + b * KT;
-                const uint64_t keys = at(k_desc, slots + (2 * j % RS) * M::kSlot), queries = at(k_desc, q_at + i * BLOCKS * 128 * 128);
+                const uint64_t keys = at(k_desc, slots + (2 * j % RS) * M::kSlot), queries = at(q_desc, q_at + i * BLOCKS * 128 * 128);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const uint64_t kd = keys + ((k >> 2) * KT * 128 >> 4) + 2 * (k & 3);
+                        const uint64_t kd = keys + ((k >> 2) * 1024 >> 4) + 2 * (k & 3);
                         if constexpr (M::kQTmem) mma_ts(d, tmem + M::kQCol + k * 8, kd, kScores, k > 0);
                         else mma_ss(d, queries + ((k >> 2) * 128 * 128 >> 4) + 2 * (k & 3), kd, kScores, k > 0);
                     }
@@ -279,7 +275,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                 const uint32_t first = j > 0;
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < KT / 16; ++k) mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, values + (k * 16 * 128 >> 4), kValues, k > 0 ? 1u : first);
+                    for (int k = 0; k < KT / 16; ++k) mma_ts(tmem + M::kOCol + i * 128, tmem + M::kSCol + b * KT + k * 8, values + (k * 2 * BLOCKS * 1024 >> 4), kValues, k > 0 ? 1u : first);
                     mma_commit(o_done(b));
                     if (i == NT - 1) mma_commit(empty((2 * j + 1) % RS));
                 }
@@ -318,7 +314,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                                          : "memory");
 #pragma unroll
                         for (int k = 0; k < kAtOnce; ++k) {
-                            const int i = w + (k0 + k) * M::kWidenWarps * 32, row = i >> 2, r = row % KT, c = (i & 3) ^ ((r >> 1) & 3);
+                            const int i = w + (k0 + k) * M::kWidenWarps * 32, row = i >> 2, r = (row / (8 * BLOCKS)) * 8 + (row & 7), c = (i & 3) ^ ((r >> 1) & 3);  // row: 128 bytes of the operand, in the order of the codes' 64
                             uint32_t o[8];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
@@ -654,7 +650,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     const int lane = threadIdx.x & 31, local = blockIdx.x * 8 + (threadIdx.x >> 5), which = blockIdx.y, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
     int x = 0, order = blockIdx.z, ranges = g.cut;
     if (g.mapped) {
-        while (g.order[x] != order) ++x;
+        x = g.at[order];
         ranges = g.ranges[x];
     } else {
         x = order * g.cut, order += g.whole;
@@ -664,9 +660,8 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     if (!sq.ok || sq.news < a.few || sq.news > a.many) return;
     const int rows = sq.news * a.group, block = (rows + kRows - 1) / kRows - 1 - order, r = block * kRows + local;
     if (block < 0 || r >= rows) return;
-    const size_t row = paged_part_row(a, g, sq, PagedPart{order, 0, ranges, x}, which, kvh, r, local, kRows), step = paged_part_row(a, g, sq, PagedPart{order, 1, ranges, x + 1}, which, kvh, r, local, kRows) - row;
     float x_row[kPer];
-    paged_join<HD, 1>(g.part_o, g.part_ml, row, step, ranges, x_row, nullptr);
+    paged_join<HD, 1>(g.part_o, g.part_ml, [&](int i) { return paged_part_row(a, g, sq, PagedPart{order, i, ranges, x + i}, which, kvh, r, local, kRows); }, ranges, x_row, nullptr);
     const size_t token = static_cast<size_t>(sq.first) + r / a.group;
     paged_store_row(static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + r % a.group) * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x_row);
 }

@@ -1,9 +1,9 @@
 // A key / value cache in pages: what its kernels share.
 //
-// A cache holds `pages` pages of P positions for every layer. A page of a layer keeps, per KV head, the rows of P positions, cut into blocks of 64
-// values: [page][head][block][position][64 values], keys and values apart. So the part of a page that one block of threads reads (a page of one head)
-// is contiguous and comes to shared memory by bulk copies, without a tensor map, whatever the page table says. Rows lie in it the way matrix
-// instructions want them in shared memory, with the 16-byte pieces of a row permuted, so that eight rows of one piece fall into eight different banks:
+// A cache holds `pages` pages of P positions for every layer. A page of a layer keeps, per KV head, the rows of P positions, eight positions together, cut into blocks of 64
+// values: [page][head][P / 8][block][8 positions][64 values], keys and values apart. So any run of whole eights of a page and head is contiguous, and comes to shared memory by one bulk copy, without a
+// tensor map, whatever the page table says. Rows lie in it the way matrix instructions want them in shared memory: groups of eight rows a constant distance apart, the 16-byte pieces of a
+// row permuted, so that eight rows of one piece fall into eight different banks:
 //   F16, BF16: rows of 128 bytes, piece c of row r at c ^ (r & 7) (the 128-byte swizzle of the tensor cores' operands);
 //   Q8:        rows of 64 bytes,  piece c of row r at c ^ ((r >> 1) & 3), and one F32 scale per row and head, [page][head][position].
 //
@@ -45,9 +45,11 @@ struct RowsView {
 
 __host__ __device__ constexpr int paged_row_bytes(int type) { return type == kPagedQ8 ? kPagedBlock : kPagedBlock * 2; }
 __device__ __forceinline__ int paged_piece(int type, int row, int piece) { return type == kPagedQ8 ? piece ^ ((row >> 1) & 3) : piece ^ (row & 7); }
-// The first byte of a page's block of a head; the page's scales of a head.
-__device__ __forceinline__ size_t paged_block_at(const PagedView& c, int type, int page, int head, int block) {
-    return (((static_cast<size_t>(page) * c.kv_heads + head) * c.blocks + block) << c.page_log2) * paged_row_bytes(type);
+// Where row r of a block lies in a run of rows that begins with a whole eight: in shared memory as in a page.
+__host__ __device__ constexpr int paged_row_at(int type, int blocks, int block, int r) { return (((r >> 3) * blocks + block) * 8 + (r & 7)) * paged_row_bytes(type); }
+// The first byte of a page's rows of a head, from row r on (a multiple of 8); the page's scales of a head.
+__device__ __forceinline__ size_t paged_rows_at(const PagedView& c, int type, int page, int head, int r) {
+    return (((static_cast<size_t>(page) * c.kv_heads + head) << c.page_log2) + r) * (c.blocks * paged_row_bytes(type));
 }
 __device__ __forceinline__ size_t paged_scales_at(const PagedView& c, int page, int head) { return (static_cast<size_t>(page) * c.kv_heads + head) << c.page_log2; }
 

@@ -176,9 +176,9 @@ __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const
             }
             if (live) atomicOr(a.c.status, kPagedSaturated);
         }
-        unsigned char* block = (kind == 1 ? a.c.k : a.c.v) + paged_block_at(a.c, a.type, place.page, h, piece >> 3);
+        unsigned char* row = (kind == 1 ? a.c.k : a.c.v) + paged_rows_at(a.c, a.type, place.page, h, 0) + paged_row_at(a.type, a.c.blocks, piece >> 3, place.row);
         if (a.type != kPagedQ8) {
-            if (live) paged_store8(block + place.row * 128 + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
+            if (live) paged_store8(row + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
             continue;
         }
 #pragma unroll
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const
             const int q = __float2int_rn(x[i] * inv);
             code[i >> 2] |= static_cast<uint32_t>(q & 0xff) << (8 * (i & 3));
         }
-        *reinterpret_cast<uint2*>(block + place.row * 64 + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
+        *reinterpret_cast<uint2*>(row + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
         if (piece == 0) (kind == 1 ? a.c.ks : a.c.vs)[paged_scales_at(a.c, place.page, h) + place.row] = d;
     }
 }
@@ -220,13 +220,13 @@ __global__ void __launch_bounds__(kPagedRowThreads) paged_read_kernel(const __gr
         const int head = min(head0 + u * kHeads, heads - 1);
         const bool value = head >= a.c.kv_heads;
         const int h = value ? head - a.c.kv_heads : head;
-        const unsigned char* block = (value ? a.c.v : a.c.k) + paged_block_at(a.c, TYPE, place.page, h, piece >> 3);
+        const unsigned char* row = (value ? a.c.v : a.c.k) + paged_rows_at(a.c, TYPE, place.page, h, 0) + paged_row_at(TYPE, a.c.blocks, piece >> 3, place.row);
         if constexpr (TYPE == kPagedQ8) {
-            const uint2 v = *reinterpret_cast<const uint2*>(block + place.row * 64 + paged_piece(TYPE, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8);
+            const uint2 v = *reinterpret_cast<const uint2*>(row + paged_piece(TYPE, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8);
             raw[u] = make_uint4(v.x, v.y, 0, 0);
             d[u] = (value ? a.c.vs : a.c.ks)[paged_scales_at(a.c, place.page, h) + place.row];
         } else {
-            raw[u] = *reinterpret_cast<const uint4*>(block + place.row * 128 + paged_piece(TYPE, place.row, piece & 7) * 16);
+            raw[u] = *reinterpret_cast<const uint4*>(row + paged_piece(TYPE, place.row, piece & 7) * 16);
         }
     }
 #pragma unroll
