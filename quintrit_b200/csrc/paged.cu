@@ -2,7 +2,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
 
@@ -154,34 +153,42 @@ int places_of(const quintrit_b200_paged_cache* c, int nt) {
 }
 
 // The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles and a start and an end of
-// about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. Where the sequences' chunks differ, as in a step that carries one
-// prompt, fewer row blocks are there than the longest chunk times the sequences: their number is taken from the tokens.
-size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, int rows, size_t limit, PagedSchedule* g) {
+// about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. `few`: the new tokens of sequences that it leaves out. Where the sequences' chunks differ,
+// the row blocks are not known here: about as many as the tokens fill, at most one more for every sequence that may be among them.
+size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, int few, int rows, size_t limit, PagedSchedule* g) {
     constexpr double kStart = 4.0, kJoin = 3.0;
     const int tile = c->head_dim == 256 ? 64 : 128, sms = c->sm_count;
-    const long long most = static_cast<long long>(r->max_new) * group, blocks = (most + rows - 1) / rows, kvh = c->kv_heads;
-    const long long all = static_cast<long long>(r->tokens) * group, m = std::max<long long>(kvh, kvh * ((all + rows - 1) / rows) / blocks);  // blocks of an order, likely
+    const long long most = static_cast<long long>(r->max_new) * group, longest_blocks = (most + rows - 1) / rows, all = static_cast<long long>(r->tokens) * group;
+    const bool even = static_cast<long long>(r->max_new) * r->sequences == r->tokens;
+    const long long m = even ? static_cast<long long>(c->kv_heads) * r->sequences : c->kv_heads;
+    const long long blocks = even ? longest_blocks : (all + rows - 1) / rows, bound = even ? blocks : all / rows + std::min<long long>(r->sequences, r->tokens / (few + 1u));
     // tiles that the row block of an order sees, if its sequence has the length that was announced
     auto tiles_of = [&](long long order) -> long long {
-        const long long first = (blocks - 1 - order) * rows / group, last = std::min<long long>(((blocks - order) * rows - 1) / group, r->max_new - 1), before = static_cast<long long>(r->max_length) - r->max_new;
+        if (!even) order = 0;
+        const long long first = (longest_blocks - 1 - order) * rows / group, last = std::min<long long>(((longest_blocks - order) * rows - 1) / group, r->max_new - 1),
+                        before = static_cast<long long>(r->max_length) - r->max_new;
         const long long high = std::max<long long>(before + last + 1, 1), low = window > 0 ? std::max<long long>(before + first - window + 1, 0) : 0;
         return std::max<long long>(1, (high - low + tile - 1) / tile);
     };
-    g->m = static_cast<int>(kvh * r->sequences), g->mapped = 0, g->whole = static_cast<int>(blocks), g->cut = 1;
+    g->m = static_cast<int>(m), g->even = even, g->orders = static_cast<int>(bound), g->mapped = 0, g->whole = static_cast<int>(bound), g->cut = 1;
     if (blocks * m < sms) {
         // Ranges of at most `length` tiles, the shortest for which they are there at once.
-        const size_t per_range = static_cast<size_t>(all) * kvh;
+        const size_t per_range = static_cast<size_t>(all) * c->kv_heads;
         const long long longest = tiles_of(0);
         long long best = longest;
         for (long long length = longest - 1; length >= 2; --length) {
-            long long parts = 0;
-            for (long long o = 0; o < blocks && parts * m <= sms; ++o) parts += (tiles_of(o) + length - 1) / length;
-            if (parts * m > sms || parts > kPagedMapped || static_cast<size_t>((longest + length - 1) / length) * per_range > limit) break;
+            long long parts = 0, mapped = 0;
+            for (long long o = 0; o < bound && mapped <= kPagedMapped; ++o) {
+                const long long n = (tiles_of(o) + length - 1) / length;
+                mapped += n;
+                if (o < blocks) parts += n;
+            }
+            if (parts * m > sms || mapped > kPagedMapped || static_cast<size_t>((longest + length - 1) / length) * per_range > limit) break;
             best = length;
         }
         if (best + kJoin >= longest) return 0;
         int x = 0;
-        for (long long o = 0; o < blocks; ++o) {
+        for (long long o = 0; o < bound; ++o) {
             const int ranges = static_cast<int>((tiles_of(o) + best - 1) / best);
             g->at[o] = static_cast<unsigned char>(x);
             for (int i = 0; i < ranges; ++i, ++x) g->order[x] = static_cast<unsigned char>(o), g->range[x] = static_cast<unsigned char>(i), g->ranges[x] = static_cast<unsigned char>(ranges);
@@ -193,15 +200,16 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
     if (left == 0) return 0;
     const double tiles = static_cast<double>(tiles_of(whole));
     const long long room = sms + (blocks * m / sms * sms - whole * m);
+    auto slots = [&](int s) { return static_cast<size_t>(bound - whole) * m * s * rows; };
     int best = 1;
     double least = 1e30;
-    for (int s = 1; s <= 24 && (s == 1 || (static_cast<size_t>(left) * g->m * s * rows <= limit && tiles / s >= 2.0)); ++s) {
+    for (int s = 1; s <= 24 && (s == 1 || (slots(s) <= limit && tiles / s >= 2.0)); ++s) {
         const double cost = static_cast<double>((left * m * s + room - 1) / room) * (std::ceil(tiles / s) + kStart) + (s > 1 ? kJoin : 0.0);
         if (cost < least * 0.97) best = s, least = cost;
     }
     if (best == 1) return 0;
     g->whole = static_cast<int>(whole), g->cut = best;
-    return static_cast<size_t>(left) * g->m * best * rows;
+    return slots(best);
 }
 template <int TYPE, int BLOCKS, int NT>
 int launch_many_of(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
@@ -221,6 +229,18 @@ int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device,
     return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 2>(a, g, device, grid, s);
 }
 
+// Launches a kernel that joins results, 256 threads to a block: it comes up while the one before it in the stream still runs, and waits for that one's end itself.
+template <typename Kernel, typename... Args>
+int launch_behind(Kernel kernel, unsigned grid, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute dependent{};
+    dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization, dependent.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(256), cfg.stream = s, cfg.attrs = &dependent, cfg.numAttrs = 1;
+    QTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    ++g_launches;
+    return QUINTRIT_OK;
+}
+
 // How a call is served: sequences of up to `few_new` new tokens by the kernel for few rows, the others by the one for many; either may have nothing to do.
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
@@ -234,10 +254,10 @@ struct PagedPlan {
     size_t part_rows;
     size_t few_bytes, many_bytes;  // of the workspace
 };
-int few_limit() { return std::getenv("QTB_FEW") ? std::atoi(std::getenv("QTB_FEW")) : 64; }
+constexpr int kPagedFewRows = 64;  // rows of a KV head up to which the kernel for few rows takes a call
 constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {
-    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = few_limit();
+    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = kPagedFewRows;
     p->many = most > limit;
     p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(std::max<long long>(8 / group, group <= 32 ? 1 : 0), r->max_new - 1));  // (a sequence alone is the longest)
     p->few_tiles = 0, p->few_share = 0, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
@@ -254,12 +274,11 @@ void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_
         const int rows = c->head_dim == 256 || most <= 128 ? 128 : 256;
         p->many_rows = rows;
         // (up to four results for every row of a block of threads on every multiprocessor, about 80 MB; no window takes more than none)
-        p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), 0, rows, static_cast<size_t>(4) * c->sm_count * rows, &p->schedule);
-        if (window > 0) p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), window, rows, p->part_rows, &p->schedule);
+        p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), 0, p->few_new, rows, static_cast<size_t>(4) * c->sm_count * rows, &p->schedule);
+        if (window > 0) p->part_rows = schedule_of(c, r, static_cast<uint32_t>(group), window, p->few_new, rows, p->part_rows, &p->schedule);
         p->many_bytes = up16(p->part_rows * row_bytes);
         const PagedSchedule& g = p->schedule;
-        const long long blocks = (most + rows - 1) / rows;
-        p->many_blocks = (g.mapped ? g.mapped : g.whole + (blocks - g.whole) * g.cut) * static_cast<long long>(g.m);
+        p->many_blocks = (g.mapped ? g.mapped : g.whole + static_cast<long long>(g.orders - g.whole) * g.cut) * g.m;
     }
 }
 }  // namespace
@@ -493,10 +512,9 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
                                                                                                                          : launch_many_type<kPagedQ8>(a, g, device, plan.many_rows, grid, s);
             if (rc != QUINTRIT_OK) return rc;
             if (plan.part_rows > 0) {
-                const int block = plan.many_rows, blocks = static_cast<int>((static_cast<long long>(rows->max_new) * group + block - 1) / block);
                 auto kernel = a.c.blocks == 1 ? paged_join_kernel<1> : a.c.blocks == 2 ? paged_join_kernel<2> : paged_join_kernel<4>;
-                kernel<<<dim3(block / 8, static_cast<unsigned>(g.m), static_cast<unsigned>(blocks - g.whole)), 256, 0, s>>>(a, g, block);
-                QTB_LAUNCH_CHECK();
+                rc = launch_behind(kernel, static_cast<unsigned>((static_cast<long long>(rows->tokens) * args->q_heads + 7) / 8), s, a, g, plan.many_rows);
+                if (rc != QUINTRIT_OK) return rc;
             }
         }
         if (plan.few_new > 0) {
@@ -508,14 +526,10 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.nt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.nt, grid, s)
                                                                                                                                 : launch_few_type<kPagedQ8>(a, device, plan.nt, grid, s);
             if (rc != QUINTRIT_OK) return rc;
-            if (plan.few_share > 0) {
+            if (plan.few_share > 1) {
                 auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;
-                cudaLaunchConfig_t cfg{};
-                cudaLaunchAttribute dependent{};
-                dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization, dependent.val.programmaticStreamSerializationAllowed = 1;
-                cfg.gridDim = dim3(rows->tokens * args->q_heads), cfg.blockDim = dim3(256), cfg.stream = s, cfg.attrs = &dependent, cfg.numAttrs = 1;
-                QTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, plan.few_share, block_rows));
-                ++g_launches;
+                rc = launch_behind(kernel, static_cast<unsigned>(plan.few_share - 1), s, a, plan.few_share, block_rows);
+                if (rc != QUINTRIT_OK) return rc;
             }
         }
         return ok();

@@ -97,6 +97,15 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased, uint32_t sel
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ long long prefix(long long v) {  // the sum of v over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, v, o);
+        if (static_cast<int>(threadIdx.x & 31) >= o) v += up;
+    }
+    return v;
+}
+
 }  // namespace paged_detail
 
 struct PagedRange {
@@ -107,19 +116,18 @@ __device__ __forceinline__ PagedRange paged_seen(const PagedAttnArgs& a, const P
     return PagedRange{a.window > 0 ? max(0, q.length - q.news - a.window + 1) & ~(kPagedTile - 1) : 0, q.length};
 }
 
-// Work shared out: the items (a sequence's KV head and block of rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles; block b of G takes the tiles
-// [b W / G, (b + 1) W / G) of all W, whatever the lengths are. What a block has of an item is a segment: a whole item's result is written as it is, others go to the workspace, at most two of a block:
+// Work shared out: the items (a sequence's KV head and block of rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles; block b of G takes W / G of all W tiles, the
+// first W % G blocks one more, whatever the lengths are. What a block has of an item is a segment: a whole item's result is written as it is, others go to the workspace, at most two of a block:
 // place 0 for the segment that its tiles begin with, place 1 for another. Every block works the items' places out for itself from the lengths (paged_share_begin), for up to kPagedShared sequences.
 constexpr int kPagedShared = 256;
 struct PagedShare {
-    long long total;
+    int total;
     int* before;  // [sequences + 1] in shared memory: tiles of the items before a sequence's
     int4* of;     // [sequences]: first token, new tokens, length, tiles of an item
 };
 struct PagedItem {
     int seq, kvh, rows0;        // rows0: the block of rows' first
-    long long begin;            // the item's first tile among all
-    int tiles;
+    int begin, tiles;           // the item's first tile among all
     PagedSequence q;
 };
 // Tiles and items of a sequence.
@@ -128,36 +136,33 @@ __device__ __forceinline__ void paged_weight(const PagedAttnArgs& a, const Paged
     const bool mine = q.ok && q.news >= a.few && q.news <= a.many;
     *tiles = max(1, (g.end - g.begin + kPagedTile - 1) / kPagedTile), *items = mine ? a.c.kv_heads * ((q.news * a.group + block_rows - 1) / block_rows) : 0;
 }
-// By all threads of a block; `before` and `of` have room for kPagedShared + 1 and kPagedShared. (32 bits hold the tiles: at most 2^16 items of 2^15 tiles, or a longer sequence alone.)
+// By all threads of a block; `before` and `of` have room for kPagedShared + 1 and kPagedShared. Tiles that 32 bits do not hold, of sequences far longer
+// than was announced, are not shared out: the call does nothing but report them.
 __device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, int block_rows, int* before, int4* of, int threads) {
     for (int s = threadIdx.x; s < a.r.sequences; s += threads) {
         int tiles, items;
         const PagedSequence q = paged_sequence(a.c, a.r, s);
         paged_weight(a, q, block_rows, &tiles, &items);
-        before[s + 1] = tiles * items;
+        before[s + 1] = static_cast<int>(min(static_cast<long long>(tiles) * items, 0x7fffffffLL));
         of[s] = make_int4(q.first, q.news, q.length, tiles);
         if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
     }
     if (threadIdx.x == 0) before[0] = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
-        int sum = 0;
+        long long sum = 0;
         for (int s0 = 0; s0 < a.r.sequences; s0 += 32) {
             const int s = s0 + threadIdx.x;
-            int v = s < a.r.sequences ? before[s + 1] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, v, o);
-                if (static_cast<int>(threadIdx.x) >= o) v += up;
-            }
-            if (s < a.r.sequences) before[s + 1] = sum + v;
-            sum += __shfl_sync(0xffffffffu, v, 31);
+            const long long v = sum + paged_detail::prefix(s < a.r.sequences ? before[s + 1] : 0);
+            if (s < a.r.sequences) before[s + 1] = static_cast<int>(v);
+            sum = __shfl_sync(0xffffffffu, v, 31);
         }
+        if (sum > 0x7fffffffLL && threadIdx.x == 0) before[a.r.sequences] = 0, atomicOr(a.c.status, kPagedBadPosition);
     }
     __syncthreads();
     return PagedShare{before[a.r.sequences], before, of};
 }
-__device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const PagedShare& w, long long tile, int block_rows) {
+__device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const PagedShare& w, int tile, int block_rows) {
     int lo = 0, hi = a.r.sequences - 1;  // the last sequence whose items begin at or before the tile
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -165,8 +170,14 @@ __device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const
         else hi = mid - 1;
     }
     const int4 of = w.of[lo];
-    const int i = static_cast<int>((tile - w.before[lo]) / of.w);
-    return PagedItem{lo, i % a.c.kv_heads, i / a.c.kv_heads * block_rows, w.before[lo] + static_cast<long long>(i) * of.w, of.w, PagedSequence{of.x, of.y, of.z, true}};
+    const int i = (tile - w.before[lo]) / of.w;
+    return PagedItem{lo, i % a.c.kv_heads, i / a.c.kv_heads * block_rows, w.before[lo] + i * of.w, of.w, PagedSequence{of.x, of.y, of.z, true}};
+}
+
+__device__ __forceinline__ int paged_share_of(int total, int blocks, int b) { return total / blocks * b + min(b, total % blocks); }  // block b's first tile
+__device__ __forceinline__ int paged_block_of(int total, int blocks, int x) {  // the block that has tile x
+    const int each = total / blocks, more = total % blocks, bound = (each + 1) * more;
+    return x < bound ? x / (each + 1) : more + (x - bound) / max(each, 1);
 }
 
 template <int TYPE, int BLOCKS> __host__ __device__ constexpr int paged_rows_bytes() { return kPagedTile * BLOCKS * paged_row_bytes(TYPE); }  // keys or values of a tile
@@ -253,12 +264,12 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    long long at = 0, until = 1, first = 0;  // this block's tiles among all
+    int at = 0, until = 1, first = 0;  // this block's tiles among all
     PagedShare shared{0, s_before, s_of};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (a.share) {
         shared = paged_share_begin(a, F::kRows, s_before, s_of, kThreads);
-        at = first = shared.total * blockIdx.x / gridDim.x, until = shared.total * (blockIdx.x + 1) / gridDim.x;
+        at = first = paged_share_of(shared.total, gridDim.x, blockIdx.x), until = paged_share_of(shared.total, gridDim.x, blockIdx.x + 1);
     }
     int base0 = 0, base1 = 0;  // units that the rings have seen
     while (at < until) {
@@ -268,7 +279,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     if (a.share) {
         const PagedItem item = paged_item_at(a, shared, at, F::kRows);
         seq = item.seq, kvh = item.kvh, r0 = item.rows0, sq = item.q;
-        const int t = static_cast<int>(at - item.begin), n = static_cast<int>(min(static_cast<long long>(item.tiles - t), until - at));
+        const int t = at - item.begin, n = min(item.tiles - t, until - at);
         range = paged_seen(a, sq);
         range.end = min(range.end, range.begin + (t + n) * kPagedTile), range.begin += t * kPagedTile;
         if (n < item.tiles) parts_place = static_cast<int>(blockIdx.x) * 2 + (at == first ? 0 : 1);
@@ -380,22 +391,35 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                         mma<BF>(sc[n], k, b[0], b[1]);
                     }
                 };
+                // (fragments are fetched a few at a time, before they are used: loads stay in their order, and one by one each would be waited for)
+                constexpr int kFrags = 4;
+                if constexpr (Q8) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    uint32_t r[4];
-                    if constexpr (Q8) {
-                        if ((ks & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice ks, then of slice ks + 1
-                            ldsm4(r, keys + paged_row_at(TYPE, BLOCKS, ks >> 2, row) + ((((ks & 3) + (lane >> 4)) ^ swz) << 4));
+                    for (int k0_ = 0; k0_ < KS / 2; k0_ += kFrags < KS / 2 ? kFrags : KS / 2) {
+                        constexpr int kHere = kFrags < KS / 2 ? kFrags : KS / 2;
+                        uint32_t r[kHere][4];  // matrices: positions 0-7 and 8-15 of a slice, then of the next slice
+#pragma unroll
+                        for (int k = 0; k < kHere; ++k) {
+                            const int ks = (k0_ + k) * 2;
+                            ldsm4(r[k], keys + paged_row_at(TYPE, BLOCKS, ks >> 2, row) + ((((ks & 3) + (lane >> 4)) ^ swz) << 4));
+                        }
+#pragma unroll
+                        for (int k = 0; k < kHere; ++k)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
-                                const uint32_t k[4] = {codes_to_half2(u0, 0x4140), codes_to_half2(u1, 0x4140), codes_to_half2(u0, 0x4342), codes_to_half2(u1, 0x4342)};
-                                score(k, ks + h);
+                                const uint32_t u0 = r[k][h * 2] ^ 0x80808080u, u1 = r[k][h * 2 + 1] ^ 0x80808080u;
+                                const uint32_t f[4] = {codes_to_half2(u0, 0x4140), codes_to_half2(u1, 0x4140), codes_to_half2(u0, 0x4342), codes_to_half2(u1, 0x4342)};
+                                score(f, (k0_ + k) * 2 + h);
                             }
-                        }
-                    } else {  // positions 0-7 and 8-15 of the slice's first 8 values, then of the others
-                        ldsm4(r, keys + paged_row_at(TYPE, BLOCKS, ks >> 2, row) + ((((ks & 3) * 2 + (lane >> 4)) ^ swz) << 4));
-                        score(r, ks);
+                    }
+                } else {
+#pragma unroll
+                    for (int k0_ = 0; k0_ < KS; k0_ += kFrags) {
+                        uint32_t r[kFrags][4];  // matrices: positions 0-7 and 8-15 of the slice's first 8 values, then of the others
+#pragma unroll
+                        for (int k = 0; k < kFrags; ++k) ldsm4(r[k], keys + paged_row_at(TYPE, BLOCKS, (k0_ + k) >> 2, row) + (((((k0_ + k) & 3) * 2 + (lane >> 4)) ^ swz) << 4));
+#pragma unroll
+                        for (int k = 0; k < kFrags; ++k) score(r[k], k0_ + k);
                     }
                 }
                 // the exponents, with masks
@@ -483,25 +507,37 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
             okay = __all_sync(0xffffffffu, mbar_wait(full + 8 * value_slot, ((n + 1) / U) & 1, abort_flag, a.spin_limit));
             if (!okay) break;
             if (there) {  // the weighted rows
+                if constexpr (Q8) {
+                    constexpr int kHere = KS / 2 < 4 ? KS / 2 : 4;
 #pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    uint32_t r[4];
-                    if constexpr (Q8) {
-                        if ((j & 1) == 0) {  // matrices: positions 0-7 and 8-15 of slice j, then of slice j + 1; a pair of bytes is two values of a position
-                            ldsm4_trans(r, values + paged_row_at(TYPE, BLOCKS, j >> 2, row) + ((((j & 3) + (lane >> 4)) ^ swz) << 4));
+                    for (int j0 = 0; j0 < KS / 2; j0 += kHere) {
+                        uint32_t r[kHere][4];  // matrices: positions 0-7 and 8-15 of slice j, then of slice j + 1; a pair of bytes is two values of a position
+#pragma unroll
+                        for (int k = 0; k < kHere; ++k) {
+                            const int j = (j0 + k) * 2;
+                            ldsm4_trans(r[k], values + paged_row_at(TYPE, BLOCKS, j >> 2, row) + ((((j & 3) + (lane >> 4)) ^ swz) << 4));
+                        }
+#pragma unroll
+                        for (int k = 0; k < kHere; ++k)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t u0 = r[h * 2] ^ 0x80808080u, u1 = r[h * 2 + 1] ^ 0x80808080u;
+                                const uint32_t u0 = r[k][h * 2] ^ 0x80808080u, u1 = r[k][h * 2 + 1] ^ 0x80808080u;
                                 const uint32_t v[4] = {codes_to_half2(u0, 0x4240), codes_to_half2(u0, 0x4341), codes_to_half2(u1, 0x4240), codes_to_half2(u1, 0x4341)};  // even values, odd values
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) mma<false>(o[j + h][n], v, pb[n][0], pb[n][1]);
+                                for (int n = 0; n < NT; ++n) mma<false>(o[(j0 + k) * 2 + h][n], v, pb[n][0], pb[n][1]);
                             }
-                        }
-                    } else {  // matrices: (positions 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-                        const int vrow = kg * 16 + (lane & 7) + ((lane >> 4) << 3);
-                        ldsm4_trans(r, values + paged_row_at(TYPE, BLOCKS, j >> 2, vrow) + ((((j & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+                    }
+                } else {
+                    const int vrow = kg * 16 + (lane & 7) + ((lane >> 4) << 3);  // matrices: (positions 0-7, values 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma<BF>(o[j][n], r, pb[n][0], pb[n][1]);
+                    for (int j0 = 0; j0 < KS; j0 += 4) {
+                        uint32_t r[4][4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) ldsm4_trans(r[k], values + paged_row_at(TYPE, BLOCKS, (j0 + k) >> 2, vrow) + (((((j0 + k) & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma<BF>(o[j0 + k][n], r[k], pb[n][0], pb[n][1]);
                     }
                 }
             }
@@ -649,33 +685,42 @@ __device__ __forceinline__ void paged_store_row(unsigned char* out, int type, co
     }
 }
 
-// The block of G whose share of W tiles has tile x.
-__device__ __forceinline__ int paged_block_of(long long x, long long total, int blocks) { return static_cast<int>(((x + 1) * blocks - 1) / total); }
-// Joins the segments of the items that were cut: a block of 8 warps per (token, query head); `blocks`, `block_rows`: of the launch whose tiles were shared out.
+// Joins the segments of the items that were cut. Where one block's tiles end and the next one's begin inside an item (`cuts` such places in the item), a block of this kernel stands for that place, and
+// takes every cuts-th row of the item: a warp a row, or all warps a row where there are many segments. `blocks`, `block_rows`: of the launch whose tiles were shared out.
 template <int BLOCKS>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnArgs a, int blocks, int block_rows) {
     constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
     __shared__ float shared[8 * 32 * (kPer + 1)];
     __shared__ int before[kPagedShared + 1];
     __shared__ int4 of[kPagedShared];
-    const int heads = a.c.kv_heads * a.group, lane = threadIdx.x & 31, t = blockIdx.x / heads, h = blockIdx.x % heads;
-    const int s = paged_sequence_of(a.r, t);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x + 1;
     const PagedShare w = paged_share_begin(a, block_rows, before, of, 256);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the segments are still being worked on; what was read above is input. Every block waits, so that none ends before them
-    if (s < 0) return;
-    const PagedSequence sq = paged_sequence(a.c, a.r, s);
-    if (!sq.ok || t < sq.first || t >= sq.first + sq.news || sq.news < a.few || sq.news > a.many) return;
-    int tiles, items;
-    paged_weight(a, sq, block_rows, &tiles, &items);
-    const int kvh = h / a.group, r = (t - sq.first) * a.group + h % a.group;
-    const long long begin = w.before[s] + static_cast<long long>(r / block_rows * a.c.kv_heads + kvh) * tiles;
-    const int b0 = paged_block_of(begin, w.total, blocks), b1 = paged_block_of(begin + tiles - 1, w.total, blocks), row = r % block_rows;
-    if (b0 == b1) return;  // it was whole
-    const int place0 = w.total * b0 / blocks == begin ? 0 : 1;
-    float x[kPer];
-    paged_join<HD, 8>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + row; }, b1 - b0 + 1, x, shared);
-    if (threadIdx.x >= 32) return;
-    paged_store_row(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x);
+    const int x = paged_share_of(w.total, blocks, b);
+    if (x <= 0 || x >= w.total) return;
+    const PagedItem item = paged_item_at(a, w, x, block_rows);
+    if (item.begin >= x) return;  // the place is between two items
+    const int b0 = paged_block_of(w.total, blocks, item.begin), b1 = paged_block_of(w.total, blocks, item.begin + item.tiles - 1), cuts = b1 - b0;
+    const int place0 = paged_share_of(w.total, blocks, b0) == item.begin ? 0 : 1, rows = min(block_rows, item.q.news * a.group - item.rows0), mine = b - b0 - 1;
+    if (mine >= cuts) return;  // (a block without tiles of its own)
+    auto out = [&](int r, const float (&v)[kPer]) {
+        const size_t t = static_cast<size_t>(item.q.first) + (item.rows0 + r) / a.group;
+        const int h = item.kvh * a.group + (item.rows0 + r) % a.group;
+        paged_store_row(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, v);
+    };
+    float v[kPer];
+    if (cuts < 8) {
+        for (int r = mine + cuts * warp; r < rows; r += cuts * 8) {
+            paged_join<HD, 1>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, nullptr);
+            out(r, v);
+        }
+    } else {
+        for (int r = mine; r < rows; r += cuts) {
+            __syncthreads();
+            paged_join<HD, 8>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, shared);
+            if (warp == 0) out(r, v);
+        }
+    }
 }
 
 }  // namespace qtb

@@ -20,12 +20,16 @@
 
 namespace qtb {
 
-// Which rows and ranges the blocks of a launch take. Row blocks count from the last one of a sequence, which sees most (order 0, 1, ...); m = KV heads x sequences of each. One block of threads
+// Which rows and ranges the blocks of a launch take. Where all sequences have as many new tokens, row blocks count from the last one of a sequence, which sees most (order 0, 1, ...), and m = KV heads x
+// sequences have each order. Where they differ (a prompt among sequences that answer), the row blocks that are there count through the sequences, each from its last one, and m = KV heads have each
+// (orders and sequences would be mostly blocks without rows: with 257 tokens next to seven single ones 1152 blocks were launched for 144 with work, 35 us instead of 27, and 21 instead of 7 to join them). One block of threads
 // per multiprocessor, so that what matters is the last of them to end: as long as row blocks fill whole waves they are taken whole; the rest, or all where there are too few,
 // are cut into ranges of equal length, whose results meet in the workspace.
 constexpr int kPagedMapped = 160;  // most (row block, range) pairs of a mapped schedule
 struct PagedSchedule {
     int m, whole, cut;                       // blocks x m: order x < whole, all of its range; else order whole + (x - whole) / cut, range (x - whole) % cut of cut
+    int even;                                // all sequences have as many new tokens
+    int orders;                              // row blocks that there are at most (times m)
     int mapped;                              // few row blocks, of different lengths: order[x], range[x] of ranges[x] instead
     unsigned char order[kPagedMapped], range[kPagedMapped], ranges[kPagedMapped], at[kPagedMapped];  // at: the first x of an order
     float* part_o;                           // [x - whole][m][rows of a block][head_dim] for what is cut; mapped: [range][KV head][packed tokens x group][head_dim]
@@ -38,6 +42,34 @@ __device__ __forceinline__ PagedPart paged_part(const PagedSchedule& g, int x) {
     if (g.mapped) return PagedPart{g.order[x], g.range[x], g.ranges[x], x};
     if (x < g.whole) return PagedPart{x, 0, 1, 0};
     return PagedPart{g.whole + (x - g.whole) / g.cut, (x - g.whole) % g.cut, g.cut, x - g.whole};
+}
+// The row blocks of sequence s that this launch serves.
+__device__ __forceinline__ int paged_row_blocks(const PagedAttnArgs& a, int s, int rows) {
+    const PagedSequence q = paged_sequence(a.c, a.r, s);
+    if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
+    return q.ok && q.news >= a.few && q.news <= a.many ? (q.news * a.group + rows - 1) / rows : 0;
+}
+// The sequence that has the x-th row block of all, and which of its own it is, or the sequence -1; by all lanes of a warp. And the row blocks of the sequences before s.
+__device__ __forceinline__ int2 paged_row_block(const PagedAttnArgs& a, int x, int rows) {
+    const int lane = threadIdx.x & 31;
+    long long sum = 0;
+    for (int s0 = 0; s0 < a.r.sequences; s0 += 32) {
+        const int mine = s0 + lane < a.r.sequences ? paged_row_blocks(a, s0 + lane, rows) : 0;
+        const long long until = sum + paged_detail::prefix(mine);
+        const unsigned int there = __ballot_sync(0xffffffffu, until > x);
+        if (there) {
+            const int first = __ffs(there) - 1;
+            return make_int2(s0 + first, static_cast<int>(x - __shfl_sync(0xffffffffu, until - mine, first)));
+        }
+        sum = __shfl_sync(0xffffffffu, until, 31);
+    }
+    return make_int2(-1, 0);
+}
+__device__ __forceinline__ long long paged_row_blocks_before(const PagedAttnArgs& a, int s, int rows) {
+    const int lane = threadIdx.x & 31;
+    long long sum = 0;
+    for (int s0 = 0; s0 < s; s0 += 32) sum += __shfl_sync(0xffffffffu, paged_detail::prefix(s0 + lane < s ? paged_row_blocks(a, s0 + lane, rows) : 0), 31);
+    return sum;
 }
 // The row of the workspace that has the result of row r (`local` of its block) for a part.
 __device__ __forceinline__ size_t paged_part_row(const PagedAttnArgs& a, const PagedSchedule& g, const PagedSequence& q, const PagedPart& part, int which, int kvh, int r, int local, int rows) {
@@ -158,13 +190,16 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const PagedPart part = paged_part(g, static_cast<int>(blockIdx.x) / g.m);
-    const int which = static_cast<int>(blockIdx.x) % g.m, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
-    const PagedSequence sq = paged_sequence(a.c, a.r, seq);
+    const int which = static_cast<int>(blockIdx.x) % g.m, kvh = which % a.c.kv_heads;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may come up beside the last wave; it waits for this launch's end before it reads
+    const int2 own = g.even ? make_int2(which / a.c.kv_heads, part.order) : paged_row_block(a, part.order, M::kRows);
+    if (own.x < 0) return;
+    const PagedSequence sq = paged_sequence(a.c, a.r, own.x);
     if (!sq.ok || sq.news < a.few || sq.news > a.many) {
         if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
         return;
     }
-    const int rows = sq.news * a.group, block = (rows + M::kRows - 1) / M::kRows - 1 - part.order, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);
+    const int rows = sq.news * a.group, block = (rows + M::kRows - 1) / M::kRows - 1 - own.y, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);
     if (block < 0) return;
     const PagedRange range = paged_part_range(a, sq, r0 / a.group, (r1 - 1) / a.group + 1, part.range, part.ranges, KT);
     const int p0 = sq.length - sq.news, tiles = range.end > range.begin ? (range.end - range.begin + KT - 1) / KT : 0, units = tiles * NT;
@@ -191,7 +226,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
         if constexpr (M::kSplitRegs) registers_down<M::kRestRegs>();
         if (warp == M::kLoadWarp) {
             // ---- pages to shared memory: per tile of positions the keys' rows, then the values' ----
-            const int* table = a.r.table + static_cast<size_t>(seq) * a.r.stride;
+            const int* table = a.r.table + static_cast<size_t>(own.x) * a.r.stride;
             const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
             constexpr int kRing = Q8 ? RW : RS;
             auto page_of = [&](int k0) {  // lane i: the page of the tile's piece i
@@ -642,28 +677,27 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
     }
 }
 
-// Joins the ranges of the row blocks that were cut: a warp per row, in the order of the ranges. Grid (rows / 8, m, row blocks that were cut, mapped: all of them).
+// Joins the ranges of the row blocks that were cut: a warp per packed token and query head, in the order of the ranges.
 template <int BLOCKS>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g, int kRows) {
     using namespace paged_detail;
     constexpr int HD = BLOCKS * kPagedBlock, kPer = HD / 32;
-    const int lane = threadIdx.x & 31, local = blockIdx.x * 8 + (threadIdx.x >> 5), which = blockIdx.y, kvh = which % a.c.kv_heads, seq = which / a.c.kv_heads;
-    int x = 0, order = blockIdx.z, ranges = g.cut;
-    if (g.mapped) {
-        x = g.at[order];
-        ranges = g.ranges[x];
-    } else {
-        x = order * g.cut, order += g.whole;
-    }
+    const int heads = a.group * a.c.kv_heads, lane = threadIdx.x & 31;
+    const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int token = static_cast<int>(row / heads), h = static_cast<int>(row % heads), kvh = h / a.group;
+    const int seq = token < a.r.tokens ? paged_sequence_of(a.r, token) : -1;
+    PagedSequence sq{};
+    if (seq >= 0) sq = paged_sequence(a.c, a.r, seq);
+    const int rows = sq.news * a.group, r = (token - sq.first) * a.group + h % a.group, own = (rows + kRows - 1) / kRows - 1 - r / kRows;
+    const long long order = g.even || seq < 0 ? own : own + paged_row_blocks_before(a, seq, kRows);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // what was read above is input. Every block waits, so that none ends before the launch that it joins
+    if (!sq.ok || sq.news < a.few || sq.news > a.many || token < sq.first || token >= sq.first + sq.news || order >= g.orders) return;
+    const int x = g.mapped ? g.at[order] : static_cast<int>(order - g.whole) * g.cut, ranges = g.mapped ? g.ranges[x] : x < 0 ? 1 : g.cut;
     if (ranges == 1) return;
-    const PagedSequence sq = paged_sequence(a.c, a.r, seq);
-    if (!sq.ok || sq.news < a.few || sq.news > a.many) return;
-    const int rows = sq.news * a.group, block = (rows + kRows - 1) / kRows - 1 - order, r = block * kRows + local;
-    if (block < 0 || r >= rows) return;
     float x_row[kPer];
-    paged_join<HD, 1>(g.part_o, g.part_ml, [&](int i) { return paged_part_row(a, g, sq, PagedPart{order, i, ranges, x + i}, which, kvh, r, local, kRows); }, ranges, x_row, nullptr);
-    const size_t token = static_cast<size_t>(sq.first) + r / a.group;
-    paged_store_row(static_cast<unsigned char*>(a.out) + (token * a.o_token + (kvh * a.group + r % a.group) * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x_row);
+    paged_join<HD, 1>(g.part_o, g.part_ml,
+                      [&](int i) { return paged_part_row(a, g, sq, PagedPart{0, i, ranges, x + i}, g.even ? seq * a.c.kv_heads + kvh : kvh, kvh, r, r % kRows, kRows); }, ranges, x_row, nullptr);
+    paged_store_row(static_cast<unsigned char*>(a.out) + (static_cast<size_t>(token) * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, x_row);
 }
 
 }  // namespace qtb

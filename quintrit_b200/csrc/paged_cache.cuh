@@ -72,7 +72,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedView& c, cons
     const bool fits = q.first >= 0 && q.first <= end && end <= r.tokens && q.length >= 0 && q.length <= (static_cast<long long>(r.stride) << c.page_log2);
     q.news = fits ? end - q.first : 0;
     q.ok = q.news > 0;
-    if (!fits && (threadIdx.x & 31) == 0) atomicOr(c.status, kPagedBadPosition);
+    if (!fits) atomicOr(c.status, kPagedBadPosition);
     return q;
 }
 
