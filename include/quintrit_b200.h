@@ -542,6 +542,17 @@ int quintrit_b200_paged_attention_workspace(const quintrit_b200_paged_cache_t* c
 int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, const quintrit_b200_paged_attention_t* args,
                                          void* stream);
 
+/* A batch (above) whose sequences share one paged cache of `pages` pages of page_tokens positions, of type F16, BF16 or Q8: a sequence takes pages as it grows and gives them back when it is rewound, so
+ * that the memory holds the tokens that there are instead of the context length for every sequence. quintrit_b200_batch_prefill, _step, _rewind, _info and _free work as before; their passes append to
+ * and attend over the pages by the functions above. Results are those of 16-bit queries and weights (and, with Q8, of 8-bit keys and values): close to, not bit for bit, those of the batch
+ * above. QUINTRIT_ERR_UNSUPPORTED for a layered model or a head_dim other than 64, 128 and 256. A call that finds too few free pages gives QUINTRIT_ERR_CONTEXT_OVERFLOW and leaves everything as
+ * it was. A key or value that is not finite is stored as quintrit_b200_paged_cache_status says; the call that stored it ends with QUINTRIT_ERR_INVALID_VALUE, its tokens taken all the same. */
+int quintrit_b200_batch_create_paged(quintrit_b200_decoder_t* decoder, uint32_t sequences, uint32_t pages, uint32_t page_tokens, int32_t type, quintrit_b200_batch_t** out_batch);
+/* The pages of a paged batch's cache, those that no sequence has, and the positions of a page (any pointer may be NULL). */
+int quintrit_b200_batch_pages(const quintrit_b200_batch_t* batch, uint32_t* out_pages, uint32_t* out_free, uint32_t* out_page_tokens);
+/* What a sequence has cached in one layer, as floats: keys (rotated) and values [tokens][kv_heads][head_dim] in host memory (either may be NULL; capacities count floats). */
+int quintrit_b200_batch_read_cache(quintrit_b200_batch_t* batch, uint32_t layer, uint32_t sequence, float* keys, size_t keys_capacity, float* values, size_t values_capacity);
+
 /* ---- batched projection on the tensor cores: out[b][n] = sum_k trit[n][k] * act[b][k] for `batch` int8 activation vectors
  * ([batch][cols], row-major), the integers quintrit_b200_gemv_i32 gives vector by vector (so every vector may carry its own
  * activation scale, as the tokens of a prompt do: quintrit-runtime/src/layer.rs:123-177 per token). out is [batch][rows]. The

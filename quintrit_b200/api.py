@@ -124,6 +124,9 @@ def load_library(build_if_missing: bool = True) -> C.CDLL:
     l.quintrit_b200_decoder_prefill.argtypes = [C.c_void_p, C.POINTER(C.c_uint32), _sz, C.c_uint32, _f32p, _sz, C.POINTER(C.c_uint32)]
     _u32p = C.POINTER(C.c_uint32)
     l.quintrit_b200_batch_create.argtypes = [C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p)]
+    l.quintrit_b200_batch_create_paged.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, C.POINTER(C.c_void_p)]
+    l.quintrit_b200_batch_pages.argtypes = [C.c_void_p, _u32p, _u32p, _u32p]
+    l.quintrit_b200_batch_read_cache.argtypes = [C.c_void_p, C.c_uint32, C.c_uint32, _f32p, _sz, _f32p, _sz]
     l.quintrit_b200_batch_free.argtypes = [C.c_void_p]
     l.quintrit_b200_batch_free.restype = None
     l.quintrit_b200_batch_info.argtypes = [C.c_void_p, _u32p, _u32p, _u32p, _sz]
@@ -502,12 +505,35 @@ class Decoder:
 class Batch:
     """Several sequences of one model decoded together (``quintrit_b200_batch_*``): every sequence has its own KV cache and
     position; a step feeds one token per listed sequence through one batched pass over the weights. The decoder must
-    outlive the batch and is not used by another thread meanwhile."""
+    outlive the batch and is not used by another thread meanwhile.
 
-    def __init__(self, decoder: "Decoder", sequences: int):
+    With ``pages`` the sequences share one cache of that many pages of ``page_tokens`` positions, stored as ``cache``
+    ("f16", "bf16" or "q8"): a sequence takes pages as it grows and gives them back when it is rewound."""
+
+    def __init__(self, decoder: "Decoder", sequences: int, pages: int | None = None, page_tokens: int = 64, cache: str = "f16"):
         self._h = C.c_void_p()
         self.decoder, self.sequences, self.vocab = decoder, sequences, decoder.vocab
-        _check(load_library().quintrit_b200_batch_create(decoder._h, sequences, C.byref(self._h)))
+        if pages is None:
+            _check(load_library().quintrit_b200_batch_create(decoder._h, sequences, C.byref(self._h)))
+            return
+        kinds = {"f16": 1, "bf16": 2, "q8": 3}
+        if cache not in kinds:
+            raise ValueError(f"cache type {cache!r}: 'f16', 'bf16' or 'q8'")
+        _check(load_library().quintrit_b200_batch_create_paged(decoder._h, sequences, pages, page_tokens, kinds[cache], C.byref(self._h)))
+
+    def pages(self):
+        """A paged batch's (pages, free pages, positions of a page)."""
+        v = [C.c_uint32(0) for _ in range(3)]
+        _check(load_library().quintrit_b200_batch_pages(self._h, *[C.byref(x) for x in v]))
+        return tuple(x.value for x in v)
+
+    def read_cache(self, layer: int, sequence: int):
+        """What a sequence of a paged batch has cached in one layer: float32 (keys, values), each [tokens][values of all KV heads]."""
+        i = self.decoder.info()
+        kv_dim = i["num_kv_heads"] * i["head_dim"]
+        k, v = (np.zeros((int(self.positions()[sequence]) if 0 <= sequence < self.sequences else 0, kv_dim), np.float32) for _ in range(2))
+        _check(load_library().quintrit_b200_batch_read_cache(self._h, layer, sequence, _p(k, _f32p), k.size, _p(v, _f32p), v.size))
+        return k, v
 
     def positions(self) -> np.ndarray:
         out = np.zeros(self.sequences, np.uint32)

@@ -5,6 +5,7 @@
 #include <sys/stat.h>
 
 #include <algorithm>
+#include <memory>
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
@@ -216,6 +217,7 @@ int check_kernel_status(unsigned int* d_counters) {  // after a synchronisation
 }  // namespace
 
 #include "decoder.cuh"
+#include "paged_batch.cuh"
 #include "layered.cuh"
 #include "moe.cuh"
 #include "gguf.hpp"
@@ -2455,11 +2457,63 @@ struct BatchTarget {
     bool own = true;                      // the decoder's own cache: a full chunk may be replayed as the captured graph
     const LayeredStore* layered = nullptr;  // layered models: the sequence store and the slot of a prompt's sequence
     int slot = 0;
+    PagedBatch* paged = nullptr;            // a paged cache instead of kc / vc: the rows of the pass and a workspace of its attention
+    quintrit_b200_paged_rows_t rows{};
+    void* space = nullptr;
+    size_t space_bytes = 0;
 };
 BatchTarget own_target(quintrit_b200_decoder* d) {
     BatchTarget t;
     t.kc = d->kc, t.vc = d->vc, t.pos = d->pf.pos;
     return t;
+}
+
+// A layer's attention over a paged cache: the projections' sums as floats, rotation and append, attention, and the codes of the output projection. The rows of floats and the rotated
+// queries lie where the contiguous cache's attention keeps the parts of its results.
+int paged_layer_attention(quintrit_b200_decoder* d, int l, int n, const BatchTarget& tg, const RopeKvArgs& rk) {
+    cudaStream_t s = d->stream;
+    quintrit_b200_paged_cache_t* cache = tg.paged->cache;
+    const size_t qd = d->q_dim, kvd = d->kv_dim, hd = d->head_dim, qkv = qd + 2 * kvd;
+    float *x = d->pf.part_acc, *q = x + size_t(n) * qkv;
+    paged_sums_kernel<<<dim3(static_cast<unsigned>((qkv + 1023) / 1024), 1, n), 256, 0, s>>>(rk, x);
+    QTB_LAUNCH_CHECK();
+    quintrit_b200_paged_append_t ap{};
+    ap.struct_size = sizeof ap, ap.type = QUINTRIT_B200_F32, ap.q_out_type = cache->type == QUINTRIT_B200_Q8 ? QUINTRIT_B200_F32 : cache->type, ap.q_heads = d->q_heads;
+    ap.d_q = x, ap.d_k = x + qd, ap.d_v = x + qd + kvd, ap.d_q_out = q;
+    ap.q_token_stride = ap.k_token_stride = ap.v_token_stride = qkv, ap.q_head_stride = ap.k_head_stride = ap.v_head_stride = hd;
+    ap.out_token_stride = qd, ap.out_head_stride = hd;
+    ap.d_cos_sin = d->cos_sin, ap.positions = d->ctx, ap.rope_dims = d->rope_dims, ap.neox = rk.neox;
+    int rc = quintrit_b200_paged_append_device(cache, l, &tg.rows, &ap, s);
+    if (rc != QUINTRIT_OK) return rc;
+    quintrit_b200_paged_attention_t at{};
+    at.struct_size = sizeof at, at.q_type = ap.q_out_type, at.out_type = QUINTRIT_B200_F32, at.q_heads = d->q_heads;
+    at.d_q = q, at.q_token_stride = qd, at.q_head_stride = hd, at.d_out = d->pf.q, at.out_token_stride = qd, at.out_head_stride = hd;
+    at.scale = 1.0f / std::sqrt(static_cast<float>(hd)), at.d_workspace = tg.space, at.workspace_bytes = tg.space_bytes;
+    if ((rc = quintrit_b200_paged_attention_device(cache, l, &tg.rows, &at, s)) != QUINTRIT_OK) return rc;
+    paged_finish_kernel<<<dim3(1, 1, n), kRowThreads, qd * sizeof(float), s>>>(d->pf.q, static_cast<int>(qd), d->norms[l * 4 + 2], d->eps, d->pf.a8_q, d->pf.s_q);
+    QTB_LAUNCH_CHECK();
+    return QUINTRIT_OK;
+}
+
+// The rows of a prompt's chunk of n tokens that ends at position `end`, and a workspace for them.
+int paged_chunk_rows(quintrit_b200_decoder* d, int n, size_t end, BatchTarget* tg) {
+    PagedBatch* p = tg->paged;
+    tg->rows = quintrit_b200_paged_rows_t{sizeof(quintrit_b200_paged_rows_t), 1, static_cast<uint32_t>(n), static_cast<uint32_t>(n), static_cast<uint32_t>(end), p->stride, p->d_chunk, p->d_chunk + 2,
+                                          p->d_table + size_t(tg->slot) * p->stride};
+    size_t need = 0;
+    const int rc = quintrit_b200_paged_attention_workspace(p->cache, &tg->rows, d->q_heads, &need);
+    if (rc != QUINTRIT_OK) return rc;
+    if (need > p->chunk_bytes) {
+        QTB_CUDA(cudaStreamSynchronize(d->stream));
+        cudaFree(p->chunk_space);
+        p->chunk_space = nullptr, p->chunk_bytes = 0;
+        QTB_CUDA(cudaMalloc(&p->chunk_space, need));
+        p->chunk_bytes = need;
+    }
+    tg->space = p->chunk_space, tg->space_bytes = p->chunk_bytes;
+    paged_chunk_kernel<<<1, 1, 0, d->stream>>>(p->d_chunk, n, static_cast<int>(end));
+    QTB_LAUNCH_CHECK();
+    return QUINTRIT_OK;
 }
 
 int prefill_layers(quintrit_b200_decoder* d, int n, const BatchTarget& tg) {
@@ -2505,26 +2559,30 @@ int prefill_layers(quintrit_b200_decoder* d, int n, const BatchTarget& tg) {
         rk.q_dim = qd, rk.kv_dim = kvd, rk.head_dim = hd, rk.rope_dims = d->rope_dims, rk.neox = d->arch != QUINTRIT_B200_ARCH_LLAMA;
         rk.q_out = d->pf.q, rk.b_q = qd;
         if (qkv_views) rk.v_q = v_q, rk.v_k = v_k, rk.v_v = v_v;
-        rk.k_cache = tg.kc + static_cast<size_t>(l) * d->ctx * kvd;
-        rk.v_cache = tg.vc + static_cast<size_t>(l) * d->ctx * kvd;
-        if (rope_rows_fit(rk)) rope_kv_rows_kernel<<<dim3(((qd + 2 * kvd) / 8 + kRopeThreads - 1) / kRopeThreads, 1, n), kRopeThreads, 0, s>>>(rk);
-        else rope_kv_kernel<<<dim3(((qd + kvd) / 2 + kvd + 255) / 256, 1, n), 256, 0, s>>>(rk);
-        QTB_LAUNCH_CHECK();
-        AttnArgs at{};
-        at.q = d->pf.q, at.b_q = qd;
-        at.k_cache = rk.k_cache, at.v_cache = rk.v_cache, at.pos = tg.pos, at.seq = tg.seq;
-        at.head_dim = hd, at.kv_dim = kvd, at.gqa = d->q_heads / d->kv_heads, at.ctx = d->ctx, at.f32_values = d->f32_values;
-        at.scale = 1.0f / std::sqrt(static_cast<float>(hd));
-        at.part_acc = d->pf.part_acc, at.b_acc = d->q_heads * 4 * hd, at.part_ms = d->pf.part_ms, at.b_ms = d->q_heads * 8;
-        launch_attention(d, at, n, s, tg.end);
-        QTB_LAUNCH_CHECK();
-        AttnFinishArgs af{};
-        af.part_acc = d->pf.part_acc, af.b_acc = d->q_heads * 4 * hd, af.part_ms = d->pf.part_ms, af.b_ms = d->q_heads * 8, af.pos = tg.pos, af.seq = tg.seq;
-        af.q_heads = d->q_heads, af.head_dim = hd, af.ctx = d->ctx;
-        af.sub_norm_w = d->norms[l * 4 + 2], af.eps = d->eps;
-        af.q_out = d->pf.a8_q, af.b_q = qd, af.scale_out = d->pf.s_q, af.b_scale = 1;
-        launch_attn_finish_rows(af, n, s);
-        QTB_LAUNCH_CHECK();
+        if (tg.paged != nullptr) {
+            if ((rc = paged_layer_attention(d, l, n, tg, rk)) != QUINTRIT_OK) return rc;
+        } else {
+            rk.k_cache = tg.kc + static_cast<size_t>(l) * d->ctx * kvd;
+            rk.v_cache = tg.vc + static_cast<size_t>(l) * d->ctx * kvd;
+            if (rope_rows_fit(rk)) rope_kv_rows_kernel<<<dim3(((qd + 2 * kvd) / 8 + kRopeThreads - 1) / kRopeThreads, 1, n), kRopeThreads, 0, s>>>(rk);
+            else rope_kv_kernel<<<dim3(((qd + kvd) / 2 + kvd + 255) / 256, 1, n), 256, 0, s>>>(rk);
+            QTB_LAUNCH_CHECK();
+            AttnArgs at{};
+            at.q = d->pf.q, at.b_q = qd;
+            at.k_cache = rk.k_cache, at.v_cache = rk.v_cache, at.pos = tg.pos, at.seq = tg.seq;
+            at.head_dim = hd, at.kv_dim = kvd, at.gqa = d->q_heads / d->kv_heads, at.ctx = d->ctx, at.f32_values = d->f32_values;
+            at.scale = 1.0f / std::sqrt(static_cast<float>(hd));
+            at.part_acc = d->pf.part_acc, at.b_acc = d->q_heads * 4 * hd, at.part_ms = d->pf.part_ms, at.b_ms = d->q_heads * 8;
+            launch_attention(d, at, n, s, tg.end);
+            QTB_LAUNCH_CHECK();
+            AttnFinishArgs af{};
+            af.part_acc = d->pf.part_acc, af.b_acc = d->q_heads * 4 * hd, af.part_ms = d->pf.part_ms, af.b_ms = d->q_heads * 8, af.pos = tg.pos, af.seq = tg.seq;
+            af.q_heads = d->q_heads, af.head_dim = hd, af.ctx = d->ctx;
+            af.sub_norm_w = d->norms[l * 4 + 2], af.eps = d->eps;
+            af.q_out = d->pf.a8_q, af.b_q = qd, af.scale_out = d->pf.s_q, af.b_scale = 1;
+            launch_attn_finish_rows(af, n, s);
+            QTB_LAUNCH_CHECK();
+        }
         if ((rc = gemm_launch(mat(l, 3), d->pf.a8_q, n, d->pf.acc_o, s, 0, view(&v_o), st, d->pf.parts[3])) != QUINTRIT_OK) return rc;
         NormQuantArgs n2{};
         n2.x = d->pf.x, n2.b_x = H, n2.acc_prev = d->pf.acc_o, n2.b_acc = H, n2.scale_prev = d->pf.s_q, n2.ws_prev = sc[3];
@@ -2621,6 +2679,7 @@ int decoder_prefill(quintrit_b200_decoder* d, const uint32_t* tokens, size_t cou
         const int n = static_cast<int>(std::min<size_t>(kPrefillMax, count - c0));
         tg.end = pos0 + c0 + n;
         QTB_CUDA(cudaMemcpyAsync(d->pf.tokens, tokens + c0, size_t(n) * sizeof(uint32_t), cudaMemcpyHostToDevice, d->stream));
+        if (tg.paged != nullptr && (rc = paged_chunk_rows(d, n, tg.end, &tg)) != QUINTRIT_OK) return rc;
         if (tg.own) QTB_CUDA(cudaMemcpyAsync(d->d_history + pos0 + c0, d->pf.tokens, size_t(n) * sizeof(uint32_t), cudaMemcpyDeviceToDevice, d->stream));
         if ((rc = enqueue_prefill_chunk(d, n, pos0 + static_cast<uint32_t>(c0), c0 + n == count, tg)) != QUINTRIT_OK) return rc;
     }
@@ -3116,6 +3175,7 @@ struct quintrit_b200_batch {
     float* logits = nullptr;               // [n_seq][vocab] of the last step
     __half* x16 = nullptr;                 // [n_seq][hidden]: the final norm's output
     LayeredStore layered;                  // layered models: states and windows of the sequences instead of kc / vc
+    std::unique_ptr<PagedBatch> paged;     // a cache in pages that the sequences share, instead of kc / vc
     std::vector<uint32_t> host_pos;        // tokens cached per sequence
     std::vector<uint32_t> staged;          // host copy of a prompt's ids for the asynchronous copies
     std::vector<void*> allocs;
@@ -3142,6 +3202,12 @@ void destroy_batch(quintrit_b200_batch* b) {
     for (cudaGraphExec_t g : b->graph)
         if (g != nullptr) cudaGraphExecDestroy(g);
     for (void* p : b->allocs) cudaFree(p);
+    if (b->paged != nullptr) {
+        quintrit_b200_paged_cache_free(b->paged->cache);
+        cudaFree(b->paged->step_space);
+        cudaFree(b->paged->chunk_space);
+        cudaFreeHost(b->paged->host_status);
+    }
     if (prev >= 0) cudaSetDevice(prev);
     b->magic = 0;
     delete b;
@@ -3207,7 +3273,41 @@ int batch_head(quintrit_b200_batch* b, int n) {
 
 }  // namespace
 
-extern "C" int quintrit_b200_batch_create(quintrit_b200_decoder_t* decoder, uint32_t sequences, quintrit_b200_batch_t** out_batch) {
+namespace {
+
+struct PagedShape {
+    uint32_t pages, page_tokens;
+    int32_t type;
+};
+
+// The pages, tables and workspaces of a batch with a paged cache.
+int paged_batch_create(quintrit_b200_batch* b, const PagedShape& shape) {
+    quintrit_b200_decoder* d = b->d;
+    b->paged = std::make_unique<PagedBatch>();
+    PagedBatch* p = b->paged.get();
+    int rc = quintrit_b200_paged_cache_create(static_cast<uint32_t>(d->device), d->layers, shape.pages, shape.page_tokens, d->kv_heads, d->head_dim, shape.type, &p->cache);
+    if (rc != QUINTRIT_OK) return rc;
+    const size_t n = b->n_seq;
+    p->stride = static_cast<uint32_t>(p->pages_for(d->ctx));
+    p->pages.resize(n);
+    p->free.reserve(shape.pages);
+    for (uint32_t i = shape.pages; i > 0; --i) p->free.push_back(static_cast<int32_t>(i - 1));
+    if ((rc = batch_alloc(b, &p->d_table, n * p->stride)) != QUINTRIT_OK || (rc = batch_alloc(b, &p->d_rows_table, n * p->stride)) != QUINTRIT_OK ||
+        (rc = batch_alloc(b, &p->d_starts, n + 1)) != QUINTRIT_OK || (rc = batch_alloc(b, &p->d_lengths, n)) != QUINTRIT_OK || (rc = batch_alloc(b, &p->d_chunk, 4)) != QUINTRIT_OK)
+        return rc;
+    for (uint32_t k = 1; k <= n; ++k) {  // enough for a step of any number of sequences
+        const quintrit_b200_paged_rows_t rows{sizeof(quintrit_b200_paged_rows_t), k, k, 1, static_cast<uint32_t>(d->ctx), p->stride, p->d_starts, p->d_lengths, p->d_rows_table};
+        size_t need = 0;
+        if ((rc = quintrit_b200_paged_attention_workspace(p->cache, &rows, d->q_heads, &need)) != QUINTRIT_OK) return rc;
+        p->step_bytes = std::max(p->step_bytes, need);
+    }
+    if (p->step_bytes > 0) QTB_CUDA(cudaMalloc(&p->step_space, p->step_bytes));
+    QTB_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&p->host_status), 16, cudaHostAllocMapped));
+    *p->host_status = 0;
+    return QUINTRIT_OK;
+}
+
+int create_batch(quintrit_b200_decoder_t* decoder, uint32_t sequences, const PagedShape* paged, quintrit_b200_batch_t** out_batch) {
     return guard([&]() -> int {
         if (out_batch == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "out_batch is NULL");
         *out_batch = nullptr;
@@ -3216,6 +3316,8 @@ extern "C" int quintrit_b200_batch_create(quintrit_b200_decoder_t* decoder, uint
         quintrit_b200_decoder* d = decoder;
         if (sequences == 0 || sequences > static_cast<uint32_t>(kGemmMaxN)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "sequences must be in [1, %d], got %u", kGemmMaxN, sequences);
         if (!prefill_available(d)) return fail(QUINTRIT_ERR_UNSUPPORTED, "this decoder has no batched pass (block-scaled or tensor-parallel model)");
+        if (paged != nullptr && d->lay) return fail(QUINTRIT_ERR_UNSUPPORTED, "a layered model keeps its sequences' states and windows itself: no paged batch");
+        if (paged != nullptr && d->q_dim > 12288) return fail(QUINTRIT_ERR_UNSUPPORTED, "query rows of %d values are too long for a paged batch (12288 at most)", d->q_dim);
         DeviceGuard g(d->device);
         if ((rc = prefill_buffers(d)) != QUINTRIT_OK) return rc;
         if (!d->lay && (rc = decoder_gemm_prepare(d)) != QUINTRIT_OK) return rc;
@@ -3229,7 +3331,12 @@ extern "C" int quintrit_b200_batch_create(quintrit_b200_decoder_t* decoder, uint
             destroy_batch(b);
             return rc;
         }
-        if ((rc = batch_alloc(b, &b->kc, n * batch_cache_stride(d))) != QUINTRIT_OK || (rc = batch_alloc(b, &b->vc, n * batch_cache_stride(d))) != QUINTRIT_OK ||
+        if (paged != nullptr && (rc = paged_batch_create(b, *paged)) != QUINTRIT_OK) {
+            destroy_batch(b);
+            return rc;
+        }
+        const size_t contiguous = paged != nullptr ? 0 : n * batch_cache_stride(d);
+        if ((rc = batch_alloc(b, &b->kc, contiguous)) != QUINTRIT_OK || (rc = batch_alloc(b, &b->vc, contiguous)) != QUINTRIT_OK ||
             (rc = batch_alloc(b, &b->d_pos, n)) != QUINTRIT_OK || (rc = batch_alloc(b, &b->d_last, n)) != QUINTRIT_OK || (rc = batch_alloc(b, &b->d_slot, n)) != QUINTRIT_OK ||
             (rc = batch_alloc(b, &b->d_chosen, n)) != QUINTRIT_OK || (rc = batch_alloc(b, &b->logits, n * d->vocab)) != QUINTRIT_OK ||
             (rc = batch_alloc(b, &b->x16, n * d->hidden)) != QUINTRIT_OK) {
@@ -3238,6 +3345,62 @@ extern "C" int quintrit_b200_batch_create(quintrit_b200_decoder_t* decoder, uint
         }
         QTB_CUDA(cudaDeviceSynchronize());
         *out_batch = b;
+        return ok();
+    });
+}
+
+}  // namespace
+
+extern "C" int quintrit_b200_batch_create(quintrit_b200_decoder_t* decoder, uint32_t sequences, quintrit_b200_batch_t** out_batch) {
+    return create_batch(decoder, sequences, nullptr, out_batch);
+}
+
+extern "C" int quintrit_b200_batch_create_paged(quintrit_b200_decoder_t* decoder, uint32_t sequences, uint32_t pages, uint32_t page_tokens, int32_t type, quintrit_b200_batch_t** out_batch) {
+    const PagedShape shape{pages, page_tokens, type};
+    return create_batch(decoder, sequences, &shape, out_batch);
+}
+
+extern "C" int quintrit_b200_batch_pages(const quintrit_b200_batch_t* batch, uint32_t* out_pages, uint32_t* out_free, uint32_t* out_page_tokens) {
+    return guard([&]() -> int {
+        const int rc = check_batch(batch);
+        if (rc != QUINTRIT_OK) return rc;
+        if (batch->paged == nullptr) return fail(QUINTRIT_ERR_UNSUPPORTED, "this batch has no paged cache");
+        if (out_pages) *out_pages = batch->paged->cache->pages;
+        if (out_free) *out_free = static_cast<uint32_t>(batch->paged->free.size());
+        if (out_page_tokens) *out_page_tokens = batch->paged->cache->page_tokens;
+        return ok();
+    });
+}
+
+extern "C" int quintrit_b200_batch_read_cache(quintrit_b200_batch_t* batch, uint32_t layer, uint32_t sequence, float* keys, size_t keys_capacity, float* values, size_t values_capacity) {
+    return guard([&]() -> int {
+        int rc = check_batch(batch);
+        if (rc != QUINTRIT_OK) return rc;
+        quintrit_b200_decoder* d = batch->d;
+        PagedBatch* p = batch->paged.get();
+        if (p == nullptr) return fail(QUINTRIT_ERR_UNSUPPORTED, "this batch has no paged cache");
+        if (layer >= static_cast<uint32_t>(d->layers)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "layer %u of %d", layer, d->layers);
+        if (sequence >= static_cast<uint32_t>(batch->n_seq)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "sequence %u of %d", sequence, batch->n_seq);
+        if (keys == nullptr && values == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "keys and values are NULL");
+        const size_t count = batch->host_pos[sequence], kvd = d->kv_dim;
+        if ((keys != nullptr && keys_capacity < count * kvd) || (values != nullptr && values_capacity < count * kvd))
+            return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "%zu cached tokens have %zu values each in keys and values", count, kvd);
+        DeviceGuard g(d->device);
+        cudaStream_t s = d->stream;
+        float* d_k = d->pf.part_acc;  // (scratch between passes)
+        for (size_t c0 = 0; c0 < count;) {
+            const size_t n = std::min<size_t>(prefill_rows(d), count - c0);
+            float* d_v = d_k + n * kvd;
+            const quintrit_b200_paged_rows_t rows{sizeof(quintrit_b200_paged_rows_t), 1, static_cast<uint32_t>(n), static_cast<uint32_t>(n), static_cast<uint32_t>(c0 + n), p->stride, p->d_chunk,
+                                                  p->d_chunk + 2, p->d_table + size_t(sequence) * p->stride};
+            paged_chunk_kernel<<<1, 1, 0, s>>>(p->d_chunk, static_cast<int>(n), static_cast<int>(c0 + n));
+            QTB_LAUNCH_CHECK();
+            if ((rc = quintrit_b200_paged_read_device(p->cache, layer, &rows, QUINTRIT_B200_F32, keys ? d_k : nullptr, values ? d_v : nullptr, s)) != QUINTRIT_OK) return rc;
+            if (keys) QTB_CUDA(cudaMemcpyAsync(keys + c0 * kvd, d_k, n * kvd * sizeof(float), cudaMemcpyDeviceToHost, s));
+            if (values) QTB_CUDA(cudaMemcpyAsync(values + c0 * kvd, d_v, n * kvd * sizeof(float), cudaMemcpyDeviceToHost, s));
+            QTB_CUDA(cudaStreamSynchronize(s));
+            c0 += n;
+        }
         return ok();
     });
 }
@@ -3272,6 +3435,7 @@ extern "C" int quintrit_b200_batch_rewind(quintrit_b200_batch_t* batch, uint32_t
         QTB_CUDA(cudaMemcpyAsync(batch->d_pos + sequence, &position, sizeof position, cudaMemcpyHostToDevice, batch->d->stream));
         QTB_CUDA(cudaStreamSynchronize(batch->d->stream));
         batch->host_pos[sequence] = position;
+        if (batch->paged != nullptr) batch->paged->trim(sequence, position);
         return ok();
     });
 }
@@ -3293,7 +3457,23 @@ extern "C" int quintrit_b200_batch_prefill(quintrit_b200_batch_t* batch, uint32_
         if (logits != nullptr && logits_capacity < static_cast<size_t>(d->vocab)) return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "logits hold %zu values, the vocabulary has %d", logits_capacity, d->vocab);
         DeviceGuard g(d->device);
         b->staged.assign(tokens, tokens + count);
+        PagedBatch* p = b->paged.get();
+        if (p != nullptr) {
+            const size_t need = p->missing(sequence, size_t(pos) + count);
+            if (need > p->free.size()) return fail(QUINTRIT_ERR_CONTEXT_OVERFLOW, "%zu tokens take %zu more pages, %zu are free", count, need, p->free.size());
+            p->grow(sequence, size_t(pos) + count);
+        }
+        struct Trim {  // a call that fails gives the pages behind the sequence's tokens back
+            quintrit_b200_batch* b;
+            uint32_t sequence;
+            ~Trim() {
+                if (b->paged != nullptr) b->paged->trim(sequence, b->host_pos[sequence]);
+            }
+        } trim{b, sequence};
+        if (p != nullptr)
+            QTB_CUDA(cudaMemcpyAsync(p->d_table + size_t(sequence) * p->stride, p->pages[sequence].data(), p->pages[sequence].size() * sizeof(int32_t), cudaMemcpyHostToDevice, d->stream));
         BatchTarget tg;
+        tg.paged = p;
         tg.kc = b->kc + sequence * batch_cache_stride(d), tg.vc = b->vc + sequence * batch_cache_stride(d), tg.pos = d->pf.pos, tg.own = false;
         tg.layered = d->lay ? &b->layered : nullptr, tg.slot = static_cast<int>(sequence);
         if ((rc = decoder_prefill(d, b->staged.data(), count, pos, &tg)) != QUINTRIT_OK) return rc;
@@ -3304,6 +3484,7 @@ extern "C" int quintrit_b200_batch_prefill(quintrit_b200_batch_t* batch, uint32_
         if (out_token) QTB_CUDA(cudaMemcpyAsync(out_token, d->d_token, sizeof(uint32_t), cudaMemcpyDeviceToHost, d->stream));
         if ((rc = decoder_check_status(d)) != QUINTRIT_OK) return rc;
         b->host_pos[sequence] = next;
+        if (p != nullptr && (rc = quintrit_b200_paged_cache_status(p->cache)) != QUINTRIT_OK) return rc;
         return ok();
     });
 }
@@ -3329,6 +3510,15 @@ extern "C" int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint
             if (tokens != nullptr && tokens[z] >= static_cast<uint32_t>(d->vocab_full)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "token id %u is not below the vocabulary size %d", tokens[z], d->vocab_full);
         }
         if (logits != nullptr && logits_capacity < count * static_cast<size_t>(d->vocab)) return fail(QUINTRIT_ERR_BUFFER_TOO_SMALL, "logits hold %zu values, %zu are needed", logits_capacity, count * static_cast<size_t>(d->vocab));
+        PagedBatch* p = b->paged.get();
+        if (p != nullptr) {
+            size_t need = 0;
+            for (int z = 0; z < n; ++z) {
+                const uint32_t sq = sequences != nullptr ? sequences[z] : static_cast<uint32_t>(z);
+                need += p->missing(sq, size_t(b->host_pos[sq]) + 1);
+            }
+            if (need > p->free.size()) return fail(QUINTRIT_ERR_CONTEXT_OVERFLOW, "the step takes %zu more pages, %zu are free", need, p->free.size());
+        }
         DeviceGuard g(d->device);
         cudaStream_t s = d->stream;
         // The sequence list is always read from device memory (one graph per step size), so "all sequences in order" is written out; list and tokens travel by value.
@@ -3347,12 +3537,29 @@ extern "C" int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint
         batch_begin_kernel<<<1, kReportTokens, 0, s>>>(begin, b->d_slot, d->lay ? d->lay->tokens : d->pf.tokens, tokens != nullptr ? nullptr : b->d_last, n);
         QTB_LAUNCH_CHECK();
         BatchTarget tg;
+        if (p != nullptr) {
+            PagedStep step;
+            for (size_t k = 0; k < count; ++k) {
+                const uint32_t sq = begin.slot[k];
+                p->grow(sq, size_t(b->host_pos[sq]) + 1);
+                step.page[k] = p->pages[sq][b->host_pos[sq] / p->cache->page_tokens];
+            }
+            paged_step_kernel<<<n, 128, 0, s>>>(step, b->d_slot, b->d_pos, p->d_table, static_cast<int>(p->stride), static_cast<int>(p->cache->page_tokens), p->d_rows_table, p->d_starts, p->d_lengths);
+            QTB_LAUNCH_CHECK();
+            tg.paged = p, tg.space = p->step_space, tg.space_bytes = p->step_bytes;
+            tg.rows = quintrit_b200_paged_rows_t{sizeof(quintrit_b200_paged_rows_t), static_cast<uint32_t>(n), static_cast<uint32_t>(n), 1, static_cast<uint32_t>(d->ctx), p->stride, p->d_starts, p->d_lengths,
+                                                 p->d_rows_table};
+        }
         tg.kc = b->kc, tg.vc = b->vc, tg.pos = b->d_pos, tg.own = false;
         tg.seq.slot = slot, tg.seq.pos_stride = 1, tg.seq.cache_stride = batch_cache_stride(d);
         auto enqueue = [&]() -> int {
             int r = d->lay ? layered_batch_layers(b, n, tg) : prefill_layers(d, n, tg);
             if (r == QUINTRIT_OK) r = batch_head(b, n);
             if (r != QUINTRIT_OK) return r;
+            if (p != nullptr) {
+                paged_report_kernel<<<1, 1, 0, s>>>(p->cache->status, p->host_status);
+                QTB_LAUNCH_CHECK();
+            }
             advance_batch_kernel<<<1, kReportTokens, 0, s>>>(b->d_pos, b->d_last, b->d_chosen, slot, n, d->d_steps, d->d_counters + 2, d->report);
             QTB_LAUNCH_CHECK();
             return QUINTRIT_OK;
@@ -3389,6 +3596,7 @@ extern "C" int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint
         if (out_tokens)
             for (size_t k = 0; k < count; ++k) out_tokens[order[k]] = d->report->chosen[k];
         for (int z = 0; z < n; ++z) b->host_pos[sequences != nullptr ? sequences[z] : static_cast<uint32_t>(z)] += 1;
+        if (p != nullptr && *const_cast<volatile unsigned int*>(p->host_status) != 0 && (rc = quintrit_b200_paged_cache_status(p->cache)) != QUINTRIT_OK) return rc;
         return ok();
     });
 }

@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 
+import quintrit_b200 as q
 from quintrit_b200 import paged
 from quintrit_b200.paged import BF16, F16, F32, Q8, _AppendC, _AttentionC, _RowsC
 
@@ -141,3 +142,12 @@ def test_calls_without_tokens_do_nothing():
 def test_no_cache_type_of_another_name():
     with pytest.raises(ValueError):
         paged.PagedCache(1, 1, 16, 1, 64, "f32")
+
+
+def test_paged_batches_refuse_what_is_no_batch():
+    lib = q.load_library()
+    out = C.c_void_p(5)
+    assert lib.quintrit_b200_batch_create_paged(None, 1, 1, 16, F16, None) == NULL
+    assert lib.quintrit_b200_batch_create_paged(None, 1, 1, 16, F16, C.byref(out)) == HANDLE and not out.value
+    assert lib.quintrit_b200_batch_pages(None, None, None, None) == HANDLE
+    assert lib.quintrit_b200_batch_read_cache(None, 0, 0, None, 0, None, 0) == HANDLE
