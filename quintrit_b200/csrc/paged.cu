@@ -77,23 +77,25 @@ void destroy(quintrit_b200_paged_cache* c) {
 }
 
 struct AppendKernel {
-    static int groups(const PagedAppendArgs& a, int heads) { return (a.q_heads + heads - 1) / heads + 2 * ((a.c.kv_heads + heads - 1) / heads); }
+    static constexpr int kValues = 16;  // of a thread
+    static int heads(const PagedAppendArgs& a) { return a.q_heads + 2 * a.c.kv_heads; }
     template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_append_kernel<LANES, TYPE, U>; }
 };
 struct ReadKernel {
-    static int groups(const PagedReadArgs& a, int heads) { return (2 * a.c.kv_heads + heads - 1) / heads; }
+    static constexpr int kValues = 8;
+    static int heads(const PagedReadArgs& a) { return 2 * a.c.kv_heads; }
     template <int LANES, int TYPE, int U> static constexpr auto of() { return paged_read_kernel<LANES, TYPE, U>; }
 };
-// A warp takes four groups of heads where that leaves a few warps for every place of the device, else one.
-template <typename Kernel, int LANES, int TYPE, typename Args>
-int launch_rows_of(const Args& a, uint32_t tokens, int heads, int sm_count, void* stream) {
-    constexpr int kHeads = 32 / LANES, kWarps = kPagedRowThreads / 32;
-    const int groups = Kernel::groups(a, kHeads);
-    const long long one = static_cast<long long>(tokens) * groups, four = static_cast<long long>(tokens) * ((groups + 3) / 4);
-    if (one > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", tokens, heads);
-    const bool many = four >= 64LL * sm_count;
-    auto kernel = many ? Kernel::template of<LANES, TYPE, 4>() : Kernel::template of<LANES, TYPE, 1>();
-    kernel<<<static_cast<unsigned int>(((many ? four : one) + kWarps - 1) / kWarps), kPagedRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+// A warp takes several groups of heads where that leaves a few warps for every place of the device, else one.
+template <typename Kernel, int HD, int TYPE, typename Args>
+int launch_rows_of(const Args& a, uint32_t tokens, int sm_count, void* stream) {
+    constexpr int LANES = HD / Kernel::kValues, kHeads = 32 / LANES, kWarps = kPagedRowThreads / 32, U = Kernel::kValues == 16 ? 2 : 4;
+    const int groups = (Kernel::heads(a) + kHeads - 1) / kHeads;
+    const long long one = static_cast<long long>(tokens) * groups, more = static_cast<long long>(tokens) * ((groups + U - 1) / U);
+    if (one > 0x7fffff00LL) return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u tokens of %d heads are too many for one call", tokens, Kernel::heads(a));
+    const bool many = more >= 64LL * sm_count;
+    auto kernel = many ? Kernel::template of<LANES, TYPE, U>() : Kernel::template of<LANES, TYPE, 1>();
+    kernel<<<static_cast<unsigned int>(((many ? more : one) + kWarps - 1) / kWarps), kPagedRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
@@ -402,12 +404,13 @@ extern "C" int quintrit_b200_paged_append_device(quintrit_b200_paged_cache_t* ca
         a.v_head = args->v_head_stride, a.o_token = args->out_token_stride, a.o_head = args->out_head_stride;
         a.q_norm = args->d_q_norm, a.k_norm = args->d_k_norm, a.eps = args->norm_eps;
         a.cos_sin = args->d_cos_sin, a.rope = static_cast<int>(args->rope_dims), a.positions = static_cast<int>(args->positions), a.neox = args->neox != 0;
-        a.vector = a.rope % (a.neox ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0;
+        const bool pieces = reinterpret_cast<uintptr_t>(a.cos_sin) % 16 == 0 && a.rope % 8 == 0;
+        a.turn = a.cos_sin == nullptr ? kPagedNoTurn : pieces && !a.neox ? kPagedTurnPairs : pieces && a.rope == static_cast<int>(cache->head_dim) ? kPagedTurnHalves : kPagedTurnAny;
         auto launch = [&](auto type) {
             constexpr int T = decltype(type)::value;
-            return cache->head_dim == 64 ? launch_rows_of<AppendKernel, 8, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream)
-                 : cache->head_dim == 128 ? launch_rows_of<AppendKernel, 16, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream)
-                                          : launch_rows_of<AppendKernel, 32, T>(a, rows->tokens, a.q_heads + 2 * a.c.kv_heads, cache->sm_count, stream);
+            return cache->head_dim == 64 ? launch_rows_of<AppendKernel, 64, T>(a, rows->tokens, cache->sm_count, stream)
+                 : cache->head_dim == 128 ? launch_rows_of<AppendKernel, 128, T>(a, rows->tokens, cache->sm_count, stream)
+                                          : launch_rows_of<AppendKernel, 256, T>(a, rows->tokens, cache->sm_count, stream);
         };
         rc = args->type == kPagedF32 ? launch(std::integral_constant<int, kPagedF32>()) : args->type == kPagedF16 ? launch(std::integral_constant<int, kPagedF16>())
                                                                                                                   : launch(std::integral_constant<int, kPagedBf16>());
@@ -429,9 +432,9 @@ extern "C" int quintrit_b200_paged_read_device(quintrit_b200_paged_cache_t* cach
         a.c = view_of(cache, layer), a.r = view_of(rows), a.type = cache->type, a.out_type = type, a.k = d_k, a.v = d_v;
         auto launch = [&](auto of) {
             constexpr int T = decltype(of)::value;
-            return cache->head_dim == 64 ? launch_rows_of<ReadKernel, 8, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream)
-                 : cache->head_dim == 128 ? launch_rows_of<ReadKernel, 16, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream)
-                                          : launch_rows_of<ReadKernel, 32, T>(a, rows->tokens, 2 * a.c.kv_heads, cache->sm_count, stream);
+            return cache->head_dim == 64 ? launch_rows_of<ReadKernel, 64, T>(a, rows->tokens, cache->sm_count, stream)
+                 : cache->head_dim == 128 ? launch_rows_of<ReadKernel, 128, T>(a, rows->tokens, cache->sm_count, stream)
+                                          : launch_rows_of<ReadKernel, 256, T>(a, rows->tokens, cache->sm_count, stream);
         };
         rc = cache->type == kPagedF16 ? launch(std::integral_constant<int, kPagedF16>()) : cache->type == kPagedBf16 ? launch(std::integral_constant<int, kPagedBf16>())
                                                                                                                      : launch(std::integral_constant<int, kPagedQ8>());

@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {  // rows 2 c, 2 c + 1 of position g (+ 8) become positions 2 c, 2 c + 1 (+ 8) of row g
-                        const uint32_t v = paged_pack2(BF ? kPagedBf16 : kPagedF16, w[2 * h], w[2 * h + 1]);
+                        const uint32_t v = paged_pack2<BF ? kPagedBf16 : kPagedF16>(w[2 * h], w[2 * h + 1]);
                         asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[n][h]) : "r"(v));
                     }
                 }
@@ -681,7 +681,7 @@ __device__ __forceinline__ void paged_store_row(unsigned char* out, int type, co
         for (int e = 0; e < PER; ++e) reinterpret_cast<float*>(out)[e] = x[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = paged_pack2(type, x[e], x[e + 1]);
+        for (int e = 0; e < PER; e += 2) reinterpret_cast<uint32_t*>(out)[e / 2] = type == kPagedF16 ? paged_pack2<kPagedF16>(x[e], x[e + 1]) : paged_pack2<kPagedBf16>(x[e], x[e + 1]);
     }
 }
 

@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     } else {
                         sums[0] = add_f32x2(sums[0], pack_f32x2(x.x, x.y)), sums[1] = add_f32x2(sums[1], pack_f32x2(y.x, y.y));
                     }
-                    w[e] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, x.x, x.y), w[e + 1] = paged_pack2(M::BF ? kPagedBf16 : kPagedF16, y.x, y.y);
+                    w[e] = paged_pack2<M::BF ? kPagedBf16 : kPagedF16>(x.x, x.y), w[e + 1] = paged_pack2<M::BF ? kPagedBf16 : kPagedF16>(y.x, y.y);
                 }
                 tmem_store16(s_at + side * (KH / 2) + c * 16, w);
             }

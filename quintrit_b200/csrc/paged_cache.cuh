@@ -95,8 +95,9 @@ __device__ __forceinline__ void paged_load8(const void* p, int type, float (&x)[
         }
     }
 }
-__device__ __forceinline__ uint32_t paged_pack2(int type, float a, float b) {
-    if (type == kPagedF16) {
+template <int TYPE>
+__device__ __forceinline__ uint32_t paged_pack2(float a, float b) {
+    if constexpr (TYPE == kPagedF16) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
@@ -107,9 +108,11 @@ __device__ __forceinline__ void paged_store8(void* p, int type, const float (&x)
     if (type == kPagedF32) {
         static_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
         static_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-        return;
+    } else if (type == kPagedF16) {  // (one branch for all eight values)
+        *static_cast<uint4*>(p) = make_uint4(paged_pack2<kPagedF16>(x[0], x[1]), paged_pack2<kPagedF16>(x[2], x[3]), paged_pack2<kPagedF16>(x[4], x[5]), paged_pack2<kPagedF16>(x[6], x[7]));
+    } else {
+        *static_cast<uint4*>(p) = make_uint4(paged_pack2<kPagedBf16>(x[0], x[1]), paged_pack2<kPagedBf16>(x[2], x[3]), paged_pack2<kPagedBf16>(x[4], x[5]), paged_pack2<kPagedBf16>(x[6], x[7]));
     }
-    *static_cast<uint4*>(p) = make_uint4(paged_pack2(type, x[0], x[1]), paged_pack2(type, x[2], x[3]), paged_pack2(type, x[4], x[5]), paged_pack2(type, x[6], x[7]));
 }
 __host__ __device__ constexpr int paged_size_of(int type) { return type == kPagedF32 ? 4 : type == kPagedQ8 ? 1 : 2; }
 

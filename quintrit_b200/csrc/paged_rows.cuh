@@ -6,10 +6,13 @@
 // rint(y / d) with d = max(|y|) / 127 of the row. All arithmetic is in 32 bits; one rounding at the end.
 // Reading (paged_read_kernel): the same rows back, code times scale, rounded to the output type.
 //
-// Eight values to a thread (16 bytes of a 16-bit type, 8 codes), 8 to 32 threads to a head: norm and maximum are exchanges within those threads, and a
-// row of the cache is written once. A warp takes U such groups of heads of one token. Both kernels are bound by the bytes they move, small calls by
+// Writing: sixteen values to a thread, two pieces of eight half a head apart, so that the pairs of a rotation lie in one thread whether they are neighbours or halves of a head (eight
+// values to a thread, the halves exchanged through shared memory: 45 us for the prompt below, now 33.5). Norm and maximum are exchanges within the 4 to 16 threads of a head. Reading: eight
+// values to a thread. A warp takes U groups of heads of one token. Both kernels are bound by the bytes they move, small calls by
 // their latency: a row's address needs four dependent reads (starts, length, page), so the heads' values are asked for before them, and where there are
-// tokens enough for it, four groups of heads share one address (U = 4).
+// tokens enough for it, groups of heads share one address (writing: two, which keep the registers at 80; four took 36 us, one 38.6; reading: four). Writing 4096 tokens of 32 + 2 x 4 heads of
+// 128 with norm, rotation and Q8: 92.5 MB in 33.5 us, 42% of the copy rate; the multiprocessors issue in 55% of their cycles, 120 instructions for sixteen values of a warp. Reading 112000 positions
+// of 4 heads of 256 values, Q8 to F16: 459 MB in 85.5 us, 82%.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -30,7 +33,7 @@ struct PagedAppendArgs {
     float eps;
     const float* cos_sin;            // [positions][rope]: cos at 2 i, sin at 2 i + 1; nullptr: no rotation
     int rope, positions, neox;
-    int vector;                      // eight values of a thread share 16-byte pieces of an angles' row: rope a multiple of 8, with neox of 16, rows on 16-byte boundaries
+    int turn;                        // PagedTurn: pairs of neighbours, rope a multiple of 8; whole heads in halves (neox); either with angles on 16-byte boundaries; else any
     int q_heads;                     // 0 where q is nullptr
 };
 
@@ -57,142 +60,138 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedView& c, const Rows
     return p;
 }
 
-template <int LANES, int TYPE, int U>  // threads of a head: head_dim / 8; type of q, k and v; groups of heads of a warp
+enum PagedTurn { kPagedNoTurn, kPagedTurnPairs, kPagedTurnHalves, kPagedTurnAny };
+
+template <int LANES, int TYPE, int U>  // threads of a head: head_dim / 16; type of q, k and v; groups of heads of a warp
 __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const __grid_constant__ PagedAppendArgs a) {
-    constexpr int kHeads = 32 / LANES, HD = LANES * 8;  // heads of a group: all of them queries, keys or values
-    __shared__ __align__(16) float exchange[kPagedRowThreads / 32][kHeads][HD];  // NEOX pairs lie half a rotation apart
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, piece = lane % LANES, e0 = piece * 8;
-    const int q_groups = (a.q_heads + kHeads - 1) / kHeads, kv_groups = (a.c.kv_heads + kHeads - 1) / kHeads, all = q_groups + 2 * kv_groups, units = (all + U - 1) / U;
+    constexpr int kHeads = 32 / LANES, HD = LANES * 16, HALF = HD / 2;
+    __shared__ __align__(16) float exchange[kPagedRowThreads / 32][kHeads][HD];  // where the values of a pair lie in two threads (kPagedTurnAny)
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LANES, e0 = lane % LANES * 8;  // this thread's values: e0 .. e0 + 7 and those half a head further
+    const int heads = a.q_heads + 2 * a.c.kv_heads, units = (heads + kHeads * U - 1) / (kHeads * U);
     const int item = blockIdx.x * (kPagedRowThreads / 32) + warp, t = item / units;
     if (t >= a.r.tokens) return;
-    const int g0 = item % units * U;
-    // group u of this warp: its kind (0 queries, 1 keys, 2 values) and this thread's head, the last one where there are no more
-    auto kind_of = [&](int g) { return g < q_groups ? 0 : g < q_groups + kv_groups ? 1 : 2; };
-    auto head_of = [&](int g, int kind) { return (g - (kind == 0 ? 0 : kind == 1 ? q_groups : q_groups + kv_groups)) * kHeads + sub; };
-    PagedRaw<TYPE> raw[U];
+    const int head0 = item % units * (kHeads * U) + sub;
+    PagedRaw<TYPE> raw[U][2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int g = min(g0 + u, all - 1), kind = kind_of(g), h = min(head_of(g, kind), (kind == 0 ? a.q_heads : a.c.kv_heads) - 1);
-        raw[u] = kind == 0 ? paged_raw<TYPE>(a.q, t * a.q_token + h * a.q_head + e0) : kind == 1 ? paged_raw<TYPE>(a.k, t * a.k_token + h * a.k_head + e0)
-                                                                                               : paged_raw<TYPE>(a.v, t * a.v_token + h * a.v_head + e0);
+    for (int u = 0; u < U; ++u) {  // (the last head again where there are no more)
+        const int h = min(head0 + u * kHeads, heads - 1), k = h - a.q_heads, v = k - a.c.kv_heads;
+        const void* from = k < 0 ? a.q : v < 0 ? a.k : a.v;
+        const size_t at = k < 0 ? t * a.q_token + h * a.q_head : v < 0 ? t * a.k_token + k * a.k_head : t * a.v_token + v * a.v_head;
+        raw[u][0] = paged_raw<TYPE>(from, at + e0), raw[u][1] = paged_raw<TYPE>(from, at + e0 + HALF);
     }
-    const PagedPlace place = paged_place(a.c, a.r, t, a.cos_sin != nullptr ? a.positions : 0x7fffffff);
+    const PagedPlace place = paged_place(a.c, a.r, t, a.turn != kPagedNoTurn ? a.positions : 0x7fffffff);
     // (a query of a token whose page does not exist is left as it was, like its row of the cache)
     if (place.page < 0) return;
-    // this thread's factors of the rotation: x_i cos_i + partner_i sin_i
+    // the angles of this thread's eight pairs: (i, i + 8) of its values, or (2 i, 2 i + 1)
+    const float* angles = a.cos_sin + static_cast<size_t>(place.pos) * a.rope;
+    const bool in[2] = {e0 < a.rope, e0 + HALF < a.rope};
     float cs[8], sn[8];
-    const int half = a.rope / 2;
-    const bool turns = a.cos_sin != nullptr && g0 < q_groups + kv_groups, rotate = turns && e0 < a.rope;
-    if (rotate) {
-        const float* row = a.cos_sin + static_cast<size_t>(place.pos) * a.rope;
-        if (a.vector && a.neox) {  // eight pairs, all first or all second values
-            const bool second = e0 >= half;
-            const float4* at = reinterpret_cast<const float4*>(row + 2 * (second ? e0 - half : e0));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 v = at[i];
-                cs[2 * i] = v.x, sn[2 * i] = second ? v.y : -v.y, cs[2 * i + 1] = v.z, sn[2 * i + 1] = second ? v.w : -v.w;
-            }
-        } else if (a.vector) {  // four pairs
-            const float4* at = reinterpret_cast<const float4*>(row + e0);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float4 v = at[i];
-                cs[4 * i] = cs[4 * i + 1] = v.x, sn[4 * i] = -v.y, sn[4 * i + 1] = v.y, cs[4 * i + 2] = cs[4 * i + 3] = v.z, sn[4 * i + 2] = -v.w, sn[4 * i + 3] = v.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = min(e0 + i, a.rope - 1);
-                const bool second = a.neox ? e >= half : (e & 1) != 0;
-                const int p = a.neox ? (second ? e - half : e) : e >> 1;
-                cs[i] = row[2 * p], sn[i] = second ? row[2 * p + 1] : -row[2 * p + 1];
-            }
-        }
+    for (int i = 0; i < 4; ++i) {
+        float4 v = make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+        if (a.turn == kPagedTurnHalves) v = reinterpret_cast<const float4*>(angles + 2 * e0)[i];
+        else if (a.turn == kPagedTurnPairs && in[i >> 1]) v = reinterpret_cast<const float4*>(angles + e0 + (i >> 1) * HALF)[i & 1];
+        cs[2 * i] = v.x, sn[2 * i] = v.y, cs[2 * i + 1] = v.z, sn[2 * i + 1] = v.w;
     }
     const float most_finite = a.type == kPagedF16 ? 65504.0f : a.type == kPagedBf16 ? 3.3895313892515355e38f : 8.507059173023462e37f;  // (Q8: 2^126, so that 127 d does not overflow)
+    // where the rows of this token lie in the cache, of head 0; a thread's pieces in them
+    const size_t row0 = paged_rows_at(a.c, a.type, place.page, 0, 0) + paged_row_at(a.type, a.c.blocks, 0, place.row), per_head = static_cast<size_t>(a.c.blocks * paged_row_bytes(a.type)) << a.c.page_log2;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const int g = g0 + u, kind = kind_of(g), h = head_of(g, kind);
-        if (g >= all) break;
-        const bool live = h < (kind == 0 ? a.q_heads : a.c.kv_heads);
-        float x[8];
-        paged_load8(raw[u].v, TYPE, x);
-        const float* w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-        if (w != nullptr) {
-            float sum = 0.0f, f[8];
-            paged_load8(w + e0, kPagedF32, f);
+        const int h = head0 + u * kHeads, k = h - a.q_heads, v = k - a.c.kv_heads;
+        const bool live = h < heads, value = v >= 0;
+        float x[16];
+        paged_load8(raw[u][0].v, TYPE, *reinterpret_cast<float(*)[8]>(x));
+        paged_load8(raw[u][1].v, TYPE, *reinterpret_cast<float(*)[8]>(x + 8));
+        if (a.q_norm != nullptr || a.k_norm != nullptr) {
+            const float* w = k < 0 ? a.q_norm : value ? nullptr : a.k_norm;
+            float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+            for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);  // (off by 2^-22 at most)
+            if (w != nullptr) {
+                float f[16];
+                paged_load8(w + e0, kPagedF32, *reinterpret_cast<float(*)[8]>(f));
+                paged_load8(w + e0 + HALF, kPagedF32, *reinterpret_cast<float(*)[8]>(f + 8));
+                const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);  // (off by 2^-22 at most)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * f[i];
+                for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * f[i];
+            }
         }
-        if (turns && kind != 2) {
-            float y[8];  // the other one of each pair
-            if (a.neox) {
-                float* row = exchange[warp][sub];
-                __syncwarp();
-                paged_store8(row + e0, kPagedF32, x);
-                __syncwarp();
-                if (a.vector) {
-                    if (rotate) paged_load8(row + (e0 >= half ? e0 - half : e0 + half), kPagedF32, y);
-                } else {
+        if (a.turn == kPagedTurnHalves && !value) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = row[e0 + i >= a.rope ? e0 + i : e0 + i >= half ? e0 + i - half : e0 + i + half];
+            for (int i = 0; i < 8; ++i) {
+                const float x0 = x[i], x1 = x[8 + i];
+                x[i] = fmaf(x0, cs[i], -(x1 * sn[i])), x[8 + i] = fmaf(x1, cs[i], x0 * sn[i]);
+            }
+        } else if (a.turn == kPagedTurnPairs && !value) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                if (in[i >> 2]) x[2 * i] = fmaf(x0, cs[i], -(x1 * sn[i])), x[2 * i + 1] = fmaf(x1, cs[i], x0 * sn[i]);
+            }
+        } else if (a.turn == kPagedTurnAny) {
+            float* row = exchange[warp][sub];
+            const int half = a.rope / 2;
+            __syncwarp();
+            paged_store8(row + e0, kPagedF32, *reinterpret_cast<float(*)[8]>(x));
+            paged_store8(row + e0 + HALF, kPagedF32, *reinterpret_cast<float(*)[8]>(x + 8));
+            __syncwarp();
+            if (!value) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int e = e0 + (i & 7) + (i >> 3) * HALF;
+                    if (e >= a.rope) continue;
+                    const bool second = a.neox ? e >= half : (e & 1) != 0;
+                    const int pair = a.neox ? (second ? e - half : e) : e >> 1;
+                    const float other = row[a.neox ? (second ? e - half : e + half) : e ^ 1], c = angles[2 * pair], s = angles[2 * pair + 1];
+                    x[i] = fmaf(x[i], c, second ? other * s : -(other * s));
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-            }
-            if (rotate && a.vector) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], cs[i], y[i] * sn[i]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = y[i];
-            } else if (rotate) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = e0 + i < a.rope ? fmaf(x[i], cs[i], y[i] * sn[i]) : x[i];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = y[i];
             }
         }
-        if (kind == 0) {
-            if (live) paged_store8(static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.q_type), a.q_type, x);
-            continue;
+        if (k < 0) {
+            unsigned char* out = static_cast<unsigned char*>(a.q_out) + (t * a.o_token + h * a.o_head + e0) * paged_size_of(a.q_type);
+            paged_store8(out, a.q_type, *reinterpret_cast<float(*)[8]>(x));
+            paged_store8(out + HALF * paged_size_of(a.q_type), a.q_type, *reinterpret_cast<float(*)[8]>(x + 8));
         }
+        if (__all_sync(0xffffffffu, k < 0 || !live)) continue;
         float amax = 0.0f;
         bool fits = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i])), fits = fits && fabsf(x[i]) <= most_finite;
-        if (!fits) {  // the nearest value that is finite and fits the type; zero for what is no number
+        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(x[i])), fits = fits && fabsf(x[i]) <= most_finite;
+        if (!fits && k >= 0) {  // the nearest value that is finite and fits the type; zero for what is no number
             amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 16; ++i) {
                 if (!(fabsf(x[i]) <= most_finite)) x[i] = isnan(x[i]) ? 0.0f : copysignf(most_finite, x[i]);
                 amax = fmaxf(amax, fabsf(x[i]));
             }
             if (live) atomicOr(a.c.status, kPagedSaturated);
         }
-        unsigned char* row = (kind == 1 ? a.c.k : a.c.v) + paged_rows_at(a.c, a.type, place.page, h, 0) + paged_row_at(a.type, a.c.blocks, piece >> 3, place.row);
+        unsigned char* row = (value ? a.c.v : a.c.k) + row0 + (value ? v : k) * per_head;
+        const int block_bytes = paged_row_at(a.type, a.c.blocks, 1, 0), piece = e0 >> 3, second = piece + HALF / 8;
         if (a.type != kPagedQ8) {
-            if (live) paged_store8(row + paged_piece(a.type, place.row, piece & 7) * 16, a.type, x);
+            if (k < 0 || !live) continue;
+            paged_store8(row + (piece >> 3) * block_bytes + paged_piece(a.type, place.row, piece & 7) * 16, a.type, *reinterpret_cast<float(*)[8]>(x));
+            paged_store8(row + (second >> 3) * block_bytes + paged_piece(a.type, place.row, second & 7) * 16, a.type, *reinterpret_cast<float(*)[8]>(x + 8));
             continue;
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (!live) continue;
+        if (k < 0 || !live) continue;
         const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = __fdividef(1.0f, d);
-        uint32_t code[2] = {0u, 0u};
+        uint32_t code[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // (|x| / d <= 127 (1 + 2^-22), which rounds to 127; x (1 / d) is off x / d by 2^-16 of a step at most)
-            const int q = __float2int_rn(x[i] * inv);
-            code[i >> 2] |= static_cast<uint32_t>(q & 0xff) << (8 * (i & 3));
+        for (int i = 0; i < 4; ++i) {  // |x| / d <= 127 (1 + 2^-22), which rounds to 127; x (1 / d) is off x / d by 2^-16 of a step at most. Added to 1.5 2^23 a number is rounded to its integer, in the low bits
+            uint32_t q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = __float_as_uint(fmaf(x[4 * i + e], inv, 12582912.0f));
+            code[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         }
-        *reinterpret_cast<uint2*>(row + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
-        if (piece == 0) (kind == 1 ? a.c.ks : a.c.vs)[paged_scales_at(a.c, place.page, h) + place.row] = d;
+        *reinterpret_cast<uint2*>(row + (piece >> 3) * block_bytes + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
+        *reinterpret_cast<uint2*>(row + (second >> 3) * block_bytes + paged_piece(a.type, place.row, (second & 7) >> 1) * 16 + (second & 1) * 8) = make_uint2(code[2], code[3]);
+        if (piece == 0) (value ? a.c.vs : a.c.ks)[paged_scales_at(a.c, place.page, value ? v : k) + place.row] = d;
     }
 }
 
