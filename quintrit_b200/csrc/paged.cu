@@ -102,11 +102,11 @@ int launch_rows_of(const Args& a, uint32_t tokens, int sm_count, void* stream) {
 
 // Whether the kernel for few rows shares its tiles out, and among how many blocks: all that the device holds, as long as each gets four tiles or so; sequences of a few tiles each, or very many
 // sequences, go one item to a block. (By the longest sequence: shorter ones leave the blocks less.)
-int few_blocks(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, long long row_blocks, int places) {
+int few_blocks(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t window, int places) {
     long long span = std::max<uint32_t>(r->max_length, 1);
     if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + r->max_new + kPagedTile);
-    const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads * row_blocks, all = tiles * items;
-    if (r->sequences > kPagedShared || tiles < 6 || all > 0x7fffffffLL || items > 8LL * places) return 0;
+    const long long tiles = (span + kPagedTile - 1) / kPagedTile, items = static_cast<long long>(r->sequences) * c->kv_heads, all = tiles * items;
+    if (r->sequences > kPagedShared || tiles < 6 || all + items * kPagedStart > 0x7fffffffLL || items > 8LL * places) return 0;
     return static_cast<int>(std::min<long long>(places, std::max<long long>(all / 4, 1)));
 }
 
@@ -134,20 +134,21 @@ int launch_few(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
 template <int TYPE, int BLOCKS>
 int launch_few_rows(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
     if (nt == 1) return launch_few<TYPE, BLOCKS, 1>(a, device, grid, s);
-    if constexpr (BLOCKS < 4)
-        if (nt > 2) return launch_few<TYPE, BLOCKS, BLOCKS == 1 ? 4 : 3>(a, device, grid, s);
+    if constexpr (TYPE == kPagedQ8 && BLOCKS == 2)
+        if (nt == 3) return launch_few<TYPE, BLOCKS, 3>(a, device, grid, s);
     return launch_few<TYPE, BLOCKS, 2>(a, device, grid, s);
 }
 template <int TYPE>
 int launch_few_type(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
     return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, nt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, nt, grid, s) : launch_few_rows<TYPE, 4>(a, device, nt, grid, s);
 }
-// Tiles of 8 rows of a block of threads: as many as its registers hold the sums of; and such blocks on all multiprocessors.
-int row_tiles_of(const quintrit_b200_paged_cache* c, long long rows) { return rows <= 8 ? 1 : rows <= 16 || c->head_dim == 256 ? 2 : c->head_dim == 128 ? 3 : 4; }
+// Blocks of the kernel for few rows on all multiprocessors, by tiles of 8 rows.
 template <int TYPE>
 int blocks_per_sm(int head_dim, int nt) {
-    return head_dim == 64 ? (nt == 1 ? PagedFew<TYPE, 1, 1>::kBlocksPerSm : nt == 2 ? PagedFew<TYPE, 1, 2>::kBlocksPerSm : PagedFew<TYPE, 1, 4>::kBlocksPerSm)
-         : head_dim == 128 ? (nt == 1 ? PagedFew<TYPE, 2, 1>::kBlocksPerSm : nt == 2 ? PagedFew<TYPE, 2, 2>::kBlocksPerSm : PagedFew<TYPE, 2, 3>::kBlocksPerSm)
+    if constexpr (TYPE == kPagedQ8)
+        if (nt == 3) return PagedFew<TYPE, 2, 3>::kBlocksPerSm;
+    return head_dim == 64 ? (nt == 1 ? PagedFew<TYPE, 1, 1>::kBlocksPerSm : PagedFew<TYPE, 1, 2>::kBlocksPerSm)
+         : head_dim == 128 ? (nt == 1 ? PagedFew<TYPE, 2, 1>::kBlocksPerSm : PagedFew<TYPE, 2, 2>::kBlocksPerSm)
                            : (nt == 1 ? PagedFew<TYPE, 4, 1>::kBlocksPerSm : PagedFew<TYPE, 4, 2>::kBlocksPerSm);
 }
 int places_of(const quintrit_b200_paged_cache* c, int nt) {
@@ -247,8 +248,7 @@ int launch_behind(Kernel kernel, unsigned grid, cudaStream_t s, const Args&... a
 struct PagedPlan {
     int few_new;             // 0: all by the kernel for many rows
     bool many;
-    int nt;                  // few: tiles of 8 rows of a block, blocks of rows of the longest chunk, blocks that the tiles are shared out among (0: an item a block)
-    long long few_tiles;
+    int nt;                  // few: tiles of 8 rows of a block, blocks that the tiles are shared out among (0: an item a block)
     int few_share;
     PagedSchedule schedule;  // many: which blocks, their number, slots of the workspace
     int many_rows;           // rows of a block of threads
@@ -256,20 +256,20 @@ struct PagedPlan {
     size_t part_rows;
     size_t few_bytes, many_bytes;  // of the workspace
 };
-constexpr int kPagedFewRows = 64;  // rows of a KV head up to which the kernel for few rows takes a call
+// Rows of a KV head up to which the kernel for few rows takes a sequence. With the few rows' kernel and the many rows' one, us: 16 sequences of 3000, heads of 128, F16: 12 rows 39 and 48,
+// 20 rows 51 and 47; Q8: 12 rows 40 and 66, 20 rows 49 and 67, 32 rows 80 and 67; heads of 64, F16: 12 rows 26 and 28, 32 rows 32 and 27; heads of 256, F16: 12 rows 58 and 59, 48 rows 104 and 61.
+inline int few_rows(const quintrit_b200_paged_cache* c) { return c->type == kPagedQ8 && c->head_dim == 128 ? 24 : 16; }
 constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {
-    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = kPagedFewRows;
+    const long long group = q_heads / c->kv_heads, most = r->max_new * group, limit = few_rows(c);
     p->many = most > limit;
-    p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(std::max<long long>(8 / group, group <= 32 ? 1 : 0), r->max_new - 1));  // (a sequence alone is the longest)
-    p->few_tiles = 0, p->few_share = 0, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
+    p->few_new = static_cast<int>(!p->many ? r->max_new : r->sequences == 1 ? 0 : std::min<long long>(std::max<long long>(8 / group, group <= limit ? 1 : 0), r->max_new - 1));  // (a sequence alone is the longest)
+    p->few_share = 0, p->part_rows = 0, p->few_bytes = p->many_bytes = 0, p->many_blocks = 0;
     const size_t row_bytes = c->head_dim * sizeof(float) + sizeof(float2);
     if (p->few_new > 0) {
-        const long long rows = p->few_new * group;
-        p->nt = row_tiles_of(c, rows);
-        p->few_tiles = (rows + 8 * p->nt - 1) / (8 * p->nt);
-        const int places = places_of(c, p->nt), share = few_blocks(c, r, 0, p->few_tiles, places);
-        p->few_share = window > 0 ? std::min(share, few_blocks(c, r, window, p->few_tiles, places)) : share;  // (no window takes more of the workspace than none)
+        p->nt = static_cast<int>((p->few_new * group + 7) / 8);
+        const int places = places_of(c, p->nt), share = few_blocks(c, r, 0, places);
+        p->few_share = window > 0 ? std::min(share, few_blocks(c, r, window, places)) : share;  // (no window takes more of the workspace than none)
         p->few_bytes = up16(static_cast<size_t>(share) * 2 * 8 * p->nt * row_bytes);
     }
     if (p->many) {
@@ -486,7 +486,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         const int group = static_cast<int>(args->q_heads / cache->kv_heads);
         PagedPlan plan;
         plan_of(cache, rows, args->q_heads, args->window, &plan);
-        if (plan.few_tiles > 65535 || plan.many_blocks > 0x7fffffffLL || static_cast<long long>(rows->tokens) * args->q_heads > 0x7fffffffLL)
+        if (plan.many_blocks > 0x7fffffffLL || static_cast<long long>(rows->tokens) * args->q_heads > 0x7fffffffLL)
             return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
         const size_t need = plan.few_bytes + plan.many_bytes;
         if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);
@@ -525,7 +525,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             const int block_rows = 8 * plan.nt;
             a.part_o = reinterpret_cast<float*>(workspace);
             a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(plan.few_share) * 2 * block_rows * cache->head_dim);
-            const dim3 grid = plan.few_share > 0 ? dim3(static_cast<unsigned>(plan.few_share)) : dim3(static_cast<unsigned>(plan.few_tiles), cache->kv_heads, rows->sequences);
+            const dim3 grid = plan.few_share > 0 ? dim3(static_cast<unsigned>(plan.few_share)) : dim3(cache->kv_heads, rows->sequences);
             rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.nt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.nt, grid, s)
                                                                                                                                 : launch_few_type<kPagedQ8>(a, device, plan.nt, grid, s);
             if (rc != QUINTRIT_OK) return rc;

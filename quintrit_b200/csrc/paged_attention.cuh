@@ -108,6 +108,8 @@ __device__ __forceinline__ long long prefix(long long v) {  // the sum of v over
 
 }  // namespace paged_detail
 
+template <int T> struct PagedTag { static constexpr int value = T; };
+
 struct PagedRange {
     int begin, end;
 };
@@ -116,34 +118,29 @@ __device__ __forceinline__ PagedRange paged_seen(const PagedAttnArgs& a, const P
     return PagedRange{a.window > 0 ? max(0, q.length - q.news - a.window + 1) & ~(kPagedTile - 1) : 0, q.length};
 }
 
-// Work shared out: the items (a sequence's KV head and block of rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles; block b of G takes W / G of all W tiles, the
-// first W % G blocks one more, whatever the lengths are. What a block has of an item is a segment: a whole item's result is written as it is, others go to the workspace, at most two of a block:
-// place 0 for the segment that its tiles begin with, place 1 for another. Every block works the items' places out for itself from the lengths (paged_share_begin), for up to kPagedShared sequences.
-constexpr int kPagedShared = 256;
+// Work shared out: the items (a sequence's KV head with all its rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles and kPagedStart places in front of
+// them; block b of G takes W / G of all W places, the first W % G blocks one more, whatever the lengths are. What a block has of an item is a segment: a whole item's result is written as it is,
+// others go to the workspace, at most two of a block: place 0 for the segment that its places begin with, place 1 for another. Every block works the items out for itself from the lengths
+// (paged_share_begin), for up to kPagedShared sequences. The places in front stand for what another segment costs a block (the end of one, the queries and the first copies of the next).
+constexpr int kPagedShared = 256, kPagedStart = 5;
 struct PagedShare {
     int total;
-    int* before;  // [sequences + 1] in shared memory: tiles of the items before a sequence's
+    int* before;  // [sequences + 1] in shared memory: places of the items before a sequence's
     int4* of;     // [sequences]: first token, new tokens, length, tiles of an item
 };
 struct PagedItem {
-    int seq, kvh, rows0;        // rows0: the block of rows' first
-    int begin, tiles;           // the item's first tile among all
+    int seq, kvh;
+    int begin, tiles;           // the item's first place among all, its tiles
     PagedSequence q;
 };
-// Tiles and items of a sequence.
-__device__ __forceinline__ void paged_weight(const PagedAttnArgs& a, const PagedSequence& q, int block_rows, int* tiles, int* items) {
-    const PagedRange g = paged_seen(a, q);
-    const bool mine = q.ok && q.news >= a.few && q.news <= a.many;
-    *tiles = max(1, (g.end - g.begin + kPagedTile - 1) / kPagedTile), *items = mine ? a.c.kv_heads * ((q.news * a.group + block_rows - 1) / block_rows) : 0;
-}
 // By all threads of a block; `before` and `of` have room for kPagedShared + 1 and kPagedShared. Tiles that 32 bits do not hold, of sequences far longer
 // than was announced, are not shared out: the call does nothing but report them.
-__device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, int block_rows, int* before, int4* of, int threads) {
+__device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, int* before, int4* of, int threads) {
     for (int s = threadIdx.x; s < a.r.sequences; s += threads) {
-        int tiles, items;
         const PagedSequence q = paged_sequence(a.c, a.r, s);
-        paged_weight(a, q, block_rows, &tiles, &items);
-        before[s + 1] = static_cast<int>(min(static_cast<long long>(tiles) * items, 0x7fffffffLL));
+        const PagedRange g = paged_seen(a, q);
+        const int tiles = max(1, (g.end - g.begin + kPagedTile - 1) / kPagedTile);
+        before[s + 1] = q.ok && q.news >= a.few && q.news <= a.many ? static_cast<int>(min((tiles + static_cast<long long>(kPagedStart)) * a.c.kv_heads, 0x7fffffffLL)) : 0;
         of[s] = make_int4(q.first, q.news, q.length, tiles);
         if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
     }
@@ -162,7 +159,7 @@ __device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, 
     __syncthreads();
     return PagedShare{before[a.r.sequences], before, of};
 }
-__device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const PagedShare& w, int tile, int block_rows) {
+__device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const PagedShare& w, int tile) {
     int lo = 0, hi = a.r.sequences - 1;  // the last sequence whose items begin at or before the tile
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -170,8 +167,8 @@ __device__ __forceinline__ PagedItem paged_item_at(const PagedAttnArgs& a, const
         else hi = mid - 1;
     }
     const int4 of = w.of[lo];
-    const int i = (tile - w.before[lo]) / of.w;
-    return PagedItem{lo, i % a.c.kv_heads, i / a.c.kv_heads * block_rows, w.before[lo] + i * of.w, of.w, PagedSequence{of.x, of.y, of.z, true}};
+    const int i = (tile - w.before[lo]) / (of.w + kPagedStart);
+    return PagedItem{lo, i, w.before[lo] + i * (of.w + kPagedStart), of.w, PagedSequence{of.x, of.y, of.z, true}};
 }
 
 __device__ __forceinline__ int paged_share_of(int total, int blocks, int b) { return total / blocks * b + min(b, total % blocks); }  // block b's first tile
@@ -268,24 +265,25 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     PagedShare shared{0, s_before, s_of};
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (a.share) {
-        shared = paged_share_begin(a, F::kRows, s_before, s_of, kThreads);
+        shared = paged_share_begin(a, s_before, s_of, kThreads);
         at = first = paged_share_of(shared.total, gridDim.x, blockIdx.x), until = paged_share_of(shared.total, gridDim.x, blockIdx.x + 1);
     }
     int base0 = 0, base1 = 0;  // units that the rings have seen
     while (at < until) {
-    int seq, kvh, r0, parts_place = -1;  // place of the workspace that the segment's result goes to, or none
+    int seq, kvh, parts_place = -1;  // place of the workspace that the segment's result goes to, or none
     PagedSequence sq;
     PagedRange range;
     if (a.share) {
-        const PagedItem item = paged_item_at(a, shared, at, F::kRows);
-        seq = item.seq, kvh = item.kvh, r0 = item.rows0, sq = item.q;
-        const int t = at - item.begin, n = min(item.tiles - t, until - at);
+        const PagedItem item = paged_item_at(a, shared, at);
+        seq = item.seq, kvh = item.kvh, sq = item.q;
+        const int tile0 = item.begin + kPagedStart, t = max(at - tile0, 0), n = min(item.tiles, until - tile0) - t;
+        if (n <= 0) break;  // (the block's places end in front of the item's tiles)
         range = paged_seen(a, sq);
         range.end = min(range.end, range.begin + (t + n) * kPagedTile), range.begin += t * kPagedTile;
         if (n < item.tiles) parts_place = static_cast<int>(blockIdx.x) * 2 + (at == first ? 0 : 1);
-        at += n;
+        at = tile0 + t + n;
     } else {
-        at = until, seq = blockIdx.z, kvh = blockIdx.y, r0 = blockIdx.x * F::kRows;
+        at = until, seq = blockIdx.y, kvh = blockIdx.x;
         sq = paged_sequence(a.c, a.r, seq);
         if (!sq.ok || sq.news < a.few || sq.news > a.many) {
             if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
@@ -293,43 +291,51 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         }
         range = paged_seen(a, sq);
     }
-    const int rows = sq.news * a.group, r1 = min(rows, r0 + F::kRows);
-    if (r0 >= rows) return;  // (only where a block takes a whole item)
-    const int t0 = r0 / a.group, t1 = (r1 - 1) / a.group + 1, p0 = sq.length - sq.news;
-    // what these rows see of it
-    const int low = a.window > 0 ? max(0, p0 + t0 - a.window + 1) & ~(kPagedTile - 1) : 0;
-    range.begin = max(range.begin, low), range.end = max(range.begin, min(range.end, max(0, p0 + t1)));
+    const int rows = sq.news * a.group, p0 = sq.length - sq.news;
+    range.end = max(range.begin, range.end);
     const int tiles = (range.end - range.begin + kPagedTile - 1) / kPagedTile;
     __syncthreads();  // the barriers are there; the segment before has left the ring
     if (warp == 8) {
         paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, base0, base1, abort_flag, a.spin_limit);
     } else {
-        // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none
-        for (int i = warp; i < F::kRows; i += 8) {
-            const int r = r0 + i, t = r / a.group, h = kvh * a.group + r % a.group;
-            float x[8];
+        // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none; all of them are asked for before the first is used
+        auto load_rows = [&](auto of) {
+            constexpr int T = decltype(of)::value;
+            PagedRaw<T> raw[NT];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.0f;
-            if (r < r1 && lane < HD / 8)
-                paged_load8(static_cast<const unsigned char*>(a.q) + ((static_cast<size_t>(sq.first) + t) * a.q_token + h * a.q_head + lane * 8) * paged_size_of(a.q_type), a.q_type, x);
-            float f = 1.0f;
-            if constexpr (Q8) {
-                float m = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const uint32_t ex = __float_as_uint(m) >> 23;  // the row's power of two, 2^(ex - 127); none for zeros, denormals and what is not finite
-                if (ex > 1 && ex < 254) {
-                    f = __uint_as_float(ex << 23);
-                    const float inv = __uint_as_float((254 - ex) << 23);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] *= inv;
-                }
+            for (int k = 0; k < NT; ++k) {
+                const int r = min(warp + k * 8, rows - 1);
+                raw[k] = paged_raw<T>(a.q, (static_cast<size_t>(sq.first) + r / a.group) * a.q_token + (kvh * a.group + r % a.group) * a.q_head + min(lane, HD / 8 - 1) * 8);
             }
-            if (lane < HD / 8) paged_store8(s_q + i * kPitch + lane * 16, BF ? kPagedBf16 : kPagedF16, x);
-            if (lane == 0) s_rowf[i] = f * a.scale;
-        }
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const int i = warp + k * 8;
+                float x[8], f = 1.0f;
+                paged_load8(raw[k].v, T, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = i < rows ? x[e] : 0.0f;
+                if constexpr (Q8) {
+                    float m = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                    const uint32_t ex = __float_as_uint(m) >> 23;  // the row's power of two, 2^(ex - 127); none for zeros, denormals and what is not finite
+                    if (ex > 1 && ex < 254) {
+                        f = __uint_as_float(ex << 23);
+                        const float inv = __uint_as_float((254 - ex) << 23);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] *= inv;
+                    }
+                }
+                if (lane < HD / 8) paged_store8(s_q + i * kPitch + lane * 16, BF ? kPagedBf16 : kPagedF16, x);
+                if (lane == 0) s_rowf[i] = f * a.scale;
+            }
+        };
+        if constexpr (TYPE != kPagedQ8) load_rows(PagedTag<TYPE>());
+        else if (a.q_type == kPagedF16) load_rows(PagedTag<kPagedF16>());
+        else if (a.q_type == kPagedBf16) load_rows(PagedTag<kPagedBf16>());
+        else load_rows(PagedTag<kPagedF32>());
         asm volatile("bar.sync 1, 256;" ::: "memory");
 
         const int turn = warp >> 2, kg = warp & 3, g = lane >> 2, c4 = lane & 3;  // positions g and g + 8 of the warp's 16, rows 2 c4 and 2 c4 + 1 of a row tile
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 #pragma unroll
             for (int i = 0; i < 2; ++i) rowf[n][i] = s_rowf[n * 8 + c4 * 2 + i], m[n][i] = -INFINITY, l[n][i] = 0.0f;
         // positions that every row sees; outside of them the masks are worked out
-        const int all_last = p0 + t0, all_first = a.window > 0 ? p0 + t1 - a.window : 0;
+        const int all_last = p0, all_first = a.window > 0 ? sq.length - a.window : 0;
         float o[KS][NT][4];
 #pragma unroll
         for (int j = 0; j < KS; ++j)
@@ -452,8 +458,8 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                     if (masked) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int rr = r0 + n * 8 + c4 * 2 + (e & 1), p = p0 + rr / a.group, j = key0 + g + 8 * (e >> 1);
-                            if (rr >= r1 || j > p || j >= range.end || (a.window > 0 && j <= p - a.window)) sc[n][e] = -INFINITY;
+                            const int rr = n * 8 + c4 * 2 + (e & 1), p = p0 + rr / a.group, j = key0 + g + 8 * (e >> 1);
+                            if (rr >= rows || j > p || j >= range.end || (a.window > 0 && j <= p - a.window)) sc[n][e] = -INFINITY;
                         }
                     }
 #pragma unroll
@@ -579,7 +585,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     // rows out: eight values to a thread
     const float* joined = reinterpret_cast<const float*>(smem);
     const float2* mls = reinterpret_cast<const float2*>(smem + 8 * F::kRows * F::kJoinPitch * 4);
-    for (int i = tid; i < (r1 - r0) * (HD / 8); i += kThreads) {
+    for (int i = tid; i < rows * (HD / 8); i += kThreads) {
         const int r = i / (HD / 8), e0 = i % (HD / 8) * 8;
         float top = -INFINITY, w[8], sum = 0.0f, x[8];
 #pragma unroll
@@ -599,8 +605,8 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
             x[0] = fmaf(w[k], u.x, x[0]), x[1] = fmaf(w[k], u.y, x[1]), x[2] = fmaf(w[k], u.z, x[2]), x[3] = fmaf(w[k], u.w, x[3]);
             x[4] = fmaf(w[k], v.x, x[4]), x[5] = fmaf(w[k], v.y, x[5]), x[6] = fmaf(w[k], v.z, x[6]), x[7] = fmaf(w[k], v.w, x[7]);
         }
-        const size_t t = static_cast<size_t>(sq.first) + (r0 + r) / a.group;
-        const int h = kvh * a.group + (r0 + r) % a.group;
+        const size_t t = static_cast<size_t>(sq.first) + r / a.group;
+        const int h = kvh * a.group + r % a.group;
         if (parts_place < 0) {
             const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (a sum that is no number stays one)
 #pragma unroll
@@ -694,18 +700,17 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
     __shared__ int before[kPagedShared + 1];
     __shared__ int4 of[kPagedShared];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x + 1;
-    const PagedShare w = paged_share_begin(a, block_rows, before, of, 256);
+    const PagedShare w = paged_share_begin(a, before, of, 256);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the segments are still being worked on; what was read above is input. Every block waits, so that none ends before them
     const int x = paged_share_of(w.total, blocks, b);
     if (x <= 0 || x >= w.total) return;
-    const PagedItem item = paged_item_at(a, w, x, block_rows);
-    if (item.begin >= x) return;  // the place is between two items
-    const int b0 = paged_block_of(w.total, blocks, item.begin), b1 = paged_block_of(w.total, blocks, item.begin + item.tiles - 1), cuts = b1 - b0;
-    const int place0 = paged_share_of(w.total, blocks, b0) == item.begin ? 0 : 1, rows = min(block_rows, item.q.news * a.group - item.rows0), mine = b - b0 - 1;
-    if (mine >= cuts) return;  // (a block without tiles of its own)
+    const PagedItem item = paged_item_at(a, w, x);
+    const int tile0 = item.begin + kPagedStart, b0 = paged_block_of(w.total, blocks, tile0), b1 = paged_block_of(w.total, blocks, tile0 + item.tiles - 1), cuts = b1 - b0;
+    const int place0 = paged_share_of(w.total, blocks, b0) >= item.begin ? 0 : 1, rows = item.q.news * a.group, mine = b - b0 - 1;
+    if (mine < 0 || mine >= cuts) return;  // the item's tiles are not cut here (the place is in front of them, or the block has none of its own)
     auto out = [&](int r, const float (&v)[kPer]) {
-        const size_t t = static_cast<size_t>(item.q.first) + (item.rows0 + r) / a.group;
-        const int h = item.kvh * a.group + (item.rows0 + r) % a.group;
+        const size_t t = static_cast<size_t>(item.q.first) + r / a.group;
+        const int h = item.kvh * a.group + r % a.group;
         paged_store_row(static_cast<unsigned char*>(a.out) + (t * a.o_token + h * a.o_head + lane * kPer) * paged_size_of(a.out_type), a.out_type, v);
     };
     float v[kPer];
