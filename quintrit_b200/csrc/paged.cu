@@ -155,11 +155,12 @@ int places_of(const quintrit_b200_paged_cache* c, int nt) {
     return c->sm_count * (c->type == kPagedQ8 ? blocks_per_sm<kPagedQ8>(static_cast<int>(c->head_dim), nt) : blocks_per_sm<kPagedF16>(static_cast<int>(c->head_dim), nt));
 }
 
-// The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles and a start and an end of
-// about four tiles more; ranges cost their results' way through memory and one more launch, about three tiles. `few`: the new tokens of sequences that it leaves out. Where the sequences' chunks differ,
+// The schedule of the kernel for many rows (PagedSchedule), and the rows of results that it takes of the workspace, at most `limit`. A block of threads costs its tiles, and for its start and
+// end about 11000 cycles; ranges cost their results' way through memory and one more launch, about 15000 more. A tile is 4300 cycles of two row tiles, 1900 of one. (1024 new tokens of 12 heads of 256 values:
+// whole row blocks 26.8 us, in ranges of 9 tiles 34; 257 tokens of 32 heads of 128, windowed, next to seven single tokens: whole 64 us, in ranges of 3 tiles 47.) `few`: the new tokens of sequences that it leaves out. Where the sequences' chunks differ,
 // the row blocks are not known here: about as many as the tokens fill, at most one more for every sequence that may be among them.
 size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t group, uint32_t window, int few, int rows, size_t limit, PagedSchedule* g) {
-    constexpr double kStart = 4.0, kJoin = 3.0;
+    const double start = rows == 256 ? 2.5 : 6.0, join = rows == 256 ? 3.5 : 8.0;
     const int tile = c->head_dim == 256 ? 64 : 128, sms = c->sm_count;
     const long long most = static_cast<long long>(r->max_new) * group, longest_blocks = (most + rows - 1) / rows, all = static_cast<long long>(r->tokens) * group;
     const bool even = static_cast<long long>(r->max_new) * r->sequences == r->tokens;
@@ -189,7 +190,7 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
             if (parts * m > sms || mapped > kPagedMapped || static_cast<size_t>((longest + length - 1) / length) * per_range > limit) break;
             best = length;
         }
-        if (best + kJoin >= longest) return 0;
+        if (static_cast<double>(best) + join >= static_cast<double>(longest)) return 0;
         int x = 0;
         for (long long o = 0; o < bound; ++o) {
             const int ranges = static_cast<int>((tiles_of(o) + best - 1) / best);
@@ -207,7 +208,7 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
     int best = 1;
     double least = 1e30;
     for (int s = 1; s <= 24 && (s == 1 || (slots(s) <= limit && tiles / s >= 2.0)); ++s) {
-        const double cost = static_cast<double>((left * m * s + room - 1) / room) * (std::ceil(tiles / s) + kStart) + (s > 1 ? kJoin : 0.0);
+        const double cost = static_cast<double>((left * m * s + room - 1) / room) * (std::ceil(tiles / s) + start) + (s > 1 ? join : 0.0);
         if (cost < least * 0.97) best = s, least = cost;
     }
     if (best == 1) return 0;
@@ -516,7 +517,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             if (rc != QUINTRIT_OK) return rc;
             if (plan.part_rows > 0) {
                 auto kernel = a.c.blocks == 1 ? paged_join_kernel<1> : a.c.blocks == 2 ? paged_join_kernel<2> : paged_join_kernel<4>;
-                rc = launch_behind(kernel, static_cast<unsigned>((static_cast<long long>(rows->tokens) * args->q_heads + 7) / 8), s, a, g, plan.many_rows);
+                rc = launch_behind(kernel, static_cast<unsigned>((static_cast<long long>(rows->tokens) * ((args->q_heads + kPagedJoinRows - 1) / kPagedJoinRows) + 7) / 8), s, a, g, plan.many_rows);
                 if (rc != QUINTRIT_OK) return rc;
             }
         }
