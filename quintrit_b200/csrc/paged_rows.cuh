@@ -180,13 +180,16 @@ __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if (k < 0 || !live) continue;
-        const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = __fdividef(1.0f, d);
+        const float d = fmaxf(amax / 127.0f, kPagedMinScale), inv = 1.0f / d;
         uint32_t code[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // |x| / d <= 127 (1 + 2^-22), which rounds to 127; x (1 / d) is off x / d by 2^-16 of a step at most. Added to 1.5 2^23 a number is rounded to its integer, in the low bits
+        for (int i = 0; i < 4; ++i) {  // |x| / d <= 127 (1 + 2^-22), which rounds to 127. Added to 1.5 2^23 a number is rounded to its integer, in the low bits
             uint32_t q[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = __float_as_uint(fmaf(x[4 * i + e], inv, 12582912.0f));
+            for (int e = 0; e < 4; ++e) {
+                const float v = x[4 * i + e], t = v * inv;
+                q[e] = __float_as_uint(fmaf(fmaf(-t, d, v), inv, t) + 12582912.0f);  // with the remainder's part the quotient of a tie is exact, so that it goes to the even code
+            }
             code[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
         }
         *reinterpret_cast<uint2*>(row + (piece >> 3) * block_bytes + paged_piece(a.type, place.row, (piece & 7) >> 1) * 16 + (piece & 1) * 8) = make_uint2(code[0], code[1]);
