@@ -3203,7 +3203,7 @@ void destroy_batch(quintrit_b200_batch* b) {
         if (g != nullptr) cudaGraphExecDestroy(g);
     for (void* p : b->allocs) cudaFree(p);
     if (b->paged != nullptr) {
-        quintrit_b200_paged_cache_free(b->paged->cache);
+        paged_cache_destroy(b->paged->cache);
         cudaFree(b->paged->step_space);
         cudaFree(b->paged->chunk_space);
         cudaFreeHost(b->paged->host_status);

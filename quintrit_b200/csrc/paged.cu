@@ -286,6 +286,8 @@ void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_
 }
 }  // namespace
 
+void qtb::paged_cache_destroy(quintrit_b200_paged_cache* cache) { destroy(cache); }
+
 extern "C" int quintrit_b200_paged_cache_create(uint32_t device_index, uint32_t layers, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, int32_t type,
                                                 quintrit_b200_paged_cache_t** out_cache) {
     return guard([&]() -> int {

@@ -14,3 +14,7 @@ struct quintrit_b200_paged_cache {
     unsigned int* status = nullptr;
     size_t layer_bytes = 0, layer_scales = 0, device_bytes = 0;
 };
+
+namespace qtb {
+void paged_cache_destroy(quintrit_b200_paged_cache* cache);  // quintrit_b200_paged_cache_free that leaves the thread's last error as it is
+}

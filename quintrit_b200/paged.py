@@ -208,14 +208,19 @@ class PagedCache:
     def attend(self, layer: int, rows: PagedRows, q, *, out=None, scale: float | None = None, cap: float = 0.0, window: int = 0, workspace=None, stream=None):
         """Attention of the new tokens' queries [tokens][query heads][head_dim] over the cached positions up to their own (the last ``window`` of them, if that
         is not 0), scores times ``scale`` (default head_dim ** -0.5), capped to ``cap`` tanh(score / ``cap``) if that is not 0. Returns ``out`` (by default
-        new, of the queries' type). ``workspace``: from ``attend_workspace``, by default allocated by torch for this call on its current stream."""
+        new, of the queries' type). ``workspace``: from ``attend_workspace``, by default allocated by torch for this call on its current stream (a call
+        on another ``stream`` brings its own)."""
         at, n = self._rows(rows), rows.tokens
         kind, heads, q_token, q_head = self._heads("q", q, n, None)
         if out is None:
             out = q.new_empty(q.shape)
         o_kind, _, o_token, o_head = self._heads("out", out, n, heads)
+        if not 0 <= window < 2 ** 31:
+            raise ValueError(f"window is 0 (none) or the number of visible positions, got {window}")
         if workspace is None:
             workspace = self.attend_workspace(rows, heads)
+            if stream is not None and stream != _torch_stream(self.device) and workspace.nbytes:  # torch would hand it out again while the call still runs there
+                raise ValueError("a call on another stream than torch's current one brings its workspace")
         elif workspace.get_device() != self.device or not workspace.is_contiguous():
             raise ValueError("the workspace is a contiguous tensor on the cache's device")
         a = _ATTENTION.pack(_ATTENTION.size, kind, o_kind, heads, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, self.head_dim ** -0.5 if scale is None else scale, cap,

@@ -251,7 +251,7 @@ def test_refusals():
     for kw, code in ((dict(pages=0), 3), (dict(pages=4, page_tokens=48), 3), (dict(pages=4, page_tokens=8), 3)):
         with pytest.raises(q.QuintritError) as e:
             q.Batch(d, 2, **kw)
-        assert e.value.code == code
+        assert e.value.code == code and "must be" in str(e.value)
     with pytest.raises(ValueError):
         q.Batch(d, 2, pages=4, cache="f32")
     for n in (0, 257):

@@ -396,3 +396,21 @@ def test_python_refusals():
     with pytest.raises(q.QuintritError) as e:
         big.status()
     assert e.value.code == 14
+
+
+def test_windows_and_workspaces_that_are_refused():
+    rows, pages, _ = make_rows(q, [1], [1000], 16)
+    cache = q.PagedCache(1, pages, 16, 2, 64)
+    x = torch.randn(1, 4, 64, device="cuda").half()
+    for window in (-1, 2 ** 31):
+        with pytest.raises(ValueError):
+            cache.attend(0, rows, x, window=window)
+    side = torch.cuda.Stream()
+    assert cache.attend_workspace(rows, 4).nbytes > 0
+    with pytest.raises(ValueError):  # torch would give the memory to others while the call runs
+        cache.attend(0, rows, x, stream=side.cuda_stream)
+    side.wait_stream(torch.cuda.current_stream())
+    out = cache.attend(0, rows, x, stream=side.cuda_stream, workspace=cache.attend_workspace(rows, 4))
+    torch.cuda.synchronize()
+    assert torch.equal(out, torch.zeros_like(out))  # a new cache holds zeros
+    cache.status()
