@@ -20,7 +20,7 @@
 //
 // Measured: a token over 65431 positions of 5 heads of 128, F16, 167.5 MB in 35.4 us, 72% of the copy rate; a token of each of 32 sequences of 1 to 4096 positions of 4 heads of 256, Q8, 173.7 MB in
 // 41.6 us, 64%. In the loop the copies run at the memory's rate; the rest is the start (places of all sequences, page numbers, the first copies: 8000 cycles), a second segment of a block, the
-// join. Five tokens of each of 16 sequences, 20 rows, Q8: 36 us, 18%: 64 positions take a group of warps 4400 cycles, which are latency (scores 1150, maximum 950, weights 1000, sums 900), and
+// join. Five tokens of each of 16 sequences, 20 rows, Q8: 35 us, 19%: 64 positions take a group of warps 4400 cycles, which are latency (scores 1150, maximum 950, weights 1000, sums 900), and
 // sums for 24 rows leave registers for nine warps on a multiprocessor.
 #pragma once
 #include "paged_cache.cuh"
@@ -197,8 +197,36 @@ struct PagedFew {
     static constexpr int kBlocksPerSm = 2 * (kSmem + (kPagedShared + 1) * 20 + 1024 + 128) <= 228 * 1024 && (NT == 1 || NT * BLOCKS <= 2) ? 2 : 1;
 };
 
+// The pages of the tiles of [begin, end), TILE positions each, for a whole warp that asks tile after tile: 32 entries of the table at a time, one to a lane, the next 32 under way meanwhile (with a read for every tile, which
+// was checked at once, a ring filled at a tile in 1700 cycles).
+template <int TILE>
+struct PagedPages {
+    const PagedView& c;
+    const int* table;
+    int begin, end, lane, step, per, now, next;  // step: positions of a piece, a page or 64 of it; per: pieces of a tile
+    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end)
+        : c(c), table(table), begin(begin), end(end), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
+        next = fetch(0);
+    }
+    __device__ __forceinline__ int fetch(int piece) const {
+        const long long k = begin + (static_cast<long long>(piece) + lane) * step;
+        return k < end ? table[k >> c.page_log2] : 0;
+    }
+    __device__ __forceinline__ int of(int tile) {  // lane i: the page of the tile's piece i
+        const int first = tile * per, at = first & 31;
+        if (at == 0) {
+            now = next, next = fetch(first + 32);
+            if (now < 0 || now >= c.pages) {
+                atomicOr(c.status, kPagedBadPage);
+                now = 0;
+            }
+        }
+        return __shfl_sync(0xffffffffu, now, (at + lane) & 31);
+    }
+};
+
 // Brings the tiles of [begin, end) of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one whole warp. base0, base1: units that the rings have seen
-// before. The pages' numbers of the tile after are asked for before a wait. Returns with its own copies landed.
+// before. Returns with its own copies landed.
 template <int TYPE, int BLOCKS, int NT>
 __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, uint32_t rings, uint32_t full, uint32_t empty,
                                                  int base0, int base1, volatile unsigned int* abort_flag, unsigned int limit) {
@@ -206,21 +234,11 @@ __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* 
     using F = PagedFew<TYPE, BLOCKS, NT>;
     constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
     const int lane = threadIdx.x & 31, P = 1 << c.page_log2, PR = min(P, kPagedTile);
-    auto page_of = [&](int k0) {  // lane i: the page of the tile's piece i
-        const int k = k0 + lane * PR;
-        if (lane * PR >= kPagedTile || k >= end) return 0;
-        int page = table[k >> c.page_log2];
-        if (page < 0 || page >= c.pages) {
-            atomicOr(c.status, kPagedBadPage);
-            page = 0;
-        }
-        return page;
-    };
-    int next = page_of(begin), tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
+    PagedPages<kPagedTile> pages_of(c, table, begin, end);
+    int tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
     bool okay = true;
     for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
-        const int pages = next, pieces = (min(kPagedTile, end - k0) + PR - 1) / PR;
-        if (k0 + kPagedTile < end) next = page_of(k0 + kPagedTile);
+        const int pages = pages_of.of(tile), pieces = (min(kPagedTile, end - k0) + PR - 1) / PR;
 #pragma unroll
         for (int value = 0; value < 2; ++value) {
             const int ring = tile & 1, n = (ring ? base1 : base0) + (tile >> 1) * 2 + value, slot = ring * U + n % U;

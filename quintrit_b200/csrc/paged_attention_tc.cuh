@@ -16,7 +16,7 @@
 // 461 us against 318 us.)
 //
 // Measured: 296 query heads of 128 over 37 KV heads, 256 tokens behind 16384, whole waves: F16 1125 TFLOP/s (69% of the library's matrix product), Q8 870; 2048 tokens of 20 heads of 128 behind
-// 14336: F16 304 us, 1059 TFLOP/s, Q8 401 us, 803; 12 heads of 256: F16 390 us, 990. Q8 waits for its weights: with one score buffer to a row tile its products and its exponentials, 3200 cycles
+// 14336: F16 304 us, 1059 TFLOP/s, Q8 396 us, 813; 12 heads of 256: F16 390 us, 990. Q8 waits for its weights: with one score buffer to a row tile its products and its exponentials, 3200 cycles
 // a tile with the scales, follow one another (two threads to a row there too, of 96 registers each: Q8 528 us, F16 342).
 #pragma once
 #include "packed_f32.cuh"
@@ -231,21 +231,11 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             const int* table = a.r.table + static_cast<size_t>(own.x) * a.r.stride;
             const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
             constexpr int kRing = Q8 ? RW : RS;
-            auto page_of = [&](int k0) {  // lane i: the page of the tile's piece i
-                const int k = k0 + lane * PR;
-                if (lane * PR >= KT || k >= range.end) return 0;
-                int page = table[k >> a.c.page_log2];
-                if (page < 0 || page >= a.c.pages) {
-                    atomicOr(a.c.status, kPagedBadPage);
-                    page = 0;
-                }
-                return page;
-            };
-            int next = tiles > 0 ? page_of(range.begin) : 0, n = 0;
+            PagedPages<KT> pages_of(a.c, table, range.begin, range.end);
+            int n = 0;
             bool okay = true;
             for (int j = 0; j < tiles && okay; ++j) {
-                const int k0 = range.begin + j * KT, pages = next, pieces = (min(KT, range.end - k0) + PR - 1) / PR;
-                if (j + 1 < tiles) next = page_of(k0 + KT);
+                const int k0 = range.begin + j * KT, pages = pages_of.of(j), pieces = (min(KT, range.end - k0) + PR - 1) / PR;
                 for (int value = 0; value < 2; ++value, ++n) {
                     const int s = n % kRing;
                     const uint32_t bar = Q8 ? raw_full(s) : full(s), to = Q8 ? raws + s * M::kRawStride : slots + s * M::kSlot;
