@@ -414,3 +414,24 @@ def test_windows_and_workspaces_that_are_refused():
     torch.cuda.synchronize()
     assert torch.equal(out, torch.zeros_like(out))  # a new cache holds zeros
     cache.status()
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hd,kvh,group", [(64, 2, 4), (128, 1, 3), (256, 1, 4)])
+def test_many_sequences_with_uneven_chunks(cache_type, hd, kvh, group):
+    """More sequences than a warp looks through at once, those with many new tokens among others with a few, one or none."""
+    new = [[1, 40, 0, 2, 130, 1, 5, 70, 33, 1, 3][i % 11] for i in range(70)]
+    check_attention(cache_type, hd, kvh, group, new, [n + (i * 37) % 400 for i, n in enumerate(new)], 32, max_new=130)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("sequences", [200, 300])
+def test_single_tokens_of_very_many_sequences(cache_type, sequences):
+    """As many as share their tiles out, and more."""
+    check_attention(cache_type, 64, 2, 4, [1] * sequences, [1 + (i * 113) % 700 for i in range(sequences)], 16)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("new,group", [(20, 4), (3, 1)])
+def test_one_head_in_more_ranges_than_a_warp_has_lanes(cache_type, new, group):
+    check_attention(cache_type, 64, 1, group, [new], [20011], 128)
