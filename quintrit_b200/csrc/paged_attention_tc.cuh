@@ -621,6 +621,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             if (lane == 0 && okay) mbar_arrive(p_full(b));
         }
         if (okay && tiles > 0) okay = values_done((tiles - 1) * NT + i);
+        if constexpr (!M::kQTmem) {  // results go out over the queries: the products that were waited for have read them; without any, the warps wait for one another's
+            if (tiles == 0) asm volatile("barrier.cta.sync 5, %0;" ::"n"(M::kSoftWarps * 32) : "memory");
+        }
         okay = __all_sync(0xffffffffu, okay && *abort_flag == 0);
         if constexpr (SIDES == 2) {
             mine->x = l, mine->y = okay ? 0.0f : 1.0f;
