@@ -642,6 +642,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         }
     }
     base0 += (tiles + 1) / 2 * 2, base1 += tiles / 2 * 2;
+    fence_async_shared();  // the next segment's copies go where the results met
     __syncthreads();
     }
 }

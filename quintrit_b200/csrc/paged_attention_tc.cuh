@@ -136,7 +136,6 @@ __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // kind::f16: F32 accumulator (1 at bit 4), A and B F16 or BF16 (1 at bits 7 and 10), B transposed (MN-major) at bit 16, N / 8 at bit 17, M / 16 at bit 24.
 __host__ __device__ constexpr uint32_t instr_desc_16(bool bf16, bool b_mn, int n) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);

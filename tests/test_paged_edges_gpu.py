@@ -4,7 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
 from tests.paged_reference import make_rows
-from tests.test_paged_gpu import DT, TYPES, filled, randn
+from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -29,4 +29,15 @@ def test_chunks_longer_than_their_sequences(cache_type, hd):
             assert int(out[s * n:first].count_nonzero()) == 0 and bool((out[first:(s + 1) * n] != 0).any(-1).all())
         assert one is None or torch.equal(out, one)
         one = out
+    cache.status()
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hd,group,new", [(64, 4, 1), (128, 4, 1), (256, 3, 1), (128, 4, 5)])
+def test_segments_that_follow_one_another_in_a_block(cache_type, hd, group, new):
+    """Blocks that end one sequence and begin the next: what the warps have written where the first one's results met does not reach the second one's keys and values."""
+    lengths = [new + 150 + (i * 211) % 1200 for i in range(120)]
+    cache, rows, qs, out = check_attention(cache_type, hd, 4, group, [new] * 120, lengths, 16, q_type="bf16" if cache_type == "bf16" else "f16")
+    for _ in range(100):
+        assert torch.equal(cache.attend(0, rows, qs), out)
     cache.status()
