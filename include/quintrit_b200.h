@@ -491,7 +491,7 @@ typedef struct quintrit_b200_paged_rows {
     uint32_t max_length;       /* no sequence is longer than this, as far as the caller knows: used to divide the work, a longer one is served too */
     uint32_t table_stride;     /* pages that a sequence's row of the table has room for */
     const int32_t* d_starts;   /* [sequences + 1], ascending: sequence s has the packed tokens d_starts[s] .. d_starts[s + 1] - 1 (none is allowed) */
-    const int32_t* d_lengths;  /* [sequences]: cached positions, the new tokens included; the last new token is at position d_lengths[s] - 1 */
+    const int32_t* d_lengths;  /* [sequences]: cached positions, the new tokens included, 2^31 - 2^16 at most; the last new token is at position d_lengths[s] - 1 */
     const int32_t* d_table;    /* [sequences][table_stride]: position p lies in page d_table[s][p / page_tokens] */
 } quintrit_b200_paged_rows_t;
 

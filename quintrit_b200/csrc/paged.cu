@@ -33,7 +33,7 @@ int check_rows(const quintrit_b200_paged_cache*, const quintrit_b200_paged_rows_
     if (r->tokens > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "at most 2^24 tokens, got %u", r->tokens);
     if (r->table_stride == 0 || r->table_stride > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "table_stride must be in [1, 2^24], got %u", r->table_stride);
     if (r->tokens != 0 && (r->max_new == 0 || r->max_new > r->tokens)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_new %u must be in [1, tokens = %u]", r->max_new, r->tokens);
-    if (r->max_length > 0x7fff0000u) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_length %u is too large", r->max_length);
+    if (r->max_length > kPagedLongest) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_length %u is too large", r->max_length);
     if (pointers && (r->d_starts == nullptr || r->d_lengths == nullptr || r->d_table == nullptr)) return fail(QUINTRIT_ERR_NULL_POINTER, "rows.d_starts, d_lengths or d_table is NULL");
     if (pointers && (reinterpret_cast<uintptr_t>(r->d_starts) % 4 != 0 || reinterpret_cast<uintptr_t>(r->d_lengths) % 4 != 0 || reinterpret_cast<uintptr_t>(r->d_table) % 4 != 0))
         return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.d_starts, d_lengths and d_table must be 4-byte aligned");

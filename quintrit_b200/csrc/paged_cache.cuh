@@ -29,6 +29,7 @@ enum PagedStatus : unsigned int {
     kPagedGaveUp = 8,       // a wait inside a kernel ran out
 };
 constexpr int kPagedBlock = 64;  // values of a block
+constexpr int kPagedLongest = 0x7fff0000;  // positions of a sequence at most: a tile, or a few for each of a launch's ranges, beyond its end is still a 32-bit number
 constexpr float kPagedMinScale = 7.888609052210118e-31f;  // 2^-100: rows of smaller values are zeros; its logarithm and its reciprocal stay normal
 constexpr int kPagedFreshScale = 0x0E;  // the bytes of a scale that no row has set: 0x0E0E0E0E is about 2^-99, a row of zeros as if it had been written
 
@@ -69,7 +70,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedView& c, cons
     PagedSequence q;
     const int end = r.starts[s + 1];
     q.first = r.starts[s], q.length = r.lengths[s];
-    const bool fits = q.first >= 0 && q.first <= end && end <= r.tokens && q.length >= 0 && q.length <= (static_cast<long long>(r.stride) << c.page_log2);
+    const bool fits = q.first >= 0 && q.first <= end && end <= r.tokens && q.length >= 0 && q.length <= min(static_cast<long long>(r.stride) << c.page_log2, static_cast<long long>(kPagedLongest));
     q.news = fits ? end - q.first : 0;
     q.ok = q.news > 0;
     if (!fits) atomicOr(c.status, kPagedBadPosition);

@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
-from tests.paged_reference import make_rows
+from tests.paged_reference import EPS, make_rows
 from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,37 @@ def test_segments_that_follow_one_another_in_a_block(cache_type, hd, group, new)
     for _ in range(100):
         assert torch.equal(cache.attend(0, rows, qs), out)
     cache.status()
+
+
+def reported(cache):
+    with pytest.raises(q.QuintritError) as e:
+        cache.status()
+    return e.value.code, str(e.value)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("new", [1, 60])
+def test_the_longest_sequences(cache_type, new):
+    """2^31 - 2^16 positions, all in one page again and again: a window's worth of the last ones is served; longer ones are left out and reported."""
+    most, window, P = 2 ** 31 - 2 ** 16, 100, 256
+    cache = q.PagedCache(1, 1, P, 1, 64, cache_type)
+    table = torch.zeros(1, 1 << 23, dtype=torch.int32, device="cuda")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    k, v = randn(P, 1, 64, seed=1), randn(P, 1, 64, seed=2)
+    cache.append(0, q.PagedRows(i32(0, P), i32(most), table, P, P, most), None, k, v)  # position p is row p % 256 (most is a multiple of it)
+    k, v = cache.read(0, q.PagedRows(i32(0, P), i32(P), table, P, P, P), dtype=torch.float32)
+    kl, vl = cache.read(0, q.PagedRows(i32(0, P), i32(most), table, P, P, most), dtype=torch.float32)
+    assert torch.equal(k, kl) and torch.equal(v, vl)
+    qs = queries(cache_type, new, 4, 64, seed=3)
+    near = cache.attend(0, q.PagedRows(i32(0, new), i32(P), table, new, new, P), qs, window=window)
+    far = cache.attend(0, q.PagedRows(i32(0, new), i32(most), table, new, new, most), qs, window=window)
+    # the same rows, perhaps in other tiles: weights rounded to the cache's type, results too
+    assert float((near.float() - far.float()).abs().max()) <= 4 * EPS[qs.dtype] * float(v.abs().max())
+    cache.status()
+    for length in (most + 1, 2 ** 31 - 1):
+        rows = q.PagedRows(i32(0, new), i32(length), table, new, new, most)
+        for kw in (dict(window=window), dict()):
+            out = cache.attend(0, rows, qs, out=torch.full_like(qs, 4), **kw)
+            assert bool((out == 4).all()) and reported(cache)[0] == 5
+        ko, _ = cache.read(0, rows, k_out=torch.full((new, 1, 64), 4.0, device="cuda"))
+        assert bool((ko == 4).all()) and reported(cache)[0] == 5
