@@ -489,10 +489,11 @@ typedef struct quintrit_b200_paged_rows {
     uint32_t tokens;           /* rows that the packed arrays of the call have */
     uint32_t max_new;          /* no sequence has more new tokens than this */
     uint32_t max_length;       /* no sequence is longer than this, as far as the caller knows: used to divide the work, a longer one is served too */
-    uint32_t table_stride;     /* pages that a sequence's row of the table has room for */
+    uint32_t table_stride;     /* from one sequence's row of the table to the next one's, in entries */
     const int32_t* d_starts;   /* [sequences + 1], ascending: sequence s has the packed tokens d_starts[s] .. d_starts[s + 1] - 1 (none is allowed) */
     const int32_t* d_lengths;  /* [sequences]: cached positions, the new tokens included, 2^31 - 2^16 at most; the last new token is at position d_lengths[s] - 1 */
     const int32_t* d_table;    /* [sequences][table_stride]: position p lies in page d_table[s][p / page_tokens] */
+    uint32_t table_pages;      /* entries of a row, at most table_stride: what lies behind them is not looked at. 0, or a struct_size without this field: table_stride */
 } quintrit_b200_paged_rows_t;
 
 /* Appends the new tokens: each query and key head is RMS-normalised with d_q_norm / d_k_norm (head_dim F32 weights; NULL: not), its first rope_dims values are rotated by its

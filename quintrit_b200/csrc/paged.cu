@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstddef>
 #include <initializer_list>
 #include <type_traits>
 
@@ -26,12 +27,17 @@ int check_layer(const quintrit_b200_paged_cache* c, uint32_t layer) {
     if (layer >= c->layers) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "layer %u of %u", layer, c->layers);
     return QUINTRIT_OK;
 }
+uint32_t table_pages_of(const quintrit_b200_paged_rows_t* r) {
+    const uint32_t pages = r->struct_size < offsetof(quintrit_b200_paged_rows_t, table_pages) + sizeof r->table_pages ? 0 : r->table_pages;
+    return pages != 0 ? pages : r->table_stride;
+}
 int check_rows(const quintrit_b200_paged_cache*, const quintrit_b200_paged_rows_t* r, bool pointers) {
     if (r == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "rows is NULL");
-    if (r->struct_size < sizeof(quintrit_b200_paged_rows_t)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.struct_size %u is too small", r->struct_size);
+    if (r->struct_size < offsetof(quintrit_b200_paged_rows_t, table_pages)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.struct_size %u is too small", r->struct_size);
     if (r->sequences == 0 || r->sequences > 65535) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "sequences must be in [1, 65535], got %u", r->sequences);
     if (r->tokens > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "at most 2^24 tokens, got %u", r->tokens);
     if (r->table_stride == 0 || r->table_stride > (1u << 24)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "table_stride must be in [1, 2^24], got %u", r->table_stride);
+    if (table_pages_of(r) > r->table_stride) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "table_pages %u is more than table_stride = %u", r->table_pages, r->table_stride);
     if (r->tokens != 0 && (r->max_new == 0 || r->max_new > r->tokens)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_new %u must be in [1, tokens = %u]", r->max_new, r->tokens);
     if (r->max_length > kPagedLongest) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "max_length %u is too large", r->max_length);
     if (pointers && (r->d_starts == nullptr || r->d_lengths == nullptr || r->d_table == nullptr)) return fail(QUINTRIT_ERR_NULL_POINTER, "rows.d_starts, d_lengths or d_table is NULL");
@@ -62,6 +68,7 @@ RowsView view_of(const quintrit_b200_paged_rows_t* r) {
     RowsView v{};
     v.starts = r->d_starts, v.lengths = r->d_lengths, v.table = r->d_table;
     v.sequences = static_cast<int>(r->sequences), v.tokens = static_cast<int>(r->tokens), v.stride = static_cast<int>(r->table_stride);
+    v.room = static_cast<int>(table_pages_of(r));
     return v;
 }
 void destroy(quintrit_b200_paged_cache* c) {

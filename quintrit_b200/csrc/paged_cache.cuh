@@ -41,7 +41,7 @@ struct PagedView {  // one layer of a cache
 };
 struct RowsView {
     const int *starts, *lengths, *table;
-    int sequences, tokens, stride;
+    int sequences, tokens, stride, room;  // of the table: from row to row, and entries of a row
 };
 
 __host__ __device__ constexpr int paged_row_bytes(int type) { return type == kPagedQ8 ? kPagedBlock : kPagedBlock * 2; }
@@ -70,7 +70,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedView& c, cons
     PagedSequence q;
     const int end = r.starts[s + 1];
     q.first = r.starts[s], q.length = r.lengths[s];
-    const bool fits = q.first >= 0 && q.first <= end && end <= r.tokens && q.length >= 0 && q.length <= min(static_cast<long long>(r.stride) << c.page_log2, static_cast<long long>(kPagedLongest));
+    const bool fits = q.first >= 0 && q.first <= end && end <= r.tokens && q.length >= 0 && q.length <= min(static_cast<long long>(r.room) << c.page_log2, static_cast<long long>(kPagedLongest));
     q.news = fits ? end - q.first : 0;
     q.ok = q.news > 0;
     if (!fits) atomicOr(c.status, kPagedBadPosition);

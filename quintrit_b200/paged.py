@@ -19,7 +19,7 @@ _sz, _vp, _u32, _i32, _f32 = C.c_size_t, C.c_void_p, C.c_uint32, C.c_int32, C.c_
 
 class _RowsC(C.Structure):
     _fields_ = [("struct_size", _u32), ("sequences", _u32), ("tokens", _u32), ("max_new", _u32), ("max_length", _u32), ("table_stride", _u32), ("d_starts", _vp),
-                ("d_lengths", _vp), ("d_table", _vp)]
+                ("d_lengths", _vp), ("d_table", _vp), ("table_pages", _u32)]
 
 
 class _AppendC(C.Structure):
@@ -99,8 +99,11 @@ class PagedRows:
         if not starts.device == lengths.device == table.device:
             raise ValueError("starts, lengths and table lie on different devices")
         self.starts, self.lengths, self.table, self.tokens = starts, lengths, table, tokens
-        # (the rows of a table may lie further apart than they are long: what lies between is not the sequence's, but pages beyond a length are never looked at)
-        self._c = _RowsC(C.sizeof(_RowsC), n, tokens, max_new, max_length, table.stride(0) if n > 1 else table.shape[1], starts.data_ptr(), lengths.data_ptr(), table.data_ptr())
+        if table.shape[1] == 0:
+            raise ValueError("a row of the table has one page at least")
+        # (the rows of a table may lie further apart than they are long: what lies between is not looked at)
+        self._c = _RowsC(C.sizeof(_RowsC), n, tokens, max_new, max_length, table.stride(0) if n > 1 else table.shape[1], starts.data_ptr(), lengths.data_ptr(), table.data_ptr(),
+                         table.shape[1])
         self._p = C.addressof(self._c)
         self.device = starts.device
         self._device = starts.get_device()

@@ -151,3 +151,11 @@ def test_paged_batches_refuse_what_is_no_batch():
     assert lib.quintrit_b200_batch_create_paged(None, 1, 1, 16, F16, C.byref(out)) == HANDLE and not out.value
     assert lib.quintrit_b200_batch_pages(None, None, None, None) == HANDLE
     assert lib.quintrit_b200_batch_read_cache(None, 0, 0, None, 0, None, 0) == HANDLE
+
+
+def test_tables_with_room_between_their_rows():
+    """table_pages came later than the rest: a caller without it is served as before."""
+    h, n = handle(), C.c_size_t(0)
+    for more, code in ((dict(table_pages=9), ARG), (dict(table_pages=8), 0), (dict(table_pages=1), 0), (dict(struct_size=_RowsC.table_pages.offset, table_pages=9), 0),
+                       (dict(struct_size=_RowsC.table_pages.offset - 1), ARG)):
+        assert call("attention_workspace", h, rows(**more), 4, C.byref(n)) == code

@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
-from tests.paged_reference import EPS, make_rows
+from tests.paged_reference import EPS, make_rows, whole
 from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
@@ -75,3 +75,27 @@ def test_the_longest_sequences(cache_type, new):
             assert bool((out == 4).all()) and reported(cache)[0] == 5
         ko, _ = cache.read(0, rows, k_out=torch.full((new, 1, 64), 4.0, device="cuda"))
         assert bool((ko == 4).all()) and reported(cache)[0] == 5
+
+
+def test_a_table_that_is_a_part_of_another():
+    """The rows of a table may lie further apart than they are long; what lies between is not the sequence's, and is not looked at."""
+    rows, pages, _ = make_rows(q, [2, 2], [40, 48], 16, seed=2)
+    cache = q.PagedCache(1, pages, 16, 2, 64)
+    wide = torch.zeros(2, 9, dtype=torch.int32, device="cuda")  # (page 0 beside the rows' own)
+    wide[:, 3:6] = rows.table
+    part = q.PagedRows(rows.starts, rows.lengths, wide[:, 3:6], 4, 2, 48)
+    x = randn(88, 2, 64, seed=1, dtype=torch.float16)
+    cache.append(0, whole(q, rows), None, x, x)
+    qs = randn(4, 4, 64, seed=3, dtype=torch.float16)
+    want = cache.attend(0, rows, qs)
+    assert torch.equal(cache.attend(0, part, qs), want)
+    assert all(torch.equal(a, b) for a, b in zip(cache.read(0, part), cache.read(0, rows)))
+    cache.status()
+    for length in (49, 60, 80):
+        long = q.PagedRows(rows.starts, torch.tensor([40, length], dtype=torch.int32, device="cuda"), wide[:, 3:6], 4, 2, 80)
+        out = cache.attend(0, long, qs, out=torch.full_like(qs, 4))
+        assert torch.equal(out[:2], want[:2]) and bool((out[2:] == 4).all()) and reported(cache)[0] == 5
+        k, v = cache.read(0, long, k_out=torch.full((4, 2, 64), 4.0, device="cuda"), v_out=torch.full((4, 2, 64), 4.0, device="cuda"))
+        assert bool((k[2:] == 4).all()) and bool((v[2:] == 4).all()) and reported(cache)[0] == 5
+    with pytest.raises(ValueError):
+        q.PagedRows(rows.starts, rows.lengths, wide[:, 3:3], 4, 2, 48)
