@@ -454,7 +454,7 @@ int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint32_t* seque
 
 /* ---- a key / value cache in pages, shared by many sequences, and its attention -----------------------------------------
  * A cache holds `pages` pages of page_tokens positions for each of `layers` layers: keys and values of kv_heads heads of head_dim values, in
- * F16, BF16, or Q8 (8-bit codes rint(x / d) with one F32 scale d = max|x| / 127 per position and head). Which pages a sequence owns, and in
+ * F16, BF16, or Q8 (8-bit codes rint(x / d) with one F32 scale d = max|x| / 127, from 2^-40 to 2^40, per position and head; values beyond 127 * 2^40 do not fit). Which pages a sequence owns, and in
  * what order, is the caller's: a page table per sequence. The reference has one contiguous F16 cache per session
  * (quintrit-runtime/src/kv_cache.rs:24-46) and no counterpart of these functions.
  *

@@ -30,8 +30,10 @@ enum PagedStatus : unsigned int {
 };
 constexpr int kPagedBlock = 64;  // values of a block
 constexpr int kPagedLongest = 0x7fff0000;  // positions of a sequence at most: a tile, or a few for each of a launch's ranges, beyond its end is still a 32-bit number
-constexpr float kPagedMinScale = 7.888609052210118e-31f;  // 2^-100: rows of smaller values are zeros; its logarithm and its reciprocal stay normal
-constexpr int kPagedFreshScale = 0x0E;  // the bytes of a scale that no row has set: 0x0E0E0E0E is about 2^-99, a row of zeros as if it had been written
+// The scales of Q8 rows: 2^-40 (rows of values below it by half are zeros) to 2^40 (larger values are saturated). Attention takes a position's part of a sum as 2^(score + log2 scale - maximum)
+// / scale, and 32 bits end at 2^-126: within these 80 powers no position is lost whose part is 2^-46 of the largest or more (with rows of zeros at 2^-100 they fell out of the sum beside values of 2^33).
+constexpr float kPagedMinScale = 9.094947017729282e-13f, kPagedMaxScale = 1099511627776.0f;
+constexpr int kPagedFreshScale = 0x2C;  // the bytes of a scale that no row has set: 0x2C2C2C2C is about 2^-39, a row of zeros as if it had been written
 
 struct PagedView {  // one layer of a cache
     unsigned char *k, *v;

@@ -3,7 +3,7 @@
 // Writing (paged_append_kernel): for every head x of a new token, y = x * w / sqrt(mean(x^2) + eps) where the head has norm weights, then pairs
 // (x0, x1) of its first `rope` values become (x0 c - x1 s, x0 s + x1 c) with the angles' row of the token's position; value heads take neither.
 // Queries are rounded to their type and written beside one another; keys and values go to their page: rounded to nearest even, or as Q8 codes
-// rint(y / d) with d = max(|y|) / 127 of the row. All arithmetic is in 32 bits; one rounding at the end.
+// rint(y / d) with d = max(|y|) / 127 of the row, from 2^-40 to 2^40. All arithmetic is in 32 bits; one rounding at the end.
 // Reading (paged_read_kernel): the same rows back, code times scale, rounded to the output type.
 //
 // Writing: sixteen values to a thread, two pieces of eight half a head apart, so that the pairs of a rotation lie in one thread whether they are neighbours or halves of a head (eight
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const
         else if (a.turn == kPagedTurnPairs && in[i >> 1]) v = reinterpret_cast<const float4*>(angles + e0 + (i >> 1) * HALF)[i & 1];
         cs[2 * i] = v.x, sn[2 * i] = v.y, cs[2 * i + 1] = v.z, sn[2 * i + 1] = v.w;
     }
-    const float most_finite = a.type == kPagedF16 ? 65504.0f : a.type == kPagedBf16 ? 3.3895313892515355e38f : 8.507059173023462e37f;  // (Q8: 2^126, so that 127 d does not overflow)
+    const float most_finite = a.type == kPagedF16 ? 65504.0f : a.type == kPagedBf16 ? 3.3895313892515355e38f : 127.0f * kPagedMaxScale;
     // where the rows of this token lie in the cache, of head 0; a thread's pieces in them
     const size_t row0 = paged_rows_at(a.c, a.type, place.page, 0, 0) + paged_row_at(a.type, a.c.blocks, 0, place.row), per_head = static_cast<size_t>(a.c.blocks * paged_row_bytes(a.type)) << a.c.page_log2;
 #pragma unroll

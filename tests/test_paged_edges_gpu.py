@@ -7,6 +7,7 @@ from tests.paged_reference import EPS, make_rows, whole
 from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
+FEW_MANY = [1, 60]  # new tokens of four heads to a key head: the kernel for few rows, the one for many
 
 
 def queries(cache_type, *shape, seed):
@@ -99,3 +100,48 @@ def test_a_table_that_is_a_part_of_another():
         assert bool((k[2:] == 4).all()) and bool((v[2:] == 4).all()) and reported(cache)[0] == 5
     with pytest.raises(ValueError):
         q.PagedRows(rows.starts, rows.lengths, wide[:, 3:3], 4, 2, 48)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", FEW_MANY)
+@pytest.mark.parametrize("size", [127 * 2.0 ** -40, 1.0, 127 * 2.0 ** 27, 127 * 2.0 ** 40])
+def test_rows_of_zeros_beside_rows_of_any_size_in_eight_bits(hd, new, size):
+    """Every position has the same score, every other value row is zeros: it has its part of the sum whatever the others' size."""
+    length = 300
+    rows, pages, _ = make_rows(q, [new], [length], 64)
+    cache = q.PagedCache(1, pages, 64, 1, hd, "q8")
+    every = whole(q, rows)
+    v = torch.full((length, 1, hd), size, device="cuda")
+    v[::2] = 0
+    cache.append(0, every, None, randn(length, 1, hd, seed=1), v)
+    cache.status()
+    out = cache.attend(0, rows, torch.zeros(new, 4, hd, device="cuda"), out=torch.empty(new, 4, hd, device="cuda"))
+    p = torch.arange(length - new, length, device="cuda", dtype=torch.float64)
+    want = (size * ((p + 1) / 2).floor() / (p + 1))[:, None, None].expand_as(out)  # position 0 is one of zeros
+    # a scale, its logarithm, its reciprocal and a weight: 2^-21 of one each at most, logarithms of up to 40 another 2^-18; the codes and F16 weights of one are exact
+    assert bool(((out.double() - want).abs() <= want * 2.0 ** -16).all())
+
+
+def test_the_range_of_eight_bits():
+    rows, pages, _ = make_rows(q, [3], [3], 16)
+    cache = q.PagedCache(1, pages, 16, 1, 64, "q8")
+    most, least = 127 * 2.0 ** 40, 2.0 ** -40
+    x = randn(3, 1, 64, seed=1)
+    x = x / x.abs().amax(-1, keepdim=True)
+    x[0] *= most
+    x[1] *= 127 * least
+    x[2] *= 20 * least
+    cache.append(0, rows, None, x, x)
+    cache.status()
+    for got in cache.read(0, rows, dtype=torch.float32):
+        step = torch.tensor([2.0 ** 40, least, least], device="cuda")[:, None, None]  # half of a step of the codes, and the scale's and the quotient's rounding
+        assert bool(((got - x).abs() <= step * (0.5 + 2.0 ** -14)).all())
+    for big in (most * 1.01, 3e38):
+        y = x.clone()
+        y[0, 0, 7], y[2, 0, 9] = big, -big
+        cache.append(0, rows, None, x, y)
+        got = cache.read(0, rows, dtype=torch.float32)[1]
+        assert abs(float(got[0, 0, 7]) / most - 1) < 1e-6 and abs(float(got[2, 0, 9]) / most + 1) < 1e-6
+        with pytest.raises(q.QuintritError) as e:
+            cache.status()
+        assert e.value.code == 5
