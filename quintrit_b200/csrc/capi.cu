@@ -3285,8 +3285,10 @@ int paged_batch_create(quintrit_b200_batch* b, const PagedShape& shape) {
     quintrit_b200_decoder* d = b->d;
     b->paged = std::make_unique<PagedBatch>();
     PagedBatch* p = b->paged.get();
-    int rc = quintrit_b200_paged_cache_create(static_cast<uint32_t>(d->device), d->layers, shape.pages, shape.page_tokens, d->kv_heads, d->head_dim, shape.type, &p->cache);
-    if (rc != QUINTRIT_OK) return rc;
+    int smem_optin = 0;
+    QTB_CUDA(cudaDeviceGetAttribute(&smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, d->device));
+    int rc = allow_max_dynamic_smem(paged_finish_kernel, smem_optin);  // (a decoder has no query rows that this does not hold)
+    if (rc != QUINTRIT_OK || (rc = quintrit_b200_paged_cache_create(static_cast<uint32_t>(d->device), d->layers, shape.pages, shape.page_tokens, d->kv_heads, d->head_dim, shape.type, &p->cache)) != QUINTRIT_OK) return rc;
     const size_t n = b->n_seq;
     p->stride = static_cast<uint32_t>(p->pages_for(d->ctx));
     p->pages.resize(n);
@@ -3317,7 +3319,6 @@ int create_batch(quintrit_b200_decoder_t* decoder, uint32_t sequences, const Pag
         if (sequences == 0 || sequences > static_cast<uint32_t>(kGemmMaxN)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "sequences must be in [1, %d], got %u", kGemmMaxN, sequences);
         if (!prefill_available(d)) return fail(QUINTRIT_ERR_UNSUPPORTED, "this decoder has no batched pass (block-scaled or tensor-parallel model)");
         if (paged != nullptr && d->lay) return fail(QUINTRIT_ERR_UNSUPPORTED, "a layered model keeps its sequences' states and windows itself: no paged batch");
-        if (paged != nullptr && d->q_dim > 12288) return fail(QUINTRIT_ERR_UNSUPPORTED, "query rows of %d values are too long for a paged batch (12288 at most)", d->q_dim);
         DeviceGuard g(d->device);
         if ((rc = prefill_buffers(d)) != QUINTRIT_OK) return rc;
         if (!d->lay && (rc = decoder_gemm_prepare(d)) != QUINTRIT_OK) return rc;

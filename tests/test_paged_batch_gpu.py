@@ -284,3 +284,18 @@ def test_refusals():
     with pytest.raises(q.QuintritError) as e:
         b.pages()
     assert e.value.code == 14
+
+
+@pytest.mark.parametrize("heads", [(191, 1, 64), (96, 2, 128), (48, 1, 256), (128, 1, 128)])
+def test_long_query_rows(heads):
+    """Rows of 12224, 12288 and 16384 values: their codes are made in more shared memory than a kernel has without asking."""
+    spec = _spec(q.ARCH_BITNET, 199, ctx=256, heads=heads)
+    prompts = _prompts([1, 30], spec["vocab"])
+    d = q.Decoder(spec)
+    want, plain = _run(d, prompts, [[1, 2], [3, 4]])
+    got, paged = _run(d, prompts, [[1, 2], [3, 4]], pages=8, page_tokens=16)
+    # (Not bit for bit at one position either: more than 16 heads to a key head take the kernel for many rows, whose exponents are fma(score, scale, -m) with m rounded to 32 bits, so that a sum of one
+    # weight is one but for |z| 2^-24, and a code that lies at a half may go the other way, in all heads of the key head at once.)
+    _near([[_far(got[k, s], want[k, s]) for s in range(2)] for k in range(3)])
+    for x in (plain, paged, d):
+        x.free()
