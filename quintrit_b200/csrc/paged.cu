@@ -45,6 +45,8 @@ int check_rows(const quintrit_b200_paged_cache*, const quintrit_b200_paged_rows_
         return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "rows.d_starts, d_lengths and d_table must be 4-byte aligned");
     return QUINTRIT_OK;
 }
+// What calls have reported so far, taken out in one step, so that a call that reports at the same time is heard now or the next time.
+__global__ void paged_take_status_kernel(unsigned int* status) { status[1] = atomicExch(status, 0u); }
 bool dense_type(int32_t t) { return t == kPagedF32 || t == kPagedF16 || t == kPagedBf16; }
 int check_array(const char* name, const void* p, int32_t type, std::initializer_list<size_t> strides) {
     if (p == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "%s is NULL", name);
@@ -362,14 +364,21 @@ extern "C" int quintrit_b200_paged_cache_status(quintrit_b200_paged_cache_t* cac
         const int rc = check_cache(cache);
         if (rc != QUINTRIT_OK) return rc;
         DeviceGuard g(cache->device);
+        std::lock_guard<std::mutex> one(cache->report);
         unsigned int bits = 0;
-        QTB_CUDA(cudaMemcpy(&bits, cache->status, sizeof bits, cudaMemcpyDeviceToHost));
+        paged_take_status_kernel<<<1, 1>>>(cache->status);
+        QTB_LAUNCH_CHECK();
+        QTB_CUDA(cudaMemcpy(&bits, cache->status + 1, sizeof bits, cudaMemcpyDeviceToHost));
         if (bits == 0) return ok();
-        QTB_CUDA(cudaMemset(cache->status, 0, sizeof bits));
-        if (bits & kPagedGaveUp) return fail(QUINTRIT_ERR_DEVICE, "the paged attention kernel on the CUDA device gave up waiting for its copies");
-        if (bits & kPagedBadPage) return fail(QUINTRIT_ERR_INVALID_VALUE, "a page table named a page that the cache does not have (%u pages)", cache->pages);
-        if (bits & kPagedBadPosition) return fail(QUINTRIT_ERR_INVALID_VALUE, "a token or length lay outside the page table, the angles or the packed rows, or a chunk was longer than announced");
-        return fail(QUINTRIT_ERR_INVALID_VALUE, "a key or value was not finite or too large for the cache's type");
+        std::string said;
+        auto add = [&](unsigned int bit, const std::string& text) {
+            if (bits & bit) said += (said.empty() ? "" : "; ") + text;
+        };
+        add(kPagedGaveUp, "the paged attention kernel on the CUDA device gave up waiting for its copies");
+        add(kPagedBadPage, "a page table named a page that the cache does not have (" + std::to_string(cache->pages) + " pages)");
+        add(kPagedBadPosition, "a token or length lay outside the page table, the angles or the packed rows, or a chunk was longer than announced");
+        add(kPagedSaturated, "a key or value was not finite or too large for the cache's type");
+        return fail(bits & kPagedGaveUp ? QUINTRIT_ERR_DEVICE : QUINTRIT_ERR_INVALID_VALUE, "%s", said.c_str());
     });
 }
 

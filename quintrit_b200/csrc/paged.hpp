@@ -2,6 +2,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <mutex>
+
 #include "../../include/quintrit_b200.h"
 
 struct quintrit_b200_paged_cache {
@@ -11,8 +13,9 @@ struct quintrit_b200_paged_cache {
     int32_t type;
     unsigned char *k = nullptr, *v = nullptr;  // [layers] of the layout of paged_cache.cuh
     float *ks = nullptr, *vs = nullptr;        // Q8: scales
-    unsigned int* status = nullptr;
+    unsigned int* status = nullptr;            // the calls' word, and what a report last took out of it
     size_t layer_bytes = 0, layer_scales = 0, device_bytes = 0;
+    std::mutex report;                         // one report at a time
 };
 
 namespace qtb {

@@ -145,3 +145,40 @@ def test_the_range_of_eight_bits():
         with pytest.raises(q.QuintritError) as e:
             cache.status()
         assert e.value.code == 5
+
+
+def test_a_report_names_all_that_was_met():
+    rows, pages, _ = make_rows(q, [2, 2], [40, 40], 16)
+    cache = q.PagedCache(1, pages, 16, 1, 64)
+    table = rows.table.clone()
+    table[0, 2] = pages
+    x = randn(4, 1, 64, seed=1)
+    x[3, 0, 5] = float("nan")
+    cache.append(0, q.PagedRows(rows.starts, rows.lengths, table, 4, 2, 40), None, x, x)
+    code, said = reported(cache)
+    assert code == 5 and "page" in said and "finite" in said
+    cache.status()
+
+
+def test_no_report_is_lost_to_one_that_is_being_read():
+    """The word is asked for while calls that set it run: each call's report comes with that answer or the next."""
+    rows, pages, _ = make_rows(q, [1], [1], 16)
+    cache = q.PagedCache(1, pages, 16, 1, 64)
+    bad = torch.full((1, 1, 64), float("nan"), device="cuda")
+    side = torch.cuda.Stream()
+    lost = 0
+    with torch.cuda.stream(side):
+        for i in range(2000):
+            for _ in range(i % 5):
+                cache.append(0, rows, None, bad, bad)
+            cache.append(0, rows, None, bad, bad)
+            seen = 0
+            for wait in (False, True):
+                if wait:
+                    side.synchronize()
+                try:
+                    cache.status()
+                except q.QuintritError:
+                    seen += 1
+            lost += seen == 0
+    assert lost == 0
