@@ -118,9 +118,11 @@ template <int T> struct PagedTag { static constexpr int value = T; };
 struct PagedRange {
     int begin, end;
 };
+// The window of a sequence's tokens: one longer than the sequence hides nothing, and the first position that a token sees is a 32-bit number with none longer.
+__device__ __forceinline__ int paged_window(const PagedAttnArgs& a, const PagedSequence& q) { return min(a.window, q.length); }
 // The positions that any new token of a sequence sees; begin is a multiple of 64.
 __device__ __forceinline__ PagedRange paged_seen(const PagedAttnArgs& a, const PagedSequence& q) {
-    return PagedRange{a.window > 0 ? max(0, q.length - q.news - a.window + 1) & ~(kPagedTile - 1) : 0, q.length};
+    return PagedRange{a.window > 0 ? max(0, q.length - q.news - paged_window(a, q) + 1) & ~(kPagedTile - 1) : 0, q.length};
 }
 
 // Work shared out: the items (a sequence's KV head with all its rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles and kPagedStart places in front of
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 #pragma unroll
             for (int i = 0; i < 2; ++i) rowf[n][i] = s_rowf[n * 8 + c4 * 2 + i], m[n][i] = -INFINITY, l[n][i] = 0.0f;
         // positions that every row sees; outside of them the masks are worked out
-        const int all_last = p0, all_first = a.window > 0 ? sq.length - a.window : 0;
+        const int window = paged_window(a, sq), all_last = p0, all_first = a.window > 0 ? sq.length - window : 0;
         float o[KS][NT][4];
 #pragma unroll
         for (int j = 0; j < KS; ++j)
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int rr = n * 8 + c4 * 2 + (e & 1), p = p0 + rr / a.group, j = key0 + g + 8 * (e >> 1);
-                            if (rr >= rows || j > p || j >= range.end || (a.window > 0 && j <= p - a.window)) sc[n][e] = -INFINITY;
+                            if (rr >= rows || j > p || j >= range.end || (a.window > 0 && j <= p - window)) sc[n][e] = -INFINITY;
                         }
                     }
 #pragma unroll

@@ -182,3 +182,16 @@ def test_no_report_is_lost_to_one_that_is_being_read():
                     seen += 1
             lost += seen == 0
     assert lost == 0
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [4, 20, 300])
+def test_windows_next_to_the_largest_number(cache_type, hd, new):
+    cache, _, _, _, _ = filled(cache_type, 2, hd, [1, 1], [new - 3, 30], 16)
+    rows, _, _ = make_rows(q, [new, new], [new - 3, 30], 16, seed=1)
+    qs = queries(cache_type, 2 * new, 8, hd, seed=3)
+    want = cache.attend(0, rows, qs)
+    assert int(want[3:new].count_nonzero()) > 0
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - new, 2 ** 30):
+        assert torch.equal(cache.attend(0, rows, qs, window=window), want), window
