@@ -3,7 +3,9 @@
 ``PagedCache`` owns the pages of all layers; which of them a sequence has is the caller's page table. ``PagedRows`` describes the new tokens of a
 call: their place in packed arrays, the lengths of their sequences and the page tables, all in device memory, so that one object serves every layer
 of a step, and a captured graph serves what its tensors hold when it is replayed. Calls are enqueued on the current torch stream of the cache's
-device (or the ``stream`` given) and do not wait; ``status()`` reports what they met.
+device (or the ``stream`` given, the number of a CUDA stream) and do not wait; ``status()`` reports what they met. Results that the caller does not bring
+are allocated on the stream that the call runs on: another stream waits for it before it reads them, and tells torch so (``record_stream``) if it may still do so
+when they are dropped.
 """
 from __future__ import annotations
 
@@ -118,7 +120,7 @@ class PagedCache:
         if dtype not in _CACHE_TYPES:
             raise ValueError(f"a paged cache is stored as {', '.join(_CACHE_TYPES)}, got {dtype!r}")
         self._lib = _lib()
-        _torch()
+        self._torch_device = _torch().device("cuda", device)
         _api._check(self._lib.quintrit_b200_paged_cache_create(device, layers, pages, page_tokens, kv_heads, head_dim, _CACHE_TYPES[dtype], C.byref(self._h)))
         self.layers, self.pages, self.page_tokens, self.kv_heads, self.head_dim, self.dtype, self.device = layers, pages, page_tokens, kv_heads, head_dim, dtype, device
 
@@ -138,6 +140,15 @@ class PagedCache:
         if kind is None:
             raise ValueError(f"{name} is float32, float16 or bfloat16, got {t.dtype}")
         return kind, shape[1], strides[0], strides[1]
+
+    def _empty(self, shape, dtype, stream):
+        """A new tensor that belongs to the stream that the call runs on: torch's allocator hands memory out, and takes it back, in the order of one stream."""
+        torch = _torch()
+        if stream is None or stream == _torch_stream(self.device):
+            return torch.empty(shape, dtype=dtype, device=self._torch_device)
+        own = torch.cuda.ExternalStream(stream, self._torch_device) if stream else torch.cuda.default_stream(self._torch_device)
+        with torch.cuda.stream(own):
+            return torch.empty(shape, dtype=dtype, device=self._torch_device)
 
     def _call(self, rc):
         if rc != 0:
@@ -160,7 +171,7 @@ class PagedCache:
         if q is not None:
             q_kind, q_heads, q_token, q_head = self._heads("q", q, n, None)
             if q_out is None:
-                q_out = q.new_empty(q.shape)
+                q_out = q.new_empty(q.shape) if stream is None else self._empty(q.shape, q.dtype, stream)
             o_kind, _, o_token, o_head = self._heads("q_out", q_out, n, q_heads)
             q_at, o_at = q.data_ptr(), q_out.data_ptr()
         else:
@@ -189,8 +200,7 @@ class PagedCache:
         ``dtype``: of the results where they are not given (default float16)."""
         at, n = self._rows(rows), rows.tokens
         if k_out is None and v_out is None:
-            torch = _torch()
-            k_out, v_out = (torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype or torch.float16, device=rows.device) for _ in range(2))
+            k_out, v_out = (self._empty((n, self.kv_heads, self.head_dim), dtype or _torch().float16, stream) for _ in range(2))
         kind = None
         for t in (k_out, v_out):
             if t is not None:
@@ -216,7 +226,7 @@ class PagedCache:
         at, n = self._rows(rows), rows.tokens
         kind, heads, q_token, q_head = self._heads("q", q, n, None)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = q.new_empty(q.shape) if stream is None else self._empty(q.shape, q.dtype, stream)
         o_kind, _, o_token, o_head = self._heads("out", out, n, heads)
         if not 0 <= window < 2 ** 31:
             raise ValueError(f"window is 0 (none) or the number of visible positions, got {window}")

@@ -195,3 +195,33 @@ def test_windows_next_to_the_largest_number(cache_type, hd, new):
     assert int(want[3:new].count_nonzero()) > 0
     for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - new, 2 ** 30):
         assert torch.equal(cache.attend(0, rows, qs, window=window), want), window
+
+
+def test_results_belong_to_the_stream_that_writes_them():
+    """Memory that was freed on torch's current stream may still be read there; memory that was freed here may still be written on the call's own."""
+    rows, pages, _ = make_rows(q, [64], [64], 16)
+    cache = q.PagedCache(1, pages, 16, 2, 64)
+    x = randn(64, 8, 64, seed=1, dtype=torch.float16)
+    ws = cache.attend_workspace(rows, 4)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    calls = (lambda: [cache.append(0, rows, x[:, :4], x[:, 4:6], x[:, 6:], stream=side.cuda_stream)], lambda: list(cache.read(0, rows, stream=side.cuda_stream)),
+             lambda: [cache.attend(0, rows, x[:, :4], workspace=ws, stream=side.cuda_stream)])
+    for call in calls:
+        shapes = [t.shape for t in call()]
+        torch.cuda.synchronize()
+        freed = [torch.empty(s, dtype=torch.float16, device="cuda") for s in shapes for _ in range(4)]
+        places = {t.data_ptr() for t in freed}
+        del freed
+        results = call()
+        mine = {t.data_ptr() for t in results}
+        assert not places & mine
+        torch.cuda.synchronize()
+        del results
+        again = [torch.empty(s, dtype=torch.float16, device="cuda") for s in shapes for _ in range(8)]
+        assert not mine & {t.data_ptr() for t in again}
+    with torch.cuda.stream(side):  # the default stream by its number
+        out = cache.read(0, rows, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], cache.read(0, rows)[0])
+    cache.status()
