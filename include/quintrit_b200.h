@@ -522,7 +522,8 @@ int quintrit_b200_paged_append_device(quintrit_b200_paged_cache_t* cache, uint32
 int quintrit_b200_paged_read_device(quintrit_b200_paged_cache_t* cache, uint32_t layer, const quintrit_b200_paged_rows_t* rows, int32_t type, void* d_k, void* d_v, void* stream);
 
 /* Attention of the new tokens over the cached positions up to their own: out = softmax(z) v with z_j = scale q.k_j, or cap tanh(scale q.k_j / cap) with cap > 0, over j <= p and,
- * with window > 0, j > p - window; query head h reads KV head h / (q_heads / kv_heads). A token that sees nothing gives zeros. q_type: that of the cache, or any of F32, F16,
+ * with window > 0, j > p - window; query head h reads KV head h / (q_heads / kv_heads). A token that sees nothing gives zeros. Pages that no new token sees any more, behind
+ * all windows, may be given back: their entries of the table are not looked at. q_type: that of the cache, or any of F32, F16,
  * BF16 over a Q8 cache; out_type: F32, F16 or BF16. Products of 16-bit operands (weights rounded to the cache's type, F16 for Q8) with F32 sums.
  * d_workspace: quintrit_b200_paged_attention_workspace bytes, 16-byte aligned, not shared with a call that may overlap; need not be kept or cleared. */
 typedef struct quintrit_b200_paged_attention {

@@ -120,9 +120,11 @@ struct PagedRange {
 };
 // The window of a sequence's tokens: one longer than the sequence hides nothing, and the first position that a token sees is a 32-bit number with none longer.
 __device__ __forceinline__ int paged_window(const PagedAttnArgs& a, const PagedSequence& q) { return min(a.window, q.length); }
+// The first position that new token t of a sequence, or any behind it, sees.
+__device__ __forceinline__ int paged_first_seen(const PagedAttnArgs& a, const PagedSequence& q, int t) { return a.window > 0 ? max(0, q.length - q.news + t - paged_window(a, q) + 1) : 0; }
 // The positions that any new token of a sequence sees; begin is a multiple of 64.
 __device__ __forceinline__ PagedRange paged_seen(const PagedAttnArgs& a, const PagedSequence& q) {
-    return PagedRange{a.window > 0 ? max(0, q.length - q.news - paged_window(a, q) + 1) & ~(kPagedTile - 1) : 0, q.length};
+    return PagedRange{paged_first_seen(a, q, 0) & ~(kPagedTile - 1), q.length};
 }
 
 // Work shared out: the items (a sequence's KV head with all its rows) stand one after the other, sequence by sequence, each as long as its sequence's tiles and kPagedStart places in front of
@@ -200,19 +202,19 @@ struct PagedFew {
 };
 
 // The pages of the tiles of [begin, end), TILE positions each, for a whole warp that asks tile after tile: 32 entries of the table at a time, one to a lane, the next 32 under way meanwhile (with a read for every tile, which
-// was checked at once, a ring filled at a tile in 1700 cycles).
+// was checked at once, a ring filled at a tile in 1700 cycles). Pieces in front of position `seen` are nobody's to look at: their pages may have been given back.
 template <int TILE>
 struct PagedPages {
     const PagedView& c;
     const int* table;
-    int begin, end, lane, step, per, now, next;  // step: positions of a piece, a page or 64 of it; per: pieces of a tile
-    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end)
-        : c(c), table(table), begin(begin), end(end), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
+    int begin, end, seen, lane, step, per, now, next;  // step: positions of a piece, a page or 64 of it; per: pieces of a tile
+    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end, int seen)
+        : c(c), table(table), begin(begin), end(end), seen(seen), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
         next = fetch(0);
     }
     __device__ __forceinline__ int fetch(int piece) const {
         const long long k = begin + (static_cast<long long>(piece) + lane) * step;
-        return k < end ? table[k >> c.page_log2] : 0;
+        return k < end && k + step > seen ? table[k >> c.page_log2] : 0;
     }
     __device__ __forceinline__ int of(int tile) {  // lane i: the page of the tile's piece i
         const int first = tile * per, at = first & 31;
@@ -227,16 +229,16 @@ struct PagedPages {
     }
 };
 
-// Brings the tiles of [begin, end) of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one whole warp. base0, base1: units that the rings have seen
-// before. Returns with its own copies landed.
+// Brings the tiles of [begin, end), of which the positions from `seen` on are looked at, of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one
+// whole warp. base0, base1: units that the rings have seen before. Returns with its own copies landed.
 template <int TYPE, int BLOCKS, int NT>
-__device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, uint32_t rings, uint32_t full, uint32_t empty,
+__device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, int seen, uint32_t rings, uint32_t full, uint32_t empty,
                                                  int base0, int base1, volatile unsigned int* abort_flag, unsigned int limit) {
     using namespace gemm_detail;
     using F = PagedFew<TYPE, BLOCKS, NT>;
     constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
     const int lane = threadIdx.x & 31, P = 1 << c.page_log2, PR = min(P, kPagedTile);
-    PagedPages<kPagedTile> pages_of(c, table, begin, end);
+    PagedPages<kPagedTile> pages_of(c, table, begin, end, seen);
     int tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
     bool okay = true;
     for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     const int tiles = (range.end - range.begin + kPagedTile - 1) / kPagedTile;
     __syncthreads();  // the barriers are there; the segment before has left the ring
     if (warp == 8) {
-        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, ring, full, empty, base0, base1, abort_flag, a.spin_limit);
+        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, paged_first_seen(a, sq, 0), ring, full, empty, base0, base1, abort_flag, a.spin_limit);
     } else {
         // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none; all of them are asked for before the first is used
         auto load_rows = [&](auto of) {

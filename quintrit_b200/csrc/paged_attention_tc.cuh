@@ -82,7 +82,7 @@ __device__ __forceinline__ size_t paged_part_row(const PagedAttnArgs& a, const P
 }
 // Range `part` of `parts` of what rows of tokens [t0, t1) see; begin is a multiple of 64.
 __device__ __forceinline__ PagedRange paged_part_range(const PagedAttnArgs& a, const PagedSequence& q, int t0, int t1, int part, int parts, int tile) {
-    const int p0 = q.length - q.news, low = a.window > 0 ? max(0, p0 + t0 - paged_window(a, q) + 1) & ~(kPagedTile - 1) : 0, high = max(low, max(0, p0 + t1));
+    const int p0 = q.length - q.news, low = paged_first_seen(a, q, t0) & ~(kPagedTile - 1), high = max(low, max(0, p0 + t1));
     const int tiles = (high - low + tile - 1) / tile, per = (tiles + parts - 1) / parts;
     return PagedRange{min(high, low + part * per * tile), min(high, low + (part + 1) * per * tile)};
 }
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             const int* table = a.r.table + static_cast<size_t>(own.x) * a.r.stride;
             const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
             constexpr int kRing = Q8 ? RW : RS;
-            PagedPages<KT> pages_of(a.c, table, range.begin, range.end);
+            PagedPages<KT> pages_of(a.c, table, range.begin, range.end, paged_first_seen(a, sq, r0 / a.group));
             int n = 0;
             bool okay = true;
             for (int j = 0; j < tiles && okay; ++j) {
@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
         }
         const float rowf = row_factor[i * 128 + local];  // what the row's scores are multiplied by: positive, the queries took the sign
         // (a row that is not there, of zeros, sees everything, so that it makes no masks necessary: a row tile of 20 rows that masked every tile for the others took 58 us instead of 47)
-        const int p = p0 + t, last = live ? min(p, range.end - 1) : range.end - 1, first = live && a.window > 0 ? max(0, p - paged_window(a, sq) + 1) : 0;
+        const int p = p0 + t, last = live ? min(p, range.end - 1) : range.end - 1, first = live ? paged_first_seen(a, sq, t) : 0;
         const bool some = r0 + i * 128 + (warp & 3) * 32 < r1;  // the same for the two warps that meet
         float m = -INFINITY, l = 0.0f;  // l: over this thread's positions
         bool okay = true;

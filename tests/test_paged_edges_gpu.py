@@ -225,3 +225,18 @@ def test_results_belong_to_the_stream_that_writes_them():
     torch.cuda.synchronize()
     assert torch.equal(out[0], cache.read(0, rows)[0])
     cache.status()
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("new,lengths", [([1, 1], [700, 9000]), ([5, 3], [333, 4097]), ([150, 40], [500, 3000])])
+def test_pages_that_the_window_has_left_behind_are_not_looked_at(cache_type, page, new, lengths):
+    for window in (1, 30, 100, 257):
+        cache, rows, _, _, _ = filled(cache_type, 2, 64, new, lengths, page, seed=2)
+        qs = queries(cache_type, rows.tokens, 8, 64, seed=3)
+        clean = cache.attend(0, rows, qs, window=window).clone()
+        cache.status()
+        for s, (n, length) in enumerate(zip(new, lengths)):
+            rows.table[s, :max(0, length - n - window + 1) // page] = -1  # given back
+        assert torch.equal(cache.attend(0, rows, qs, window=window), clean)
+        cache.status()
