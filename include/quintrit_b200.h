@@ -464,7 +464,8 @@ int quintrit_b200_batch_step(quintrit_b200_batch_t* batch, const uint32_t* seque
  * nothing. Calls that write the same positions, or read what another writes, are ordered by the caller; otherwise calls may overlap.
  *
  * Device data that is out of range (a page number, a token or length outside the table, the angles or the packed rows; a chunk longer than max_new) is
- * skipped, and quintrit_b200_paged_cache_status reports it. The rows behind the last sequence (d_starts[sequences] and up) are left as they were. */
+ * skipped, and quintrit_b200_paged_cache_status reports it: the rows of the cache and of the results that it stands for are left as they were (attention: those of every new token of the
+ * sequence that sees such a page). The rows behind the last sequence (d_starts[sequences] and up) are left as they were. */
 #define QUINTRIT_B200_F32 0
 #define QUINTRIT_B200_F16 1
 #define QUINTRIT_B200_BF16 2

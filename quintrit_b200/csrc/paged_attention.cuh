@@ -113,6 +113,9 @@ __device__ __forceinline__ long long prefix(long long v) {  // the sum of v over
 
 }  // namespace paged_detail
 
+// In the place of a partial result's maximum and sum: the row is not to be written, for want of a page.
+__device__ __forceinline__ float2 paged_left_out() { return make_float2(-INFINITY, -1.0f); }
+
 template <int T> struct PagedTag { static constexpr int value = T; };
 
 struct PagedRange {
@@ -203,13 +206,15 @@ struct PagedFew {
 
 // The pages of the tiles of [begin, end), TILE positions each, for a whole warp that asks tile after tile: 32 entries of the table at a time, one to a lane, the next 32 under way meanwhile (with a read for every tile, which
 // was checked at once, a ring filled at a tile in 1700 cycles). Pieces in front of position `seen` are nobody's to look at: their pages may have been given back.
+// A page that the cache does not have is reported and raises `bad`; page 0 stands in for it, and the results are not written.
 template <int TILE>
 struct PagedPages {
     const PagedView& c;
     const int* table;
+    volatile unsigned int* bad;
     int begin, end, seen, lane, step, per, now, next;  // step: positions of a piece, a page or 64 of it; per: pieces of a tile
-    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end, int seen)
-        : c(c), table(table), begin(begin), end(end), seen(seen), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
+    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end, int seen, volatile unsigned int* bad)
+        : c(c), table(table), bad(bad), begin(begin), end(end), seen(seen), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
         next = fetch(0);
     }
     __device__ __forceinline__ int fetch(int piece) const {
@@ -222,7 +227,7 @@ struct PagedPages {
             now = next, next = fetch(first + 32);
             if (now < 0 || now >= c.pages) {
                 atomicOr(c.status, kPagedBadPage);
-                now = 0;
+                *bad = 1, now = 0;
             }
         }
         return __shfl_sync(0xffffffffu, now, (at + lane) & 31);
@@ -233,12 +238,12 @@ struct PagedPages {
 // whole warp. base0, base1: units that the rings have seen before. Returns with its own copies landed.
 template <int TYPE, int BLOCKS, int NT>
 __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, int seen, uint32_t rings, uint32_t full, uint32_t empty,
-                                                 int base0, int base1, volatile unsigned int* abort_flag, unsigned int limit) {
+                                                 int base0, int base1, volatile unsigned int* abort_flag, volatile unsigned int* bad_flag, unsigned int limit) {
     using namespace gemm_detail;
     using F = PagedFew<TYPE, BLOCKS, NT>;
     constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
     const int lane = threadIdx.x & 31, P = 1 << c.page_log2, PR = min(P, kPagedTile);
-    PagedPages<kPagedTile> pages_of(c, table, begin, end, seen);
+    PagedPages<kPagedTile> pages_of(c, table, begin, end, seen, bad_flag);
     int tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
     bool okay = true;
     for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     unsigned char* s_q = smem + F::kBody;                                       // [kRows][kPitch]
     float* s_rowf = reinterpret_cast<float*>(s_q + F::kRows * kPitch);          // [kRows]: what a row's score is multiplied by
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_rowf + F::kRows);
-    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U);
+    volatile unsigned int *abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U), *bad_flag = abort_flag + 1;  // bad: the segment's sequence has a page that is not there
     __shared__ int s_before[kPagedShared + 1];
     __shared__ int4 s_of[kPagedShared];
     const uint32_t full = smem_u32(bars), empty = full + 16 * U;
@@ -321,9 +326,10 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     const int rows = sq.news * a.group, p0 = sq.length - sq.news;
     range.end = max(range.begin, range.end);
     const int tiles = (range.end - range.begin + kPagedTile - 1) / kPagedTile;
+    if (tid == 0) *bad_flag = 0;
     __syncthreads();  // the barriers are there; the segment before has left the ring
     if (warp == 8) {
-        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, paged_first_seen(a, sq, 0), ring, full, empty, base0, base1, abort_flag, a.spin_limit);
+        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, paged_first_seen(a, sq, 0), ring, full, empty, base0, base1, abort_flag, bad_flag, a.spin_limit);
     } else {
         // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none; all of them are asked for before the first is used
         auto load_rows = [&](auto of) {
@@ -610,10 +616,15 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     __syncthreads();
     if (*abort_flag != 0) return;
     // rows out: eight values to a thread
+    const bool left_out = *bad_flag != 0;
     const float* joined = reinterpret_cast<const float*>(smem);
     const float2* mls = reinterpret_cast<const float2*>(smem + 8 * F::kRows * F::kJoinPitch * 4);
     for (int i = tid; i < rows * (HD / 8); i += kThreads) {
         const int r = i / (HD / 8), e0 = i % (HD / 8) * 8;
+        if (left_out) {
+            if (parts_place >= 0 && e0 == 0) a.part_ml[static_cast<size_t>(parts_place) * F::kRows + r] = paged_left_out();
+            continue;
+        }
         float top = -INFINITY, w[8], sum = 0.0f, x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, mls[k * F::kRows + r].x);
@@ -652,14 +663,19 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 }
 
 // Joins results: weights 2^(m_i - m) over `count` of them, the i-th in row row_of(i) of the workspace, for the values of one warp's lanes (kPer each), by the WARPS warps of a block in turn, a few results at
-// a time so that their reads overlap; in the same order whenever it is asked for. Returns the row's normalised values, in the first warp.
+// a time so that their reads overlap; in the same order whenever it is asked for. The row's normalised values are the first warp's; returns whether they are to be written.
 template <int HD, int WARPS, typename RowOf>
-__device__ __forceinline__ void paged_join(const float* part_o, const float2* part_ml, RowOf row_of, int count, float (&x)[HD / 32], float* shared) {
+__device__ __forceinline__ bool paged_join(const float* part_o, const float2* part_ml, RowOf row_of, int count, float (&x)[HD / 32], float* shared) {
     using namespace paged_detail;
     constexpr int kPer = HD / 32;
     const int lane = threadIdx.x & 31, warp = WARPS > 1 ? threadIdx.x >> 5 : 0;
     float top = -INFINITY;
-    for (int i = lane; i < count; i += 32) top = fmaxf(top, part_ml[row_of(i)].x);
+    bool left_out = false;
+    for (int i = lane; i < count; i += 32) {
+        const float2 v = part_ml[row_of(i)];
+        top = fmaxf(top, v.x), left_out = left_out || v.y < 0.0f;
+    }
+    left_out = __any_sync(0xffffffffu, left_out);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.0f;
@@ -695,7 +711,7 @@ __device__ __forceinline__ void paged_join(const float* part_o, const float2* pa
         for (int e = 0; e < kPer; ++e) mine[e] = x[e];
         mine[kPer] = sum;
         __syncthreads();
-        if (warp != 0) return;
+        if (warp != 0) return false;
 #pragma unroll
         for (int w = 1; w < WARPS; ++w) {
             const float* other = shared + (w * 32 + lane) * (kPer + 1);
@@ -707,6 +723,7 @@ __device__ __forceinline__ void paged_join(const float* part_o, const float2* pa
     const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) x[e] *= inv;
+    return !left_out;
 }
 template <int PER>
 __device__ __forceinline__ void paged_store_row(unsigned char* out, int type, const float (&x)[PER]) {
@@ -744,14 +761,12 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constan
     float v[kPer];
     if (cuts < 8) {
         for (int r = mine + cuts * warp; r < rows; r += cuts * 8) {
-            paged_join<HD, 1>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, nullptr);
-            out(r, v);
+            if (paged_join<HD, 1>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, nullptr)) out(r, v);
         }
     } else {
         for (int r = mine; r < rows; r += cuts) {
             __syncthreads();
-            paged_join<HD, 8>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, shared);
-            if (warp == 0) out(r, v);
+            if (paged_join<HD, 8>(a.part_o, a.part_ml, [&](int i) { return static_cast<size_t>((b0 + i) * 2 + (i == 0 ? place0 : 0)) * block_rows + r; }, cuts + 1, v, shared)) out(r, v);
         }
     }
 }

@@ -110,7 +110,7 @@ struct PagedMany {
     static constexpr bool kSplitRegs = NT == 2;
     static constexpr int kLaunchRegs = Q8 ? 128 : 168, kSoftRegs = Q8 ? 200 : 216, kRestRegs = Q8 ? 56 : 72;
     static_assert(!kSplitRegs || kSoftWarps * 32 * kSoftRegs + (kThreads - kSoftWarps * 32) * kRestRegs <= kThreads * kLaunchRegs, "more registers than the block was launched with");
-    static constexpr int kBars = 2 * kSlots + 2 * kRaws + 3 * NB + 2;
+    static constexpr int kBars = 2 * kSlots + 2 * kRaws + 3 * NB + 3;
     static constexpr int kNeed = 1024 + kQBytes + kSlots * kSlot + kRaws * kRawStride + kFactors * KT * 12 + (SIDES == 2 ? 2048 : 0) + NT * 512 + kStageOwn + kBars * 8 + 16;
     static constexpr int kSmem = kNeed > 116 * 1024 ? kNeed : 116 * 1024;  // one block per multiprocessor: it takes all of its tensor memory
     static constexpr int kOCol = 0, kSCol = 256, kQCol = BLOCKS == 4 ? 384 : 128;  // tensor memory columns: O (of row tile i at 128 i), S (buffer b at KT b behind), Q
@@ -185,9 +185,9 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
     auto s_full = [&](int b) { return tail + 8u * b; };                     // scores of a buffer
     auto p_full = [&](int b) { return tail + 8u * (NB + b); };               // weights of a buffer
     auto o_done = [&](int b) { return tail + 8u * (2 * NB + b); };               // the value products of a buffer's weights
-    const uint32_t q_full = tail + 8u * (3 * NB), drained = q_full + 8u;
+    const uint32_t q_full = tail + 8u * (3 * NB), drained = q_full + 8u, pages_known = drained + 8u;  // the last: every page number was looked at
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bars + M::kBars);
-    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1);
+    volatile unsigned int *abort_flag = reinterpret_cast<volatile unsigned int*>(tmem_slot + 1), *bad_flag = abort_flag + 1;  // bad: the sequence has a page that is not there
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const PagedPart part = paged_part(g, static_cast<int>(blockIdx.x) / g.m);
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
         for (int s = 0; s < M::kRaws; ++s) mbar_init(raw_full(s), 1), mbar_init(raw_empty(s), M::kWidenWarps);
         for (int b = 0; b < NB; ++b) mbar_init(s_full(b), 1), mbar_init(p_full(b), 4 * SIDES), mbar_init(o_done(b), 1);
         mbar_init(q_full, M::kSoftWarps);
-        mbar_init(drained, 1);
-        *abort_flag = 0;
+        mbar_init(drained, 1), mbar_init(pages_known, 1);
+        *abort_flag = 0, *bad_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == M::kMmaWarp) {
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             const int* table = a.r.table + static_cast<size_t>(own.x) * a.r.stride;
             const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
             constexpr int kRing = Q8 ? RW : RS;
-            PagedPages<KT> pages_of(a.c, table, range.begin, range.end, paged_first_seen(a, sq, r0 / a.group));
+            PagedPages<KT> pages_of(a.c, table, range.begin, range.end, paged_first_seen(a, sq, r0 / a.group), bad_flag);
             int n = 0;
             bool okay = true;
             for (int j = 0; j < tiles && okay; ++j) {
@@ -259,6 +259,8 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     }
                 }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pages_known);
             for (int back = max(0, n - kRing); back < n; ++back) mbar_wait(Q8 ? raw_full(back % kRing) : full(back % kRing), (back / kRing) & 1, abort_flag, a.spin_limit, false);
         } else if (warp == M::kMmaWarp) {
             // ---- all products: one thread issues them, but the warp stays together, so that descriptors live in uniform registers (issued by a lane on its own, eight products took as long to issue
@@ -623,6 +625,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
         if constexpr (!M::kQTmem) {  // results go out over the queries: the products that were waited for have read them; without any, the warps wait for one another's
             if (tiles == 0) asm volatile("barrier.cta.sync 5, %0;" ::"n"(M::kSoftWarps * 32) : "memory");
         }
+        if (okay) okay = __all_sync(0xffffffffu, mbar_wait(pages_known, 0, abort_flag, a.spin_limit));
         okay = __all_sync(0xffffffffu, okay && *abort_flag == 0);
         if constexpr (SIDES == 2) {
             mine->x = l, mine->y = okay ? 0.0f : 1.0f;
@@ -633,10 +636,11 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
         if (!okay && lane == 0) atomicOr(a.c.status, kPagedGaveUp);
         if (okay) {
             fence_after();
+            const bool left_out = *bad_flag != 0;
             const float inv = part.ranges > 1 ? 1.0f : l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
             const int wr = r0 + i * 128 + (warp & 3) * 32;  // the warp's first row
             const size_t row = paged_part_row(a, g, sq, part, which, kvh, r, i * 128 + local, M::kRows);
-            if (tiles > 0 || part.ranges == 1) {  // (of a range in which the rows see nothing only the sums below are read)
+            if (!left_out && (tiles > 0 || part.ranges == 1)) {  // (of a range in which the rows see nothing only the sums below are read)
 #pragma unroll 1
                 for (int c = side * HH; c < (side + 1) * HH; c += 32) {
                     uint32_t o[32];
@@ -668,7 +672,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     }
                 }
             }
-            if (live && part.ranges > 1 && side == 0) g.part_ml[row] = make_float2(m, l);
+            if (live && part.ranges > 1 && side == 0) g.part_ml[row] = left_out ? paged_left_out() : make_float2(m, l);
         }
     }
     fence_before();
@@ -713,12 +717,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     auto sums_of = [&](int k, int i) { return i < ranges[k] && ranges[k] > 1 ? g.part_ml[from[k] + i * step[k]] : make_float2(-INFINITY, 0.0f); };
     float top[ROWS], total[ROWS] = {}, x[ROWS][kPer] = {};
     float2 ml[ROWS];
+    bool left_out[ROWS];
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) ml[k] = sums_of(k, lane);
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-        top[k] = ml[k].x;
-        for (int i = lane + 32; i < most; i += 32) top[k] = fmaxf(top[k], sums_of(k, i).x);
+        top[k] = ml[k].x, left_out[k] = ml[k].y < 0.0f;
+        for (int i = lane + 32; i < most; i += 32) {
+            const float2 v = sums_of(k, i);
+            top[k] = fmaxf(top[k], v.x), left_out[k] = left_out[k] || v.y < 0.0f;
+        }
+        left_out[k] = __any_sync(0xffffffffu, left_out[k]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
     }
@@ -749,7 +758,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     }
 #pragma unroll
     for (int k = 0; k < ROWS; ++k) {
-        if (ranges[k] == 1) continue;
+        if (ranges[k] == 1 || left_out[k]) continue;
         const float inv = total[k] > 0.0f ? 1.0f / total[k] : total[k] == 0.0f ? 0.0f : total[k];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[k][e] *= inv;

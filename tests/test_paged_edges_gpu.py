@@ -240,3 +240,27 @@ def test_pages_that_the_window_has_left_behind_are_not_looked_at(cache_type, pag
             rows.table[s, :max(0, length - n - window + 1) // page] = -1  # given back
         assert torch.equal(cache.attend(0, rows, qs, window=window), clean)
         cache.status()
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hd,new,lengths", [(64, [1, 1, 1], [40, 40, 40]), (128, [1] * 3, [5000, 9000, 3000]), (64, [3, 3, 3], [900, 20001, 70]), (128, [70, 70, 70], [70, 90, 4000]),
+                                            (256, [40, 40, 40], [100, 2000, 300]), (128, [64, 64, 64], [9000, 20000, 9000]), (64, [1, 130, 3], [3000, 9000, 40])])
+def test_a_sequence_with_a_page_that_is_not_there_is_left_out(cache_type, hd, new, lengths):
+    """Nothing is written for it, whether one block has it whole or many have ranges of it; the others are as they were."""
+    cache, rows, _, _, _ = filled(cache_type, 2, hd, new, lengths, 16, seed=2)
+    qs = queries(cache_type, rows.tokens, 8, hd, seed=3)
+    clean = cache.attend(0, rows, qs).clone()
+    cache.status()
+    a, b = rows.starts[1:3].tolist()
+    for at, page in ((0, -1), ((lengths[1] - 1) // 16, cache.pages), (lengths[1] // 40, 1 << 30)):
+        table = rows.table.clone()
+        table[1, at] = page
+        out = cache.attend(0, q.PagedRows(rows.starts, rows.lengths, table, rows.tokens, max(new), max(lengths)), qs, out=torch.full_like(qs, 4))
+        assert torch.equal(out[:a], clean[:a]) and torch.equal(out[b:], clean[b:])
+        seen = (out[a:b] != 4).flatten(1).any(1)
+        see = torch.arange(lengths[1] - new[1], lengths[1], device="cuda") >= at * 16  # tokens that see a position of the page
+        assert not bool(seen[see].any())
+        assert torch.equal(out[a:b][seen], clean[a:b][seen])  # (tokens that do not see the page may have been answered)
+        assert reported(cache)[0] == 5
+    assert torch.equal(cache.attend(0, rows, qs), clean)
+    cache.status()
