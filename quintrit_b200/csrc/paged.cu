@@ -70,7 +70,7 @@ RowsView view_of(const quintrit_b200_paged_rows_t* r) {
     RowsView v{};
     v.starts = r->d_starts, v.lengths = r->d_lengths, v.table = r->d_table;
     v.sequences = static_cast<int>(r->sequences), v.tokens = static_cast<int>(r->tokens), v.stride = static_cast<int>(r->table_stride);
-    v.room = static_cast<int>(table_pages_of(r));
+    v.room = static_cast<int>(table_pages_of(r)), v.most = static_cast<int>(r->max_new);
     return v;
 }
 void destroy(quintrit_b200_paged_cache* c) {
@@ -521,12 +521,11 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         a.scale = args->cap > 0.0f ? args->scale / args->cap : args->scale * kLog2e;
         a.cap = args->cap * kLog2e;
         a.window = static_cast<int>(args->window);
-        a.most = static_cast<int>(rows->max_new);
         a.spin_limit = kPagedSpin;
         const int device = cache->device;
         unsigned char* workspace = static_cast<unsigned char*>(args->d_workspace);
         if (plan.many) {
-            a.few = plan.few_new + 1, a.many = a.most;
+            a.few = plan.few_new + 1, a.many = a.r.most;
             PagedSchedule& g = plan.schedule;
             g.part_o = reinterpret_cast<float*>(workspace + plan.few_bytes), g.part_ml = reinterpret_cast<float2*>(g.part_o + plan.part_rows * cache->head_dim);
             const unsigned grid = static_cast<unsigned>(plan.many_blocks);

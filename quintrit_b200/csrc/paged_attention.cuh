@@ -48,7 +48,6 @@ struct PagedAttnArgs {
     float* part_o;           // [blocks][2][rows of a block][head_dim], where the tiles are shared out
     float2* part_ml;         // [blocks][2][rows of a block]
     int few, many;           // new tokens of the sequences that this launch serves: few <= n <= many
-    int most;                // new tokens of the longest chunk as announced: the grid has no rows for more
     unsigned int spin_limit;
 };
 
@@ -154,7 +153,7 @@ __device__ __forceinline__ PagedShare paged_share_begin(const PagedAttnArgs& a, 
         const int tiles = max(1, (g.end - g.begin + kPagedTile - 1) / kPagedTile);
         before[s + 1] = q.ok && q.news >= a.few && q.news <= a.many ? static_cast<int>(min((tiles + static_cast<long long>(kPagedStart)) * a.c.kv_heads, 0x7fffffffLL)) : 0;
         of[s] = make_int4(q.first, q.news, q.length, tiles);
-        if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
+        if (q.news > a.r.most) atomicOr(a.c.status, kPagedBadPosition);
     }
     if (threadIdx.x == 0) before[0] = 0;
     __syncthreads();
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         at = until, seq = blockIdx.y, kvh = blockIdx.x;
         sq = paged_sequence(a.c, a.r, seq);
         if (!sq.ok || sq.news < a.few || sq.news > a.many) {
-            if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
+            if (sq.news > a.r.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
             return;
         }
         range = paged_seen(a, sq);

@@ -50,7 +50,7 @@ __device__ __forceinline__ PagedPart paged_part(const PagedSchedule& g, int x) {
 // The row blocks of sequence s that this launch serves.
 __device__ __forceinline__ int paged_row_blocks(const PagedAttnArgs& a, int s, int rows) {
     const PagedSequence q = paged_sequence(a.c, a.r, s);
-    if (q.news > a.most) atomicOr(a.c.status, kPagedBadPosition);
+    if (q.news > a.r.most) atomicOr(a.c.status, kPagedBadPosition);
     return q.ok && q.news >= a.few && q.news <= a.many ? (q.news * a.group + rows - 1) / rows : 0;
 }
 // The sequence that has the x-th row block of all, and which of its own it is, or the sequence -1; by all lanes of a warp. And the row blocks of the sequences before s.
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
     if (own.x < 0) return;
     const PagedSequence sq = paged_sequence(a.c, a.r, own.x);
     if (!sq.ok || sq.news < a.few || sq.news > a.many) {
-        if (sq.news > a.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
+        if (sq.news > a.r.most && tid == 0) atomicOr(a.c.status, kPagedBadPosition);
         return;
     }
     const int rows = sq.news * a.group, block = (rows + M::kRows - 1) / M::kRows - 1 - own.y, r0 = block * M::kRows, r1 = min(rows, r0 + M::kRows);

@@ -44,6 +44,7 @@ struct PagedView {  // one layer of a cache
 struct RowsView {
     const int *starts, *lengths, *table;
     int sequences, tokens, stride, room;  // of the table: from row to row, and entries of a row
+    int most;                             // new tokens of a sequence, as announced
 };
 
 __host__ __device__ constexpr int paged_row_bytes(int type) { return type == kPagedQ8 ? kPagedBlock : kPagedBlock * 2; }

@@ -48,7 +48,7 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedView& c, const Rows
     const PagedSequence sq = paged_sequence(c, r, s);
     if (!sq.ok || t < sq.first || t >= sq.first + sq.news) return p;
     p.pos = sq.length - sq.news + (t - sq.first);
-    if (p.pos < 0 || p.pos >= positions) {
+    if (p.pos < 0 || p.pos >= positions || sq.news > r.most) {
         if ((threadIdx.x & 31) == 0) atomicOr(c.status, kPagedBadPosition);
         return p;
     }

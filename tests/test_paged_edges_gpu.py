@@ -264,3 +264,25 @@ def test_a_sequence_with_a_page_that_is_not_there_is_left_out(cache_type, hd, ne
         assert reported(cache)[0] == 5
     assert torch.equal(cache.attend(0, rows, qs), clean)
     cache.status()
+
+
+def test_chunks_longer_than_announced():
+    rows, pages, _ = make_rows(q, [2, 5, 2], [40, 40, 40], 16, seed=2)
+    cache = q.PagedCache(1, pages, 16, 2, 64)
+    every = whole(q, rows)
+    x = randn(120, 2, 64, seed=1, dtype=torch.float16)
+    cache.append(0, every, None, x, x)
+    qs = randn(9, 4, 64, seed=3, dtype=torch.float16)
+    short = q.PagedRows(rows.starts, rows.lengths, rows.table, 9, 4, 40)
+    clean = cache.attend(0, rows, qs)
+    cache.status()
+    before = cache.read(0, every)
+    out = cache.append(0, short, qs, x[20:29], x[30:39], q_out=torch.full_like(qs, 4))
+    assert bool((out[2:7] == 4).all()) and torch.equal(out[:2], qs[:2]) and reported(cache)[0] == 5
+    after = cache.read(0, every)
+    assert all(torch.equal(a[40:80], b[40:80]) and not torch.equal(a, b) for a, b in zip(after, before))
+    cache.append(0, every, None, x, x)
+    k, _ = cache.read(0, short, k_out=torch.full((9, 2, 64), 4.0, dtype=torch.float16, device="cuda"))
+    assert bool((k[2:7] == 4).all()) and torch.equal(k[:2], x[38:40]) and reported(cache)[0] == 5
+    out = cache.attend(0, short, qs, out=torch.full_like(qs, 4))
+    assert bool((out[2:7] == 4).all()) and torch.equal(out[:2], clean[:2]) and torch.equal(out[7:], clean[7:]) and reported(cache)[0] == 5
