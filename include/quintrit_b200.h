@@ -535,7 +535,7 @@ typedef struct quintrit_b200_paged_attention {
     size_t q_token_stride, q_head_stride;
     void* d_out;
     size_t out_token_stride, out_head_stride;
-    float scale, cap;
+    float scale, cap;          /* scale from -2^30 to 2^30; cap finite, 0: none */
     uint32_t window;
     void* d_workspace;
     size_t workspace_bytes;

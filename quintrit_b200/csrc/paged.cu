@@ -17,6 +17,9 @@ using namespace qtb;
 namespace {
 
 constexpr uint32_t kMagicPaged = 0x51545047u;  // "QTPG"
+// A cap below the first leaves all scores as good as equal, and none above the last touches a score of 16-bit keys and queries; between them, with a scale of up to 2^30, scale / cap and its products with
+// the scales of Q8 rows are ordinary 32-bit numbers.
+constexpr float kPagedLeastCap = 9.31322574615478515625e-10f, kPagedMostCap = 3.777893186295716e22f, kPagedMostScale = 1073741824.0f;  // 2^-30, 2^75, 2^30
 constexpr unsigned int kPagedSpin = 1u << 17;  // tries of a wait (up to 20 us each) before it gives up
 
 int check_cache(const quintrit_b200_paged_cache* c) {
@@ -495,7 +498,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "q_type %d: the cache's type, or F32, F16 or BF16 over a Q8 cache", args->q_type);
         if (!dense_type(args->out_type)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "out_type %d: F32, F16 or BF16", args->out_type);
         if ((rc = check_heads(cache, args->q_heads)) != QUINTRIT_OK) return rc;
-        if (!std::isfinite(args->scale)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "scale must be finite");
+        if (!(std::fabs(args->scale) <= kPagedMostScale)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "scale must be in [-2^30, 2^30]");
         if (!(args->cap >= 0.0f) || !std::isfinite(args->cap)) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "cap must be finite and not negative (0: none)");
         if (args->window > 0x7fffffffu) return fail(QUINTRIT_ERR_INVALID_ARGUMENT, "window %u is too large", args->window);
         if (rows->tokens == 0) return ok();
@@ -518,8 +521,9 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         a.q = args->d_q, a.q_token = args->q_token_stride, a.q_head = args->q_head_stride, a.q_type = args->q_type;
         a.out = args->d_out, a.o_token = args->out_token_stride, a.o_head = args->out_head_stride, a.out_type = args->out_type;
         a.group = group;
-        a.scale = args->cap > 0.0f ? args->scale / args->cap : args->scale * kLog2e;
-        a.cap = args->cap * kLog2e;
+        const bool level = args->cap > 0.0f && args->cap < kPagedLeastCap, capped = !level && args->cap > 0.0f && args->cap <= kPagedMostCap;
+        a.scale = level ? 0.0f : capped ? args->scale / args->cap : args->scale * kLog2e;
+        a.cap = capped ? args->cap * kLog2e : 0.0f;
         a.window = static_cast<int>(args->window);
         a.spin_limit = kPagedSpin;
         const int device = cache->device;

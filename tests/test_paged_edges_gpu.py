@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
-from tests.paged_reference import EPS, make_rows, whole
+from tests.paged_reference import EPS, attention, attention_bound, make_rows, whole
 from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
@@ -286,3 +286,35 @@ def test_chunks_longer_than_announced():
     assert bool((k[2:7] == 4).all()) and torch.equal(k[:2], x[38:40]) and reported(cache)[0] == 5
     out = cache.attend(0, short, qs, out=torch.full_like(qs, 4))
     assert bool((out[2:7] == 4).all()) and torch.equal(out[:2], clean[:2]) and torch.equal(out[7:], clean[7:]) and reported(cache)[0] == 5
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("new", FEW_MANY)
+@pytest.mark.parametrize("cap", [50.0, 1e3, 1e5, 1e9, 1e30, 3e38])
+def test_caps_far_above_the_scores(cache_type, new, cap):
+    """A cap changes a score z by z^3 / (3 cap^2); what is computed is off no further than scores without a cap."""
+    cache, rows, k, v, first = filled(cache_type, 2, 64, [new], [200], 16)
+    qs = queries(cache_type, new, 8, 64, seed=3)
+    out = cache.attend(0, rows, qs, out=torch.empty(new, 8, 64, device="cuda"), scale=1.0, cap=cap)
+    want, mass, size = attention(qs, rows, k, v, first, 1.0, cap)
+    # (the capped score is off by eight half steps more: the quotient, the tangent by 2^-20 of itself, the product)
+    bound = attention_bound(want, mass, size * (1 + 16 / 72), 200, 64, qs.dtype, torch.float32, v, cache_type == "q8", qs.dtype)
+    off = (out.double() - want).abs()
+    assert bool((off <= bound).all()), f"off by {float((off / bound).max()):.2f} bounds"
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("new", FEW_MANY)
+def test_caps_and_scales_next_to_nothing(cache_type, new):
+    """Scores below 2^-30 leave all weights equal."""
+    cache, rows, k, v, first = filled(cache_type, 2, 64, [new], [200], 16)
+    qs = queries(cache_type, new, 8, 64, seed=3)
+    want, mass, size = attention(qs * 0, rows, k, v, first, 0.0)
+    bound = attention_bound(want, mass, size, 200, 64, qs.dtype, torch.float32, v, cache_type == "q8", qs.dtype)
+    for kw in (dict(cap=1e-10), dict(cap=1e-40), dict(scale=0.0), dict(scale=1e-12), dict(scale=1e-40), dict(scale=0.0, cap=1e-40), dict(scale=2.0 ** 30, cap=1e-30)):
+        out = cache.attend(0, rows, qs, out=torch.empty(new, 8, 64, device="cuda"), **kw)
+        assert bool(((out.double() - want).abs() <= bound).all()), kw
+    for scale in (2.0 ** 31, -3e38, float('inf')):
+        with pytest.raises(q.QuintritError) as e:
+            cache.attend(0, rows, qs, scale=scale)
+        assert e.value.code == 2
