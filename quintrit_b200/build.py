@@ -67,6 +67,8 @@ def _compile(source: str, force: bool, verbose: bool, extra) -> tuple:
     stamp, want = obj + ".srchash", _source_hash(_included(path))
     if not force and os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read().strip() == want:
         return obj, ""
+    if os.path.exists(stamp):  # (an object that a compilation left half written, or that was written and not stamped, is nobody's)
+        os.remove(stamp)
     flags = [f for f in NVCC_FLAGS if f != "-shared"]
     cmd = [_nvcc(), *(["-Xptxas", "-v"] if verbose else []), *flags, *extra, "-c", "-o", obj, path]
     r = subprocess.run(cmd, capture_output=True, text=True)
