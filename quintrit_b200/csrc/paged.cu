@@ -191,16 +191,20 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
         // Ranges of at most `length` tiles, the shortest for which they are there at once.
         const size_t per_range = static_cast<size_t>(all) * c->kv_heads;
         const long long longest = tiles_of(0);
-        long long best = longest;
-        for (long long length = longest - 1; length >= 2; --length) {
+        auto fits = [&](long long length) {  // longer ranges are fewer
             long long parts = 0, mapped = 0;
             for (long long o = 0; o < bound && mapped <= kPagedMapped; ++o) {
                 const long long n = (tiles_of(o) + length - 1) / length;
                 mapped += n;
                 if (o < blocks) parts += n;
             }
-            if (parts * m > sms || mapped > kPagedMapped || static_cast<size_t>((longest + length - 1) / length) * per_range > limit) break;
-            best = length;
+            return parts * m <= sms && mapped <= kPagedMapped && static_cast<size_t>((longest + length - 1) / length) * per_range <= limit;
+        };
+        long long best = longest;
+        for (long long low = 2; low < best;) {
+            const long long mid = (low + best) / 2;
+            if (fits(mid)) best = mid;
+            else low = mid + 1;
         }
         if (static_cast<double>(best) + join >= static_cast<double>(longest)) return 0;
         int x = 0;

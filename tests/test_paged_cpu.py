@@ -1,5 +1,6 @@
 """What the paged cache's entry points refuse, without a GPU: a refused call looks at its arguments only, so a handle that owns no memory will do."""
 import ctypes as C
+import time
 
 import pytest
 
@@ -159,3 +160,13 @@ def test_tables_with_room_between_their_rows():
     for more, code in ((dict(table_pages=9), ARG), (dict(table_pages=8), 0), (dict(table_pages=1), 0), (dict(struct_size=_RowsC.table_pages.offset, table_pages=9), 0),
                        (dict(struct_size=_RowsC.table_pages.offset - 1), ARG)):
         assert call("attention_workspace", h, rows(**more), 4, C.byref(n)) == code
+
+
+@pytest.mark.parametrize("head_dim,kv_heads,q_heads,new,sequences", [(64, 1, 4, 60, 1), (128, 4, 32, 257, 2), (256, 4, 12, 200, 1)])
+def test_a_call_is_planned_in_no_time_whatever_length_is_announced(head_dim, kv_heads, q_heads, new, sequences):
+    h, n = handle(head_dim=head_dim, kv_heads=kv_heads), C.c_size_t(0)
+    r = rows(sequences=sequences, tokens=new + sequences - 1, max_new=new, max_length=0x7fff0000, table_stride=1 << 23)
+    t = time.perf_counter()
+    for _ in range(20):
+        assert call("attention_workspace", h, r, q_heads, C.byref(n)) == 0 and n.value > 0
+    assert time.perf_counter() - t < 0.5
