@@ -299,3 +299,82 @@ def test_long_query_rows(heads):
     _near([[_far(got[k, s], want[k, s]) for s in range(2)] for k in range(3)])
     for x in (plain, paged, d):
         x.free()
+
+
+class _ByOperators:
+    """A decoder's passes over a paged cache put together from the operators, called one by one through ``PagedCache``, and the integer products and 32-bit steps of the model's definition (the
+    oracle's) around them: what a batch's passes give, bit for bit."""
+
+    def __init__(self, spec, sequences, cache, page_tokens):
+        import torch
+
+        self.t, self.spec, self.kind = torch, spec, cache
+        H, I, qh, kvh, hd = (spec[k] for k in ("hidden", "inter", "q_heads", "kv_heads", "head_dim"))
+        shapes = [(qh * hd, H), (kvh * hd, H), (kvh * hd, H), (H, qh * hd), (I, H), (I, H), (H, I)]
+        self.weights = [oracle.unpack_planar(w, *shapes[i % 7]).astype(np.float64).T for i, w in enumerate(spec["weights"])]
+        per = -(-spec["ctx"] // page_tokens)
+        self.cache = q.PagedCache(spec["layers"], sequences * per, page_tokens, kvh, hd, cache)
+        self.table = torch.randperm(sequences * per, generator=torch.Generator().manual_seed(1)).to(torch.int32).reshape(sequences, per).cuda()
+        self.angles = torch.tensor(np.stack([oracle.rope_cache(p, spec["rope_dims"], spec["rope_theta"]) for p in range(spec["ctx"])])).cuda()
+        self.embed = np.asarray(spec["embed"], np.uint16).view(np.float16).reshape(-1, H).astype(np.float32)
+        self.head = np.asarray(spec["embed"] if spec["lm_head"] is None else spec["lm_head"], np.uint16).reshape(-1, H)
+
+    def rows(self, sequences, new, lengths, longest):
+        i32 = lambda v: self.t.tensor(v, dtype=self.t.int32, device="cuda")
+        return q.PagedRows(i32([0] + list(np.cumsum(new))), i32(lengths), self.table[i32(sequences).long()], int(sum(new)), max(new), longest)
+
+    def project(self, rows, l, *which):
+        """Rows of 32-bit values through projections: [rows][outputs] each."""
+        out = [[] for _ in which]
+        for x in rows:
+            codes, s = oracle.quantize_int8(x)
+            for o, k in zip(out, which):
+                o.append(oracle.rescale((codes.astype(np.float64) @ self.weights[l * 7 + k]).astype(np.int32), float(self.spec["scales"][l * 7 + k]), float(s)))
+        return [np.stack(o) for o in out]
+
+    def forward(self, tokens, rows, wanted):
+        """Logits of the packed tokens `wanted`."""
+        spec, torch = self.spec, self.t
+        qh, kvh, hd = (spec[k] for k in ("q_heads", "kv_heads", "head_dim"))
+        norm = lambda x, w: x if w is None else np.stack([oracle.rms_norm(r, w, spec["eps"]) for r in x])
+        x = self.embed[np.asarray(tokens, np.int64)]
+        n = len(x)
+        for l in range(spec["layers"]):
+            w = spec["norms"][l * 4:l * 4 + 4]
+            heads = [torch.tensor(y).reshape(n, -1, hd).cuda() for y in self.project(norm(x, w[0]), l, 0, 1, 2)]
+            q_out = torch.empty(n, qh, hd, dtype={"f16": torch.float16, "bf16": torch.bfloat16, "q8": torch.float32}[self.kind], device="cuda")
+            self.cache.append(l, rows, *heads, q_out=q_out, cos_sin=self.angles, neox=spec["arch"] != q.ARCH_LLAMA)
+            o = self.cache.attend(l, rows, q_out, out=torch.empty(n, qh, hd, device="cuda"), scale=float(np.float32(1) / np.sqrt(np.float32(hd))))
+            x = x + self.project(norm(o.reshape(n, -1).cpu().numpy(), w[2]), l, 3)[0]
+            g, u = self.project(norm(x, w[1]), l, 4, 5)
+            y = np.stack([(oracle.relu2_mul if spec["arch"] == q.ARCH_BITNET else oracle.swiglu)(a, b) for a, b in zip(g, u)])
+            x = x + self.project(norm(y, w[3]), l, 6)[0]
+        self.cache.status()
+        last = [oracle.f32_to_f16_bits(r) for r in norm(x[wanted], spec["out_norm"])]
+        return np.stack([[oracle.vec_dot_f16(row, r) for row in self.head] for r in last])
+
+
+@pytest.mark.parametrize("cache,page_tokens", [("f16", 16), ("bf16", 64), ("q8", 32)])
+@pytest.mark.parametrize("arch,heads", [(q.ARCH_LLAMA, (4, 2, 64)), (q.ARCH_BITNET, (4, 1, 64)), (q.ARCH_LLAMA, (6, 2, 128)), (q.ARCH_BITNET, (3, 1, 256)), (q.ARCH_LLAMA, (40, 1, 64))])
+def test_passes_are_the_operators_one_by_one(arch, heads, cache, page_tokens):
+    spec = _spec(arch, 200, ctx=512, heads=heads, tied=arch == q.ARCH_BITNET)
+    lengths = [1, 3, 150, 41, 333]
+    prompts = _prompts(lengths, spec["vocab"])
+    fed = [synth.prompt_tokens(70 + k, len(lengths), spec["vocab"]) for k in range(3)]
+    d = q.Decoder(spec)
+    got, b = _run(d, prompts, fed, pages=sum(-(-(n + 3) // page_tokens) for n in lengths), page_tokens=page_tokens, cache=cache)
+    one = _ByOperators(spec, len(lengths), cache, page_tokens)
+    want = [np.concatenate([one.forward(p, one.rows([s], [len(p)], [len(p)], len(p)), [len(p) - 1]) for s, p in enumerate(prompts)])]
+    every = sorted(range(len(lengths)), key=lambda s: -lengths[s])  # a step takes its longest sequences first; where their tiles are cut into ranges goes by that
+    for k, tokens in enumerate(fed):
+        out = one.forward([tokens[s] for s in every], one.rows(every, [1] * len(every), [lengths[s] + k + 1 for s in every], spec["ctx"]), list(range(len(every))))
+        want.append(out[np.argsort(every)])
+    want = np.stack(want).astype(np.float32)
+    for s, n in enumerate(lengths):
+        whole = one.rows([s], [n + 3], [n + 3], n + 3)
+        for l in range(spec["layers"]):
+            for x, y in zip(b.read_cache(l, s), one.cache.read(l, whole, dtype=one.t.float32)):
+                assert np.array_equal(x, y.reshape(n + 3, -1).cpu().numpy()), (s, l)
+    assert np.array_equal(got.view(np.uint32), want.view(np.uint32))
+    for x in (b, d):
+        x.free()
