@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
-from tests.paged_reference import EPS, attention, attention_bound, make_rows, whole
+from tests.paged_reference import EPS, attention, attention_bound, make_rows, places, whole
 from tests.test_paged_gpu import TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
@@ -290,7 +290,7 @@ def test_chunks_longer_than_announced():
 
 @pytest.mark.parametrize("cache_type", TYPES)
 @pytest.mark.parametrize("new", FEW_MANY)
-@pytest.mark.parametrize("cap", [50.0, 1e3, 1e5, 1e9, 1e30, 3e38])
+@pytest.mark.parametrize("cap", [50.0, 64.0, 64.1, 1e3, 1e5, 1e9, 1e30, 3e38])
 def test_caps_far_above_the_scores(cache_type, new, cap):
     """A cap changes a score z by z^3 / (3 cap^2); what is computed is off no further than scores without a cap."""
     cache, rows, k, v, first = filled(cache_type, 2, 64, [new], [200], 16)
@@ -318,3 +318,27 @@ def test_caps_and_scales_next_to_nothing(cache_type, new):
         with pytest.raises(q.QuintritError) as e:
             cache.attend(0, rows, qs, scale=scale)
         assert e.value.code == 2
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new,group,lengths", [([1], 1, [20011]), ([1], 4, [65431]), ([3], 1, [20011]), ([20], 4, [20011]), ([130], 4, [9001]), ([700], 2, [2900]), ([1, 1, 1], 4, [9001, 40, 20011]),
+                                               ([1, 3, 1, 2] * 10, 3, [100 + 471 * i for i in range(40)]), ([1, 70, 3, 200], 4, [9001, 3000, 20011, 700])])
+@pytest.mark.parametrize("window", [0, 4097])
+def test_every_position_counts_once(cache_type, hd, new, group, lengths, window):
+    """All scores are zero and a value is 0 or 1: a result is a count over a count, and one position too many or too few among 65431 is seen, at whatever edge of a tile, range or segment."""
+    rows, pages, _ = make_rows(q, new, lengths, 64, seed=4)
+    cache = q.PagedCache(1, pages, 64, 1, hd, cache_type)
+    every = whole(q, rows)
+    k, v = randn(every.tokens, 1, hd, seed=1), (randn(every.tokens, 1, hd, seed=2) > 0).float()
+    cache.append(0, every, None, k, v)
+    qs = torch.zeros(rows.tokens, group, hd, device="cuda", dtype=torch.bfloat16 if cache_type == "bf16" else torch.float16)
+    out = cache.attend(0, rows, qs, out=torch.empty(qs.shape, device="cuda"), window=window)
+    count = torch.cat([torch.zeros(1, hd, device="cuda", dtype=torch.float64), v[:, 0].double().cumsum(0)])
+    s, p = (torch.tensor(x, device="cuda") for x in zip(*places(rows)))
+    first = every.starts.long()[s]
+    low = (p - window + 1).clamp_min(0) if window else torch.zeros_like(p)
+    want = (count[first + p + 1] - count[first + low]) / (p + 1 - low)[:, None].double()
+    # The weights are one and counts are exact, but for two roundings of the quotient. Q8 adds reciprocals of scales: up to 64 in a row, a range's tiles and the ranges, fewer than 256 terms, half a step each.
+    assert bool(((out.double() - want[:, None]).abs() <= want[:, None] * 2.0 ** (-16 if cache_type == "q8" else -22)).all())
+    cache.status()
