@@ -132,27 +132,27 @@ int allow_smem(Kernel kernel, int bytes, int device, std::atomic<uint64_t>& done
     return QUINTRIT_OK;
 }
 
-template <int TYPE, int BLOCKS, int NT>
+template <int TYPE, int BLOCKS, int NT, bool FAR>
 int launch_few(const PagedAttnArgs& a, int device, dim3 grid, cudaStream_t s) {
     using F = PagedFew<TYPE, BLOCKS, NT>;
     static_assert(F::kSmem <= 227 * 1024, "the ring does not fit");
     static std::atomic<uint64_t> done{0};
-    const int rc = allow_smem(paged_few_kernel<TYPE, BLOCKS, NT>, F::kSmem, device, done);
+    const int rc = allow_smem(paged_few_kernel<TYPE, BLOCKS, NT, FAR>, F::kSmem, device, done);
     if (rc != QUINTRIT_OK) return rc;
-    paged_few_kernel<TYPE, BLOCKS, NT><<<grid, F::kThreads, F::kSmem, s>>>(a);
+    paged_few_kernel<TYPE, BLOCKS, NT, FAR><<<grid, F::kThreads, F::kSmem, s>>>(a);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
-template <int TYPE, int BLOCKS>
+template <int TYPE, int BLOCKS, bool FAR>
 int launch_few_rows(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
-    if (nt == 1) return launch_few<TYPE, BLOCKS, 1>(a, device, grid, s);
+    if (nt == 1) return launch_few<TYPE, BLOCKS, 1, FAR>(a, device, grid, s);
     if constexpr (TYPE == kPagedQ8 && BLOCKS == 2)
-        if (nt == 3) return launch_few<TYPE, BLOCKS, 3>(a, device, grid, s);
-    return launch_few<TYPE, BLOCKS, 2>(a, device, grid, s);
+        if (nt == 3) return launch_few<TYPE, BLOCKS, 3, FAR>(a, device, grid, s);
+    return launch_few<TYPE, BLOCKS, 2, FAR>(a, device, grid, s);
 }
-template <int TYPE>
+template <int TYPE, bool FAR>
 int launch_few_type(const PagedAttnArgs& a, int device, int nt, dim3 grid, cudaStream_t s) {
-    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1>(a, device, nt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2>(a, device, nt, grid, s) : launch_few_rows<TYPE, 4>(a, device, nt, grid, s);
+    return a.c.blocks == 1 ? launch_few_rows<TYPE, 1, FAR>(a, device, nt, grid, s) : a.c.blocks == 2 ? launch_few_rows<TYPE, 2, FAR>(a, device, nt, grid, s) : launch_few_rows<TYPE, 4, FAR>(a, device, nt, grid, s);
 }
 // Blocks of the kernel for few rows on all multiprocessors, by tiles of 8 rows.
 template <int TYPE>
@@ -231,22 +231,34 @@ size_t schedule_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged
     g->whole = static_cast<int>(whole), g->cut = best;
     return slots(best);
 }
-template <int TYPE, int BLOCKS, int NT>
+template <int TYPE, int BLOCKS, int NT, bool FAR>
 int launch_many_of(const PagedAttnArgs& a, const PagedSchedule& g, int device, unsigned grid, cudaStream_t s) {
     using M = PagedMany<TYPE, BLOCKS, NT>;
     static_assert(M::kSmem <= 227 * 1024, "the rings do not fit");
     static std::atomic<uint64_t> done{0};
-    const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS, NT>, M::kSmem, device, done);
+    const int rc = allow_smem(paged_many_kernel<TYPE, BLOCKS, NT, FAR>, M::kSmem, device, done);
     if (rc != QUINTRIT_OK) return rc;
-    paged_many_kernel<TYPE, BLOCKS, NT><<<grid, M::kThreads, M::kSmem, s>>>(a, g);
+    paged_many_kernel<TYPE, BLOCKS, NT, FAR><<<grid, M::kThreads, M::kSmem, s>>>(a, g);
     QTB_LAUNCH_CHECK();
     return QUINTRIT_OK;
 }
-template <int TYPE>
+template <int TYPE, bool FAR>
 int launch_many_type(const PagedAttnArgs& a, const PagedSchedule& g, int device, int rows, unsigned grid, cudaStream_t s) {
-    if (a.c.blocks == 4) return launch_many_of<TYPE, 4, 1>(a, g, device, grid, s);
-    if (rows == 128) return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 1>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 1>(a, g, device, grid, s);
-    return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 2>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 2>(a, g, device, grid, s);
+    if (a.c.blocks == 4) return launch_many_of<TYPE, 4, 1, FAR>(a, g, device, grid, s);
+    if (rows == 128) return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 1, FAR>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 1, FAR>(a, g, device, grid, s);
+    return a.c.blocks == 1 ? launch_many_of<TYPE, 1, 2, FAR>(a, g, device, grid, s) : launch_many_of<TYPE, 2, 2, FAR>(a, g, device, grid, s);
+}
+// By the cache's type and the cap. Up to a cap of 64 one exponential's error of 2^-22 of the cap is 2^-16 of a weight and below its rounding; in the same kernels the series took 52.5 us of a mixed batch
+// under a cap of 30 instead of 49.6, and, not even called, 421 us of 2048 tokens over Q8 instead of 410.
+constexpr float kPagedNearCap = 64.0f;
+template <typename Launch>
+int by_type(const PagedAttnArgs& a, int32_t type, Launch launch) {
+    auto with = [&](auto far) {
+        constexpr bool FAR = decltype(far)::value;
+        return type == kPagedF16 ? launch(std::integral_constant<int, kPagedF16>(), std::bool_constant<FAR>()) : type == kPagedBf16 ? launch(std::integral_constant<int, kPagedBf16>(), std::bool_constant<FAR>())
+                                                                                                                           : launch(std::integral_constant<int, kPagedQ8>(), std::bool_constant<FAR>());
+    };
+    return a.cap > kPagedNearCap * kLog2e ? with(std::true_type()) : with(std::false_type());
 }
 
 // Launches a kernel that joins results, 256 threads to a block: it comes up while the one before it in the stream still runs, and waits for that one's end itself.
@@ -537,8 +549,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             PagedSchedule& g = plan.schedule;
             g.part_o = reinterpret_cast<float*>(workspace + plan.few_bytes), g.part_ml = reinterpret_cast<float2*>(g.part_o + plan.part_rows * cache->head_dim);
             const unsigned grid = static_cast<unsigned>(plan.many_blocks);
-            rc = cache->type == kPagedF16 ? launch_many_type<kPagedF16>(a, g, device, plan.many_rows, grid, s) : cache->type == kPagedBf16 ? launch_many_type<kPagedBf16>(a, g, device, plan.many_rows, grid, s)
-                                                                                                                         : launch_many_type<kPagedQ8>(a, g, device, plan.many_rows, grid, s);
+            rc = by_type(a, cache->type, [&](auto type, auto far) { return launch_many_type<decltype(type)::value, decltype(far)::value>(a, g, device, plan.many_rows, grid, s); });
             if (rc != QUINTRIT_OK) return rc;
             if (plan.part_rows > 0) {
                 auto kernel = a.c.blocks == 1 ? paged_join_kernel<1> : a.c.blocks == 2 ? paged_join_kernel<2> : paged_join_kernel<4>;
@@ -552,8 +563,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
             a.part_o = reinterpret_cast<float*>(workspace);
             a.part_ml = reinterpret_cast<float2*>(a.part_o + static_cast<size_t>(plan.few_share) * 2 * block_rows * cache->head_dim);
             const dim3 grid = plan.few_share > 0 ? dim3(static_cast<unsigned>(plan.few_share)) : dim3(cache->kv_heads, rows->sequences);
-            rc = cache->type == kPagedF16 ? launch_few_type<kPagedF16>(a, device, plan.nt, grid, s) : cache->type == kPagedBf16 ? launch_few_type<kPagedBf16>(a, device, plan.nt, grid, s)
-                                                                                                                                : launch_few_type<kPagedQ8>(a, device, plan.nt, grid, s);
+            rc = by_type(a, cache->type, [&](auto type, auto far) { return launch_few_type<decltype(type)::value, decltype(far)::value>(a, device, plan.nt, grid, s); });
             if (rc != QUINTRIT_OK) return rc;
             if (plan.few_share > 1) {
                 auto kernel = a.c.blocks == 1 ? paged_combine_kernel<1> : a.c.blocks == 2 ? paged_combine_kernel<2> : paged_combine_kernel<4>;

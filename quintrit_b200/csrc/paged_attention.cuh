@@ -68,11 +68,14 @@ __device__ __forceinline__ float rcp(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// tanh, off by 2^-20 of itself: below 1/4 the first terms of its series (the next one is 2^-21.5 of the sum there), else from one exponential, 1 - 2 / (1 + e^2x), which is off by about 2^-22 of one whatever x
-// is (so that alone, under a cap of 10^5, it spoiled scores by hundredths); the infinities of the exponential give -1 and 1.
+// tanh from one exponential: 1 - 2 / (1 + e^2x), off by about 2^-22 of one whatever x is; the infinities of the exponential give -1 and 1. SMALL: off by 2^-20 of itself, as a cap far above the scores asks
+// for (the exponential alone spoils them by hundredths under a cap of 10^5): below 1/4 the first terms of the series, the next of which is 2^-21.5 of their sum there.
+template <bool SMALL>
 __device__ __forceinline__ float tanh_of(float x) {
+    const float y = 1.0f - 2.0f * rcp(1.0f + ex2(x * (2.0f * kLog2e)));
+    if constexpr (!SMALL) return y;
     const float t = x * x, near = fmaf(x * t, fmaf(t, fmaf(t, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), x);
-    return fabsf(x) < 0.25f ? near : 1.0f - 2.0f * rcp(1.0f + ex2(x * (2.0f * kLog2e)));
+    return fabsf(x) < 0.25f ? near : y;
 }
 
 template <bool BF16>
@@ -209,15 +212,15 @@ struct PagedFew {
 
 // The pages of the tiles of [begin, end), TILE positions each, for a whole warp that asks tile after tile: 32 entries of the table at a time, one to a lane, the next 32 under way meanwhile (with a read for every tile, which
 // was checked at once, a ring filled at a tile in 1700 cycles). Pieces in front of position `seen` are nobody's to look at: their pages may have been given back.
-// A page that the cache does not have is reported and raises `bad`; page 0 stands in for it, and the results are not written.
+// A page that the cache does not have is reported; page 0 stands in for it, and `bad` (of the lane that asked for it) says that the results are not to be written.
 template <int TILE>
 struct PagedPages {
     const PagedView& c;
     const int* table;
-    volatile unsigned int* bad;
+    bool bad;
     int begin, end, seen, lane, step, per, now, next;  // step: positions of a piece, a page or 64 of it; per: pieces of a tile
-    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end, int seen, volatile unsigned int* bad)
-        : c(c), table(table), bad(bad), begin(begin), end(end), seen(seen), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
+    __device__ __forceinline__ PagedPages(const PagedView& c, const int* table, int begin, int end, int seen)
+        : c(c), table(table), bad(false), begin(begin), end(end), seen(seen), lane(threadIdx.x & 31), step(min(1 << c.page_log2, kPagedTile)), per(TILE / step), now(0) {
         next = fetch(0);
     }
     __device__ __forceinline__ int fetch(int piece) const {
@@ -230,7 +233,7 @@ struct PagedPages {
             now = next, next = fetch(first + 32);
             if (now < 0 || now >= c.pages) {
                 atomicOr(c.status, kPagedBadPage);
-                *bad = 1, now = 0;
+                bad = true, now = 0;
             }
         }
         return __shfl_sync(0xffffffffu, now, (at + lane) & 31);
@@ -238,15 +241,15 @@ struct PagedPages {
 };
 
 // Brings the tiles of [begin, end), of which the positions from `seen` on are looked at, of one KV head into the two rings, tile i into ring i & 1, keys and values one unit after the other; run by one
-// whole warp. base0, base1: units that the rings have seen before. Returns with its own copies landed.
+// whole warp. base0, base1: units that the rings have seen before. Returns with its own copies landed, whether a page that this lane asked for is not there.
 template <int TYPE, int BLOCKS, int NT>
-__device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, int seen, uint32_t rings, uint32_t full, uint32_t empty,
-                                                 int base0, int base1, volatile unsigned int* abort_flag, volatile unsigned int* bad_flag, unsigned int limit) {
+__device__ __forceinline__ bool paged_load_tiles(const PagedView& c, const int* table, int head, int begin, int end, int seen, uint32_t rings, uint32_t full, uint32_t empty,
+                                                 int base0, int base1, volatile unsigned int* abort_flag, unsigned int limit) {
     using namespace gemm_detail;
     using F = PagedFew<TYPE, BLOCKS, NT>;
     constexpr int kRow = paged_row_bytes(TYPE), kRows = paged_rows_bytes<TYPE, BLOCKS>(), U = F::kUnits;
     const int lane = threadIdx.x & 31, P = 1 << c.page_log2, PR = min(P, kPagedTile);
-    PagedPages<kPagedTile> pages_of(c, table, begin, end, seen, bad_flag);
+    PagedPages<kPagedTile> pages_of(c, table, begin, end, seen);
     int tile = 0, asked0 = base0, asked1 = base1;  // units asked for, of either ring
     bool okay = true;
     for (int k0 = begin; k0 < end && okay; k0 += kPagedTile, ++tile) {
@@ -270,9 +273,10 @@ __device__ __forceinline__ void paged_load_tiles(const PagedView& c, const int* 
     }
     for (int ring = 0; ring < 2; ++ring)
         for (int asked = ring ? asked1 : asked0, n = max(ring ? base1 : base0, asked - U); n < asked; ++n) mbar_wait(full + 8 * (ring * U + n % U), (n / U) & 1, abort_flag, limit, false);
+    return pages_of.bad;
 }
 
-template <int TYPE, int BLOCKS, int NT>
+template <int TYPE, int BLOCKS, int NT, bool FAR>  // FAR: the cap is far above the scores
 __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew<TYPE, BLOCKS, NT>::kBlocksPerSm) paged_few_kernel(const __grid_constant__ PagedAttnArgs a) {
     using namespace gemm_detail;
     using namespace paged_detail;
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     unsigned char* s_q = smem + F::kBody;                                       // [kRows][kPitch]
     float* s_rowf = reinterpret_cast<float*>(s_q + F::kRows * kPitch);          // [kRows]: what a row's score is multiplied by
     uint64_t* bars = reinterpret_cast<uint64_t*>(s_rowf + F::kRows);
-    volatile unsigned int *abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U), *bad_flag = abort_flag + 1;  // bad: the segment's sequence has a page that is not there
+    volatile unsigned int* abort_flag = reinterpret_cast<volatile unsigned int*>(bars + 4 * U);
     __shared__ int s_before[kPagedShared + 1];
     __shared__ int4 s_of[kPagedShared];
     const uint32_t full = smem_u32(bars), empty = full + 16 * U;
@@ -329,10 +333,10 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
     const int rows = sq.news * a.group, p0 = sq.length - sq.news;
     range.end = max(range.begin, range.end);
     const int tiles = (range.end - range.begin + kPagedTile - 1) / kPagedTile;
-    if (tid == 0) *bad_flag = 0;
+    bool bad = false;
     __syncthreads();  // the barriers are there; the segment before has left the ring
     if (warp == 8) {
-        paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, paged_first_seen(a, sq, 0), ring, full, empty, base0, base1, abort_flag, bad_flag, a.spin_limit);
+        bad = paged_load_tiles<TYPE, BLOCKS, NT>(a.c, a.r.table + static_cast<size_t>(seq) * a.r.stride, kvh, range.begin, range.end, paged_first_seen(a, sq, 0), ring, full, empty, base0, base1, abort_flag, a.spin_limit);
     } else {
         // queries: a warp takes rows warp, warp + 8, ...; a lane 8 values or none; all of them are asked for before the first is used
         auto load_rows = [&](auto of) {
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 #pragma unroll
             for (int i = 0; i < 2; ++i) rowf[n][i] = s_rowf[n * 8 + c4 * 2 + i], m[n][i] = -INFINITY, l[n][i] = 0.0f;
         // positions that every row sees; outside of them the masks are worked out
-        const int window = paged_window(a, sq), all_last = p0, all_first = a.window > 0 ? sq.length - window : 0;
+        const int all_last = p0, all_first = a.window > 0 ? sq.length - a.window : 0;
         float o[KS][NT][4];
 #pragma unroll
         for (int j = 0; j < KS; ++j)
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                     }
                     if (a.cap > 0.0f) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[n][e] = a.cap * tanh_of(sc[n][e]);
+                        for (int e = 0; e < 4; ++e) sc[n][e] = a.cap * tanh_of<FAR>(sc[n][e]);
                     }
                     if constexpr (Q8) {
 #pragma unroll
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int rr = n * 8 + c4 * 2 + (e & 1), p = p0 + rr / a.group, j = key0 + g + 8 * (e >> 1);
-                            if (rr >= rows || j > p || j >= range.end || (a.window > 0 && j <= p - window)) sc[n][e] = -INFINITY;
+                            if (rr >= rows || j > p || j >= range.end || (a.window > 0 && j <= static_cast<int>(static_cast<unsigned int>(p) - a.window))) sc[n][e] = -INFINITY;
                         }
                     }
 #pragma unroll
@@ -616,18 +620,13 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
                 }
         }
     }
-    __syncthreads();
+    const bool left_out = __syncthreads_or(bad);  // the segment's sequence has a page that is not there
     if (*abort_flag != 0) return;
     // rows out: eight values to a thread
-    const bool left_out = *bad_flag != 0;
     const float* joined = reinterpret_cast<const float*>(smem);
     const float2* mls = reinterpret_cast<const float2*>(smem + 8 * F::kRows * F::kJoinPitch * 4);
     for (int i = tid; i < rows * (HD / 8); i += kThreads) {
         const int r = i / (HD / 8), e0 = i % (HD / 8) * 8;
-        if (left_out) {
-            if (parts_place >= 0 && e0 == 0) a.part_ml[static_cast<size_t>(parts_place) * F::kRows + r] = paged_left_out();
-            continue;
-        }
         float top = -INFINITY, w[8], sum = 0.0f, x[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, mls[k * F::kRows + r].x);
@@ -649,6 +648,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         const size_t t = static_cast<size_t>(sq.first) + r / a.group;
         const int h = kvh * a.group + r % a.group;
         if (parts_place < 0) {
+            if (left_out) continue;
             const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // (a sum that is no number stays one)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] *= inv;
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(PagedFew<TYPE, BLOCKS, NT>::kThreads, PagedFew
         } else {
             const size_t row = static_cast<size_t>(parts_place) * F::kRows + r;
             paged_store8(a.part_o + row * HD + e0, kPagedF32, x);
-            if (e0 == 0) a.part_ml[row] = make_float2(top, sum);
+            if (e0 == 0) a.part_ml[row] = left_out ? paged_left_out() : make_float2(top, sum);
         }
     }
     base0 += (tiles + 1) / 2 * 2, base1 += tiles / 2 * 2;

@@ -159,7 +159,7 @@ template <int N> __device__ __forceinline__ void registers_down() { asm volatile
 
 }  // namespace paged_detail
 
-template <int TYPE, int BLOCKS, int NT>
+template <int TYPE, int BLOCKS, int NT, bool FAR>  // FAR: the cap is far above the scores
 __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) paged_many_kernel(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PagedSchedule g) {
     using namespace gemm_detail;
     using namespace paged_detail;
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
             const int* table = a.r.table + static_cast<size_t>(own.x) * a.r.stride;
             const int P = 1 << a.c.page_log2, PR = min(P, kPagedTile);
             constexpr int kRing = Q8 ? RW : RS;
-            PagedPages<KT> pages_of(a.c, table, range.begin, range.end, paged_first_seen(a, sq, r0 / a.group), bad_flag);
+            PagedPages<KT> pages_of(a.c, table, range.begin, range.end, paged_first_seen(a, sq, r0 / a.group));
             int n = 0;
             bool okay = true;
             for (int j = 0; j < tiles && okay; ++j) {
@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     }
                 }
             }
+            if (pages_of.bad) *bad_flag = 1;
             __syncwarp();
             if (lane == 0) mbar_arrive(pages_known);
             for (int back = max(0, n - kRing); back < n; ++back) mbar_wait(Q8 ? raw_full(back % kRing) : full(back % kRing), (back / kRing) & 1, abort_flag, a.spin_limit, false);
@@ -526,7 +527,7 @@ __global__ void __launch_bounds__(PagedMany<TYPE, BLOCKS, NT>::kThreads, 1) page
                     for (int e = 0; e < 32; ++e) {
                         float x = __uint_as_float(s[c][e]);
                         if constexpr (Q8) x *= reinterpret_cast<const float*>(f)[c * 32 + e];
-                        x = a.cap * tanh_of(x * rowf);
+                        x = a.cap * tanh_of<FAR>(x * rowf);
                         if constexpr (Q8) x += reinterpret_cast<const float*>(f)[KT + c * 32 + e];
                         s[c][e] = __float_as_uint(x);
                     }
