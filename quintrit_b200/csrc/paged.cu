@@ -524,7 +524,7 @@ extern "C" int quintrit_b200_paged_attention_device(quintrit_b200_paged_cache_t*
         const int group = static_cast<int>(args->q_heads / cache->kv_heads);
         PagedPlan plan;
         plan_of(cache, rows, args->q_heads, args->window, &plan);
-        if (plan.many_blocks > 0x7fffffffLL || static_cast<long long>(rows->tokens) * args->q_heads > 0x7fffffffLL)
+        if (plan.many_blocks > 0x7fffffffLL || static_cast<long long>(rows->tokens) * args->q_heads > 0x7fff0000LL)  // (rows are counted in 32 bits, up to whole row blocks)
             return fail(QUINTRIT_ERR_INVALID_SHAPE, "%u new tokens of %u query heads are too many for one call", rows->max_new, args->q_heads);
         const size_t need = plan.few_bytes + plan.many_bytes;
         if (need > 0 && args->d_workspace == nullptr) return fail(QUINTRIT_ERR_NULL_POINTER, "d_workspace is NULL, %zu bytes are needed", need);

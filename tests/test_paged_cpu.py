@@ -170,3 +170,9 @@ def test_a_call_is_planned_in_no_time_whatever_length_is_announced(head_dim, kv_
     for _ in range(20):
         assert call("attention_workspace", h, r, q_heads, C.byref(n)) == 0 and n.value > 0
     assert time.perf_counter() - t < 0.5
+
+
+def test_more_rows_than_can_be_counted_are_refused():
+    h = handle(kv_heads=1)
+    for tokens, q_heads in ((1 << 24, 128), ((1 << 24) - 1, 128), (1 << 15, 65536)):
+        assert call("attention_device", h, 0, rows(tokens=tokens, max_new=tokens), attention(q_heads=q_heads, q_token_stride=64 * q_heads, out_token_stride=64 * q_heads), None) == SHAPE
