@@ -285,8 +285,9 @@ struct PagedPlan {
     size_t part_rows;
     size_t few_bytes, many_bytes;  // of the workspace
 };
-// Rows of a KV head up to which the kernel for few rows takes a sequence. With the few rows' kernel and the many rows' one, us: 16 sequences of 3000, heads of 128, F16: 12 rows 39 and 48,
-// 20 rows 51 and 47; Q8: 12 rows 40 and 66, 20 rows 49 and 67, 32 rows 80 and 67; heads of 64, F16: 12 rows 26 and 28, 32 rows 32 and 27; heads of 256, F16: 12 rows 58 and 59, 48 rows 104 and 61.
+// Rows of a KV head up to which the kernel for few rows takes a sequence: two row tiles of 8, three where their sums' registers are there. With it and with the many rows' kernel, us, 16 sequences of 3000, 4 KV heads,
+// 8, 12 and 16 rows: F16, heads of 64: 22, 24, 25 and 32, 32, 32; of 128: 29, 31, 31 and 38, 38, 39; of 256: 45, 54, 55 and 54, 57, 56; Q8, heads of 64: 21, 23, 23 and 43, 43, 44; of 128: 22, 29, 30 and 46, 47, 46
+// (20 and 24 rows: 36, 37 and 47, 47); of 256: 35, 43, 45 and 62, 65, 66.
 inline int few_rows(const quintrit_b200_paged_cache* c) { return c->type == kPagedQ8 && c->head_dim == 128 ? 24 : 16; }
 constexpr size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 void plan_of(const quintrit_b200_paged_cache* c, const quintrit_b200_paged_rows_t* r, uint32_t q_heads, uint32_t window, PagedPlan* p) {

@@ -8,7 +8,7 @@
 // Q8 rows: k_j = ks_j a_j, v_j = vs_j b_j with integer codes. The codes go into the products as they are (exact in F16), ks_j multiplies the score, and
 // vs_j goes into the exponent: with y_j = z_j + log2(vs_j) the weights w_j = 2^(y_j - m), m the maximum of y, are what multiplies b_j, and l = sum w_j / vs_j.
 // So the weights that are rounded to F16 lie in [0, 256] whatever the scales are, and the cache's limits on them keep the terms of l from vanishing. Queries are scaled by a power of two per row to a maximum in [1, 2),
-// which is exact, so BF16 and F32 queries of any size meet F16 codes.
+// which is exact, so BF16 and F32 queries of any size meet F16 codes (F32 queries are rounded to F16's 11 bits then).
 //
 // Bound by the rows' bytes: 2 G flops per byte of a 16-bit cache. A block of threads takes one KV head of one sequence, up to 16 rows of queries (24 of 128 values, Q8; a row
 // is a (token, head of the group)) and a range of its positions; one warp brings the pages, tile by tile of 64 positions, into a ring in shared memory with bulk copies;

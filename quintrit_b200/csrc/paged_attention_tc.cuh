@@ -15,9 +15,9 @@
 // positions and four buffers kept the threads busier and the tensor cores less: an instruction over 64 positions took 87 cycles, one over 128 took 100. 64-value heads apart, 2048 tokens behind 14336:
 // 461 us against 318 us.)
 //
-// Measured: 296 query heads of 128 over 37 KV heads, 256 tokens behind 16384, whole waves: F16 1125 TFLOP/s (69% of the library's matrix product), Q8 870; 2048 tokens of 20 heads of 128 behind
-// 14336: F16 304 us, 1059 TFLOP/s, Q8 396 us, 813; 12 heads of 256: F16 390 us, 990. Q8 waits for its weights: with one score buffer to a row tile its products and its exponentials, 3200 cycles
-// a tile with the scales, follow one another (two threads to a row there too, of 96 registers each: Q8 528 us, F16 342).
+// Measured: 296 query heads of 128 over 37 KV heads, 256 tokens behind 16384, whole waves: F16 1141 TFLOP/s (70% of the library's matrix product), Q8 851; 2048 tokens of 20 heads of 128 behind
+// 14336: F16 314 us, 1027 TFLOP/s, Q8 398 us, 809; 12 heads of 256: F16 382 us, 1013. With one score buffer to a row tile its products and its exponentials, 3200 cycles
+// a tile with Q8's scales, follow one another (two threads to a row there too, of 96 registers each: Q8 528 us, F16 342).
 #pragma once
 #include "packed_f32.cuh"
 #include "paged_attention.cuh"

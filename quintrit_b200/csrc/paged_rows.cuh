@@ -7,11 +7,11 @@
 // Reading (paged_read_kernel): the same rows back, code times scale, rounded to the output type.
 //
 // Writing: sixteen values to a thread, two pieces of eight half a head apart, so that the pairs of a rotation lie in one thread whether they are neighbours or halves of a head (eight
-// values to a thread, the halves exchanged through shared memory: 45 us for the prompt below, now 33.5). Norm and maximum are exchanges within the 4 to 16 threads of a head. Reading: eight
+// values to a thread, the halves exchanged through shared memory: 40 us for the prompt below, now 29). Norm and maximum are exchanges within the 4 to 16 threads of a head. Reading: eight
 // values to a thread. A warp takes U groups of heads of one token. Both kernels are bound by the bytes they move, small calls by
 // their latency: a row's address needs four dependent reads (starts, length, page), so the heads' values are asked for before them, and where there are
-// tokens enough for it, groups of heads share one address (writing: two, which keep the registers at 80; four took 36 us, one 38.6; reading: four). Writing 4096 tokens of 32 + 2 x 4 heads of
-// 128 with norm, rotation and Q8: 92.5 MB in 33.5 us, 42% of the copy rate; the multiprocessors issue in 55% of their cycles, 120 instructions for sixteen values of a warp. Reading 112000 positions
+// tokens enough for it, groups of heads share one address (writing: two, which keep the registers at 80; four took 36 us with the rows' way back, one 38.6, two 33.5; reading: four). Writing 4096 tokens of 32 + 2 x 4 heads of
+// 128 with norm, rotation and Q8: 79.8 MB in 28.7 us, 42% of the copy rate; the multiprocessors issue in 55% of their cycles, 120 instructions for sixteen values of a warp. Reading 112000 positions
 // of 4 heads of 256 values, Q8 to F16: 459 MB in 85.5 us, 82%.
 #pragma once
 #include "paged_cache.cuh"
