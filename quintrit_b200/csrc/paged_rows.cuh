@@ -105,16 +105,24 @@ __global__ void __launch_bounds__(kPagedRowThreads, 3) paged_append_kernel(const
         paged_load8(raw[u][1].v, TYPE, *reinterpret_cast<float(*)[8]>(x + 8));
         if (a.q_norm != nullptr || a.k_norm != nullptr) {
             const float* w = k < 0 ? a.q_norm : value ? nullptr : a.k_norm;
-            float sum = 0.0f;
+            float sum = 0.0f, eps = a.eps;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (w != nullptr && sum == INFINITY) {  // squares beyond 32 bits (the same for all threads of a head): of the values over 2^70 instead, beside which eps is nothing
+                const unsigned int head = (0xffffffffu >> (32 - LANES)) << (sub * LANES);
+                sum = 0.0f, eps = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] *= 0x1p-70f, sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(head, sum, o);
+            }
             if (w != nullptr) {
                 float f[16];
                 paged_load8(w + e0, kPagedF32, *reinterpret_cast<float(*)[8]>(f));
                 paged_load8(w + e0 + HALF, kPagedF32, *reinterpret_cast<float(*)[8]>(f + 8));
-                const float inv = rsqrtf(sum * (1.0f / HD) + a.eps);  // (off by 2^-22 at most)
+                const float inv = rsqrtf(sum * (1.0f / HD) + eps);  // (off by 2^-22 at most)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[i] = x[i] * inv * f[i];
             }

@@ -3,8 +3,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import quintrit_b200 as q
-from tests.paged_reference import EPS, attention, attention_bound, make_rows, places, whole
-from tests.test_paged_gpu import TYPES, check_attention, filled, randn
+from tests.paged_reference import EPS, attention, attention_bound, make_rows, places, whole, written
+from tests.test_paged_gpu import DT, TYPES, check_attention, filled, randn
 
 pytestmark = pytest.mark.gpu
 FEW_MANY = [1, 60]  # new tokens of four heads to a key head: the kernel for few rows, the one for many
@@ -289,16 +289,16 @@ def test_chunks_longer_than_announced():
 
 
 @pytest.mark.parametrize("cache_type", TYPES)
-@pytest.mark.parametrize("new", FEW_MANY)
+@pytest.mark.parametrize("hd,new", [(64, 1), (64, 3), (64, 60), (128, 1), (128, 3), (128, 5), (128, 20), (128, 60), (256, 1), (256, 3), (256, 60)])
 @pytest.mark.parametrize("cap", [50.0, 64.0, 64.1, 1e3, 1e5, 1e9, 1e30, 3e38])
-def test_caps_far_above_the_scores(cache_type, new, cap):
+def test_caps_far_above_the_scores(cache_type, hd, new, cap):
     """A cap changes a score z by z^3 / (3 cap^2); what is computed is off no further than scores without a cap."""
-    cache, rows, k, v, first = filled(cache_type, 2, 64, [new], [200], 16)
-    qs = queries(cache_type, new, 8, 64, seed=3)
-    out = cache.attend(0, rows, qs, out=torch.empty(new, 8, 64, device="cuda"), scale=1.0, cap=cap)
+    cache, rows, k, v, first = filled(cache_type, 2, hd, [new], [200], 16)
+    qs = queries(cache_type, new, 8, hd, seed=3)
+    out = cache.attend(0, rows, qs, out=torch.empty(new, 8, hd, device="cuda"), scale=1.0, cap=cap)
     want, mass, size = attention(qs, rows, k, v, first, 1.0, cap)
     # (the capped score is off by eight half steps more: the quotient, the tangent by 2^-20 of itself, the product)
-    bound = attention_bound(want, mass, size * (1 + 16 / 72), 200, 64, qs.dtype, torch.float32, v, cache_type == "q8", qs.dtype)
+    bound = attention_bound(want, mass, size * (1 + 16 / (hd + 8)), 200, hd, qs.dtype, torch.float32, v, cache_type == "q8", qs.dtype)
     off = (out.double() - want).abs()
     assert bool((off <= bound).all()), f"off by {float((off / bound).max()):.2f} bounds"
 
@@ -342,3 +342,23 @@ def test_every_position_counts_once(cache_type, hd, new, group, lengths, window)
     # The weights are one and counts are exact, but for two roundings of the quotient. Q8 adds reciprocals of scales: up to 64 in a row, a range's tiles and the ranges, fewer than 256 terms, half a step each.
     assert bool(((out.double() - want[:, None]).abs() <= want[:, None] * 2.0 ** (-16 if cache_type == "q8" else -22)).all())
     cache.status()
+
+
+@pytest.mark.parametrize("hd,in_type", [(64, "f32"), (128, "bf16"), (256, "f32")])
+def test_norms_of_values_whose_squares_leave_32_bits(hd, in_type):
+    """A head of such values is as long as any other behind its norm; its neighbours in a warp are what they are without it."""
+    rows, pages, _ = make_rows(q, [6], [6], 16)
+    cache = q.PagedCache(1, pages, 16, 3, hd, "f16")
+    size = torch.tensor([1.0, 1e19, 1e25, 3e37, 1e-3, 1e20], device="cuda")[:, None, None]
+    x = randn(6, 10, hd, seed=1)
+    x = (x / x.abs().amax(-1, keepdim=True) * torch.where(torch.arange(10, device="cuda")[:, None] % 2 == 0, size, torch.ones_like(size))).to(DT[in_type])
+    w = 1 + 0.3 * randn(hd, seed=2)
+    out = cache.append(0, rows, x[:, :4], x[:, 4:7], x[:, 7:], q_norm=w, k_norm=w, eps=1e-6, q_out=torch.empty(6, 4, hd, device="cuda"))
+    k, _ = cache.read(0, rows, dtype=torch.float32)
+    at = torch.arange(6, device="cuda")
+    for got, heads, half in ((out, x[:, :4], 0.0), (k, x[:, 4:7], EPS[torch.float16])):
+        want = written(heads, w, 1e-6, None, False, at)
+        bound = want.abs() * half + want.abs().amax(-1, keepdim=True) * (hd / 2 + 16) * 2.0 ** -24
+        assert bool(((got.double() - want).abs() <= bound).all())
+    with pytest.raises(q.QuintritError):  # the values themselves are too large for F16
+        cache.status()
